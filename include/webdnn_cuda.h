@@ -333,6 +333,67 @@ int wdc_attention(wdc_context* ctx, const wdc_attention_desc* d, const float* q,
  * negated when bit 7 is set, bit-identical to the reference's table lookup.  Both buffers 16-byte aligned. */
 int wdc_decode_eightbit(wdc_context* ctx, const void* codes, float* out, int64_t n, float scale);
 
+/* ---- a decoder's cache in 8 bits --------------------------------------------------------------
+ * Keys and values of the tokens a decoder has seen, in pages of one pool (no counterpart in the reference, whose graphs
+ * keep nothing between runs).  A page holds page_tokens tokens of one sequence:
+ *   codes  int8    [2 (keys, values)][kv_heads][page_tokens][head_size]
+ *   scales float32 [2][kv_heads]
+ * and a number is code * scale.  A pool of several layers is [layers][pages] of these: a page has the same index in every
+ * layer, and the calls of one layer take the address of that layer's first page.
+ * page_table is int32 [batch][table_pages]: the pages of each sequence in order.  lengths is int32 [batch]: the tokens of
+ * each sequence, those of this call included; counts is int32 [batch] or NULL: how many of them are new, the last ones (NULL:
+ * `tokens` of each).  Row i of k, v, q and y is a sequence's i-th new token; rows from its count on are padding.
+ * page_tokens is 16, 32, 64 or 128, head_size 32, 64 or 128 (else WDC_ERR_UNSUPPORTED).  Strides are non-negative multiples
+ * of 4 floats, buffers 16-byte aligned (int32 ones and scales 4-byte).
+ * A sequence whose length is negative, beyond its table row or below its count, a count outside 0 .. tokens, and a page outside
+ * 0 .. pages - 1 are left out on the device (nothing of them is read or written, their rows of y are zero or do without that
+ * page's tokens) and the next waiting call returns WDC_ERR_INVALID once. */
+typedef struct wdc_cache_append_desc {
+  int64_t pages, kv_heads, page_tokens, head_size;
+  int64_t batch, tokens, table_pages;
+  int64_t k_sb, k_sh, k_st; /* strides of k: sequence, head, token */
+  int64_t v_sb, v_sh, v_st;
+} wdc_cache_append_desc;
+/* Writes the new tokens.  The scale of a page and head is max |x| / 127 over its tokens: where the page holds older tokens it
+ * only grows, and their codes are then rounded again, rint(code * old scale / new scale).  A new code is rint(x / scale), ties
+ * to even.  A page and head that is given an infinity or a NaN stands for NaN until its first token is written again.
+ * No page may be that of two sequences of the call, other than pages that the call does not write. */
+int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d, const float* k, const float* v, void* codes,
+                     float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts);
+typedef struct wdc_cache_attention_desc {
+  int64_t pages, kv_heads, page_tokens, head_size;
+  int64_t batch, tokens, table_pages;
+  int64_t heads; /* of the queries, a multiple of kv_heads: head h reads the keys of head h / (heads / kv_heads) */
+  int64_t q_sb, q_sh, q_st;
+  int64_t y_sb, y_sh, y_st;
+  float scale;
+} wdc_cache_attention_desc;
+/* y = softmax(scale * q k^T) v of every new token over its sequence's tokens up to itself, all of them in the cache
+ * already (wdc_cache_append first).  Rows of padding are zero, and so are those of an empty sequence. */
+int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
+                        const float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts,
+                        float* y);
+/* Copies pages, codes and scales, in every layer: page from[i] to page to[i] for i < n.  from and to are HOST arrays, read before
+ * the call returns.  No page may be written twice, nor read and written. */
+typedef struct wdc_cache_pages_desc {
+  int64_t layers, pages, kv_heads, page_tokens, head_size;
+} wdc_cache_pages_desc;
+int wdc_cache_copy_pages(wdc_context* ctx, const wdc_cache_pages_desc* d, void* codes, float* scales, int64_t n,
+                         const int32_t* from, const int32_t* to);
+
+/* Log probabilities under softmax(logits), logits [rows][vocab] with rows row_stride floats apart (no counterpart in the
+ * reference, which ends at Softmax).  Any of the results may be NULL (top_ids and top_logprobs together):
+ *   logprob [rows]             of the tokens int32 [rows] (NULL: no logprob); NaN for a token outside 0 .. vocab - 1
+ *   entropy [rows]             -sum p log p, in nats
+ *   top_ids int32 [rows][top], top_logprobs [rows][top]  the `top` largest logits, largest first, ties by the lower index
+ * 0 <= top <= 32 and top <= vocab; vocab < 2^31.  Logits of -inf have no part in the sums; a row with nothing else, with +inf or
+ * with a NaN has NaN in place of every logarithm, and in the order a NaN stands above everything. */
+typedef struct wdc_logprobs_desc {
+  int64_t rows, vocab, row_stride, top;
+} wdc_logprobs_desc;
+int wdc_token_logprobs(wdc_context* ctx, const wdc_logprobs_desc* d, const float* logits, const int32_t* tokens,
+                       float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs);
+
 /* ---- LSTM -----------------------------------------------------------------------------------
  * ONNX LSTM, forward direction, default activations, no peepholes (not in the reference; ONNX
  * operator spec).  X [T, Bt, I], W [4H, I], R [4H, H], bias [8H] or NULL, h0/c0 [Bt, H] or NULL;

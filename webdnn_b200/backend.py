@@ -25,7 +25,7 @@ from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 
-from .lib import (DTYPE_CODE, ConvDesc, CudaBackendError, GemmDesc, Library, PoolDesc, i64_array)
+from .lib import (DTYPE_CODE, ConvDesc, CudaBackendError, GemmDesc, Library, LogprobsDesc, PoolDesc, i64_array)
 
 NP_DTYPE = {"float32": np.float32, "int32": np.int32, "bool": np.uint8}
 
@@ -146,6 +146,19 @@ class CudaSharedBuffer:
         if self.ref_count == 0 and self.ptr is not None:
             self.context._free(self.ptr)
             self.ptr = None
+
+
+class BorrowedBuffer(CudaSharedBuffer):
+    """Device memory of someone else's, which it leaves alone and whose owner it keeps alive."""
+
+    def __init__(self, context: "WebDNNCudaContext", byte_length: int, ptr: int, owner):
+        self.context, self.byte_length, self.ptr, self.owner = context, byte_length, ptr, owner
+        self.ref_count = 1
+
+    def dispose(self) -> None:
+        self.ref_count -= 1
+        if self.ref_count == 0:
+            self.ptr = self.owner = None
 
 
 class CudaTensor(TensorImpl):
@@ -274,6 +287,7 @@ class WebDNNCudaContext:
         self.handle = None
         self.precision = "tf32x3"
         self.profile = False      # backendOptions.cuda.profile: NVTX range "name(opType)" around every node
+        self.caches: Dict[str, object] = {}   # add_cache
 
     # --- lifecycle
     def initialize(self) -> None:
@@ -392,6 +406,21 @@ class WebDNNCudaContext:
     def empty_tensor(self, dims: Sequence[int], data_type: str = "float32", layout: str = "nchw") -> CudaTensor:
         return CudaTensor(self, dims, data_type, layout=layout)
 
+    def borrow_tensor(self, address: int, dims: Sequence[int], data_type: str = "float32", owner=None) -> CudaTensor:
+        """A tensor over device memory that another library of the process allocated on this GPU (row-major, 16-byte
+        aligned); ``owner`` is kept alive with it.  The context's work on it is queued on the context's stream: what
+        other streams do with the memory has to be ordered by the caller (``stream_handle``, ``sync``)."""
+        if address % 16:
+            raise ValueError("borrow_tensor: the memory is not 16-byte aligned")
+        size = 4
+        for d in dims:
+            if d < 0:
+                raise ValueError("borrow_tensor: negative dimension")
+            size *= d
+        if size and not address:
+            raise ValueError("borrow_tensor: no memory")
+        return CudaTensor(self, dims, data_type, BorrowedBuffer(self, size, address, owner))
+
     def move_tensor(self, tensor, option=None) -> CudaTensor:
         if isinstance(tensor, EightbitCPUTensor):
             return self.decode_eightbit(tensor.codes, tensor.scale, tensor.dims)
@@ -403,6 +432,16 @@ class WebDNNCudaContext:
         """``t`` holds a constant of the model: nothing queued from now on writes it (``wdc_declare_constant``)."""
         t.constant = True
         self._call("wdc_declare_constant", c_void_p(t.ptr), t.length * 4)
+
+    def add_cache(self, name: str, cache) -> None:
+        """Makes a ``PagedCache`` of this context known to its graphs, whose CudaCacheAttention nodes name it.  It stays for the
+        context's life: recorded runs hold its address, like a weight's."""
+        if cache.context is not self:
+            raise ValueError("add_cache: the cache belongs to another context")
+        if name in self.caches:
+            raise ValueError(f"add_cache: there is a cache {name!r} already")
+        cache.registered = True
+        self.caches[name] = cache
 
     def decode_eightbit(self, codes: np.ndarray, scale: float, dims: Sequence[int]) -> CudaTensor:
         """float32 tensor from the 8-bit codes of a WDN2 container: the codes (1 byte per element)
@@ -554,6 +593,45 @@ class WebDNNCudaContext:
             self._call("wdc_gemm_columns", byref(desc), columns, *operands)
         else:
             self._call("wdc_gemm", byref(desc), *operands)
+
+    def token_logprobs(self, logits: CudaTensor, tokens: Optional[CudaTensor] = None, top: int = 0,
+                       vocab: Optional[int] = None, out: Optional[Sequence[Optional[CudaTensor]]] = None):
+        """Log probabilities under softmax(logits) (``wdc_token_logprobs``): (logprob, entropy, top_ids, top_logprobs).
+
+        ``logits`` float32 [..., n], of which the first ``vocab`` columns count (all, if not given); ``tokens`` int32, one
+        for each row (without: logprob is None); ``top`` up to 32 best alternatives, ties by the lower index (0: the last two
+        are None).  Results have the leading dims of ``logits``; they are written to ``out`` where that is given, in which an
+        entry of None leaves that result out."""
+        self.asserts_cuda_tensor(logits)
+        if logits.ndim < 1 or logits.data_type != "float32" or logits.layout != "nchw":
+            raise TypeError("token_logprobs: logits are float32 rows")
+        width = logits.dims[-1]
+        lead, vocab = logits.dims[:-1], width if vocab is None else int(vocab)
+        rows = logits.length // width if width else 0
+        if not 0 < vocab <= width:
+            raise ValueError(f"token_logprobs: vocab {vocab} of rows of {width}")
+        if not 0 <= top <= min(32, vocab):
+            raise ValueError(f"token_logprobs: top {top} is not 0 .. {min(32, vocab)}")
+        if tokens is not None:
+            self.asserts_cuda_tensor(tokens)
+            if tokens.data_type != "int32" or tokens.length != rows:
+                raise TypeError(f"token_logprobs: tokens are one int32 for each of {rows} rows")
+        if out is None:
+            out = (self.empty_tensor(lead) if tokens is not None else None, self.empty_tensor(lead),
+                   self.empty_tensor(lead + [top], "int32") if top else None, self.empty_tensor(lead + [top]) if top else None)
+        else:
+            if len(out) != 4 or (tokens is None and out[0] is not None):
+                raise ValueError("token_logprobs: out is (logprob, entropy, top_ids, top_logprobs)")
+            for t, n, kind in zip(out, (rows, rows, rows * top, rows * top), ("float32", "float32", "int32", "float32")):
+                if t is not None:
+                    self.asserts_cuda_tensor(t)
+                    if t.length != n or t.data_type != kind:
+                        raise ValueError(f"token_logprobs: a result has {n} values of {kind}")
+        if rows:
+            at = [c_void_p(t.ptr) if t is not None and t.length else None for t in out]
+            self._call("wdc_token_logprobs", byref(LogprobsDesc(rows, vocab, width, top)), c_void_p(logits.ptr),
+                       c_void_p(tokens.ptr) if tokens is not None else None, *at)
+        return tuple(out)
 
     def conv2d(self, desc: ConvDesc, x, w, scale, shift, residual, y) -> None:
         def p(t):

@@ -82,6 +82,9 @@ struct wdc_context {
   std::vector<ProfRec> prof;
 };
 
+// The word behind status_word's first that the kernels over a paged cache set when they leave something out.
+constexpr int WDC_STATUS_CACHE = 1;
+
 int wdc_fail(wdc_context* ctx, int code, const char* fmt, ...);
 int wdc_check_cuda(wdc_context* ctx, cudaError_t e, const char* what);
 int wdc_check_launch(wdc_context* ctx, const char* kernel);

@@ -480,6 +480,10 @@ static int report_device_status(wdc_context* ctx) {
     *word = 0;
     return wdc_fail(ctx, WDC_ERR_DEVICE_WAIT, "a bounded device-side wait expired (kernel status %d)", code);
   }
+  if (word[WDC_STATUS_CACHE] != 0) {
+    word[WDC_STATUS_CACHE] = 0;
+    return wdc_fail(ctx, WDC_ERR_INVALID, "a cache call was given a length, count or page out of range; that part was left out");
+  }
   return WDC_OK;
 }
 

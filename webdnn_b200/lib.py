@@ -62,6 +62,24 @@ class AttentionDesc(Structure):
                                        "k_st", "v_sb", "v_sh", "v_st", "y_sb", "y_sh", "y_st")] + [("scale", c_float)]
 
 
+class CacheAppendDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("pages", "kv_heads", "page_tokens", "head_size", "batch", "tokens", "table_pages",
+                                       "k_sb", "k_sh", "k_st", "v_sb", "v_sh", "v_st")]
+
+
+class CacheAttentionDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("pages", "kv_heads", "page_tokens", "head_size", "batch", "tokens", "table_pages",
+                                       "heads", "q_sb", "q_sh", "q_st", "y_sb", "y_sh", "y_st")] + [("scale", c_float)]
+
+
+class CachePagesDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("layers", "pages", "kv_heads", "page_tokens", "head_size")]
+
+
+class LogprobsDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("rows", "vocab", "row_stride", "top")]
+
+
 class PoolDesc(Structure):
     _fields_ = [(n, c_int64) for n in (
         "batch", "ch", "in_h", "in_w", "out_h", "out_w", "k_h", "k_w", "stride_h", "stride_w",
@@ -87,6 +105,10 @@ SIGNATURES = {
     "wdc_instance_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                   ctypes.c_double]),
     "wdc_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "wdc_cache_append": (c_int, [c_void_p, POINTER(CacheAppendDesc)] + [c_void_p] * 7),
+    "wdc_cache_attention": (c_int, [c_void_p, POINTER(CacheAttentionDesc)] + [c_void_p] * 7),
+    "wdc_cache_copy_pages": (c_int, [c_void_p, POINTER(CachePagesDesc), c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "wdc_token_logprobs": (c_int, [c_void_p, POINTER(LogprobsDesc)] + [c_void_p] * 6),
     "wdc_decode_eightbit": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_float]),
     "wdc_capture_begin": (c_int, [c_void_p]),
     "wdc_capture_end": (c_int, [c_void_p, POINTER(c_void_p)]),

@@ -357,6 +357,62 @@ class CudaAttention(OperatorImpl):
         return [y]
 
 
+class CudaCacheAttention(OperatorImpl):
+    """A decoder layer's self-attention over a paged 8-bit cache: the new tokens' keys and values are appended, then the
+    new tokens attend to their sequences.  No operator of the reference, whose graphs keep nothing between runs.
+
+    Inputs q, k, v [batch, tokens, width], page_table [batch, pages], lengths [batch] and, optionally, counts [batch] (int32, as
+    ``PagedCache.batch`` gives them); the result is [batch, tokens, heads * head_size].  Attributes: ``cache``, the name the
+    cache was given (``WebDNNCudaContext.add_cache``); ``layer``; ``scale`` (1 / sqrt(head_size) unless given); ``heads``
+    and ``q_column``, ``k_column``, ``v_column`` where an operand is some columns of its tensor."""
+
+    def __init__(self):
+        super().__init__("cuda")
+
+    def initialize(self, attribute):
+        self.cache = get_attr_string(attribute, "cache", "")
+        self.layer = get_attr_int(attribute, "layer", 0)
+        self.heads = get_attr_int(attribute, "heads", 0) or None
+        scale = get_attr_float(attribute, "scale", 0.0)
+        self.scale = scale if any(a.name == "scale" for a in attribute) else None
+        self.columns = [get_attr_int(attribute, f"{key}_column", 0) for key in ("q", "k", "v")]
+
+    def run(self, context, inputs, n_outputs):
+        context.asserts_cuda_tensor_array(inputs)
+        if len(inputs) not in (5, 6):
+            raise ValueError("CudaCacheAttention: inputs are q, k, v, page_table, lengths and, optionally, counts")
+        cache = context.caches.get(self.cache)
+        if cache is None:
+            raise ValueError(f"CudaCacheAttention: the context has no cache {self.cache!r}")
+        q, k, v, *where = inputs
+        cache.append(self.layer, k, v, *where, k_column=self.columns[1], v_column=self.columns[2])
+        return [cache.attention(self.layer, q, *where, heads=self.heads, q_column=self.columns[0], scale=self.scale)]
+
+
+class CudaTokenLogProbs(OperatorImpl):
+    """Log probabilities of given tokens, entropy and the ``top`` best alternatives of softmax(logits).  No operator of the
+    reference, whose graphs end at Softmax (softmax.ts:15-59).
+
+    Inputs logits [..., vocab] and, optionally, tokens (int32, one for each row); results logprob (with tokens only), entropy,
+    and with ``top`` top_ids and top_logprobs."""
+
+    def __init__(self):
+        super().__init__("cuda")
+
+    def initialize(self, attribute):
+        self.top = get_attr_int(attribute, "top", 0)
+
+    def run(self, context, inputs, n_outputs):
+        context.asserts_cuda_tensor_array(inputs)
+        logits = context.canonical(inputs[0])
+        outs = [t for t in context.token_logprobs(logits, inputs[1] if len(inputs) > 1 else None, self.top) if t is not None]
+        if logits is not inputs[0]:
+            logits.dispose()
+        for t in outs[n_outputs:]:
+            t.dispose()
+        return outs[:n_outputs]
+
+
 def _packed_weight(context: WebDNNCudaContext, w: CudaTensor) -> CudaTensor:
     """[Cout, Cin/g, kh, kw] -> [Cout, kh, kw, Cin/g], cached on the (persistent) weight tensor."""
     pk = w.aux.get("krsc")
@@ -1135,6 +1191,8 @@ def get_op_entries() -> List[OperatorEntry]:
         E("CudaGemmRelu", 1, None, "cuda", lambda: CudaGemm(relu=True)),
         E("CudaMatMulBias", 1, None, "cuda", CudaMatMulBias),
         E("CudaAttention", 1, None, "cuda", CudaAttention),
+        E("CudaCacheAttention", 1, None, "cuda", CudaCacheAttention),
+        E("CudaTokenLogProbs", 1, None, "cuda", CudaTokenLogProbs),
         E("MatMul", 1, None, "cuda", CudaMatMul),
         E("Conv", 1, None, "cuda", CudaConv),
         E("CudaConvFused", 1, None, "cuda", lambda: CudaConv(fused=True)),

@@ -17,7 +17,7 @@ from typing import Dict, List, Tuple
 
 import numpy as np
 
-from .onnx_io import FLOAT, Graph, Model, ValueInfo, make_node, make_tensor
+from .onnx_io import FLOAT, INT32, Graph, Model, ValueInfo, make_node, make_tensor
 
 
 class _Builder:
@@ -243,6 +243,31 @@ def lstm(seq: int = 128, batch: int = 64, input_size: int = 256, hidden: int = 5
     return b.model([("X", [seq, batch, input_size])],
                    [(y, [seq, 1, batch, hidden]), (yh, [1, batch, hidden]), (yc, [1, batch, hidden])],
                    name="lstm")
+
+
+def decoder(vocab: int = 1000, d: int = 256, heads: int = 8, kv_heads: int = 2, layers: int = 4, ffn: int = 1024,
+            positions: int = 4096, top: int = 8, cache: str = "cache") -> Model:
+    """Post-norm decoder whose layers attend over a paged 8-bit cache (``PagedCache``, known to the context as ``cache``), any
+    number of sequences and new tokens.  Inputs, all int32: token_ids and places [batch, tokens] (of rows behind a
+    sequence's count: anything), page_table, lengths and counts as ``PagedCache.batch`` gives them, rows [n]: which of the
+    batch * tokens rows have their logits computed, and tokens [n]: whose log probabilities are wanted.  Outputs of those
+    rows: logprob, entropy [n], top_ids and top_logprobs [n, top]."""
+    b = _Builder(0)
+    t = _Transformer(b, 0, d, heads, ffn)
+    table = b.init("embedding", b.rng.standard_normal((vocab, d)).astype(np.float32))
+    place = b.init("place_embedding", b.rng.standard_normal((positions, d)).astype(np.float32))
+    h = b.node("Add", [b.node("Gather", [table, "token_ids"], axis=0)[0], b.node("Gather", [place, "places"], axis=0)[0]])[0]
+    for layer in range(layers):
+        q, k, v = t.linear(h, d, d), t.linear(h, d, kv_heads * t.dh), t.linear(h, d, kv_heads * t.dh)
+        a = b.node("CudaCacheAttention", [q, k, v, "page_table", "lengths", "counts"], cache=cache, layer=layer)[0]
+        h = t.add_norm(h, t.linear(a, d, d))
+        h = t.add_norm(h, t.feed_forward(h))
+    h = b.node("Gather", [b.node("Reshape", [h, t.shape([-1, d])])[0], "rows"], axis=0)[0]
+    outs = b.node("CudaTokenLogProbs", [t.linear(h, d, vocab), "tokens"], n_out=4, top=top)
+    ints = [("token_ids", 2), ("places", 2), ("page_table", 2), ("lengths", 1), ("counts", 1), ("rows", 1), ("tokens", 1)]
+    g = Graph("decoder", b.nodes, b.inits, [ValueInfo(n, INT32, [0] * rank) for n, rank in ints],
+              [ValueInfo(o, kind, []) for o, kind in zip(outs, (FLOAT, FLOAT, INT32, FLOAT))])
+    return Model(g, ir_version=7, opset_import=[("", 13)], producer_name="webdnn_b200.zoo")
 
 
 def make_input(shape, kind: str = "normal", seed: int = 1) -> np.ndarray:
