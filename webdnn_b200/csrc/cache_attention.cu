@@ -1,12 +1,11 @@
 // Attention of new tokens over a paged cache in 8 bits:  y = softmax(scale * q k^T) v,  k = code * (scale of page and head).
 // The reference has no such operator.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include "paged_cache.cuh"
 
 namespace {
-
-constexpr int THREADS = 128;
 
 struct CacheAttArgs {
   const float* q;
@@ -17,68 +16,405 @@ struct CacheAttArgs {
   int* status;
   int64_t pages, table_pages;
   int64_t q_sb, q_sh, q_st, y_sb, y_sh, y_st;
-  int tokens, heads, kv_heads, group, page_tokens;
-  float scale_log2;   // scale * log2(e): the softmax runs on exp2
+  int batch, tokens, heads, kv_heads, group, page_tokens;
+  int row_tiles, splits;
+  float *part_rows, *part_stats;   // of every unit and split: O of its rows; m, M and l
+  float scale_log2;                // scale * log2(e): the softmax runs on exp2
 };
 
-// One CTA per (sequence, new token, query head); warp w takes tokens w, w + 4, ..., a lane DH / 32 channels, and the warps'
-// maxima, sums and rows are joined at the end.
+// A unit of work is eight rows of one sequence and key head, row = new token * group + query head of the group, and one of
+// `splits` ranges of the tokens they see.  Its four warps take tiles of 32 tokens in turn, each through a ring of its own in shared
+// memory that asynchronous copies fill three tiles ahead, so that no warp waits for another before the end.
+//
+// Both products run on mma.m16n8k16 with float16 operands and 32-bit sums.  A code (-127 .. 127) is exact in float16; a
+// query is split into a high and a low half, 22 bits together, and so is a weight.  The halves are the two halves of the
+// instruction's 16 rows: eight rows with both halves are one instruction, and their sums meet in one thread's registers.
+//
+// Weights carry the value scale of their page.  With s the scores (base 2) and lv = log2(value scale) of a group of 16 tokens,
+//   m = max s,  l = sum 2^(s - m);      M = max (s + lv),  O = sum 2^(s + lv - M) code,      y = O 2^(M - m) / l,
+// so that what is split into halves is relative to the largest term of O, whatever the pages' scales are.
+constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, STAGES = 3, ROWS = 8;
+constexpr float WEIGHT_BITS = 14.f;        // weights are up to 2^14: both halves stay in float16's normal range
+constexpr int QUERY_BITS = 13;             // a row's queries are scaled to less than 2^14
+
 template <int DH>
-__global__ void __launch_bounds__(THREADS) cache_attention_kernel(const CacheAttArgs a) {
-  constexpr int C = DH / 32, WARPS = THREADS / 32;
+struct Layout {
+  static constexpr int SCALES = 2 * TILE * DH;                       // behind a stage's keys and values: four scales
+  static constexpr int STAGE = SCALES + 16, RING = STAGES * STAGE;
+  static constexpr int STRIDE = DH + 4, STATS = ROWS * STRIDE;       // floats: a row when the warps join; behind them m, M, l
+  static constexpr int PART = STATS + 3 * ROWS;
+  static constexpr int SMEM = WARPS * (RING > PART * 4 ? RING : PART * 4);
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// Two halves of a pair: h = x in float16, l = what is missing.
+__device__ __forceinline__ void split(float x, float y, uint32_t& h, uint32_t& l) {
+  const __half2 hi = __floats2half2_rn(x, y);
+  const float2 back = __half22float2(hi);
+  h = half2_bits(hi);
+  l = half2_bits(__floats2half2_rn(x - back.x, y - back.y));
+}
+// Two bytes of a word of codes + 128 as float16: 0x6400 + byte is 1024 + byte.
+template <int SELECT>
+__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
+  const uint32_t u = __byte_perm(w, 0x64646464u, SELECT);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+  return half2_bits(v);
+}
+
+// Where the 16-byte chunk `c` of token `t` lies in a tile of keys or values: as in memory, chunks of a 128-byte line exchanged
+// so that the eight (16-byte loads), sixteen (8) or 32 (4) threads that load at a time meet different banks.
+template <int DH>
+__device__ __forceinline__ int key_at(int t, int c) {
+  const int x = t * (DH / 16) + c;
+  return (DH == 128 ? x ^ (t & 1) << 2 : x) * 16;
+}
+template <int DH>
+__device__ __forceinline__ int value_at(int t, int c) {
+  const int x = t * (DH / 16) + c;
+  return (DH == 32 ? x ^ (t >> 2 & 1) << 1 : x ^ (t >> 1 & 3) << 1) * 16;
+}
+template <int BYTES>
+__device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[BYTES / 4]) {
+  if (BYTES == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[BYTES > 4] = v.y; w[BYTES / 8] = v.z; w[BYTES / 4 - 1] = v.w;
+  } else if (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[BYTES / 4 - 1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; i++) w[i] ^= 0x80808080u;
+}
+
+__device__ __forceinline__ float finite_or_0(float x) { return x == -INFINITY ? 0.f : x; }   // a reference to subtract
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+
+template <int DH>
+__global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const CacheAttArgs a) {
+  constexpr int STEPS = DH / 16;                  // of the score product's sum; also columns of O a thread and key row
+  constexpr int KB = DH == 32 ? 8 : 16;           // bytes of a key a thread loads at a time
+  constexpr int VB = DH / 8;                      // bytes of a value row a thread loads
+  using L = Layout<DH>;
+  extern __shared__ __align__(16) unsigned char smem[];
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = (int)(blockIdx.x % (unsigned)a.heads), rest = (int)(blockIdx.x / (unsigned)a.heads);
-  const int i = rest % a.tokens, b = rest / a.tokens;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int part = (int)(blockIdx.x % (unsigned)a.splits), unit = (int)(blockIdx.x / (unsigned)a.splits);
+  const int tile = unit % a.row_tiles, bh = unit / a.row_tiles, kvh = bh % a.kv_heads, b = bh / a.kv_heads;
   const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages * a.page_tokens, a.status);
-  const int last = i < span.count ? span.length - span.count + i : -1;   // the token itself
-  const float* q = pdl_after(a.q) + b * a.q_sb + h * a.q_sh + i * a.q_st;
-  float qc[C], o[C], m = -INFINITY, l = 0.f;
+  const int row = tile * ROWS + g, token = row / a.group, head = kvh * a.group + row % a.group;   // this thread's row
+  const int last = token < span.count ? span.length - span.count + token : -1;    // the last token it sees
+  const int top_token = min((tile * ROWS + ROWS - 1) / a.group, span.count - 1);  // the tile's last row that is no padding
+  const int seen = tile * ROWS / a.group < span.count ? span.length - span.count + top_token + 1 : 0;
+  const int tiles = (seen + TILE - 1) / TILE;
+  const int first = (int)((int64_t)part * tiles / a.splits), end = (int)((int64_t)(part + 1) * tiles / a.splits);
+  const int32_t* table = a.page_table + (int64_t)b * a.table_pages;
+  const int64_t block_bytes = (int64_t)a.page_tokens * DH, side_bytes = a.kv_heads * block_bytes;
+  unsigned char* ring = smem + warp * L::RING;
+
+  // Copies tile i of the sequence to a stage; bit 0 and 1 of the answer: its two groups of 16 tokens are there.
+  auto fetch = [&](int i, int stage) -> uint32_t {
+    uint32_t there = 0;
+    unsigned char* to = ring + stage * L::STAGE;
 #pragma unroll
-  for (int c = 0; c < C; c++) {
-    qc[c] = last >= 0 ? pdl_ld(q + lane * C + c) * a.scale_log2 : 0.f;
-    o[c] = 0.f;
-  }
-  for (int t = warp; t <= last; t += WARPS) {
-    const int page = cache_page(a.page_table + (int64_t)b * a.table_pages, t / a.page_tokens, a.pages, a.status);
-    if (page < 0) continue;
-    const int64_t block = (int64_t)page * 2 * a.kv_heads + h / a.group;
-    const int8_t* k = pdl_after(a.codes) + (block * a.page_tokens + t % a.page_tokens) * DH + lane * C;
-    const int8_t* v = k + (int64_t)a.kv_heads * a.page_tokens * DH;
-    float s = 0.f;
+    for (int group = 0; group < 2; group++) {
+      const int t0 = i * TILE + group * 16;
+      const int page = i < end && t0 < seen ? cache_page(table, t0 / a.page_tokens, a.pages, a.status) : -1;
+      if (page >= 0) {
+        there |= 1u << group;
+        const int64_t block = (int64_t)page * 2 * a.kv_heads + kvh;
+        const int8_t* k = a.codes + block * block_bytes + (t0 % a.page_tokens) * DH;
 #pragma unroll
-    for (int c = 0; c < C; c++) s = fmaf(qc[c], (float)k[c], s);
-#pragma unroll
-    for (int w = 1; w < 32; w <<= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= pdl_ld(a.scales + block);
-    const float vs = pdl_ld(a.scales + block + a.kv_heads);
-    const float top = fmaxf(m, s);
-    const float keep = top == -INFINITY ? 1.f : exp2f(m - top), e = top == -INFINITY ? 0.f : exp2f(s - top);
-    l = l * keep + e;
-#pragma unroll
-    for (int c = 0; c < C; c++) o[c] = o[c] * keep + e * vs * (float)v[c];
-    m = s == s ? top : s;
-  }
-  __shared__ float ms[WARPS], ls[WARPS], os[WARPS][DH];
-  if (lane == 0) {
-    ms[warp] = m;
-    ls[warp] = l;
-  }
-#pragma unroll
-  for (int c = 0; c < C; c++) os[warp][lane * C + c] = o[c];
-  __syncthreads();
-  if ((int)threadIdx.x < DH) {
-    float top = -INFINITY, total = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) top = fmaxf(top, ms[w]);
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      const float f = ms[w] == -INFINITY ? 0.f : exp2f(ms[w] - top);
-      total = fmaf(ls[w], f, total);
-      sum = fmaf(os[w][threadIdx.x], f, sum);
+        for (int j = 0; j < 16 * DH / 512; j++) {
+          const int x = lane + 32 * j, r = x / (DH / 16), c = x % (DH / 16);
+          copy16(smem_u32(to + key_at<DH>(group * 16 + r, c)), k + x * 16);
+          copy16(smem_u32(to + TILE * DH + value_at<DH>(group * 16 + r, c)), k + side_bytes + x * 16);
+        }
+        if (lane < 2) copy4(smem_u32(to + L::SCALES + (group * 2 + lane) * 4), a.scales + block + lane * a.kv_heads);
+      }
     }
-    a.y[b * a.y_sb + h * a.y_sh + i * a.y_st + threadIdx.x] = total == 0.f ? 0.f : sum / total;
+    copies_commit();
+    return there;
+  };
+  int next = first + warp;
+  uint32_t there[STAGES];
+#pragma unroll
+  for (int s = 0; s < STAGES; s++, next += WARPS) there[s] = fetch(next, s);
+
+  // this row's queries, scaled by a power of two, in halves: step j of the sum covers channels at(j) .. + 3 of thread t
+  uint32_t q[STEPS][4];
+  float row_scale;
+  {
+    const float* qp = pdl_after(a.q) + b * a.q_sb + head * a.q_sh + token * a.q_st;
+    float4 x[STEPS];
+    float peak = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+      const int at = DH == 32 ? t * 8 + j * 4 : (j / 4) * 64 + t * 16 + (j % 4) * 4;
+      x[j] = last >= 0 ? pdl_ld(reinterpret_cast<const float4*>(qp + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      peak = fmaxf(fmaxf(fmaxf(peak, fabsf(x[j].x)), fmaxf(fabsf(x[j].y), fabsf(x[j].z))), fabsf(x[j].w));
+    }
+    peak = quad_max(peak);
+    // 2^(its exponent), no less than 2^-100: smaller queries than that weigh nothing
+    const int e = max((int)(__float_as_uint(peak) >> 23) - 127, -100);
+    const float up = exp2f((float)(QUERY_BITS - e));
+    row_scale = exp2f((float)(e - QUERY_BITS)) * a.scale_log2;
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) {
+      split(x[j].x * up, x[j].y * up, q[j][0], q[j][1]);
+      split(x[j].z * up, x[j].w * up, q[j][2], q[j][3]);
+    }
   }
+
+  float o[DH / 8][4], m = -INFINITY, big = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int d = 0; d < DH / 8; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[d][i] = 0.f;
+
+  for (int i = first + warp, stage = 0; i < end; i += WARPS) {
+    copies_wait<STAGES - 1>();
+    __syncwarp();
+    const unsigned char* tile_at = ring + stage * L::STAGE;
+    const float4 sc = *reinterpret_cast<const float4*>(tile_at + L::SCALES);    // keys, values of both groups
+    uint32_t here = there[0];
+#pragma unroll
+    for (int s = 1; s < STAGES; s++) here = stage == s ? there[s] : here;
+    float s[4][2];
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < STEPS; j += KB / 4) {
+        uint32_t w[KB / 4];
+        load_words<KB>(tile_at + (DH == 32 ? key_at<DH>(n * 8 + g, t >> 1) + (t & 1) * 8 : key_at<DH>(n * 8 + g, j + t)), w);
+#pragma unroll
+        for (int k = 0; k < KB / 4; k++) mma(c, q[j + k], two_codes<0x4140>(w[k]), two_codes<0x4342>(w[k]));
+      }
+      const float by = row_scale * (n < 2 ? sc.x : sc.z);
+      s[n][0] = (c[0] + c[2]) * by;
+      s[n][1] = (c[1] + c[3]) * by;
+    }
+    // what this row does not see
+    const int t0 = i * TILE + 2 * t;
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        if (t0 + n * 8 + k > last || !(here >> (n >> 1) & 1)) s[n][k] = -INFINITY;
+    const float top0 = quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
+    const float top1 = quad_max(fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
+    const float lv0 = here & 1 ? log2f(sc.y) : -INFINITY, lv1 = here & 2 ? log2f(sc.w) : -INFINITY;
+    const float m_new = fmaxf(m, fmaxf(top0, top1));
+    const float big_new = fmaxf(big, fmaxf(top0 + lv0, top1 + lv1));
+    const float m_ref = finite_or_0(m_new), big_ref = finite_or_0(big_new);
+    l *= exp2f(m - m_ref);
+    // a scale that is no number makes NaN of the rows that see it
+    const float f0 = lv0 < INFINITY ? exp2f(fminf(m_ref + lv0 - big_ref + WEIGHT_BITS, 126.f)) : NAN;
+    const float f1 = lv1 < INFINITY ? exp2f(fminf(m_ref + lv1 - big_ref + WEIGHT_BITS, 126.f)) : NAN;
+    if (__any_sync(0xffffffffu, big_new != big)) {
+      const float keep = exp2f(big - big_ref);
+#pragma unroll
+      for (int d = 0; d < DH / 8; d++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[d][k] *= keep;
+    }
+    m = m_new;
+    big = big_new;
+    uint32_t p[2][4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      float w[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const bool none = s[n][k] == -INFINITY;
+        const float e = exp2f(s[n][k] - m_ref);
+        l += none ? 0.f : e;
+        w[k] = none ? 0.f : e * (n < 2 ? f0 : f1);
+      }
+      split(w[0], w[1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
+    }
+    const unsigned char* values = tile_at + TILE * DH;
+#pragma unroll
+    for (int group = 0; group < 2; group++) {
+      uint32_t v[4][VB / 4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int key = group * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
+        load_words<VB>(values + value_at<DH>(key, g * VB / 16) + g * VB % 16, v[r]);
+      }
+#pragma unroll
+      for (int w = 0; w < VB / 4; w++) {
+        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+        const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+        mma(o[w * 4 + 0], p[group], two_codes<0x4140>(a0), two_codes<0x4140>(b0));
+        mma(o[w * 4 + 1], p[group], two_codes<0x4342>(a0), two_codes<0x4342>(b0));
+        mma(o[w * 4 + 2], p[group], two_codes<0x4140>(a1), two_codes<0x4140>(b1));
+        mma(o[w * 4 + 3], p[group], two_codes<0x4342>(a1), two_codes<0x4342>(b1));
+      }
+    }
+    __syncwarp();
+    const uint32_t fetched = fetch(next, stage);
+#pragma unroll
+    for (int s = 0; s < STAGES; s++) there[s] = stage == s ? fetched : there[s];
+    next += WARPS;
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  }
+
+  // the warps' results: channel c of row g is in thread c / (2 * DH / 8), its two halves beside one another
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  copies_wait<0>();
+  __syncthreads();
+  float* parts = reinterpret_cast<float*>(smem);
+  {
+    float* mine = parts + warp * L::PART;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int d = 0; d < DH / 8; d += 4)
+        *reinterpret_cast<float4*>(mine + g * L::STRIDE + (2 * t + k) * (DH / 8) + d) =
+            make_float4(o[d][k] + o[d][k + 2], o[d + 1][k] + o[d + 1][k + 2], o[d + 2][k] + o[d + 2][k + 2], o[d + 3][k] + o[d + 3][k + 2]);
+    if (t == 0) {
+      float* stats = mine + L::STATS;
+      stats[g] = m;
+      stats[ROWS + g] = big;
+      stats[2 * ROWS + g] = l;
+    }
+  }
+  __syncthreads();
+  constexpr int PER = THREADS / ROWS;             // threads a row, DH / PER channels each
+  const int r = threadIdx.x / PER, c0 = threadIdx.x % PER * (DH / PER);
+  float mw[WARPS], bw[WARPS], lw[WARPS], m_all = -INFINITY, big_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) {
+    const float* stats = parts + w * L::PART + L::STATS;
+    mw[w] = stats[r];
+    bw[w] = stats[ROWS + r];
+    lw[w] = stats[2 * ROWS + r];
+    m_all = fmaxf(m_all, mw[w]);
+    big_all = fmaxf(big_all, bw[w]);
+  }
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) {
+    l_all = fmaf(lw[w], exp2f(mw[w] - finite_or_0(m_all)), l_all);
+    bw[w] = exp2f(bw[w] - finite_or_0(big_all));
+  }
+  float out[DH / PER];
+#pragma unroll
+  for (int c = 0; c < DH / PER; c++) {
+    out[c] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) out[c] = fmaf(parts[w * L::PART + r * L::STRIDE + c0 + c], bw[w], out[c]);
+  }
+  const int out_row = tile * ROWS + r;
+  if (out_row >= a.tokens * a.group) return;
+  if (a.splits == 1) {
+    const float by = l_all == 0.f ? 0.f : exp2f(big_all - finite_or_0(m_all) - WEIGHT_BITS) / l_all;
+    float* y = a.y + b * a.y_sb + (kvh * a.group + out_row % a.group) * a.y_sh + out_row / a.group * a.y_st + c0;
+#pragma unroll
+    for (int c = 0; c < DH / PER; c++) y[c] = out[c] * by;
+  } else {
+    const int64_t at = ((int64_t)unit * a.splits + part) * ROWS + r;
+    float* to = a.part_rows + at * DH + c0;
+#pragma unroll
+    for (int c = 0; c < DH / PER; c++) to[c] = out[c];
+    if (c0 == 0) {
+      a.part_stats[at * 3] = m_all;
+      a.part_stats[at * 3 + 1] = big_all;
+      a.part_stats[at * 3 + 2] = l_all;
+    }
+  }
+}
+
+// Joins the parts of a row, one warp each.
+template <int DH>
+__global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAttArgs a) {
+  pdl_wait();
+  constexpr int C = DH / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.batch * a.kv_heads * a.tokens * a.group) return;
+  const int in = (int)(row % (a.tokens * a.group)), bh = (int)(row / (a.tokens * a.group)), kvh = bh % a.kv_heads, b = bh / a.kv_heads;
+  const int64_t at = (((int64_t)bh * a.row_tiles + in / ROWS) * a.splits) * ROWS + in % ROWS;   // of part 0; then ROWS further
+  const float* stats = pdl_after(a.part_stats);
+  const float* rows = pdl_after(a.part_rows);
+  float m = -INFINITY, big = -INFINITY, l = 0.f, o[C];
+  for (int s = lane; s < a.splits; s += 32) {
+    m = fmaxf(m, stats[(at + s * ROWS) * 3]);
+    big = fmaxf(big, stats[(at + s * ROWS) * 3 + 1]);
+  }
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, w));
+  }
+#pragma unroll
+  for (int c = 0; c < C; c++) o[c] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; s++) {
+    const float* st = stats + (at + s * ROWS) * 3;
+    l = fmaf(st[2], exp2f(st[0] - finite_or_0(m)), l);
+    const float f = exp2f(st[1] - finite_or_0(big));
+#pragma unroll
+    for (int c = 0; c < C; c++) o[c] = fmaf(rows[(at + s * ROWS) * DH + lane * C + c], f, o[c]);
+  }
+  const float by = l == 0.f ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
+  float* y = a.y + b * a.y_sb + (kvh * a.group + in % a.group) * a.y_sh + in / a.group * a.y_st + lane * C;
+#pragma unroll
+  for (int c = 0; c < C; c++) y[c] = o[c] * by;
+}
+
+template <int DH>
+int launch(wdc_context* ctx, CacheAttArgs& a) {
+  static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
+  WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "wdc_cache_attention: device index out of range");
+  if (!opted_in[ctx->device]) {
+    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::SMEM));
+    opted_in[ctx->device] = true;
+  }
+  const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = 2 * ctx->sm_count;
+  const int64_t tiles = ceil_div64(a.table_pages * a.page_tokens, TILE);
+  int64_t splits = ceil_div64(4 * slots, units);
+  if (splits > ceil_div64(tiles, WARPS)) splits = ceil_div64(tiles, WARPS);
+  if (splits < 1) splits = 1;
+  a.splits = (int)splits;
+  WDC_REQUIRE(ctx, units * splits < (1ll << 31), "wdc_cache_attention: batch exceeds the grid");
+  float* scratch = nullptr;
+  if (splits > 1) {
+    CACHE_TRY(wdc_alloc(ctx, units * splits * ROWS * (DH + 3) * 4, (void**)&scratch));
+    a.part_rows = scratch;
+    a.part_stats = scratch + units * splits * ROWS * DH;
+  }
+  wdc_launch_pdl(ctx, cache_attention_kernel<DH>, dim3((unsigned)(units * splits)), dim3(THREADS), Layout<DH>::SMEM, a);
+  int s = wdc_check_launch(ctx, "cache_attention_kernel");
+  if (s == WDC_OK && splits > 1) {
+    const int64_t rows = (int64_t)a.batch * a.heads * a.tokens;
+    wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)ceil_div64(rows, 4)), dim3(128), 0, a);
+    s = wdc_check_launch(ctx, "cache_attention_join_kernel");
+  }
+  if (scratch) wdc_free(ctx, scratch);   // stream-ordered: reused only by work queued after the kernels
+  return s;
 }
 
 }  // namespace
@@ -102,14 +438,19 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   WDC_REQUIRE(ctx, cache_aligned(q, 16) && cache_aligned(codes, 16) && cache_aligned(y, 16) && cache_aligned(scales, 4) &&
               cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4),
               "wdc_cache_attention: buffers are not aligned");
-  CacheAttArgs a = {q, (const int8_t*)codes, scales, page_table, lengths, counts, y, ctx->status_word, d->pages,
-                    d->table_pages, d->q_sb, d->q_sh, d->q_st, d->y_sb, d->y_sh, d->y_st, (int)d->tokens, (int)d->heads,
-                    (int)d->kv_heads, (int)(d->heads / d->kv_heads), (int)d->page_tokens, d->scale * 1.4426950408889634f};
-  const int64_t ctas = d->batch * d->tokens * d->heads;
-  WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_cache_attention: batch exceeds the grid");
+  CacheAttArgs a = {};
+  a.q = q; a.codes = (const int8_t*)codes; a.scales = scales;
+  a.page_table = page_table; a.lengths = lengths; a.counts = counts;
+  a.y = y; a.status = ctx->status_word;
+  a.pages = d->pages; a.table_pages = d->table_pages;
+  a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
+  a.y_sb = d->y_sb; a.y_sh = d->y_sh; a.y_st = d->y_st;
+  a.batch = (int)d->batch; a.tokens = (int)d->tokens; a.heads = (int)d->heads; a.kv_heads = (int)d->kv_heads;
+  a.group = (int)(d->heads / d->kv_heads); a.page_tokens = (int)d->page_tokens;
+  WDC_REQUIRE(ctx, d->tokens * a.group < (1ll << 31) - ROWS && d->batch * d->heads * d->tokens < (1ll << 31),
+              "wdc_cache_attention: batch exceeds the grid");
+  a.row_tiles = (int)ceil_div64(d->tokens * a.group, ROWS);
+  a.scale_log2 = d->scale * 1.4426950408889634f;
   DeviceGuard g(ctx->device);
-  auto kernel = d->head_size == 32 ? cache_attention_kernel<32> : d->head_size == 64 ? cache_attention_kernel<64>
-                                                                                      : cache_attention_kernel<128>;
-  wdc_launch_pdl(ctx, kernel, dim3((unsigned)ctas), dim3(THREADS), 0, a);
-  return wdc_check_launch(ctx, "cache_attention_kernel");
+  return d->head_size == 32 ? launch<32>(ctx, a) : d->head_size == 64 ? launch<64>(ctx, a) : launch<128>(ctx, a);
 }
