@@ -6,7 +6,10 @@
 
 namespace {
 
-constexpr int THREADS = 256, TOP_MOST = 32;
+constexpr int WARPS = 8, THREADS = 32 * WARPS, EACH = 4;      // float4 a thread and round
+constexpr int TOP_MOST = 32, PARTS_MOST = 8;
+constexpr int KEPT = 1024;                                     // keys that the candidates' list holds
+constexpr int PART_LEAST = 4096;                               // logits of a part, where a row is cut into several
 
 struct LogprobArgs {
   const float* logits;
@@ -14,10 +17,10 @@ struct LogprobArgs {
   float *logprob, *entropy, *top_logprobs;
   int32_t* top_ids;
   int64_t row_stride;
-  int vocab, top;
+  int vocab, top, parts;
 };
 
-// A key that orders by value, NaN above everything and -0 as 0, then by the lower index.
+// A key that orders by value, NaN above everything and -0 as 0, then by the lower index.  No key is 0.
 __device__ __forceinline__ uint64_t order_key(float x, int index) {
   uint32_t bits = x == x ? __float_as_uint(x + 0.f) : 0x7fffffffu;
   bits = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
@@ -27,52 +30,242 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   const uint32_t bits = (uint32_t)(key >> 32);
   return __uint_as_float(bits & 0x80000000u ? bits & 0x7fffffffu : ~bits);
 }
+__device__ __forceinline__ float exp_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
 
-// s = sum e^(x - m), t = sum (x - m) e^(x - m), without terms of x = -inf.
+// s = sum e^(x - m), t = sum (x - m) e^(x - m).  A difference below -200, whose exponential is 0, counts as -200 in t: it may be
+// infinite, and infinity times 0 is NaN.  A NaN or +inf makes s NaN.
 struct Sums {
   float m, s, t;
 };
-__device__ __forceinline__ Sums joined(Sums a, Sums b) {
-  if (a.m == -INFINITY) return b;
-  if (b.m == -INFINITY) return a;
-  const float m = fmaxf(a.m, b.m), fa = expf(a.m - m), fb = expf(b.m - m);
-  Sums r;
-  r.m = m;
-  r.s = a.s * fa + b.s * fb;
-  // (a difference whose exponential is 0 is cut off: times the sum it could be infinite, and 0 times that NaN)
-  r.t = fa * fmaf(a.s, fmaxf(a.m - m, -200.f), a.t) + fb * fmaf(b.s, fmaxf(b.m - m, -200.f), b.t);
-  return r;
+__device__ __forceinline__ void raise_to(Sums& a, float m) {
+  if (m > a.m) {
+    const float d = a.m - m, f = exp_of(d);
+    a.t = f * fmaf(a.s, fmaxf(d, -200.f), a.t);
+    a.s *= f;
+    a.m = m;
+  }
+}
+__device__ __forceinline__ void add(Sums& a, Sums b) {
+  raise_to(a, b.m);
+  raise_to(b, a.m);
+  a.s += b.s;
+  a.t += b.t;
+}
+__device__ __forceinline__ void take(Sums& a, float x, float ref) {
+  const float d = x - ref, e = exp_of(d);
+  a.s += e;
+  a.t = fmaf(fmaxf(d, -200.f), e, a.t);
 }
 
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobArgs a) {
-  pdl_wait();
-  __shared__ Sums parts[THREADS / 32];
-  __shared__ uint64_t best[THREADS / 32];
+// Keys of a warp, one a lane: sorted, largest in lane 0; and the 32 largest of two sorted lists, `b` given backwards.
+__device__ __forceinline__ uint64_t exchange(uint64_t key, int with, bool larger) {
+  const uint64_t other = __shfl_xor_sync(0xffffffffu, key, with);
+  return (key > other) == larger ? key : other;
+}
+__device__ __forceinline__ uint64_t warp_sorted(uint64_t key) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int w = size / 2; w > 0; w /= 2) key = exchange(key, w, !(lane & w) == !(lane & size));
+  return key;
+}
+__device__ __forceinline__ uint64_t warp_joined(uint64_t a, uint64_t b_backwards) {
+  const int lane = threadIdx.x & 31;
+  uint64_t key = a > b_backwards ? a : b_backwards;
+#pragma unroll
+  for (int w = 16; w > 0; w /= 2) key = exchange(key, w, !(lane & w));
+  return key;
+}
+
+struct Shared {
+  uint64_t kept[KEPT];                 // candidates, in no order
+  uint64_t lists[WARPS][32];
+  uint64_t part_lists[PARTS_MOST][32]; // of the parts of a row, in the first CTA of its cluster
+  Sums part_sums[PARTS_MOST];
+  Sums sums[WARPS];
+  uint64_t best[WARPS];
+  unsigned int count;
+};
+
+// The 32 largest of the warps' sorted lists, to lists[0].  All threads; a barrier at both ends.
+__device__ __forceinline__ void join_lists(Shared& sh, uint64_t sorted) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.x;
-  const float* x = pdl_after(a.logits) + row * a.row_stride;
-  Sums sums = {-INFINITY, 0.f, 0.f};
-  for (int i = threadIdx.x; i < a.vocab; i += THREADS) {
-    const float v = pdl_ld(x + i);
-    if (v != -INFINITY) sums = joined(sums, {v, 1.f + (v - v), v - v});   // (v - v: NaN for infinity and NaN)
+  sh.lists[warp][lane] = sorted;
+  __syncthreads();
+#pragma unroll
+  for (int step = WARPS / 2; step > 0; step /= 2) {
+    if (warp < step) sh.lists[warp][lane] = warp_joined(sh.lists[warp][lane], sh.lists[warp + step][31 - lane]);
+    __syncthreads();
   }
+}
+__device__ __forceinline__ uint64_t sorted_part_of_kept(const Shared& sh, int count) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t key = 0;
+  for (int at = warp * 32; at < count; at += THREADS) {
+    const uint64_t more = warp_sorted(at + lane < count ? sh.kept[at + lane] : 0);
+    key = warp_joined(key, __shfl_sync(0xffffffffu, more, 31 - lane));
+  }
+  return key;
+}
+
+__device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// One CTA per row, or a cluster of `parts` where rows are few, each on a range of the row.  A round is EACH float4 a thread.
+//
+// Candidates for the best `top`: `floor_key` is a key that `top` logits of the range are known to be above; what a round has above
+// it goes to a list in shared memory.  Where more might come than the list has room for (always in the first round), the floor is
+// raised first, to just below the `top`-th largest of the threads' largest keys of the round: at most `top` threads hold
+// anything above that, EACH * 4 keys each.  A list that is nearly full is cut to its `top` largest, which raises the floor too.
+template <bool kTop, bool kCluster>
+__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobArgs a) {
+  __shared__ Shared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = kCluster ? (int)(blockIdx.x % (unsigned)a.parts) : 0;
+  const int64_t row = kCluster ? blockIdx.x / (unsigned)a.parts : blockIdx.x;
+  if (kCluster) cluster_arrive();   // this CTA has begun: the others may write to its shared memory (waited for below)
+  if (threadIdx.x == 0) sh.count = 0;
+  pdl_wait();
+  const float* x = pdl_after(a.logits) + row * a.row_stride;
+  // float4 from the first 16-byte boundary on; what is before and behind them goes by single floats, to the first part
+  const int before = min((int)(-(intptr_t)x >> 2 & 3), a.vocab), quads = (a.vocab - before) / 4;
+  const int begin = kCluster ? (int)((int64_t)rank * quads / a.parts) : 0;
+  const int end = kCluster ? (int)((int64_t)(rank + 1) * quads / a.parts) : quads;
+  const float4* x4 = reinterpret_cast<const float4*>(x + before);
+
+  Sums sums = {-INFINITY, 0.f, 0.f};
+  uint64_t floor_key = 0;
+  float floor_value = -INFINITY;
+  int have = 0;
+  if (rank == 0) {
+    const int singles = a.vocab - quads * 4;       // up to six
+    if ((int)threadIdx.x < singles) {
+      const int i = (int)threadIdx.x < before ? (int)threadIdx.x : quads * 4 + (int)threadIdx.x;
+      const float v = pdl_ld(x + i);
+      raise_to(sums, v);
+      take(sums, v, sums.m == -INFINITY ? 0.f : sums.m);
+      if (kTop) sh.kept[threadIdx.x] = order_key(v, i);
+    }
+    if (kTop && threadIdx.x == 0) sh.count = singles;
+    have = singles;
+  }
+  for (int base = begin; base < end; base += THREADS * EACH) {
+    float4 f[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; j++) {
+      const int at = base + j * THREADS + (int)threadIdx.x;
+      f[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    float peak = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < EACH; j++) peak = fmaxf(fmaxf(fmaxf(f[j].x, f[j].y), fmaxf(f[j].z, f[j].w)), peak);
+    raise_to(sums, peak);
+    const float ref = sums.m == -INFINITY ? 0.f : sums.m;
+#pragma unroll
+    for (int j = 0; j < EACH; j++) {
+      take(sums, f[j].x, ref);
+      take(sums, f[j].y, ref);
+      take(sums, f[j].z, ref);
+      take(sums, f[j].w, ref);
+    }
+    if (kTop) {
+      const int first = before + 4 * (base + (int)threadIdx.x);
+      const auto each = [&](auto what) {
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+          if (base + j * THREADS + (int)threadIdx.x >= end) break;
+          const int i = first + 4 * j * THREADS;
+          what(order_key(f[j].x, i));
+          what(order_key(f[j].y, i + 1));
+          what(order_key(f[j].z, i + 2));
+          what(order_key(f[j].w, i + 3));
+        }
+      };
+      uint64_t mine = 0;
+      if (peak >= floor_value) each([&](uint64_t key) { mine = key > mine ? key : mine; });
+      const int wanting = __syncthreads_count(mine > floor_key);
+      if (wanting == 0) continue;
+      if (have + wanting * EACH * 4 > KEPT) {
+        join_lists(sh, warp_sorted(mine));
+        uint64_t least = sh.lists[0][a.top - 1];
+        if (least > floor_key + 1) floor_key = least - 1;
+        if (have + a.top * EACH * 4 > KEPT) {
+          const uint64_t sorted = sorted_part_of_kept(sh, have);
+          __syncthreads();                         // lists[0] and the candidates have been read
+          join_lists(sh, sorted);
+          least = sh.lists[0][a.top - 1];
+          if (least > floor_key + 1) floor_key = least - 1;
+          if (warp == 0) sh.kept[lane] = sh.lists[0][lane];
+          if (threadIdx.x == 0) sh.count = a.top;  // (there are more candidates than that)
+        }
+        __syncthreads();
+        floor_value = floor_key ? key_value(floor_key) : -INFINITY;
+      }
+      if (mine > floor_key)
+        each([&](uint64_t key) {
+          if (key > floor_key) sh.kept[atomicAdd(&sh.count, 1u)] = key;
+        });
+      __syncthreads();
+      have = (int)sh.count;
+    }
+  }
+
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1)
-    sums = joined(sums, {__shfl_xor_sync(0xffffffffu, sums.m, w), __shfl_xor_sync(0xffffffffu, sums.s, w),
-                         __shfl_xor_sync(0xffffffffu, sums.t, w)});
-  if (lane == 0) parts[warp] = sums;
+    add(sums, {__shfl_xor_sync(0xffffffffu, sums.m, w), __shfl_xor_sync(0xffffffffu, sums.s, w),
+               __shfl_xor_sync(0xffffffffu, sums.t, w)});
+  if (lane == 0) sh.sums[warp] = sums;
   __syncthreads();
-  sums = parts[0];
-  for (int w = 1; w < THREADS / 32; w++) sums = joined(sums, parts[w]);
-  const float log_s = logf(sums.s);
+  if (kTop) join_lists(sh, sorted_part_of_kept(sh, have));
+  sums = sh.sums[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; w++) add(sums, sh.sums[w]);
+  uint64_t best = kTop ? sh.lists[0][lane] : 0;
+  if (kCluster) {
+    cluster_wait();
+    if (warp == 0) {
+      if (kTop)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at(&sh.part_lists[rank][31 - lane], 0)), "l"(best) : "memory");
+      if (lane < 3)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_at(&sh.part_sums[rank].m + lane, 0)),
+                     "f"(lane == 0 ? sums.m : lane == 1 ? sums.s : sums.t) : "memory");
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+    for (int r = 1; r < a.parts; r++) {
+      add(sums, sh.part_sums[r]);
+      if (kTop) best = warp_joined(best, sh.part_lists[r][lane]);
+    }
+  }
   const bool none = sums.m == -INFINITY;
+  const float log_s = none ? NAN : logf(sums.s);
   if (threadIdx.x == 0) {
     if (a.logprob) {
       const int token = pdl_ld(a.tokens + row);
-      a.logprob[row] = none || token < 0 || token >= a.vocab ? NAN : x[token] - sums.m - log_s;
+      a.logprob[row] = token < 0 || token >= a.vocab ? NAN : pdl_ld(x + token) - sums.m - log_s;
     }
-    if (a.entropy) a.entropy[row] = none ? NAN : log_s - sums.t / sums.s;
+    if (a.entropy) a.entropy[row] = log_s - sums.t / sums.s;
   }
+  if (!kTop) return;
+  if (sums.s == sums.s) {
+    if (warp == 0 && lane < a.top) {
+      a.top_ids[row * a.top + lane] = (int32_t)~(uint32_t)best;
+      a.top_logprobs[row * a.top + lane] = key_value(best) - sums.m - log_s;
+    }
+    return;
+  }
+  // a NaN, which no maximum above shows: the next largest key of the whole row, `top` times
   uint64_t below = ~0ull;
   for (int k = 0; k < a.top; k++) {
     uint64_t mine = 0;
@@ -81,17 +274,44 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
       if (key < below && key > mine) mine = key;
     }
 #pragma unroll
-    for (int w = 1; w < 32; w <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, w));
+    for (int w = 1; w < 32; w <<= 1) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, mine, w);
+      mine = mine > other ? mine : other;
+    }
     __syncthreads();
-    if (lane == 0) best[warp] = mine;
+    if (lane == 0) sh.best[warp] = mine;
     __syncthreads();
-    for (int w = 0; w < THREADS / 32; w++) mine = max(mine, best[w]);
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) mine = mine > sh.best[w] ? mine : sh.best[w];
     below = mine;
     if (threadIdx.x == 0) {
       a.top_ids[row * a.top + k] = (int32_t)~(uint32_t)mine;
-      a.top_logprobs[row * a.top + k] = none ? NAN : key_value(mine) - sums.m - log_s;
+      a.top_logprobs[row * a.top + k] = NAN;
     }
   }
+}
+
+template <bool kTop>
+cudaError_t launch(wdc_context* ctx, const LogprobArgs& a, int64_t rows) {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * a.parts));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  if (a.parts > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)a.parts;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs++;
+  }
+  if (ctx->opt_pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs++;
+  }
+  return a.parts > 1 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kTop, true>, a)
+                     : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kTop, false>, a);
 }
 
 }  // namespace
@@ -111,9 +331,15 @@ extern "C" int wdc_token_logprobs(wdc_context* ctx, const wdc_logprobs_desc* d, 
               (long long)d->top, (long long)d->vocab, TOP_MOST);
   if (d->rows == 0) return WDC_OK;
   WDC_REQUIRE(ctx, logits && (tokens || !logprob) && !top_ids == !top_logprobs, "wdc_token_logprobs: null argument");
+  for (const void* p : {(const void*)logits, (const void*)tokens, (const void*)logprob, (const void*)entropy,
+                        (const void*)top_ids, (const void*)top_logprobs})
+    WDC_REQUIRE(ctx, (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "wdc_token_logprobs: buffers are not aligned");
   DeviceGuard g(ctx->device);
   LogprobArgs a = {logits, tokens, logprob, entropy, top_logprobs, top_ids, d->row_stride, (int)d->vocab,
-                   top_ids ? (int)d->top : 0};
-  wdc_launch_pdl(ctx, token_logprobs_kernel, dim3((unsigned)d->rows), dim3(THREADS), 0, a);
+                   top_ids ? (int)d->top : 0, 1};
+  while (a.parts < PARTS_MOST && d->rows * a.parts < 2 * ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
+  WDC_REQUIRE(ctx, d->rows * a.parts < (1ll << 31), "wdc_token_logprobs: rows exceed the grid");
+  const cudaError_t e = a.top ? launch<true>(ctx, a, d->rows) : launch<false>(ctx, a, d->rows);
+  WDC_CUDA(ctx, e);
   return wdc_check_launch(ctx, "token_logprobs_kernel");
 }
