@@ -16,7 +16,7 @@ struct CacheAttArgs {
   int* status;
   int64_t pages, table_pages;
   int64_t q_sb, q_sh, q_st, y_sb, y_sh, y_st;
-  int batch, tokens, heads, kv_heads, group, page_tokens;
+  int batch, tokens, heads, kv_heads, group, page_shift;   // 2^page_shift tokens a page
   int row_tiles, splits;
   float *part_rows, *part_stats;   // of every unit and split: O of its rows; m, M and l
   float scale_log2;                // scale * log2(e): the softmax runs on exp2
@@ -31,24 +31,29 @@ struct CacheAttArgs {
 // instruction's 16 rows: eight rows with both halves are one instruction, and their sums meet in one thread's registers.
 //
 // Weights carry the value scale of their page.  With s the scores (base 2) and lv = log2(value scale) of a group of 16 tokens,
-//   m = max s,  l = sum 2^(s - m);      M = max (s + lv),  O = sum 2^(s + lv - M) code,      y = O 2^(M - m) / l,
-// so that what is split into halves is relative to the largest term of O, whatever the pages' scales are.
-constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, STAGES = 3, ROWS = 8;
+//   m = max s,  l = sum 2^(s - m);      M = max (s + [lv]),  O = sum 2^(s + lv - M) code,      y = O 2^(M - m) / l,
+// so that what is split into halves is relative to the largest term of O, whatever the pages' scales are.  ([lv] is the scale's
+// binary exponent: the maxima need no logarithm, and the weights take the scale itself.)
+constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, ROWS = 8;
 constexpr float WEIGHT_BITS = 14.f;        // weights are up to 2^14: both halves stay in float16's normal range
 constexpr int QUERY_BITS = 13;             // a row's queries are scaled to less than 2^14
 
 template <int DH>
 struct Layout {
-  static constexpr int SCALES = 2 * TILE * DH;                       // behind a stage's keys and values: four scales
-  static constexpr int STAGE = SCALES + 16, RING = STAGES * STAGE;
+  static constexpr int CTAS = DH == 128 ? 2 : 4;                     // per SM: what registers and shared memory have room for
+  static constexpr int STAGES = 3;
+  static constexpr int SCALES = 2 * TILE * DH;                       // behind a stage's keys and values: four scales, and
+  static constexpr int THERE = SCALES + 16;                          // which of its two groups of 16 tokens are there
+  static constexpr int STAGE = SCALES + 128, RING = STAGES * STAGE;  // (128-byte lines, for value_at)
   static constexpr int STRIDE = DH + 4, STATS = ROWS * STRIDE;       // floats: a row when the warps join; behind them m, M, l
   static constexpr int PART = STATS + 3 * ROWS;
   static constexpr int SMEM = WARPS * (RING > PART * 4 ? RING : PART * 4);
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int TO, int FROM>
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
@@ -104,62 +109,107 @@ __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)
   for (int i = 0; i < BYTES / 4; i++) w[i] ^= 0x80808080u;
 }
 
+__device__ __forceinline__ float exp2_of(float x) {      // results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// A value scale as 2^e * f, 1 <= f < 2 (0: e = -infinity; no number: f is NaN).
+__device__ __forceinline__ void exponent_of(float scale, float& e, float& f) {
+  const bool small = scale < 1.2e-38f;                       // (below the normal range)
+  const uint32_t bits = __float_as_uint(small ? scale * 16777216.f : scale);
+  e = scale > 0.f && scale < INFINITY ? (float)((int)(bits >> 23) - (small ? 151 : 127)) : scale == 0.f ? -INFINITY : 0.f;
+  f = scale < INFINITY ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : NAN;
+}
+
 __device__ __forceinline__ float finite_or_0(float x) { return x == -INFINITY ? 0.f : x; }   // a reference to subtract
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 
+// Asynchronous copies of 16 tokens' keys and values by a warp.  `k` and `v` are at this lane's 16 bytes.
+template <int DH, int GROUP>
+__device__ __forceinline__ void copy_group(uint32_t to_k, uint32_t to_v, const int8_t* k, const int8_t* v) {
+  constexpr int AT = GROUP * 16 * DH;
+  copy16<AT, 0>(to_k, k);
+  copy16<AT, 0>(to_v, v);
+  if (DH >= 64) {
+    // (128: eight rows of a line's exchange pattern are two copies, so that every other copy's is the other half's)
+    copy16<AT + (DH >= 64 ? 512 : 0), DH >= 64 ? 512 : 0>(to_k, k);
+    copy16<AT + (DH >= 64 ? 512 : 0), DH >= 64 ? 512 : 0>(DH == 128 ? to_v ^ 64 : to_v, v);
+  }
+  if (DH == 128) {
+    copy16<AT + 1024, 1024>(to_k, k);
+    copy16<AT + 1024, 1024>(to_v, v);
+    copy16<AT + 1536, 1536>(to_k, k);
+    copy16<AT + 1536, 1536>(to_v ^ 64, v);
+  }
+}
+
 template <int DH>
-__global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const CacheAttArgs a) {
+__global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_kernel(const CacheAttArgs a) {
   constexpr int STEPS = DH / 16;                  // of the score product's sum; also columns of O a thread and key row
   constexpr int KB = DH == 32 ? 8 : 16;           // bytes of a key a thread loads at a time
   constexpr int VB = DH / 8;                      // bytes of a value row a thread loads
   using L = Layout<DH>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int part = (int)(blockIdx.x % (unsigned)a.splits), unit = (int)(blockIdx.x / (unsigned)a.splits);
   const int tile = unit % a.row_tiles, bh = unit / a.row_tiles, kvh = bh % a.kv_heads, b = bh / a.kv_heads;
-  const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages * a.page_tokens, a.status);
+  const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
   const int row = tile * ROWS + g, token = row / a.group, head = kvh * a.group + row % a.group;   // this thread's row
-  const int last = token < span.count ? span.length - span.count + token : -1;    // the last token it sees
-  const int top_token = min((tile * ROWS + ROWS - 1) / a.group, span.count - 1);  // the tile's last row that is no padding
-  const int seen = tile * ROWS / a.group < span.count ? span.length - span.count + top_token + 1 : 0;
+  const int before = span.length - span.count;
+  // the last token that this row sees (rows of padding see all: nobody reads theirs), and those of the tile's first and last row
+  const int first_token = tile * ROWS / a.group, top_token = min((tile * ROWS + ROWS - 1) / a.group, span.count - 1);
+  const int last = token < span.count ? before + token : 0x7fffffff;
+  const int seen_by_all = before + first_token + 1;
+  const int seen = first_token < span.count ? before + top_token + 1 : 0;
   const int tiles = (seen + TILE - 1) / TILE;
   const int first = (int)((int64_t)part * tiles / a.splits), end = (int)((int64_t)(part + 1) * tiles / a.splits);
   const int32_t* table = a.page_table + (int64_t)b * a.table_pages;
-  const int64_t block_bytes = (int64_t)a.page_tokens * DH, side_bytes = a.kv_heads * block_bytes;
   unsigned char* ring = smem + warp * L::RING;
 
-  // Copies tile i of the sequence to a stage; bit 0 and 1 of the answer: its two groups of 16 tokens are there.
-  auto fetch = [&](int i, int stage) -> uint32_t {
-    uint32_t there = 0;
-    unsigned char* to = ring + stage * L::STAGE;
+  // a lane's place in a group of 16 tokens, in memory and in a stage
+  const uint32_t page_bytes = (uint32_t)(2 * a.kv_heads * DH) << a.page_shift, side_bytes = page_bytes / 2;
+  const int8_t* codes = a.codes + (int64_t)kvh * (DH << a.page_shift) + lane * 16;
+  const uint32_t to_k = smem_u32(ring + key_at<DH>(lane / (DH / 16), lane % (DH / 16)));
+  const uint32_t to_v = smem_u32(ring + TILE * DH + value_at<DH>(lane / (DH / 16), lane % (DH / 16)));
+  const float* scales = a.scales + kvh + (lane & 1) * a.kv_heads;
+  const uint32_t to_scale = smem_u32(ring + L::SCALES + (lane & 1) * 4);
+
+  // the pages of a tile's two groups of 16 tokens (-1: nothing is there), and their copies to a stage
+  const auto pages_of = [&](int i, int (&page)[2]) {
 #pragma unroll
     for (int group = 0; group < 2; group++) {
       const int t0 = i * TILE + group * 16;
-      const int page = i < end && t0 < seen ? cache_page(table, t0 / a.page_tokens, a.pages, a.status) : -1;
-      if (page >= 0) {
-        there |= 1u << group;
-        const int64_t block = (int64_t)page * 2 * a.kv_heads + kvh;
-        const int8_t* k = a.codes + block * block_bytes + (t0 % a.page_tokens) * DH;
-#pragma unroll
-        for (int j = 0; j < 16 * DH / 512; j++) {
-          const int x = lane + 32 * j, r = x / (DH / 16), c = x % (DH / 16);
-          copy16(smem_u32(to + key_at<DH>(group * 16 + r, c)), k + x * 16);
-          copy16(smem_u32(to + TILE * DH + value_at<DH>(group * 16 + r, c)), k + side_bytes + x * 16);
-        }
-        if (lane < 2) copy4(smem_u32(to + L::SCALES + (group * 2 + lane) * 4), a.scales + block + lane * a.kv_heads);
-      }
+      page[group] = i < end && t0 < seen ? cache_page(table, t0 >> a.page_shift, a.pages, a.status) : -1;
+    }
+  };
+  const auto fetch = [&](int i, const int (&page)[2], uint32_t stage_at) {
+    const uint32_t in_page = (uint32_t)(i * TILE) & ((1u << a.page_shift) - 1);
+    if (page[0] >= 0) {
+      const int8_t* k = codes + (uint64_t)(uint32_t)page[0] * page_bytes + in_page * DH;
+      copy_group<DH, 0>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
+      if (lane < 2) copy4(to_scale + stage_at, scales + (uint64_t)(uint32_t)page[0] * (uint32_t)(2 * a.kv_heads));
+    }
+    if (page[1] >= 0) {
+      const uint32_t at = a.page_shift == 4 ? 0 : in_page + 16;
+      const int8_t* k = codes + (uint64_t)(uint32_t)page[1] * page_bytes + at * DH;
+      copy_group<DH, 1>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
+      if (lane < 2) copy4(to_scale + stage_at + 8, scales + (uint64_t)(uint32_t)page[1] * (uint32_t)(2 * a.kv_heads));
     }
     copies_commit();
-    return there;
+    if (lane == 0) *reinterpret_cast<int*>(ring + stage_at + L::THERE) = (page[0] >= 0 ? 1 : 0) | (page[1] >= 0 ? 2 : 0);
   };
-  int next = first + warp;
-  uint32_t there[STAGES];
+  int next = first + warp, page[2];
 #pragma unroll
-  for (int s = 0; s < STAGES; s++, next += WARPS) there[s] = fetch(next, s);
+  for (int s = 0; s < L::STAGES; s++, next += WARPS) {
+    pages_of(next, page);
+    fetch(next, page, s * L::STAGE);
+  }
+  pages_of(next, page);
 
   // this row's queries, scaled by a power of two, in halves: step j of the sum covers channels at(j) .. + 3 of thread t
   uint32_t q[STEPS][4];
@@ -171,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
       const int at = DH == 32 ? t * 8 + j * 4 : (j / 4) * 64 + t * 16 + (j % 4) * 4;
-      x[j] = last >= 0 ? pdl_ld(reinterpret_cast<const float4*>(qp + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[j] = token < span.count ? pdl_ld(reinterpret_cast<const float4*>(qp + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
       peak = fmaxf(fmaxf(fmaxf(peak, fabsf(x[j].x)), fmaxf(fabsf(x[j].y), fabsf(x[j].z))), fabsf(x[j].w));
     }
     peak = quad_max(peak);
@@ -192,14 +242,13 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
 #pragma unroll
     for (int i = 0; i < 4; i++) o[d][i] = 0.f;
 
-  for (int i = first + warp, stage = 0; i < end; i += WARPS) {
-    copies_wait<STAGES - 1>();
+  uint32_t stage_at = 0;
+  for (int i = first + warp; i < end; i += WARPS) {
+    copies_wait<L::STAGES - 1>();
     __syncwarp();
-    const unsigned char* tile_at = ring + stage * L::STAGE;
+    const unsigned char* tile_at = ring + stage_at;
     const float4 sc = *reinterpret_cast<const float4*>(tile_at + L::SCALES);    // keys, values of both groups
-    uint32_t here = there[0];
-#pragma unroll
-    for (int s = 1; s < STAGES; s++) here = stage == s ? there[s] : here;
+    const int there = *reinterpret_cast<const int*>(tile_at + L::THERE);
     float s[4][2];
 #pragma unroll
     for (int n = 0; n < 4; n++) {
@@ -216,24 +265,28 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
       s[n][1] = (c[1] + c[3]) * by;
     }
     // what this row does not see
-    const int t0 = i * TILE + 2 * t;
+    const bool whole = (i + 1) * TILE <= seen_by_all && there == 3;
+    if (!whole) {
+      const int t0 = i * TILE + 2 * t;
 #pragma unroll
-    for (int n = 0; n < 4; n++)
+      for (int n = 0; n < 4; n++)
 #pragma unroll
-      for (int k = 0; k < 2; k++)
-        if (t0 + n * 8 + k > last || !(here >> (n >> 1) & 1)) s[n][k] = -INFINITY;
+        for (int k = 0; k < 2; k++)
+          if (t0 + n * 8 + k > last || !(there >> (n >> 1) & 1)) s[n][k] = -INFINITY;
+    }
     const float top0 = quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
     const float top1 = quad_max(fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
-    const float lv0 = here & 1 ? log2f(sc.y) : -INFINITY, lv1 = here & 2 ? log2f(sc.w) : -INFINITY;
+    float e0, e1, f0, f1;
+    exponent_of(sc.y, e0, f0);
+    exponent_of(sc.w, e1, f1);
     const float m_new = fmaxf(m, fmaxf(top0, top1));
-    const float big_new = fmaxf(big, fmaxf(top0 + lv0, top1 + lv1));
+    const float big_new = fmaxf(big, fmaxf(top0 + e0, top1 + e1));
     const float m_ref = finite_or_0(m_new), big_ref = finite_or_0(big_new);
-    l *= exp2f(m - m_ref);
-    // a scale that is no number makes NaN of the rows that see it
-    const float f0 = lv0 < INFINITY ? exp2f(fminf(m_ref + lv0 - big_ref + WEIGHT_BITS, 126.f)) : NAN;
-    const float f1 = lv1 < INFINITY ? exp2f(fminf(m_ref + lv1 - big_ref + WEIGHT_BITS, 126.f)) : NAN;
+    l *= exp2_of(m - m_ref);
+    f0 *= exp2_of(fminf(m_ref + e0 - big_ref + WEIGHT_BITS, 126.f));
+    f1 *= exp2_of(fminf(m_ref + e1 - big_ref + WEIGHT_BITS, 126.f));
     if (__any_sync(0xffffffffu, big_new != big)) {
-      const float keep = exp2f(big - big_ref);
+      const float keep = exp2_of(big - big_ref);
 #pragma unroll
       for (int d = 0; d < DH / 8; d++)
 #pragma unroll
@@ -241,19 +294,25 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
     }
     m = m_new;
     big = big_new;
-    uint32_t p[2][4];
+    float w[4][2];
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      float w[2];
+    for (int n = 0; n < 4; n++)
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const bool none = s[n][k] == -INFINITY;
-        const float e = exp2f(s[n][k] - m_ref);
-        l += none ? 0.f : e;
-        w[k] = none ? 0.f : e * (n < 2 ? f0 : f1);
+        const float e = exp2_of(s[n][k] - m_ref);
+        l += e;
+        w[n][k] = e * (n < 2 ? f0 : f1);
       }
-      split(w[0], w[1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
+    if (!whole) {                                  // (a scale that is no number is for the rows that see it)
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          if (s[n][k] == -INFINITY) w[n][k] = 0.f;
     }
+    uint32_t p[2][4];
+#pragma unroll
+    for (int n = 0; n < 4; n++) split(w[n][0], w[n][1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
     const unsigned char* values = tile_at + TILE * DH;
 #pragma unroll
     for (int group = 0; group < 2; group++) {
@@ -274,11 +333,10 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
       }
     }
     __syncwarp();
-    const uint32_t fetched = fetch(next, stage);
-#pragma unroll
-    for (int s = 0; s < STAGES; s++) there[s] = stage == s ? fetched : there[s];
+    fetch(next, page, stage_at);
     next += WARPS;
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    pages_of(next, page);
+    stage_at = stage_at == (L::STAGES - 1) * L::STAGE ? 0 : stage_at + L::STAGE;
   }
 
   // the warps' results: channel c of row g is in thread c / (2 * DH / 8), its two halves beside one another
@@ -330,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
   const int out_row = tile * ROWS + r;
   if (out_row >= a.tokens * a.group) return;
   if (a.splits == 1) {
-    const float by = l_all == 0.f ? 0.f : exp2f(big_all - finite_or_0(m_all) - WEIGHT_BITS) / l_all;
+    const float by = l_all == 0.f || out_row / a.group >= span.count ? 0.f : exp2f(big_all - finite_or_0(m_all) - WEIGHT_BITS) / l_all;
     float* y = a.y + b * a.y_sb + (kvh * a.group + out_row % a.group) * a.y_sh + out_row / a.group * a.y_st + c0;
 #pragma unroll
     for (int c = 0; c < DH / PER; c++) y[c] = out[c] * by;
@@ -347,18 +405,19 @@ __global__ void __launch_bounds__(THREADS, 2) cache_attention_kernel(const Cache
   }
 }
 
-// Joins the parts of a row, one warp each.
+// Joins the parts of a row, one CTA each: warp w takes parts w, w + 4, ...
 template <int DH>
-__global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAttArgs a) {
+__global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const CacheAttArgs a) {
   pdl_wait();
   constexpr int C = DH / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.kv_heads * a.tokens * a.group) return;
-  const int in = (int)(row % (a.tokens * a.group)), bh = (int)(row / (a.tokens * a.group)), kvh = bh % a.kv_heads, b = bh / a.kv_heads;
-  const int64_t at = (((int64_t)bh * a.row_tiles + in / ROWS) * a.splits) * ROWS + in % ROWS;   // of part 0; then ROWS further
+  __shared__ float sums[WARPS][DH + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = (int)(blockIdx.x % (unsigned)(a.tokens * a.group)), bh = (int)(blockIdx.x / (unsigned)(a.tokens * a.group));
+  const int kvh = bh % a.kv_heads, b = bh / a.kv_heads, token = row / a.group;
+  const int64_t at = (((int64_t)bh * a.row_tiles + row / ROWS) * a.splits) * ROWS + row % ROWS;   // of part 0; then ROWS further
   const float* stats = pdl_after(a.part_stats);
-  const float* rows = pdl_after(a.part_rows);
+  const float* rows = pdl_after(a.part_rows) + lane * C;
+  const int count = a.counts ? pdl_ld(a.counts + b) : a.tokens;
   float m = -INFINITY, big = -INFINITY, l = 0.f, o[C];
   for (int s = lane; s < a.splits; s += 32) {
     m = fmaxf(m, stats[(at + s * ROWS) * 3]);
@@ -372,17 +431,27 @@ __global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAt
 #pragma unroll
   for (int c = 0; c < C; c++) o[c] = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < a.splits; s++) {
+  for (int s = warp; s < a.splits; s += WARPS) {
     const float* st = stats + (at + s * ROWS) * 3;
     l = fmaf(st[2], exp2f(st[0] - finite_or_0(m)), l);
     const float f = exp2f(st[1] - finite_or_0(big));
 #pragma unroll
-    for (int c = 0; c < C; c++) o[c] = fmaf(rows[(at + s * ROWS) * DH + lane * C + c], f, o[c]);
+    for (int c = 0; c < C; c++) o[c] = fmaf(rows[(at + s * ROWS) * DH + c], f, o[c]);
   }
-  const float by = l == 0.f ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
-  float* y = a.y + b * a.y_sb + (kvh * a.group + in % a.group) * a.y_sh + in / a.group * a.y_st + lane * C;
 #pragma unroll
-  for (int c = 0; c < C; c++) y[c] = o[c] * by;
+  for (int c = 0; c < C; c++) sums[warp][lane * C + c] = o[c];
+  if (lane == 0) sums[warp][DH] = l;
+  __syncthreads();
+  if ((int)threadIdx.x >= DH) return;
+  float total = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) {
+    total += sums[w][DH];
+    sum += sums[w][threadIdx.x];
+  }
+  // (a count out of range leaves l at 0)
+  const float by = total == 0.f || token >= count ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / total;
+  a.y[b * a.y_sb + (kvh * a.group + row % a.group) * a.y_sh + token * a.y_st + threadIdx.x] = sum * by;
 }
 
 template <int DH>
@@ -393,8 +462,8 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
     WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::SMEM));
     opted_in[ctx->device] = true;
   }
-  const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = 2 * ctx->sm_count;
-  const int64_t tiles = ceil_div64(a.table_pages * a.page_tokens, TILE);
+  const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = Layout<DH>::CTAS * ctx->sm_count;
+  const int64_t tiles = ceil_div64(a.table_pages << a.page_shift, TILE);
   int64_t splits = ceil_div64(4 * slots, units);
   if (splits > ceil_div64(tiles, WARPS)) splits = ceil_div64(tiles, WARPS);
   if (splits < 1) splits = 1;
@@ -409,8 +478,7 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
   wdc_launch_pdl(ctx, cache_attention_kernel<DH>, dim3((unsigned)(units * splits)), dim3(THREADS), Layout<DH>::SMEM, a);
   int s = wdc_check_launch(ctx, "cache_attention_kernel");
   if (s == WDC_OK && splits > 1) {
-    const int64_t rows = (int64_t)a.batch * a.heads * a.tokens;
-    wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)ceil_div64(rows, 4)), dim3(128), 0, a);
+    wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)(a.batch * a.heads * a.tokens)), dim3(THREADS), 0, a);
     s = wdc_check_launch(ctx, "cache_attention_join_kernel");
   }
   if (scratch) wdc_free(ctx, scratch);   // stream-ordered: reused only by work queued after the kernels
@@ -446,7 +514,8 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
   a.y_sb = d->y_sb; a.y_sh = d->y_sh; a.y_st = d->y_st;
   a.batch = (int)d->batch; a.tokens = (int)d->tokens; a.heads = (int)d->heads; a.kv_heads = (int)d->kv_heads;
-  a.group = (int)(d->heads / d->kv_heads); a.page_tokens = (int)d->page_tokens;
+  a.group = (int)(d->heads / d->kv_heads); a.page_shift = 4;
+  while (1 << a.page_shift < d->page_tokens) a.page_shift++;
   WDC_REQUIRE(ctx, d->tokens * a.group < (1ll << 31) - ROWS && d->batch * d->heads * d->tokens < (1ll << 31),
               "wdc_cache_attention: batch exceeds the grid");
   a.row_tiles = (int)ceil_div64(d->tokens * a.group, ROWS);

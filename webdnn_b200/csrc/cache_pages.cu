@@ -17,7 +17,7 @@ struct AppendArgs {
   int* status;
   int64_t pages, table_pages;
   int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
-  int tokens, slots, kv_heads, page_tokens, head_size;
+  int tokens, slots, kv_heads, page_shift, quad_shift;   // 2^page_shift tokens a page, 2^quad_shift float4 a head
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -28,60 +28,84 @@ __device__ __forceinline__ int quantise(float x, float scale) {
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
   return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)(d & 255) << 24;
 }
+// Four codes rint(x / scale) without a division where it cannot matter: x * (1 / scale) is within 3e-5 of the rounded quotient
+// (|x / scale| <= 127, three roundings of 2^-24), so where it is further than that from a half the nearest whole number is
+// the same, and is read off the sum with 1.5 * 2^23, whose last bits are that number.  About one quadruple in 1200 divides.
+// inverse: 0 where 1 / scale might leave the normal range.
+__device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inverse) {
+  const float magic = 12582912.f;
+  const float4 t = make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse);
+  const float4 r = make_float4(t.x + magic, t.y + magic, t.z + magic, t.w + magic);
+  const float off = fmaxf(fmaxf(fabsf(t.x - (r.x - magic)), fabsf(t.y - (r.y - magic))),
+                          fmaxf(fabsf(t.z - (r.z - magic)), fabsf(t.w - (r.w - magic))));
+  if (off < 0.4999f && inverse > 0.f)
+    return __byte_perm(__byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x0040),
+                       __byte_perm(__float_as_uint(r.z), __float_as_uint(r.w), 0x0040), 0x5410);
+  return pack4(quantise(x.x, scale), quantise(x.y, scale), quantise(x.z, scale), quantise(x.w, scale));
+}
 
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
-// Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.
+// Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.  The new numbers are read
+// once and wait in registers for their scale, HELD float4 a thread (a whole page).
+template <int HELD>
 __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
   pdl_wait();
   const int part = (int)(blockIdx.x % (unsigned)(2 * a.kv_heads));
   const int rest = (int)(blockIdx.x / (unsigned)(2 * a.kv_heads));
   const int slot = rest % a.slots, b = rest / a.slots;
   const int is_v = part >= a.kv_heads, head = part - is_v * a.kv_heads;
-  const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages * a.page_tokens, a.status);
+  const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
   if (span.count == 0) return;
-  const int start = span.length - span.count, index = start / a.page_tokens + slot;
-  const int first = index * a.page_tokens;                       // the page's first token
+  const int start = span.length - span.count, index = (start >> a.page_shift) + slot;
+  const int first = index << a.page_shift;                       // the page's first token
   if (first >= span.length) return;
   const int page = cache_page(a.page_table + (int64_t)b * a.table_pages, index, a.pages, a.status);
   if (page < 0) return;
-  const int lo = max(start, first), hi = min(span.length, first + a.page_tokens);
+  const int lo = max(start, first), hi = min(span.length, first + (1 << a.page_shift));
   const float* x = is_v ? pdl_after(a.v) + b * a.v_sb + head * a.v_sh + (lo - start) * a.v_st
                         : pdl_after(a.k) + b * a.k_sb + head * a.k_sh + (lo - start) * a.k_st;
   const int64_t row = is_v ? a.v_st : a.k_st;
-  const int quads = a.head_size / 4, n = (hi - lo) * quads;
+  const int n = (hi - lo) << a.quad_shift, quad = (1 << a.quad_shift) - 1;      // float4 of the new tokens
   const int64_t block = ((int64_t)page * 2 + is_v) * a.kv_heads + head;
-  uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes + block * a.page_tokens * a.head_size);
+  uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes) + (block << (a.page_shift + a.quad_shift));
 
   __shared__ uint32_t peaks[APPEND_THREADS / 32];
   uint32_t peak = 0;
-  for (int i = threadIdx.x; i < n; i += APPEND_THREADS) {
-    const float4 f = pdl_ld(reinterpret_cast<const float4*>(x + (i / quads) * row) + i % quads);
-    peak = max(max(max(peak, abs_bits(f.x)), max(abs_bits(f.y), abs_bits(f.z))), abs_bits(f.w));
+  float4 f[HELD];
+#pragma unroll
+  for (int j = 0; j < HELD; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS;
+    f[j] = i < n ? pdl_ld(reinterpret_cast<const float4*>(x + (i >> a.quad_shift) * row) + (i & quad)) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  const float before = lo > first ? pdl_ld(a.scales + block) : 0.f;
+#pragma unroll
+  for (int j = 0; j < HELD; j++)
+    peak = max(max(max(peak, abs_bits(f[j].x)), max(abs_bits(f[j].y), abs_bits(f[j].z))), abs_bits(f[j].w));
   peak = __reduce_max_sync(0xffffffffu, peak);
   if ((threadIdx.x & 31) == 0) peaks[threadIdx.x >> 5] = peak;
-  const float before = lo > first ? *pdl_after(a.scales + block) : 0.f;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < APPEND_THREADS / 32; i++) peak = max(peak, peaks[i]);
   const float fresh = __fdiv_rn(__uint_as_float(peak), 127.f);
   const float scale = lo > first && !(fresh > before) && fresh == fresh ? before : fresh;
   const bool usable = scale > 0.f && scale < INFINITY;            // (all zero, or it stands for NaN: codes of 0)
+  const float inverse = scale > 1e-30f ? __frcp_rn(scale) : 0.f;
 
   if (lo > first && scale > before) {
-    const int old = (lo - first) * quads;
+    const int old = (lo - first) << a.quad_shift;
     for (int i = threadIdx.x; i < old; i += APPEND_THREADS) {
-      const uint32_t w = *pdl_after(codes + i);
+      const uint32_t w = pdl_ld(codes + i);
       int c[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) c[j] = usable ? quantise(__fmul_rn((float)(int8_t)(w >> (8 * j)), before), scale) : 0;
       codes[i] = pack4(c[0], c[1], c[2], c[3]);
     }
   }
-  uint32_t* to = codes + (lo - first) * quads;
-  for (int i = threadIdx.x; i < n; i += APPEND_THREADS) {
-    const float4 f = pdl_ld(reinterpret_cast<const float4*>(x + (i / quads) * row) + i % quads);
-    to[i] = usable ? pack4(quantise(f.x, scale), quantise(f.y, scale), quantise(f.z, scale), quantise(f.w, scale)) : 0u;
+  uint32_t* to = codes + ((lo - first) << a.quad_shift);
+#pragma unroll
+  for (int j = 0; j < HELD; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS;
+    if (i < n) to[i] = usable ? quantise4(f[j], scale, inverse) : 0u;
   }
   if (threadIdx.x == 0) a.scales[block] = scale;
 }
@@ -141,12 +165,18 @@ extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d
               "wdc_cache_append: buffers are not aligned");
   AppendArgs a = {k, v, (int8_t*)codes, scales, page_table, lengths, counts, ctx->status_word, d->pages, d->table_pages,
                   d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st, (int)d->tokens,
-                  (int)((d->tokens + d->page_tokens - 2) / d->page_tokens + 1), (int)d->kv_heads, (int)d->page_tokens,
-                  (int)d->head_size};
+                  (int)((d->tokens + d->page_tokens - 2) / d->page_tokens + 1), (int)d->kv_heads, 4, 3};
+  while (1 << a.page_shift < d->page_tokens) a.page_shift++;
+  while (4 << a.quad_shift < d->head_size) a.quad_shift++;
   const int64_t ctas = d->batch * a.slots * 2 * d->kv_heads;
   WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_cache_append: batch exceeds the grid");
+  // float4 of a page's new tokens a thread: of all its tokens, or of as many as the call can bring
+  const int64_t most = (d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * d->head_size / 4;
+  auto kernel = most <= APPEND_THREADS       ? cache_append_kernel<1>
+                : most <= 4 * APPEND_THREADS ? cache_append_kernel<4>
+                : most <= 8 * APPEND_THREADS ? cache_append_kernel<8> : cache_append_kernel<16>;
   DeviceGuard g(ctx->device);
-  wdc_launch_pdl(ctx, cache_append_kernel, dim3((unsigned)ctas), dim3(APPEND_THREADS), 0, a);
+  wdc_launch_pdl(ctx, kernel, dim3((unsigned)ctas), dim3(APPEND_THREADS), 0, a);
   return wdc_check_launch(ctx, "cache_append_kernel");
 }
 
