@@ -33,17 +33,20 @@ struct CacheAttArgs {
 // Weights carry the value scale of their page.  With s the scores (base 2) and lv = log2(value scale) of a group of 16 tokens,
 //   m = max s,  l = sum 2^(s - m);      M = max (s + [lv]),  O = sum 2^(s + lv - M) code,      y = O 2^(M - m) / l,
 // so that what is split into halves is relative to the largest term of O, whatever the pages' scales are.  ([lv] is the scale's
-// binary exponent: the maxima need no logarithm, and the weights take the scale itself.)
+// binary exponent: the maxima need no logarithm, and the weights take the scale itself.)  M need not be that maximum, only no
+// less: it starts HEADROOM above what the first tile has, and rises only when a term would pass it, so that O is rarely scaled
+// again.  A tile's tokens of one page are a group: 32 of them, or 16 where pages hold no more (GROUPS).
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, ROWS = 8;
-constexpr float WEIGHT_BITS = 14.f;        // weights are up to 2^14: both halves stay in float16's normal range
+constexpr float WEIGHT_BITS = 14.f;        // weights are less than 2^15: both halves stay in float16's normal range
+constexpr float HEADROOM = 3.f;
 constexpr int QUERY_BITS = 13;             // a row's queries are scaled to less than 2^14
 
 template <int DH>
 struct Layout {
-  static constexpr int CTAS = DH == 128 ? 2 : 4;                     // per SM: what registers and shared memory have room for
-  static constexpr int STAGES = 3;
-  static constexpr int SCALES = 2 * TILE * DH;                       // behind a stage's keys and values: four scales, and
-  static constexpr int THERE = SCALES + 16;                          // which of its two groups of 16 tokens are there
+  static constexpr int CTAS = DH == 128 ? 3 : 4;                     // per SM: what registers and shared memory have room for
+  static constexpr int STAGES = DH == 128 ? 2 : 3;
+  static constexpr int SCALES = 2 * TILE * DH;                       // behind a stage's keys and values: its groups' scales, and
+  static constexpr int THERE = SCALES + 16;                          // which of its groups are there
   static constexpr int STAGE = SCALES + 128, RING = STAGES * STAGE;  // (128-byte lines, for value_at)
   static constexpr int STRIDE = DH + 4, STATS = ROWS * STRIDE;       // floats: a row when the warps join; behind them m, M, l
   static constexpr int PART = STATS + 3 * ROWS;
@@ -128,26 +131,25 @@ __device__ __forceinline__ float quad_max(float x) {
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 
-// Asynchronous copies of 16 tokens' keys and values by a warp.  `k` and `v` are at this lane's 16 bytes.
-template <int DH, int GROUP>
-__device__ __forceinline__ void copy_group(uint32_t to_k, uint32_t to_v, const int8_t* k, const int8_t* v) {
-  constexpr int AT = GROUP * 16 * DH;
-  copy16<AT, 0>(to_k, k);
-  copy16<AT, 0>(to_v, v);
+// Asynchronous copies of 16 tokens' keys and values by a warp.  `k` and `v` are at this lane's 16 bytes; MORE: how far behind.
+template <int DH, int TO, int MORE>
+__device__ __forceinline__ void copy_half(uint32_t to_k, uint32_t to_v, const int8_t* k, const int8_t* v) {
+  copy16<TO, MORE>(to_k, k);
+  copy16<TO, MORE>(to_v, v);
   if (DH >= 64) {
     // (128: eight rows of a line's exchange pattern are two copies, so that every other copy's is the other half's)
-    copy16<AT + (DH >= 64 ? 512 : 0), DH >= 64 ? 512 : 0>(to_k, k);
-    copy16<AT + (DH >= 64 ? 512 : 0), DH >= 64 ? 512 : 0>(DH == 128 ? to_v ^ 64 : to_v, v);
+    copy16<TO + (DH >= 64 ? 512 : 0), MORE + (DH >= 64 ? 512 : 0)>(to_k, k);
+    copy16<TO + (DH >= 64 ? 512 : 0), MORE + (DH >= 64 ? 512 : 0)>(DH == 128 ? to_v ^ 64 : to_v, v);
   }
   if (DH == 128) {
-    copy16<AT + 1024, 1024>(to_k, k);
-    copy16<AT + 1024, 1024>(to_v, v);
-    copy16<AT + 1536, 1536>(to_k, k);
-    copy16<AT + 1536, 1536>(to_v ^ 64, v);
+    copy16<TO + 1024, MORE + 1024>(to_k, k);
+    copy16<TO + 1024, MORE + 1024>(to_v, v);
+    copy16<TO + 1536, MORE + 1536>(to_k, k);
+    copy16<TO + 1536, MORE + 1536>(to_v ^ 64, v);
   }
 }
 
-template <int DH>
+template <int DH, int GROUPS>
 __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_kernel(const CacheAttArgs a) {
   constexpr int STEPS = DH / 16;                  // of the score product's sum; also columns of O a thread and key row
   constexpr int KB = DH == 32 ? 8 : 16;           // bytes of a key a thread loads at a time
@@ -179,31 +181,33 @@ __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_ker
   const float* scales = a.scales + kvh + (lane & 1) * a.kv_heads;
   const uint32_t to_scale = smem_u32(ring + L::SCALES + (lane & 1) * 4);
 
-  // the pages of a tile's two groups of 16 tokens (-1: nothing is there), and their copies to a stage
-  const auto pages_of = [&](int i, int (&page)[2]) {
+  // the pages of a tile's groups (-1: nothing is there), and their copies to a stage
+  constexpr int SIZE = TILE / GROUPS;
+  const auto pages_of = [&](int i, int (&page)[GROUPS]) {
 #pragma unroll
-    for (int group = 0; group < 2; group++) {
-      const int t0 = i * TILE + group * 16;
+    for (int group = 0; group < GROUPS; group++) {
+      const int t0 = i * TILE + group * SIZE;
       page[group] = i < end && t0 < seen ? cache_page(table, t0 >> a.page_shift, a.pages, a.status) : -1;
     }
   };
-  const auto fetch = [&](int i, const int (&page)[2], uint32_t stage_at) {
-    const uint32_t in_page = (uint32_t)(i * TILE) & ((1u << a.page_shift) - 1);
-    if (page[0] >= 0) {
-      const int8_t* k = codes + (uint64_t)(uint32_t)page[0] * page_bytes + in_page * DH;
-      copy_group<DH, 0>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
-      if (lane < 2) copy4(to_scale + stage_at, scales + (uint64_t)(uint32_t)page[0] * (uint32_t)(2 * a.kv_heads));
-    }
-    if (page[1] >= 0) {
-      const uint32_t at = a.page_shift == 4 ? 0 : in_page + 16;
-      const int8_t* k = codes + (uint64_t)(uint32_t)page[1] * page_bytes + at * DH;
-      copy_group<DH, 1>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
-      if (lane < 2) copy4(to_scale + stage_at + 8, scales + (uint64_t)(uint32_t)page[1] * (uint32_t)(2 * a.kv_heads));
+  const auto fetch = [&](int i, const int (&page)[GROUPS], uint32_t stage_at) {
+    int there = 0;
+#pragma unroll
+    for (int group = 0; group < GROUPS; group++) {
+      if (page[group] < 0) continue;
+      there |= 1 << group;
+      // (a group of 16 is a page of 16, from its first token on)
+      const uint32_t in_page = GROUPS == 2 ? 0 : (uint32_t)(i * TILE) & ((1u << a.page_shift) - 1);
+      const int8_t* k = codes + ((uint64_t)(uint32_t)page[group] * page_bytes + in_page * DH);
+      if (GROUPS == 1 || group == 0) copy_half<DH, 0, 0>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
+      if (GROUPS == 1) copy_half<DH, 16 * DH, 16 * DH>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
+      else if (group == 1) copy_half<DH, 16 * DH, 0>(to_k + stage_at, to_v + stage_at, k, k + side_bytes);
+      if (lane < 2) copy4(to_scale + stage_at + group * 8, scales + (uint64_t)(uint32_t)page[group] * (uint32_t)(2 * a.kv_heads));
     }
     copies_commit();
-    if (lane == 0) *reinterpret_cast<int*>(ring + stage_at + L::THERE) = (page[0] >= 0 ? 1 : 0) | (page[1] >= 0 ? 2 : 0);
+    if (lane == 0) *reinterpret_cast<int*>(ring + stage_at + L::THERE) = there;
   };
-  int next = first + warp, page[2];
+  int next = first + warp, page[GROUPS];
 #pragma unroll
   for (int s = 0; s < L::STAGES; s++, next += WARPS) {
     pages_of(next, page);
@@ -247,8 +251,15 @@ __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_ker
     copies_wait<L::STAGES - 1>();
     __syncwarp();
     const unsigned char* tile_at = ring + stage_at;
-    const float4 sc = *reinterpret_cast<const float4*>(tile_at + L::SCALES);    // keys, values of both groups
+    float key_scale[GROUPS], value_scale[GROUPS];
+#pragma unroll
+    for (int group = 0; group < GROUPS; group++) {
+      const float2 sc = *reinterpret_cast<const float2*>(tile_at + L::SCALES + group * 8);
+      key_scale[group] = sc.x;
+      value_scale[group] = sc.y;
+    }
     const int there = *reinterpret_cast<const int*>(tile_at + L::THERE);
+    constexpr int PER = 4 / GROUPS;                // sets of eight tokens a group
     float s[4][2];
 #pragma unroll
     for (int n = 0; n < 4; n++) {
@@ -260,48 +271,53 @@ __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_ker
 #pragma unroll
         for (int k = 0; k < KB / 4; k++) mma(c, q[j + k], two_codes<0x4140>(w[k]), two_codes<0x4342>(w[k]));
       }
-      const float by = row_scale * (n < 2 ? sc.x : sc.z);
+      const float by = row_scale * key_scale[n / PER];
       s[n][0] = (c[0] + c[2]) * by;
       s[n][1] = (c[1] + c[3]) * by;
     }
     // what this row does not see
-    const bool whole = (i + 1) * TILE <= seen_by_all && there == 3;
+    const bool whole = (i + 1) * TILE <= seen_by_all && there == (1 << GROUPS) - 1;
     if (!whole) {
       const int t0 = i * TILE + 2 * t;
 #pragma unroll
       for (int n = 0; n < 4; n++)
 #pragma unroll
         for (int k = 0; k < 2; k++)
-          if (t0 + n * 8 + k > last || !(there >> (n >> 1) & 1)) s[n][k] = -INFINITY;
+          if (t0 + n * 8 + k > last || !(there >> (n / PER) & 1)) s[n][k] = -INFINITY;
     }
-    const float top0 = quad_max(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])));
-    const float top1 = quad_max(fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
-    float e0, e1, f0, f1;
-    exponent_of(sc.y, e0, f0);
-    exponent_of(sc.w, e1, f1);
-    const float m_new = fmaxf(m, fmaxf(top0, top1));
-    const float big_new = fmaxf(big, fmaxf(top0 + e0, top1 + e1));
-    const float m_ref = finite_or_0(m_new), big_ref = finite_or_0(big_new);
-    l *= exp2_of(m - m_ref);
-    f0 *= exp2_of(fminf(m_ref + e0 - big_ref + WEIGHT_BITS, 126.f));
-    f1 *= exp2_of(fminf(m_ref + e1 - big_ref + WEIGHT_BITS, 126.f));
-    if (__any_sync(0xffffffffu, big_new != big)) {
-      const float keep = exp2_of(big - big_ref);
+    float e[GROUPS], f[GROUPS], m_new = m, big_new = -INFINITY;
+#pragma unroll
+    for (int group = 0; group < GROUPS; group++) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = group * PER; n < (group + 1) * PER; n++) top = fmaxf(top, fmaxf(s[n][0], s[n][1]));
+      top = quad_max(top);
+      exponent_of(value_scale[group], e[group], f[group]);
+      m_new = fmaxf(m_new, top);
+      big_new = fmaxf(big_new, top + e[group]);
+    }
+    if (__any_sync(0xffffffffu, big_new > big)) {
+      big_new = big_new > big ? big_new + HEADROOM : big;
+      const float keep = exp2_of(big - finite_or_0(big_new));
 #pragma unroll
       for (int d = 0; d < DH / 8; d++)
 #pragma unroll
         for (int k = 0; k < 4; k++) o[d][k] *= keep;
+      big = big_new;
     }
+    const float m_ref = finite_or_0(m_new), big_ref = finite_or_0(big);
+    l *= exp2_of(m - m_ref);
     m = m_new;
-    big = big_new;
+#pragma unroll
+    for (int group = 0; group < GROUPS; group++) f[group] *= exp2_of(fminf(m_ref + e[group] - big_ref + WEIGHT_BITS, 126.f));
     float w[4][2];
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const float e = exp2_of(s[n][k] - m_ref);
-        l += e;
-        w[n][k] = e * (n < 2 ? f0 : f1);
+        const float p = exp2_of(s[n][k] - m_ref);
+        l += p;
+        w[n][k] = p * f[n / PER];
       }
     if (!whole) {                                  // (a scale that is no number is for the rows that see it)
 #pragma unroll
@@ -315,21 +331,21 @@ __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_ker
     for (int n = 0; n < 4; n++) split(w[n][0], w[n][1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
     const unsigned char* values = tile_at + TILE * DH;
 #pragma unroll
-    for (int group = 0; group < 2; group++) {
+    for (int half = 0; half < 2; half++) {
       uint32_t v[4][VB / 4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int key = group * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
+        const int key = half * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
         load_words<VB>(values + value_at<DH>(key, g * VB / 16) + g * VB % 16, v[r]);
       }
 #pragma unroll
       for (int w = 0; w < VB / 4; w++) {
         const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
         const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-        mma(o[w * 4 + 0], p[group], two_codes<0x4140>(a0), two_codes<0x4140>(b0));
-        mma(o[w * 4 + 1], p[group], two_codes<0x4342>(a0), two_codes<0x4342>(b0));
-        mma(o[w * 4 + 2], p[group], two_codes<0x4140>(a1), two_codes<0x4140>(b1));
-        mma(o[w * 4 + 3], p[group], two_codes<0x4342>(a1), two_codes<0x4342>(b1));
+        mma(o[w * 4 + 0], p[half], two_codes<0x4140>(a0), two_codes<0x4140>(b0));
+        mma(o[w * 4 + 1], p[half], two_codes<0x4342>(a0), two_codes<0x4342>(b0));
+        mma(o[w * 4 + 2], p[half], two_codes<0x4140>(a1), two_codes<0x4140>(b1));
+        mma(o[w * 4 + 3], p[half], two_codes<0x4342>(a1), two_codes<0x4342>(b1));
       }
     }
     __syncwarp();
@@ -454,17 +470,18 @@ __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const Cac
   a.y[b * a.y_sb + (kvh * a.group + row % a.group) * a.y_sh + token * a.y_st + threadIdx.x] = sum * by;
 }
 
-template <int DH>
+template <int DH, int GROUPS>
 int launch(wdc_context* ctx, CacheAttArgs& a) {
   static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
   WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "wdc_cache_attention: device index out of range");
   if (!opted_in[ctx->device]) {
-    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DH>::SMEM));
+    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Layout<DH>::SMEM));
     opted_in[ctx->device] = true;
   }
   const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = Layout<DH>::CTAS * ctx->sm_count;
   const int64_t tiles = ceil_div64(a.table_pages << a.page_shift, TILE);
-  int64_t splits = ceil_div64(4 * slots, units);
+  int64_t splits = ceil_div64(slots, units);
   if (splits > ceil_div64(tiles, WARPS)) splits = ceil_div64(tiles, WARPS);
   if (splits < 1) splits = 1;
   a.splits = (int)splits;
@@ -475,7 +492,7 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
     a.part_rows = scratch;
     a.part_stats = scratch + units * splits * ROWS * DH;
   }
-  wdc_launch_pdl(ctx, cache_attention_kernel<DH>, dim3((unsigned)(units * splits)), dim3(THREADS), Layout<DH>::SMEM, a);
+  wdc_launch_pdl(ctx, cache_attention_kernel<DH, GROUPS>, dim3((unsigned)(units * splits)), dim3(THREADS), Layout<DH>::SMEM, a);
   int s = wdc_check_launch(ctx, "cache_attention_kernel");
   if (s == WDC_OK && splits > 1) {
     wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)(a.batch * a.heads * a.tokens)), dim3(THREADS), 0, a);
@@ -521,5 +538,8 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   a.row_tiles = (int)ceil_div64(d->tokens * a.group, ROWS);
   a.scale_log2 = d->scale * 1.4426950408889634f;
   DeviceGuard g(ctx->device);
-  return d->head_size == 32 ? launch<32>(ctx, a) : d->head_size == 64 ? launch<64>(ctx, a) : launch<128>(ctx, a);
+  const bool small = d->page_tokens < TILE;
+  if (d->head_size == 32) return small ? launch<32, 2>(ctx, a) : launch<32, 1>(ctx, a);
+  if (d->head_size == 64) return small ? launch<64, 2>(ctx, a) : launch<64, 1>(ctx, a);
+  return small ? launch<128, 2>(ctx, a) : launch<128, 1>(ctx, a);
 }

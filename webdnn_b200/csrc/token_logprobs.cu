@@ -8,7 +8,7 @@ namespace {
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS, EACH = 4;      // float4 a thread and round
 constexpr int TOP_MOST = 32, PARTS_MOST = 8;
-constexpr int KEPT = 1024;                                     // keys that the candidates' list holds
+constexpr int KEPT = 192;                                      // keys that a warp's list of candidates holds
 constexpr int PART_LEAST = 4096;                               // logits of a part, where a row is cut into several
 
 struct LogprobArgs {
@@ -83,31 +83,31 @@ __device__ __forceinline__ uint64_t warp_joined(uint64_t a, uint64_t b_backwards
 }
 
 struct Shared {
-  uint64_t kept[KEPT];                 // candidates, in no order
+  uint64_t kept[WARPS][KEPT];          // a warp's candidates, in no order
   uint64_t lists[WARPS][32];
   uint64_t part_lists[PARTS_MOST][32]; // of the parts of a row, in the first CTA of its cluster
   Sums part_sums[PARTS_MOST];
   Sums sums[WARPS];
   uint64_t best[WARPS];
-  unsigned int count;
+  unsigned long long floor_key;
 };
 
-// The 32 largest of the warps' sorted lists, to lists[0].  All threads; a barrier at both ends.
-__device__ __forceinline__ void join_lists(Shared& sh, uint64_t sorted) {
+// The 32 largest of `count` sorted lists in shared memory, to list 0.  All threads; a barrier at both ends.
+__device__ __forceinline__ void join_lists(uint64_t (*lists)[32], int count) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  sh.lists[warp][lane] = sorted;
   __syncthreads();
-#pragma unroll
-  for (int step = WARPS / 2; step > 0; step /= 2) {
-    if (warp < step) sh.lists[warp][lane] = warp_joined(sh.lists[warp][lane], sh.lists[warp + step][31 - lane]);
+  for (int step = count / 2; step > 0; step /= 2) {
+    if (warp < step) lists[warp][lane] = warp_joined(lists[warp][lane], lists[warp + step][31 - lane]);
     __syncthreads();
   }
 }
-__device__ __forceinline__ uint64_t sorted_part_of_kept(const Shared& sh, int count) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t key = 0;
-  for (int at = warp * 32; at < count; at += THREADS) {
-    const uint64_t more = warp_sorted(at + lane < count ? sh.kept[at + lane] : 0);
+// The 32 largest of a warp's candidates, sorted.
+__device__ __forceinline__ uint64_t warp_best(const uint64_t* kept, int have) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  uint64_t key = warp_sorted(lane < have ? kept[lane] : 0);
+  for (int at = 32; at < have; at += 32) {
+    const uint64_t more = warp_sorted(at + lane < have ? kept[at + lane] : 0);
     key = warp_joined(key, __shfl_sync(0xffffffffu, more, 31 - lane));
   }
   return key;
@@ -123,10 +123,9 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 
 // One CTA per row, or a cluster of `parts` where rows are few, each on a range of the row.  A round is EACH float4 a thread.
 //
-// Candidates for the best `top`: `floor_key` is a key that `top` logits of the range are known to be above; what a round has above
-// it goes to a list in shared memory.  Where more might come than the list has room for (always in the first round), the floor is
-// raised first, to just below the `top`-th largest of the threads' largest keys of the round: at most `top` threads hold
-// anything above that, EACH * 4 keys each.  A list that is nearly full is cut to its `top` largest, which raises the floor too.
+// Candidates for the best `top`: the floor is a key that `top` logits of the range are known to be above.  After the first round it
+// is just below the `top`-th largest of the threads' largest keys; from then on every warp keeps what is above it in a list of its
+// own, without a barrier.  A list that might overflow is cut to its `top` largest, which raises the floor for all.
 template <bool kTop, bool kCluster>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobArgs a) {
   __shared__ Shared sh;
@@ -134,7 +133,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
   const int rank = kCluster ? (int)(blockIdx.x % (unsigned)a.parts) : 0;
   const int64_t row = kCluster ? blockIdx.x / (unsigned)a.parts : blockIdx.x;
   if (kCluster) cluster_arrive();   // this CTA has begun: the others may write to its shared memory (waited for below)
-  if (threadIdx.x == 0) sh.count = 0;
+  if (kTop && threadIdx.x == 0) sh.floor_key = 0;
   pdl_wait();
   const float* x = pdl_after(a.logits) + row * a.row_stride;
   // float4 from the first 16-byte boundary on; what is before and behind them goes by single floats, to the first part
@@ -145,18 +144,17 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
 
   Sums sums = {-INFINITY, 0.f, 0.f};
   uint64_t floor_key = 0;
-  float floor_value = -INFINITY;
-  int have = 0;
-  if (rank == 0) {
+  uint64_t* kept = sh.kept[warp];
+  int have = 0;                                    // candidates of this warp
+  if (rank == 0 && warp == 0) {
     const int singles = a.vocab - quads * 4;       // up to six
-    if ((int)threadIdx.x < singles) {
-      const int i = (int)threadIdx.x < before ? (int)threadIdx.x : quads * 4 + (int)threadIdx.x;
+    if (lane < singles) {
+      const int i = lane < before ? lane : quads * 4 + lane;
       const float v = pdl_ld(x + i);
       raise_to(sums, v);
       take(sums, v, sums.m == -INFINITY ? 0.f : sums.m);
-      if (kTop) sh.kept[threadIdx.x] = order_key(v, i);
+      if (kTop) kept[lane] = order_key(v, i);
     }
-    if (kTop && threadIdx.x == 0) sh.count = singles;
     have = singles;
   }
   for (int base = begin; base < end; base += THREADS * EACH) {
@@ -166,9 +164,10 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
       const int at = base + j * THREADS + (int)threadIdx.x;
       f[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    float peak = -INFINITY;
+    float peaks[EACH];
 #pragma unroll
-    for (int j = 0; j < EACH; j++) peak = fmaxf(fmaxf(fmaxf(f[j].x, f[j].y), fmaxf(f[j].z, f[j].w)), peak);
+    for (int j = 0; j < EACH; j++) peaks[j] = fmaxf(fmaxf(f[j].x, f[j].y), fmaxf(f[j].z, f[j].w));
+    const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
     raise_to(sums, peak);
     const float ref = sums.m == -INFINITY ? 0.f : sums.m;
 #pragma unroll
@@ -180,43 +179,53 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
     }
     if (kTop) {
       const int first = before + 4 * (base + (int)threadIdx.x);
-      const auto each = [&](auto what) {
+      if (base == begin) {
+        uint64_t mine = 0;
 #pragma unroll
         for (int j = 0; j < EACH; j++) {
           if (base + j * THREADS + (int)threadIdx.x >= end) break;
-          const int i = first + 4 * j * THREADS;
-          what(order_key(f[j].x, i));
-          what(order_key(f[j].y, i + 1));
-          what(order_key(f[j].z, i + 2));
-          what(order_key(f[j].w, i + 3));
+          // the largest of the four, and the first of those
+          const int i = first + 4 * j * THREADS + (f[j].x == peaks[j] ? 0 : f[j].y == peaks[j] ? 1 : f[j].z == peaks[j] ? 2 : 3);
+          const uint64_t key = order_key(peaks[j], i);
+          mine = key > mine ? key : mine;
         }
-      };
-      uint64_t mine = 0;
-      if (peak >= floor_value) each([&](uint64_t key) { mine = key > mine ? key : mine; });
-      const int wanting = __syncthreads_count(mine > floor_key);
-      if (wanting == 0) continue;
-      if (have + wanting * EACH * 4 > KEPT) {
-        join_lists(sh, warp_sorted(mine));
-        uint64_t least = sh.lists[0][a.top - 1];
-        if (least > floor_key + 1) floor_key = least - 1;
-        if (have + a.top * EACH * 4 > KEPT) {
-          const uint64_t sorted = sorted_part_of_kept(sh, have);
-          __syncthreads();                         // lists[0] and the candidates have been read
-          join_lists(sh, sorted);
-          least = sh.lists[0][a.top - 1];
-          if (least > floor_key + 1) floor_key = least - 1;
-          if (warp == 0) sh.kept[lane] = sh.lists[0][lane];
-          if (threadIdx.x == 0) sh.count = a.top;  // (there are more candidates than that)
-        }
-        __syncthreads();
-        floor_value = floor_key ? key_value(floor_key) : -INFINITY;
+        sh.lists[warp][lane] = warp_sorted(mine);
+        join_lists(sh.lists, WARPS);
+        floor_key = sh.lists[0][a.top - 1];
+        if (floor_key) floor_key--;                // (fewer than `top` threads have any)
+        __syncthreads();                           // (the lists are used again)
+      } else {
+        const uint64_t raised = *(volatile unsigned long long*)&sh.floor_key;
+        floor_key = raised > floor_key ? raised : floor_key;
       }
-      if (mine > floor_key)
-        each([&](uint64_t key) {
-          if (key > floor_key) sh.kept[atomicAdd(&sh.count, 1u)] = key;
-        });
-      __syncthreads();
-      have = (int)sh.count;
+      const float floor_value = floor_key ? key_value(floor_key) : -INFINITY;
+      if (!__any_sync(0xffffffffu, peak >= floor_value)) continue;
+#pragma unroll
+      for (int j = 0; j < EACH; j++) {
+        const bool inside = base + j * THREADS + (int)threadIdx.x < end;
+        if (!__any_sync(0xffffffffu, inside && peaks[j] >= floor_value)) continue;
+        const int i = first + 4 * j * THREADS;
+        const float v[4] = {f[j].x, f[j].y, f[j].z, f[j].w};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const uint64_t key = order_key(v[c], i + c);
+          const bool above = inside && key > floor_key && v[c] == v[c];
+          const unsigned who = __ballot_sync(0xffffffffu, above);
+          if (above) kept[have + __popc(who & ((1u << lane) - 1))] = key;
+          have += __popc(who);
+        }
+        if (have > KEPT - 128) {
+          const uint64_t key = warp_best(kept, have), least = __shfl_sync(0xffffffffu, key, a.top - 1) - 1;
+          __syncwarp();
+          kept[lane] = key;
+          have = a.top;                            // (there were more than that)
+          if (least > floor_key) {
+            floor_key = least;
+            if (lane == 0) atomicMax(&sh.floor_key, least);
+          }
+          __syncwarp();
+        }
+      }
     }
   }
 
@@ -225,17 +234,20 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
     add(sums, {__shfl_xor_sync(0xffffffffu, sums.m, w), __shfl_xor_sync(0xffffffffu, sums.s, w),
                __shfl_xor_sync(0xffffffffu, sums.t, w)});
   if (lane == 0) sh.sums[warp] = sums;
-  __syncthreads();
-  if (kTop) join_lists(sh, sorted_part_of_kept(sh, have));
+  if (kTop) {
+    sh.lists[warp][lane] = warp_best(kept, have);
+    join_lists(sh.lists, WARPS);
+  } else {
+    __syncthreads();
+  }
   sums = sh.sums[0];
 #pragma unroll
   for (int w = 1; w < WARPS; w++) add(sums, sh.sums[w]);
-  uint64_t best = kTop ? sh.lists[0][lane] : 0;
   if (kCluster) {
     cluster_wait();
     if (warp == 0) {
       if (kTop)
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at(&sh.part_lists[rank][31 - lane], 0)), "l"(best) : "memory");
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at(&sh.part_lists[rank][lane], 0)), "l"(sh.lists[0][lane]) : "memory");
       if (lane < 3)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_at(&sh.part_sums[rank].m + lane, 0)),
                      "f"(lane == 0 ? sums.m : lane == 1 ? sums.s : sums.t) : "memory");
@@ -243,10 +255,8 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    for (int r = 1; r < a.parts; r++) {
-      add(sums, sh.part_sums[r]);
-      if (kTop) best = warp_joined(best, sh.part_lists[r][lane]);
-    }
+    for (int r = 1; r < a.parts; r++) add(sums, sh.part_sums[r]);
+    if (kTop) join_lists(sh.part_lists, a.parts);
   }
   const bool none = sums.m == -INFINITY;
   const float log_s = none ? NAN : logf(sums.s);
@@ -260,6 +270,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
   if (!kTop) return;
   if (sums.s == sums.s) {
     if (warp == 0 && lane < a.top) {
+      const uint64_t best = kCluster ? sh.part_lists[0][lane] : sh.lists[0][lane];
       a.top_ids[row * a.top + lane] = (int32_t)~(uint32_t)best;
       a.top_logprobs[row * a.top + lane] = key_value(best) - sums.m - log_s;
     }
