@@ -241,6 +241,72 @@ def test_attention(cuda_context, size, c, heads, kv_heads, lengths, counts):
     cache.dispose()
 
 
+PROMPTS = [
+    # enough rows of new tokens for the tensor-core kernel: 37 tiles of 128 rows
+    (64, 128, 16, 8, [300, 500], [290, 300]), (16, 64, 8, 8, [200, 150, 131], [200, 100, 131]),
+    (128, 128, 12, 4, [900], [700]), (32, 64, 30, 10, [150, 151], [90, 33]), (16, 128, 10, 10, [64, 65, 300, 63], [64, 1, 129, 63]),
+    (64, 64, 64, 2, [80, 1000], [80, 77]), (32, 128, 5, 5, [1000, 999], [513, 512]), (64, 128, 20, 20, [2000, 70], [100, 70]),
+]
+
+
+@pytest.mark.parametrize("size,c,heads,kv_heads,lengths,counts", PROMPTS)
+def test_attention_of_prompts(cuda_context, size, c, heads, kv_heads, lengths, counts):
+    rng = np.random.default_rng(size + c + heads + len(lengths))
+    ctx = cuda_context
+    cache = PagedCache(ctx, 1, sum(-(-n // size) for n in lengths) + 1, kv_heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, lengths)
+    q = rng.standard_normal((len(lengths), max(counts), heads, c)).astype(f32)
+    before = ctx.stats()["tensor_core_launches"]
+    got = run_attention(ctx, cache, q, table, lengths, counts)
+    assert ctx.stats()["tensor_core_launches"] == before + 1
+    want, tol = reference_attention(q, codes[0], scales[0], table, lengths, counts, size, c ** -0.5)
+    assert np.abs(got - want).max() <= tol
+    for b, n in enumerate(counts):
+        assert not got[b, n:].any()                   # padding
+    cache.dispose()
+
+
+def test_prompts_with_sharp_scores_missing_pages_and_scales_that_are_no_numbers(cuda_context):
+    rng = np.random.default_rng(20)
+    ctx, size, c, heads = cuda_context, 16, 64, 20
+    cache = PagedCache(ctx, 1, 41, heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, [300, 320])
+    scales[0, table[0, :19], 0] *= np.linspace(0.2, 8, 19, dtype=f32)[:, None]
+    scales[0, table[0, 18], 1] = 0
+    scales[0, table[1, 12], 1, 3] = np.nan            # tokens 192 .. of the second sequence, one head's values
+    scales[0, table[1, 5], 0, 4] = np.inf             # tokens 80 ..: another's keys
+    set_pool(cache, codes, scales)
+    lengths, counts = [300, 320], [170, 310]
+    q = (rng.standard_normal((2, 310, heads, c)) * np.where(np.arange(heads) % 3 == 0, 20, 1)[:, None]).astype(f32)
+    got = run_attention(ctx, cache, q, table, lengths, counts, scale=0.3)
+    first = np.arange(310) + 10
+    assert np.isnan(got[1, first >= 192, 3]).all() and np.isfinite(got[1, first < 192, 3]).all()
+    assert np.isnan(got[1, first >= 80, 4]).all() and np.isfinite(got[1, first < 80, 4]).all()
+    scales[0, table[1, 12], 1, 3] = scales[0, table[1, 5], 0, 4] = 0
+    want, tol = reference_attention(q, codes[0], scales[0], table, lengths, counts, size, float(f32(0.3)))
+    fine = np.isfinite(got)
+    assert np.abs(got - want)[fine].max() <= tol and fine.mean() > 0.9
+    # a page out of range: its tokens are left out
+    set_pool(cache, codes, scales)
+    holes = table.copy()
+    holes[0, 3] = 41
+    ts = [dev(ctx, a) for a in (q.reshape(2, 310, -1), holes, np.array(lengths, np.int32), np.array(counts, np.int32))]
+    y = cache.attention(0, *ts, scale=0.3)
+    with pytest.raises(CudaBackendError, match="out of range"):
+        ctx.sync()
+    got = y.get_data().reshape(q.shape)
+    shorter = table.copy()
+    shorter[0, 3:19] = table[0, 4:20]
+    k_lengths = [300 - size, 320]
+    want0, tol0 = reference_attention(q[:1], codes[0], scales[0], shorter[:1], k_lengths[:1], counts[:1], size, float(f32(0.3)))
+    assert np.abs(got[0] - want0[0]).max() <= tol0
+    for t in ts + [y]:
+        t.dispose()
+    cache.dispose()
+
+
 @pytest.mark.parametrize("tokens", [1, 70])
 def test_sharp_and_tiny_scores(cuda_context, tokens):
     """Scores spread over hundreds of units, the largest at the end, and queries of very different magnitudes."""

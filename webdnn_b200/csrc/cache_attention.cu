@@ -3,26 +3,9 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include "paged_cache.cuh"
+#include "cache_attention.cuh"
 
 namespace {
-
-struct CacheAttArgs {
-  const float* q;
-  const int8_t* codes;
-  const float* scales;
-  const int32_t *page_table, *lengths, *counts;
-  float* y;
-  int* status;
-  int64_t pages, table_pages;
-  int64_t q_sb, q_sh, q_st, y_sb, y_sh, y_st;
-  int batch, tokens, heads, kv_heads, group, page_shift;   // 2^page_shift tokens a page
-  int row_tiles;
-  int splits;                      // CTAs of a unit; 0: the tiles of all units are shared out
-  float *part_rows, *part_stats;   // of every unit and split, or two of every CTA: O of a unit's rows; m, M and l
-  int* part_plan;                  // first tile of each sequence in the order of all, their number, tiles of a CTA
-  float scale_log2;                // scale * log2(e): the softmax runs on exp2
-};
 
 // A unit of work is eight rows of one sequence and key head, row = new token * group + query head of the group, and the tiles of 32
 // tokens of that sequence.  The warps of a CTA take tiles in turn, each through a ring of its own in shared memory that asynchronous
@@ -48,9 +31,10 @@ struct CacheAttArgs {
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, ROWS = 8;
 constexpr int PLAN_MOST = 512;             // sequences whose tiles are shared out
 constexpr int BEGIN = 8;
-constexpr float WEIGHT_BITS = 14.f;        // weights are less than 2^15: both halves stay in float16's normal range
 constexpr float HEADROOM = 3.f;
-constexpr int QUERY_BITS = 13;             // a row's queries are scaled to less than 2^14
+// Tiles whose weighted values the tensor core adds up before the sum goes to one of the thread's own.  It rounds towards zero, 2^-25
+// of the sum at each of two additions a tile: 44 in a row were 1.3e-6 short, 1000 would be 3e-5.  (Folding costs 4% of 3 x 40001.)
+constexpr int FOLD = 16;
 
 template <int DH>
 struct Layout {
@@ -80,26 +64,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// Two halves of a pair: h = x in float16, l = what is missing.
-__device__ __forceinline__ void split(float x, float y, uint32_t& h, uint32_t& l) {
-  const __half2 hi = __floats2half2_rn(x, y);
-  const float2 back = __half22float2(hi);
-  h = half2_bits(hi);
-  l = half2_bits(__floats2half2_rn(x - back.x, y - back.y));
-}
 // Two bytes of a word of codes + 128 as float16.  A byte alone is a number below float16's normal range, byte * 2^-24, which the
 // product takes exactly: a key's score is then 2^24 of that sum, less 128 times the sum of the query's channels.  (Sums of weighted
 // values cancel, so that the 128 has to go before them: 0x6400 + byte is 1024 + byte.)
 template <int SELECT>
 __device__ __forceinline__ uint32_t two_bytes(uint32_t w) { return __byte_perm(w, 0, SELECT); }
-template <int SELECT>
-__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
-  const uint32_t u = __byte_perm(w, 0x64646464u, SELECT);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return half2_bits(v);
-}
-
 // Where the 16-byte chunk `c` of token `t` lies in a tile of keys or values: as in memory, chunks of a 128-byte line exchanged
 // so that the eight (16-byte loads), sixteen (8) or 32 (4) threads that load at a time meet different banks.
 template <int DH>
@@ -127,20 +96,6 @@ __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)
   for (int i = 0; i < BYTES / 4; i++) w[i] ^= 0x80808080u;
 }
 
-__device__ __forceinline__ float exp2_of(float x) {      // results below 2^-126 are 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// A value scale as 2^e * f, 1 <= f < 2 (0: e = -infinity; no number: f is NaN).
-__device__ __forceinline__ void exponent_of(float scale, float& e, float& f) {
-  const bool small = scale < 1.2e-38f;                       // (below the normal range)
-  const uint32_t bits = __float_as_uint(small ? scale * 16777216.f : scale);
-  e = scale > 0.f && scale < INFINITY ? (float)((int)(bits >> 23) - (small ? 151 : 127)) : scale == 0.f ? -INFINITY : 0.f;
-  f = scale < INFINITY ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : NAN;
-}
-
-__device__ __forceinline__ float finite_or_0(float x) { return x == -INFINITY ? 0.f : x; }   // a reference to subtract
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -313,15 +268,12 @@ next_segment:
       peak = fmaxf(fmaxf(fmaxf(peak, fabsf(x[j].x)), fmaxf(fabsf(x[j].y), fabsf(x[j].z))), fabsf(x[j].w));
     }
     peak = quad_max(peak);
-    // 2^(its exponent), no less than 2^-100: smaller queries than that weigh nothing
-    const int e = max((int)(__float_as_uint(peak) >> 23) - 127, -100);
-    const float up = exp2f((float)(QUERY_BITS - e));
-    row_scale = exp2f((float)(e - QUERY_BITS)) * a.scale_log2 * 16777216.f;
+    const float up = query_scale(peak, a.scale_log2 * 16777216.f, row_scale);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
-      split(x[j].x * up, x[j].y * up, q[j][0], q[j][1]);
-      split(x[j].z * up, x[j].w * up, q[j][2], q[j][3]);
+      split_halves(x[j].x * up, x[j].y * up, q[j][0], q[j][1]);
+      split_halves(x[j].z * up, x[j].w * up, q[j][2], q[j][3]);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const float2 both = __half22float2(*reinterpret_cast<const __half2*>(&q[j][k]));
@@ -339,8 +291,31 @@ next_segment:
 #pragma unroll
     for (int i = 0; i < 4; i++) o[d][i] = 0.f;
 
+  // sums of FOLD tiles and more, in local memory: channels of this thread's two columns, relative to 2^total_big
+  float total_room[DH / 4], total_big = -INFINITY;
+  volatile float* total = total_room;
+  int added = 0;
   uint32_t stage_at = 0;
   for (int i = first + warp; i < end; i += WARPS) {
+    if (added == FOLD) {
+      const float keep = exp2_of(total_big - finite_or_0(big));
+      const bool some = total_big > -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        float before[DH / 8];
+#pragma unroll
+        for (int d = 0; d < DH / 8; d++) before[d] = total[k * (DH / 8) + d];      // (all loads before the first store)
+#pragma unroll
+        for (int d = 0; d < DH / 8; d++) {
+          const float sum = o[d][k] + o[d][k + 2];
+          total[k * (DH / 8) + d] = some ? fmaf(before[d], keep, sum) : sum;
+          o[d][k] = o[d][k + 2] = 0.f;
+        }
+      }
+      total_big = fmaxf(big, -1e30f);
+      added = 0;
+    }
+    added++;
     copies_wait<L::STAGES - 1>();
     __syncwarp();
     const unsigned char* tile_at = ring + stage_at;
@@ -421,7 +396,7 @@ next_segment:
     }
     uint32_t p[2][4];
 #pragma unroll
-    for (int n = 0; n < 4; n++) split(w[n][0], w[n][1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
+    for (int n = 0; n < 4; n++) split_halves(w[n][0], w[n][1], p[n >> 1][(n & 1) * 2], p[n >> 1][(n & 1) * 2 + 1]);
     const unsigned char* values = tile_at + TILE * DH;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
@@ -456,6 +431,13 @@ next_segment:
   float* parts = reinterpret_cast<float*>(smem);
   {
     float* mine = parts + warp * L::PART;
+    const float keep = exp2_of(total_big - finite_or_0(big));
+    if (total_big > -INFINITY) {
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int d = 0; d < DH / 8; d++) o[d][k] = fmaf(total[k * (DH / 8) + d], keep, o[d][k]);
+    }
 #pragma unroll
     for (int k = 0; k < 2; k++)
 #pragma unroll
@@ -659,6 +641,10 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   a.row_tiles = (int)ceil_div64(d->tokens * a.group, ROWS);
   a.scale_log2 = d->scale * 1.4426950408889634f;
   DeviceGuard g(ctx->device);
+  {
+    const int s = wdc_cache_attention_tc(ctx, a, (int)d->head_size);
+    if (s != WDC_ERR_UNSUPPORTED) return s;
+  }
   const bool small = d->page_tokens < TILE;
   if (d->head_size == 32) return small ? launch<32, 2>(ctx, a) : launch<32, 1>(ctx, a);
   if (d->head_size == 64) return small ? launch<64, 2>(ctx, a) : launch<64, 1>(ctx, a);
