@@ -4,14 +4,16 @@
 //
 // One CTA owns 128 rows of one sequence and key head, row = new token * group + query head of the group, and walks the tokens that
 // they see in chunks of 64:
-//   S  = Q K_chunk^T     two tcgen05.mma.kind::f16 products, M = 128, N = 64, K = head size: low half, high half.  Q is the A
-//                        operand in TENSOR MEMORY, K_chunk the B operand in shared memory
-//   P  = weights         by the 128 row threads (thread r = row r = TMEM lane r), in halves back to tensor memory
+//   S  = Q K_chunk^T     two tcgen05.mma.kind::f16 products, M = 128, N = 64, K = head size: low half, high half of Q, both operands
+//                        in shared memory
+//   P  = weights         by the row threads, in halves to TENSOR MEMORY, as the next A operand
 //   Oc = P V_chunk       two products, M = 128, N = head size, K = 64; V_chunk^T the B operand in shared memory
 //   O  = O * keep + Oc   in the row threads' registers, rounded to nearest
-// Warps 0-3 are row threads, 4-7 bring keys and values in and widen the codes to float16 in the tensor core's K-major layout with
-// 128-byte swizzle (values transposed on the way), three chunks deep; warp 7 issues the products too.  S has two buffers: while a
-// chunk's rows are turned into weights, the tensor core works on the last chunk's values and the next one's scores.
+// Warps 0-7 are row threads, two of a row (= TMEM lane): each has half of the chunk's scores and half of O's channels, and they
+// exchange their maxima through shared memory.  Warps 8-11 bring values in and 12-14 keys, widening the codes to float16 in the tensor
+// core's K-major layout with 128-byte swizzle (values transposed on the way), three chunks deep; warp 15 issues the products.  S and P
+// have two buffers: while a chunk's rows are turned into weights, the tensor core works on the last chunk's values and the next
+// one's scores.
 //
 // Bound: the row threads, about 18 instructions a score, against 16 cycles of the tensor pipe for four of them; measured below.
 // Every mbarrier wait is bounded (2 s): on expiry the CTA records a status code, raises its abort flag, frees its TMEM and returns.
@@ -22,13 +24,19 @@
 
 namespace {
 
-constexpr int BQ = 128, BK = 64, STAGES = 3, THREADS = 256;   // (a ninth warp would leave each 168 registers)
+constexpr int BQ = 128, BK = 64, STAGES = 3;
+constexpr int ROW_THREADS = 256, VALUE_THREADS = 128, KEY_THREADS = 96, ISSUER = 15, THREADS = 512;
+// 128 registers a thread at launch; four groups of four warps: 2 * 160 + 2 * 96 = 4 * 128
+constexpr int ROW_REGISTERS = 160, OTHER_REGISTERS = 96;
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
 
 struct Shared {
   unsigned long long kv_full[STAGES], kv_empty[STAGES], s_full[2], q_ready, p_ready, o_full;
   float key_scale[STAGES][4], exponent[STAGES][4], fraction[STAGES][4];   // of a chunk's groups of 16 tokens (values: 2^e * f)
   int there[STAGES];                                                      // which of the groups are there
+  float2 tops[2][2][BQ];                                                  // maxima of a row's halves, of two chunks
+  float row_scale[BQ], sums[BQ];
+  int row_stop[2];                                                        // of two chunks: a row thread's wait has expired
   unsigned int tmem_base;
   volatile int abort_flag;
 };
@@ -57,7 +65,7 @@ __device__ __forceinline__ unsigned long long global_ns() {
   return t;
 }
 // Bounded wait.  Returns false if the wait was abandoned (time limit or CTA-wide abort).
-__device__ __noinline__ bool mbar_wait_slow(unsigned long long* bar, uint32_t parity, Shared* sh, int* status, int code) {
+__device__ __forceinline__ bool mbar_wait_slow(unsigned long long* bar, uint32_t parity, Shared* sh, int* status, int code) {
   const unsigned long long t0 = global_ns();
   for (;;) {
     for (int i = 0; i < 1024; i++)
@@ -108,6 +116,18 @@ __device__ __forceinline__ void umma_one(uint32_t tmem_c, uint32_t tmem_a, uint3
       "r"(tmem_a), "r"(desc_lo), "r"(desc_top), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same with A in shared memory.
+__device__ __forceinline__ void umma_shared(uint32_t tmem_c, uint32_t a_lo, uint32_t b_lo, uint32_t desc_top, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_c),
+      "r"(a_lo), "r"(b_lo), "r"(desc_top), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void umma_commit_one(unsigned long long* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -138,9 +158,12 @@ template <int DH>
 struct Tile {
   static constexpr int K_BLOCK = BK * 128;                 // 64 tokens x 64 channels
   static constexpr int KEYS = 0, VALUES = DH / 64 * K_BLOCK, STAGE = 2 * VALUES;
-  static constexpr int SMEM = STAGES * STAGE + 1024;
-  // tensor-memory columns
-  static constexpr int Q_HI = 0, Q_LO = DH / 2, S = DH, P_HI = S + 2 * BK, P_LO = P_HI + BK / 2, O = P_LO + BK / 2, COLS = 512;
+  static constexpr int Q_BLOCK = BQ * 128;                 // 128 rows x 64 channels; high halves, then low ones, behind the stages
+  static constexpr int Q_HI = STAGES * STAGE, Q_LO = Q_HI + DH / 64 * Q_BLOCK;
+  static constexpr int OUT_STRIDE = DH + 4;                // floats of a row of the result, over all of this at the end
+  static constexpr int SMEM = Q_LO + DH / 64 * Q_BLOCK + 1024;
+  static constexpr int S = 0, P = 2 * BK, O = 4 * BK, COLS = 512;   // tensor-memory columns; S and P of two chunks
+  static_assert(BQ * OUT_STRIDE * 4 <= SMEM - 1024, "the result's place");
 };
 
 template <int DH>
@@ -152,18 +175,18 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
-      mbar_init(&sh.kv_full[s], 4);
+      mbar_init(&sh.kv_full[s], (VALUE_THREADS + KEY_THREADS) / 32);
       mbar_init(&sh.kv_empty[s], 1);
     }
     mbar_init(&sh.s_full[0], 1);
     mbar_init(&sh.s_full[1], 1);
-    mbar_init(&sh.q_ready, 4);
-    mbar_init(&sh.p_ready, 4);
+    mbar_init(&sh.q_ready, ROW_THREADS / 32);
+    mbar_init(&sh.p_ready, ROW_THREADS / 32);
     mbar_init(&sh.o_full, 1);
-    sh.abort_flag = 0;
+    sh.abort_flag = sh.row_stop[0] = sh.row_stop[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 7) {
+  if (warp == ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(T::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -184,52 +207,59 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   const int chunks = (seen + BK - 1) / BK;
 
   bool ok = true;
-  if (warp < 4) {
+  if (warp < ROW_THREADS / 32) {
     // ============================================================================ row threads
-    const uint32_t lane_base = tmem_base + ((uint32_t)(warp * 32) << 16);
-    const int row = tile * BQ + (int)threadIdx.x, token = row / a.group, head = kvh * a.group + row % a.group;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ROW_REGISTERS));
+    constexpr int HALF = DH / 2;                   // channels of O (and of Q, to be stored) a thread
+    const uint32_t lane_base = tmem_base + ((uint32_t)(warp % 4 * 32) << 16);
+    const int in_tile = (int)threadIdx.x % BQ, half = (int)threadIdx.x / BQ;
+    const int token = (tile * BQ + in_tile) / a.group;
     const int last = token < span.count ? before + token : 0x7fffffff;
-    float row_scale;
     {
-      const float* qp = pdl_after(a.q) + b * a.q_sb + head * a.q_sh + token * a.q_st;
-      float peak = 0.f;
-      if (token < span.count) {
-#pragma unroll 8
-        for (int c = 0; c < DH; c += 4) {
-          const float4 x = pdl_ld(reinterpret_cast<const float4*>(qp + c));
-          peak = fmaxf(fmaxf(fmaxf(peak, fabsf(x.x)), fmaxf(fabsf(x.y), fabsf(x.z))), fabsf(x.w));
-        }
-      }
-      const float up = query_scale(peak, a.scale_log2, row_scale);
+      // the tile's queries, whole rows by a warp: scaled by a power of two, in halves, to shared memory (layout as of the keys)
+      constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
+      const int c = lane % LANES * 4;
+      float4 x[PASSES];
 #pragma unroll
-      for (int c0 = 0; c0 < DH; c0 += 16) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int c = 0; c < 16; c += 4) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (token < span.count) x = pdl_ld(reinterpret_cast<const float4*>(qp + c0 + c));
-          split_halves(x.x * up, x.y * up, hi[c / 2], lo[c / 2]);
-          split_halves(x.z * up, x.w * up, hi[c / 2 + 1], lo[c / 2 + 1]);
-        }
-        tmem_st8(lane_base + (uint32_t)(T::Q_HI + c0 / 2), hi);
-        tmem_st8(lane_base + (uint32_t)(T::Q_LO + c0 / 2), lo);
+      for (int i = 0; i < PASSES; i++) {
+        const int r = (warp * PASSES + i) * TOGETHER + lane / LANES, of_row = tile * BQ + r, at = of_row / a.group;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at < span.count)
+          x[i] = pdl_ld(reinterpret_cast<const float4*>(pdl_after(a.q) + b * a.q_sb + (kvh * a.group + of_row % a.group) * a.q_sh + at * a.q_st + c));
       }
-      tmem_stored();
-      before_sync();
+#pragma unroll
+      for (int i = 0; i < PASSES; i++) {
+        const int r = (warp * PASSES + i) * TOGETHER + lane / LANES;
+        float peak = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+        for (int w = 1; w < LANES; w <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, w));
+        float row_scale;
+        const float up = query_scale(peak, a.scale_log2, row_scale);
+        if (lane % LANES == 0) sh.row_scale[r] = row_scale;
+        uint2 hi, lo;
+        split_halves(x[i].x * up, x[i].y * up, hi.x, lo.x);
+        split_halves(x[i].z * up, x[i].w * up, hi.y, lo.y);
+        unsigned char* to = stages + T::Q_HI + c / 64 * T::Q_BLOCK + r * 128 + ((c % 64 / 8) ^ (r & 7)) * 16 + c % 8 * 2;
+        *reinterpret_cast<uint2*>(to) = hi;
+        *reinterpret_cast<uint2*>(to + (T::Q_LO - T::Q_HI)) = lo;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // (the tensor core reads what was stored)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_ready);
+      asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
     }
-    float o[DH], m = -INFINITY, big = -INFINITY, l = 0.f, keep = 0.f;
+    const float row_scale = sh.row_scale[in_tile];
+    float o[HALF], m = -INFINITY, big = -INFINITY, l = 0.f, keep = 0.f;
 #pragma unroll
-    for (int c = 0; c < DH; c++) o[c] = 0.f;
+    for (int c = 0; c < HALF; c++) o[c] = 0.f;
     const auto add_values = [&](int chunk) {       // O of a chunk, whose weights were relative to `big` of that time
-      if (!mbar_wait(&sh.o_full, (uint32_t)(chunk & 1), &sh, a.status, 82)) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh.o_full, (uint32_t)(chunk & 1), &sh, a.status, 82))) return false;
       after_sync();
 #pragma unroll
-      for (int c0 = 0; c0 < DH; c0 += 32) {
+      for (int c0 = 0; c0 < HALF; c0 += 32) {
         float oc[32];
-        tmem_ld16(lane_base + (uint32_t)(T::O + c0), oc);
-        tmem_ld16(lane_base + (uint32_t)(T::O + c0 + 16), oc + 16);
+        tmem_ld16(lane_base + (uint32_t)(T::O + half * HALF + c0), oc);
+        tmem_ld16(lane_base + (uint32_t)(T::O + half * HALF + c0 + 16), oc + 16);
         tmem_loaded();
 #pragma unroll
         for (int c = 0; c < 32; c++) o[c0 + c] = fmaf(o[c0 + c], keep, oc[c]);
@@ -239,228 +269,274 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     };
     for (int j = 0; j < chunks; j++) {
       const int st = j % STAGES;
-      ok = mbar_wait(&sh.kv_full[st], (uint32_t)(j / STAGES & 1), &sh, a.status, 80) &&
+      ok = ok && mbar_wait(&sh.kv_full[st], (uint32_t)(j / STAGES & 1), &sh, a.status, 80) &&
            mbar_wait(&sh.s_full[j & 1], (uint32_t)(j >> 1 & 1), &sh, a.status, 81);
-      if (!ok) break;
+      // (on expiry all row threads leave together, behind the barrier below)
+      if (!ok) sh.row_stop[j & 1] = 1;
+      __syncwarp();
       after_sync();
-      float s[BK];
-#pragma unroll
-      for (int c0 = 0; c0 < BK; c0 += 16) tmem_ld16(lane_base + (uint32_t)(T::S + (j & 1) * BK + c0), s + c0);
+      float s[32];
+      tmem_ld16(lane_base + (uint32_t)(T::S + (j & 1) * BK + half * 32), s);
+      tmem_ld16(lane_base + (uint32_t)(T::S + (j & 1) * BK + half * 32 + 16), s + 16);
       tmem_loaded();
-      float e[4], f[4], m_new = m, big_new = big;
-      const int there = sh.there[st];
-      const bool whole = (j + 1) * BK <= seen_by_all && there == 15;
+      const int there = sh.there[st] >> (half * 2), t0 = j * BK + half * 32;
+      const bool whole = (j + 1) * BK <= seen_by_all && sh.there[st] == 15;
+      float e[2], f[2], top_s = -INFINITY, top_big = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const float by = row_scale * sh.key_scale[st][g];
-        e[g] = sh.exponent[st][g];
-        f[g] = sh.fraction[st][g];
+      for (int g = 0; g < 2; g++) {
+        const float by = row_scale * sh.key_scale[st][half * 2 + g];
+        e[g] = sh.exponent[st][half * 2 + g];
+        f[g] = sh.fraction[st][half * 2 + g];
 #pragma unroll
         for (int c = g * 16; c < g * 16 + 16; c++) s[c] *= by;
-      }
-      if (!whole) {
+        if (!whole) {
 #pragma unroll
-        for (int c = 0; c < BK; c++)
-          if (j * BK + c > last || !(there >> (c / 16) & 1)) s[c] = -INFINITY;
-      }
+          for (int c = g * 16; c < g * 16 + 16; c++)
+            if (t0 + c > last || !(there >> g & 1)) s[c] = -INFINITY;
+        }
+        float top = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        float top = s[g * 16];
-#pragma unroll
-        for (int c = 1; c < 16; c++) top = fmaxf(top, s[g * 16 + c]);
-        m_new = fmaxf(m_new, top);
-        big_new = fmaxf(big_new, top + e[g]);
+        for (int c = g * 16; c < g * 16 + 16; c++) top = fmaxf(top, s[c]);
+        top_s = fmaxf(top_s, top);
+        top_big = fmaxf(top_big, top + e[g]);
       }
+      sh.tops[j & 1][half][in_tile] = make_float2(top_s, top_big);
+      asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
+      if (((volatile int*)sh.row_stop)[j & 1]) {
+        ok = false;
+        break;
+      }
+      const float2 other = sh.tops[j & 1][half ^ 1][in_tile];
+      const float m_new = fmaxf(m, fmaxf(top_s, other.x)), big_new = fmaxf(big, fmaxf(top_big, other.y));
       const float m_ref = finite_or_0(m_new), big_ref = finite_or_0(big_new);
       l *= exp2_of(m - m_ref);
       const float keep_new = exp2_of(big - big_ref);
       m = m_new;
       big = big_new;
-      uint32_t hi[BK / 2], lo[BK / 2];
+      const uint32_t to = lane_base + (uint32_t)(T::P + (j & 1) * BK + half * 16);   // (chunk j - 2's values are done: o_full)
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
+      for (int g = 0; g < 2; g++) {
         const float by = f[g] * exp2_of(fminf(m_ref + e[g] - big_ref + WEIGHT_BITS, 126.f));
         float sum = 0.f;
+        uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int c = g * 16; c < g * 16 + 16; c += 2) {
-          const float p0 = exp2_of(s[c] - m_ref), p1 = exp2_of(s[c + 1] - m_ref);
+        for (int c = 0; c < 16; c += 2) {
+          const float s0 = s[g * 16 + c], s1 = s[g * 16 + c + 1];
+          const float p0 = exp2_of(s0 - m_ref), p1 = exp2_of(s1 - m_ref);
           sum += p0 + p1;
           float w0 = p0 * by, w1 = p1 * by;
           if (!whole) {                            // (a scale that is no number is for the rows that see it)
-            w0 = s[c] == -INFINITY ? 0.f : w0;
-            w1 = s[c + 1] == -INFINITY ? 0.f : w1;
+            w0 = s0 == -INFINITY ? 0.f : w0;
+            w1 = s1 == -INFINITY ? 0.f : w1;
           }
           split_halves(w0, w1, hi[c / 2], lo[c / 2]);
         }
         l += sum;
+        tmem_st8(to + (uint32_t)(g * 8), hi);
+        tmem_st8(to + (uint32_t)(BK / 2 + g * 8), lo);
       }
-      if (j > 0) {
-        ok = add_values(j - 1);
-        if (!ok) break;
-      }
+      if (j > 0) ok = add_values(j - 1);
       keep = keep_new;
-#pragma unroll
-      for (int c = 0; c < BK / 2; c += 8) {
-        tmem_st8(lane_base + (uint32_t)(T::P_HI + c), hi + c);
-        tmem_st8(lane_base + (uint32_t)(T::P_LO + c), lo + c);
-      }
       tmem_stored();
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_ready);
     }
     if (ok && chunks > 0) ok = add_values(chunks - 1);
-    if (ok && row < a.tokens * a.group) {
-      const float by = l == 0.f || token >= span.count ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
-      const bool some = by != 0.f || token < span.count;     // (padding: 0, whatever the sums are)
-      float* y = a.y + b * a.y_sb + head * a.y_sh + token * a.y_st;
+    // the halves' sums
+    if (half) sh.sums[in_tile] = l;
+    asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
+    if (!half) {
+      l += sh.sums[in_tile];
+      sh.tops[0][0][in_tile].x = l;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
+    l = sh.tops[0][0][in_tile].x;
+    // The result through shared memory, so that rows are written whole: every product that reads it has completed.  (Not ok: it may
+    // have not, and nothing is written.)
+    const float by = l == 0.f ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
+    float* out = reinterpret_cast<float*>(stages);
+    if (ok && token < span.count) {
 #pragma unroll
-      for (int c = 0; c < DH; c += 4)
-        *reinterpret_cast<float4*>(y + c) = some ? make_float4(o[c] * by, o[c + 1] * by, o[c + 2] * by, o[c + 3] * by)
-                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < HALF; c += 4)
+        *reinterpret_cast<float4*>(out + in_tile * T::OUT_STRIDE + half * HALF + c) = make_float4(o[c] * by, o[c + 1] * by, o[c + 2] * by, o[c + 3] * by);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
+    constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
+#pragma unroll 4
+    for (int i = 0; i < PASSES; i++) {
+      const int r = (warp * PASSES + i) * TOGETHER + lane / LANES, of_row = tile * BQ + r, at = of_row / a.group, c = lane % LANES * 4;
+      if (!ok || of_row >= a.tokens * a.group) continue;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);                              // (padding)
+      if (at < span.count) x = *reinterpret_cast<const float4*>(out + r * T::OUT_STRIDE + c);
+      *reinterpret_cast<float4*>(a.y + b * a.y_sb + (kvh * a.group + of_row % a.group) * a.y_sh + at * a.y_st + c) = x;
     }
   } else {
-    // ============================================================================ keys and values
-    const int id = (int)threadIdx.x - 128;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
     const int32_t* table = a.page_table + (int64_t)b * a.table_pages;
     const int64_t block_bytes = (int64_t)DH << a.page_shift, side_bytes = block_bytes * a.kv_heads;
-    // keys: a thread takes half a head of one token (or all of it in two threads' stead); values: 8 tokens, 8 channels
-    const int key = id & 63, part = id >> 6, octet = id & 7, column = id >> 3;
-    constexpr int KW = DH / 8, VN = DH == 128 ? 8 : 4;               // words of a key half; channels of a value octet
-    const auto at = [&](int token) -> const int8_t* {                // a token's keys, or null
-      if (token >= seen) return nullptr;
-      const int page = cache_page(table, token >> a.page_shift, a.pages, a.status);
-      if (page < 0) return nullptr;
-      return a.codes + ((int64_t)page * 2 * a.kv_heads + kvh) * block_bytes + (token & ((1 << a.page_shift) - 1)) * DH;
+    const int8_t* mine = pdl_after(a.codes) + kvh * block_bytes;
+    // Lane g of a warp has the page of a chunk's group g (-1: not there).  A table entry is read two chunks before its codes are
+    // fetched, and looked at a chunk later: nothing waits for it.
+    const auto entry_of = [&](int j) {
+      const int t0 = j * BK + lane * 16;
+      return lane < 4 && t0 < seen ? pdl_ld(table + (t0 >> a.page_shift)) : -1;
     };
-    uint32_t kw[KW], vw[8][VN / 4];
-    const auto load = [&](int j) {
-      const int8_t* k = j < chunks ? at(j * BK + key) : nullptr;
-      const int8_t* v = j < chunks ? at(j * BK + octet * 8) : nullptr;
-#pragma unroll
-      for (int i = 0; i < KW; i += 4) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (k) x = pdl_ld(reinterpret_cast<const uint4*>(pdl_after(k) + part * (DH / 2) + i * 4));
-        kw[i] = x.x; kw[i + 1] = x.y; kw[i + 2] = x.z; kw[i + 3] = x.w;
-      }
-#pragma unroll
-      for (int r = 0; r < 8; r++)
-#pragma unroll
-        for (int i = 0; i < VN / 4; i++)
-          vw[r][i] = v ? pdl_ld(reinterpret_cast<const uint32_t*>(pdl_after(v) + side_bytes + r * DH + column * VN) + i) : 0u;
+    const auto page_of = [&](int entry, int j) {
+      if (entry >= 0 && entry < a.pages) return entry;
+      if (lane < 4 && j * BK + lane * 16 < seen) a.status[WDC_STATUS_CACHE] = 1;
+      return -1;
     };
-    const auto convert = [&](int j) {
-      const int st = j % STAGES;
-      if (!mbar_wait(&sh.kv_empty[st], (uint32_t)(j / STAGES & 1) ^ 1, &sh, a.status, 83)) return false;
-      unsigned char* stage = stages + st * T::STAGE;
-      // keys: row = token, 128 bytes of 64 channels, 16-byte pieces exchanged by the row's last three bits
-      uint32_t w[KW][2];
-#pragma unroll
-      for (int i = 0; i < KW; i++) {
-        const uint32_t u = kw[i] ^ 0x80808080u;
-        w[i][0] = two_codes<0x4140>(u);
-        w[i][1] = two_codes<0x4342>(u);
-      }
-#pragma unroll
-      for (int i = 0; i < KW; i += 2) {
-        const int channel = part * (DH / 2) + i * 4;                 // of the piece's eight
-        store16(stage + T::KEYS + channel / 64 * T::K_BLOCK + key * 128 + ((channel % 64 / 8) ^ (key & 7)) * 16, w[i][0], w[i][1],
-                w[i + 1][0], w[i + 1][1]);
-      }
-      // values: row = channel, 128 bytes of 64 tokens
-#pragma unroll
-      for (int i = 0; i < VN / 4; i++) {
-        uint32_t out[4][4];                                          // [channel][pair of tokens]
-#pragma unroll
-        for (int r = 0; r < 8; r += 2) {
-          const uint32_t x = vw[r][i] ^ 0x80808080u, y = vw[r + 1][i] ^ 0x80808080u;
-          const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
-          out[0][r / 2] = two_codes<0x4140>(lo);
-          out[1][r / 2] = two_codes<0x4342>(lo);
-          out[2][r / 2] = two_codes<0x4140>(hi);
-          out[3][r / 2] = two_codes<0x4342>(hi);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const int channel = column * VN + i * 4 + c;
-          store16(stage + T::VALUES + channel * 128 + (octet ^ (channel & 7)) * 16, out[c][0], out[c][1], out[c][2], out[c][3]);
-        }
-      }
-      if (id < 4) {
-        const int t0 = j * BK + id * 16;
-        const int page = t0 < seen ? cache_page(table, t0 >> a.page_shift, a.pages, a.status) : -1;
-        const float* scales = pdl_after(a.scales) + (int64_t)max(page, 0) * 2 * a.kv_heads + kvh;
-        float e, f;
-        exponent_of(page >= 0 ? pdl_ld(scales + a.kv_heads) : 0.f, e, f);
-        sh.key_scale[st][id] = page >= 0 ? pdl_ld(scales) : 0.f;
-        sh.exponent[st][id] = e;
-        sh.fraction[st][id] = f;
-        const unsigned there = __ballot_sync(15u, page >= 0);
-        if (id == 0) sh.there[st] = (int)there;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor core reads what was stored here
+    const auto codes_at = [&](int pages, int j, int in_chunk) -> const int8_t* {        // a token's keys, or null
+      const int page = __shfl_sync(0xffffffffu, pages, in_chunk / 16), token = j * BK + in_chunk;
+      return page < 0 ? nullptr : mine + (int64_t)page * 2 * side_bytes + (token & ((1 << a.page_shift) - 1)) * DH;
+    };
+    const auto stage_free = [&](int j) { return mbar_wait(&sh.kv_empty[j % STAGES], (uint32_t)(j / STAGES & 1) ^ 1, &sh, a.status, 83); };
+    const auto filled = [&](int st) {                // this warp's part of a stage
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // (the tensor core reads what was stored)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.kv_full[st]);
-      load(j + 1);
-      return true;
     };
-    load(0);
-    if (warp < 7) {
-      for (int j = 0; j < chunks && ok; j++) ok = convert(j);
-    } else {
+    const uint32_t flip = 0x80808080u;
+    if (warp < (ROW_THREADS + VALUE_THREADS) / 32) {
+      // ========================================================================== values: 8 tokens by 8 (or 4) channels a thread
+      // row = channel, 128 bytes of 64 tokens, 16-byte pieces exchanged by the row's last three bits
+      const int id = (int)threadIdx.x - ROW_THREADS, octet = id & 7, column = id >> 3;
+      constexpr int VN = DH / 16, WORDS = VN / 4;
+      uint32_t w[8][WORDS];
+      const auto load = [&](const int8_t* from) {
+#pragma unroll
+        for (int r = 0; r < 8; r++)
+#pragma unroll
+          for (int i = 0; i < WORDS; i++)
+            w[r][i] = from ? pdl_ld(reinterpret_cast<const uint32_t*>(from + side_bytes + r * DH + column * VN) + i) : 0u;
+      };
+      int pages = page_of(entry_of(0), 0), next_entry = entry_of(1);
+      load(codes_at(pages, 0, octet * 8));
+      for (int j = 0; j < chunks; j++) {
+        const int st = j % STAGES;
+        ok = stage_free(j);
+        if (!ok) break;
+        const int these = pages;
+        pages = page_of(next_entry, j + 1);
+        next_entry = entry_of(j + 2);
+        float key_scale = 0.f, value_scale = 0.f;
+        if (id < 4 && these >= 0) {
+          const float* scales = pdl_after(a.scales) + (int64_t)these * 2 * a.kv_heads + kvh;
+          key_scale = pdl_ld(scales);
+          value_scale = pdl_ld(scales + a.kv_heads);
+        }
+        unsigned char* to = stages + st * T::STAGE + T::VALUES;
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+          uint32_t out[4][4];                                                  // [channel][pair of tokens]
+#pragma unroll
+          for (int r = 0; r < 8; r += 2) {
+            const uint32_t x = w[r][i] ^ flip, y = w[r + 1][i] ^ flip;
+            const uint32_t lo = __byte_perm(x, y, 0x5140), hi = __byte_perm(x, y, 0x7362);
+            out[0][r / 2] = two_codes<0x4140>(lo);
+            out[1][r / 2] = two_codes<0x4342>(lo);
+            out[2][r / 2] = two_codes<0x4140>(hi);
+            out[3][r / 2] = two_codes<0x4342>(hi);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int channel = column * VN + i * 4 + c;
+            store16(to + channel * 128 + (octet ^ (channel & 7)) * 16, out[c][0], out[c][1], out[c][2], out[c][3]);
+          }
+        }
+        load(codes_at(pages, j + 1, octet * 8));
+        if (id < 4) {
+          exponent_of(value_scale, sh.exponent[st][id], sh.fraction[st][id]);
+          sh.key_scale[st][id] = key_scale;
+          const unsigned there = __ballot_sync(15u, these >= 0);
+          if (id == 0) sh.there[st] = (int)there;
+        }
+        filled(st);
+      }
+    } else if (warp < ISSUER) {
+      // ========================================================================== keys: pieces of 16 bytes `part` and `part` + 4 of a
+      // token (four threads read 64 bytes of a row), two or three tokens a thread.  row = token, 128 bytes of 64 channels
+      const int id = (int)threadIdx.x - ROW_THREADS - VALUE_THREADS, part = id & 3, key0 = id >> 2;
+      constexpr int EACH = 3, STEP = KEY_THREADS / 4, PIECES = DH / 64;
+      uint4 w[EACH][PIECES];
+      const auto load = [&](int n, int pages, int j) {
+        const int key = key0 + n * STEP;
+        const int8_t* from = codes_at(pages, j, key % BK);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++)
+          w[n][i] = from && key < BK ? pdl_ld(reinterpret_cast<const uint4*>(from) + i * 4 + part) : make_uint4(0, 0, 0, 0);
+      };
+      int pages = page_of(entry_of(0), 0), next_entry = entry_of(1);
+#pragma unroll
+      for (int n = 0; n < EACH; n++) load(n, pages, 0);
+      for (int j = 0; j < chunks; j++) {
+        const int st = j % STAGES;
+        ok = stage_free(j);
+        if (!ok) break;
+        pages = page_of(next_entry, j + 1);
+        next_entry = entry_of(j + 2);
+#pragma unroll
+        for (int n = 0; n < EACH; n++) {
+          const int key = key0 + n * STEP;
+          if (key < BK) {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {       // (codes 16 (4 i + part) .. : block i, pieces 2 part and 2 part + 1)
+              unsigned char* to = stages + st * T::STAGE + T::KEYS + i * T::K_BLOCK + key * 128;
+              const uint32_t x = w[n][i].x ^ flip, y = w[n][i].y ^ flip, z = w[n][i].z ^ flip, u = w[n][i].w ^ flip;
+              store16(to + ((2 * part) ^ (key & 7)) * 16, two_codes<0x4140>(x), two_codes<0x4342>(x), two_codes<0x4140>(y), two_codes<0x4342>(y));
+              store16(to + ((2 * part + 1) ^ (key & 7)) * 16, two_codes<0x4140>(z), two_codes<0x4342>(z), two_codes<0x4140>(u), two_codes<0x4342>(u));
+            }
+          }
+          load(n, pages, j + 1);
+        }
+        filled(st);
+      }
+    } else if (elect_one()) {
       // ========================================================================== the products
       const uint32_t idesc_s = make_idesc(BK), idesc_o = make_idesc(DH);
+      const uint32_t q_hi = (uint32_t)make_smem_desc(smem_u32(stages + T::Q_HI)), q_lo = (uint32_t)make_smem_desc(smem_u32(stages + T::Q_LO));
       const auto scores = [&](int j) {
         const int st = j % STAGES;
         if (!mbar_wait(&sh.kv_full[st], (uint32_t)(j / STAGES & 1), &sh, a.status, 84)) return false;
         after_sync();
         const uint64_t desc = make_smem_desc(smem_u32(stages + st * T::STAGE + T::KEYS));
         const uint32_t lo0 = (uint32_t)desc, top = (uint32_t)(desc >> 32), to = tmem_base + T::S + (uint32_t)(j & 1) * BK;
-        if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; half++)
+        for (int half = 0; half < 2; half++)
 #pragma unroll
-            for (int k = 0; k < DH / 16; k++)
-              umma_one(to, tmem_base + (half ? T::Q_HI : T::Q_LO) + (uint32_t)(k * 8),
-                       lo0 + (uint32_t)((k / 4 * T::K_BLOCK + k % 4 * 32) >> 4), top, idesc_s, half | k ? 1u : 0u);
-          umma_commit_one(&sh.s_full[j & 1]);
-        }
-        __syncwarp();
+          for (int k = 0; k < DH / 16; k++)
+            umma_shared(to, (half ? q_hi : q_lo) + (uint32_t)((k / 4 * T::Q_BLOCK + k % 4 * 32) >> 4),
+                        lo0 + (uint32_t)((k / 4 * T::K_BLOCK + k % 4 * 32) >> 4), top, idesc_s, half | k ? 1u : 0u);
+        umma_commit_one(&sh.s_full[j & 1]);
         return true;
       };
-      if (chunks > 0) ok = convert(0);
-      if (ok && chunks > 1) ok = convert(1);
-      ok = ok && mbar_wait(&sh.q_ready, 0, &sh, a.status, 85);
+      ok = mbar_wait(&sh.q_ready, 0, &sh, a.status, 85);
       after_sync();
       if (ok && chunks > 0) ok = scores(0);
-      if (ok && chunks > 1) ok = scores(1);
       for (int j = 0; j < chunks && ok; j++) {
-        if (j + 2 < chunks) ok = convert(j + 2);
+        // (the scores that were in the next buffer are weights already: p_ready of chunk j - 1)
+        if (j + 1 < chunks) ok = scores(j + 1);
         ok = ok && mbar_wait(&sh.p_ready, (uint32_t)(j & 1), &sh, a.status, 86);
         if (!ok) break;
         after_sync();
         const int st = j % STAGES;
         const uint64_t desc = make_smem_desc(smem_u32(stages + st * T::STAGE + T::VALUES));
         const uint32_t lo0 = (uint32_t)desc, top = (uint32_t)(desc >> 32);
-        if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; half++)
+        for (int half = 0; half < 2; half++)
 #pragma unroll
-            for (int k = 0; k < BK / 16; k++)
-              umma_one(tmem_base + T::O, tmem_base + (half ? T::P_HI : T::P_LO) + (uint32_t)(k * 8), lo0 + (uint32_t)(k * 2), top,
-                       idesc_o, half | k ? 1u : 0u);
-          umma_commit_one(&sh.kv_empty[st]);
-          umma_commit_one(&sh.o_full);
-        }
-        __syncwarp();
-        // (chunk j's scores are weights: their buffer is free)
-        if (j + 2 < chunks) ok = scores(j + 2);
+          for (int k = 0; k < BK / 16; k++)
+            umma_one(tmem_base + T::O, tmem_base + (uint32_t)(T::P + (j & 1) * BK + (half ? 0 : BK / 2) + k * 8), lo0 + (uint32_t)(k * 2), top,
+                     idesc_o, half | k ? 1u : 0u);
+        umma_commit_one(&sh.kv_empty[st]);
+        umma_commit_one(&sh.o_full);
       }
     }
   }
   before_sync();
   __syncthreads();
-  if (warp == 7) {
+  if (warp == ISSUER) {
     after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(T::COLS));
   }
