@@ -4,9 +4,10 @@
 //
 // One CTA owns 128 rows of one sequence and key head, row = new token * group + query head of the group, and walks the tokens that
 // they see in chunks of 64:
-//   S  = Q K_chunk^T     two tcgen05.mma.kind::f16 products, M = 128, N = 64, K = head size: low half, high half of Q, both operands
-//                        in shared memory
-//   P  = weights         by the row threads, in halves to TENSOR MEMORY, as the next A operand
+//   S  = Q K_chunk^T     two tcgen05.mma.kind::f16 products, M = 128, N = 64, K = head size: low half, high half.  Q is the A
+//                        operand in TENSOR MEMORY (from shared memory each chunk would read all of it again: 768 cycles of the
+//                        ports at 128 bytes), K_chunk the B operand in shared memory
+//   P  = weights         by the row threads, in halves to tensor memory, as the next A operand
 //   Oc = P V_chunk       two products, M = 128, N = head size, K = 64; V_chunk^T the B operand in shared memory
 //   O  = O * keep + Oc   in the row threads' registers, rounded to nearest
 // Warps 0-7 are row threads, two of a row (= TMEM lane): each has half of the chunk's scores and half of O's channels, and they
@@ -116,18 +117,6 @@ __device__ __forceinline__ void umma_one(uint32_t tmem_c, uint32_t tmem_a, uint3
       "r"(tmem_a), "r"(desc_lo), "r"(desc_top), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// The same with A in shared memory.
-__device__ __forceinline__ void umma_shared(uint32_t tmem_c, uint32_t a_lo, uint32_t b_lo, uint32_t desc_top, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%1, %3};\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_c),
-      "r"(a_lo), "r"(b_lo), "r"(desc_top), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 __device__ __forceinline__ void umma_commit_one(unsigned long long* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -158,11 +147,11 @@ template <int DH>
 struct Tile {
   static constexpr int K_BLOCK = BK * 128;                 // 64 tokens x 64 channels
   static constexpr int KEYS = 0, VALUES = DH / 64 * K_BLOCK, STAGE = 2 * VALUES;
-  static constexpr int Q_BLOCK = BQ * 128;                 // 128 rows x 64 channels; high halves, then low ones, behind the stages
-  static constexpr int Q_HI = STAGES * STAGE, Q_LO = Q_HI + DH / 64 * Q_BLOCK;
+  static constexpr int Q = STAGES * STAGE, Q_STRIDE = 4 * DH + 16;   // queries on their way: a row's high halves, then the low ones
   static constexpr int OUT_STRIDE = DH + 4;                // floats of a row of the result, over all of this at the end
-  static constexpr int SMEM = Q_LO + DH / 64 * Q_BLOCK + 1024;
-  static constexpr int S = 0, P = 2 * BK, O = 4 * BK, COLS = 512;   // tensor-memory columns; S and P of two chunks
+  static constexpr int SMEM = Q + BQ * Q_STRIDE + 1024;
+  // tensor-memory columns; S and P of two chunks
+  static constexpr int Q_HI = 0, Q_LO = DH / 2, S = DH, P = S + 2 * BK, O = P + 2 * BK, COLS = 512;
   static_assert(BQ * OUT_STRIDE * 4 <= SMEM - 1024, "the result's place");
 };
 
@@ -216,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     const int token = (tile * BQ + in_tile) / a.group;
     const int last = token < span.count ? before + token : 0x7fffffff;
     {
-      // the tile's queries, whole rows by a warp: scaled by a power of two, in halves, to shared memory (layout as of the keys)
+      // the tile's queries, whole rows by a warp: scaled by a power of two, in halves, through shared memory to tensor memory
       constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
       const int c = lane % LANES * 4;
       float4 x[PASSES];
@@ -239,14 +228,27 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         uint2 hi, lo;
         split_halves(x[i].x * up, x[i].y * up, hi.x, lo.x);
         split_halves(x[i].z * up, x[i].w * up, hi.y, lo.y);
-        unsigned char* to = stages + T::Q_HI + c / 64 * T::Q_BLOCK + r * 128 + ((c % 64 / 8) ^ (r & 7)) * 16 + c % 8 * 2;
+        unsigned char* to = stages + T::Q + r * T::Q_STRIDE + c * 2;
         *reinterpret_cast<uint2*>(to) = hi;
-        *reinterpret_cast<uint2*>(to + (T::Q_LO - T::Q_HI)) = lo;
+        *reinterpret_cast<uint2*>(to + 2 * DH) = lo;
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // (the tensor core reads what was stored)
+      asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
+      // (16 bytes are eight channels, four columns)
+      const unsigned char* from = stages + T::Q + in_tile * T::Q_STRIDE + half * DH;
+#pragma unroll
+      for (int i = 0; i < DH / 16; i += 2) {
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+          const uint4 x = *reinterpret_cast<const uint4*>(from + part * 2 * DH + i * 16);
+          const uint4 y = *reinterpret_cast<const uint4*>(from + part * 2 * DH + i * 16 + 16);
+          const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          tmem_st8(lane_base + (uint32_t)((part ? T::Q_LO : T::Q_HI) + half * (DH / 4) + i * 4), w);
+        }
+      }
+      tmem_stored();
+      before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_ready);
-      asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
     }
     const float row_scale = sh.row_scale[in_tile];
     float o[HALF], m = -INFINITY, big = -INFINITY, l = 0.f, keep = 0.f;
@@ -495,7 +497,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     } else if (elect_one()) {
       // ========================================================================== the products
       const uint32_t idesc_s = make_idesc(BK), idesc_o = make_idesc(DH);
-      const uint32_t q_hi = (uint32_t)make_smem_desc(smem_u32(stages + T::Q_HI)), q_lo = (uint32_t)make_smem_desc(smem_u32(stages + T::Q_LO));
       const auto scores = [&](int j) {
         const int st = j % STAGES;
         if (!mbar_wait(&sh.kv_full[st], (uint32_t)(j / STAGES & 1), &sh, a.status, 84)) return false;
@@ -506,8 +507,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         for (int half = 0; half < 2; half++)
 #pragma unroll
           for (int k = 0; k < DH / 16; k++)
-            umma_shared(to, (half ? q_hi : q_lo) + (uint32_t)((k / 4 * T::Q_BLOCK + k % 4 * 32) >> 4),
-                        lo0 + (uint32_t)((k / 4 * T::K_BLOCK + k % 4 * 32) >> 4), top, idesc_s, half | k ? 1u : 0u);
+            umma_one(to, tmem_base + (uint32_t)((half ? T::Q_HI : T::Q_LO) + k * 8), lo0 + (uint32_t)((k / 4 * T::K_BLOCK + k % 4 * 32) >> 4),
+                     top, idesc_s, half | k ? 1u : 0u);
         umma_commit_one(&sh.s_full[j & 1]);
         return true;
       };
