@@ -155,9 +155,31 @@ struct Tile {
   static_assert(BQ * OUT_STRIDE * 4 <= SMEM - 1024, "the result's place");
 };
 
+// The rows of a tile that a warp of the row threads reads or writes whole, and a lane's four channels of them.
+template <int DH>
+struct WholeRows {
+  static constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
+  int group, row, token, head, channel;
+  __device__ WholeRows(const CacheAttArgs& a, int tile, int warp, int lane) : group(a.group) {
+    row = warp * PASSES * TOGETHER + lane / LANES;
+    token = (tile * BQ + row) / group;
+    head = tile * BQ + row - token * group;
+    channel = lane % LANES * 4;
+  }
+  __device__ void next() {
+    row += TOGETHER;
+    head += TOGETHER;
+    while (head >= group) {
+      head -= group;
+      token++;
+    }
+  }
+};
+
 template <int DH>
 __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const CacheAttArgs a) {
   using T = Tile<DH>;
+  using Rows = WholeRows<DH>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Shared sh;
   unsigned char* stages = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -205,32 +227,35 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     const int token = (tile * BQ + in_tile) / a.group;
     const int last = token < span.count ? before + token : 0x7fffffff;
     {
-      // the tile's queries, whole rows by a warp: scaled by a power of two, in halves, through shared memory to tensor memory
-      constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
-      const int c = lane % LANES * 4;
-      float4 x[PASSES];
+      // The tile's queries, whole rows by a warp: scaled by a power of two, in halves, through shared memory to tensor memory.  (A
+      // loop that is short in code: what runs once waits for its instructions, about as long as they are.)
+      Rows rows(a, tile, warp, lane);
+#pragma unroll 1
+      for (int i = 0; i < Rows::PASSES; i += 4) {
+        float4 x[4];
+        int r[4];
 #pragma unroll
-      for (int i = 0; i < PASSES; i++) {
-        const int r = (warp * PASSES + i) * TOGETHER + lane / LANES, of_row = tile * BQ + r, at = of_row / a.group;
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < span.count)
-          x[i] = pdl_ld(reinterpret_cast<const float4*>(pdl_after(a.q) + b * a.q_sb + (kvh * a.group + of_row % a.group) * a.q_sh + at * a.q_st + c));
-      }
+        for (int k = 0; k < 4; k++, rows.next()) {
+          r[k] = rows.row;
+          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (rows.token < span.count)
+            x[k] = pdl_ld(reinterpret_cast<const float4*>(pdl_after(a.q) + b * a.q_sb + (kvh * a.group + rows.head) * a.q_sh + rows.token * a.q_st + rows.channel));
+        }
 #pragma unroll
-      for (int i = 0; i < PASSES; i++) {
-        const int r = (warp * PASSES + i) * TOGETHER + lane / LANES;
-        float peak = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+        for (int k = 0; k < 4; k++) {
+          float peak = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
 #pragma unroll
-        for (int w = 1; w < LANES; w <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, w));
-        float row_scale;
-        const float up = query_scale(peak, a.scale_log2, row_scale);
-        if (lane % LANES == 0) sh.row_scale[r] = row_scale;
-        uint2 hi, lo;
-        split_halves(x[i].x * up, x[i].y * up, hi.x, lo.x);
-        split_halves(x[i].z * up, x[i].w * up, hi.y, lo.y);
-        unsigned char* to = stages + T::Q + r * T::Q_STRIDE + c * 2;
-        *reinterpret_cast<uint2*>(to) = hi;
-        *reinterpret_cast<uint2*>(to + 2 * DH) = lo;
+          for (int w = 1; w < Rows::LANES; w <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, w));
+          float row_scale;
+          const float up = query_scale(peak, a.scale_log2, row_scale);
+          if (rows.channel == 0) sh.row_scale[r[k]] = row_scale;
+          uint2 hi, lo;
+          split_halves(x[k].x * up, x[k].y * up, hi.x, lo.x);
+          split_halves(x[k].z * up, x[k].w * up, hi.y, lo.y);
+          unsigned char* to = stages + T::Q + r[k] * T::Q_STRIDE + rows.channel * 2;
+          *reinterpret_cast<uint2*>(to) = hi;
+          *reinterpret_cast<uint2*>(to + 2 * DH) = lo;
+        }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
       // (16 bytes are eight channels, four columns)
@@ -364,14 +389,13 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         *reinterpret_cast<float4*>(out + in_tile * T::OUT_STRIDE + half * HALF + c) = make_float4(o[c] * by, o[c + 1] * by, o[c + 2] * by, o[c + 3] * by);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(ROW_THREADS) : "memory");
-    constexpr int LANES = DH / 4, TOGETHER = 32 / LANES, PASSES = BQ / (ROW_THREADS / 32) / TOGETHER;
-#pragma unroll 4
-    for (int i = 0; i < PASSES; i++) {
-      const int r = (warp * PASSES + i) * TOGETHER + lane / LANES, of_row = tile * BQ + r, at = of_row / a.group, c = lane % LANES * 4;
-      if (!ok || of_row >= a.tokens * a.group) continue;
+    Rows rows(a, tile, warp, lane);
+#pragma unroll 1
+    for (int i = 0; i < Rows::PASSES; i++, rows.next()) {
+      if (!ok || rows.token >= a.tokens) continue;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);                              // (padding)
-      if (at < span.count) x = *reinterpret_cast<const float4*>(out + r * T::OUT_STRIDE + c);
-      *reinterpret_cast<float4*>(a.y + b * a.y_sb + (kvh * a.group + of_row % a.group) * a.y_sh + at * a.y_st + c) = x;
+      if (rows.token < span.count) x = *reinterpret_cast<const float4*>(out + rows.row * T::OUT_STRIDE + rows.channel);
+      *reinterpret_cast<float4*>(a.y + b * a.y_sb + (kvh * a.group + rows.head) * a.y_sh + rows.token * a.y_st + rows.channel) = x;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGISTERS));
