@@ -56,13 +56,13 @@ __device__ __forceinline__ void exponent_of(float scale, float& e, float& f) {
 }
 
 __device__ __forceinline__ float finite_or_0(float x) { return x == -INFINITY ? 0.f : x; }   // a reference to subtract
-// The power of two that a row of queries is scaled by, 2^(QUERY_BITS - exponent of its largest), and what its scores are to be
-// scaled by for it.  No exponent below -100: smaller queries than that weigh nothing.
 __device__ __forceinline__ float power_of_2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+// What a row of queries is scaled by, 2^(QUERY_BITS - exponent of its largest) with the sign of `scale`, and what its scores are to be
+// scaled by for it, which is not negative.  No exponent below -100: smaller queries than that weigh nothing.
 __device__ __forceinline__ float query_scale(float peak, float scale, float& row_scale) {
   const int e = max((int)(__float_as_uint(peak) >> 23) - 127, -100);
-  row_scale = power_of_2(e - QUERY_BITS) * scale;
-  return power_of_2(QUERY_BITS - e);
+  row_scale = power_of_2(e - QUERY_BITS) * fabsf(scale);
+  return copysignf(power_of_2(QUERY_BITS - e), scale);
 }
 
 // For many new tokens (cache_attention_tc.cu); WDC_ERR_UNSUPPORTED where the other kernel is to run.

@@ -308,14 +308,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
       tmem_loaded();
       const int there = sh.there[st] >> (half * 2), t0 = j * BK + half * 32;
       const bool whole = (j + 1) * BK <= seen_by_all && sh.there[st] == 15;
-      float e[2], f[2], top_s = -INFINITY, top_big = -INFINITY;
+      float by[2], e[2], f[2], top_s = -INFINITY, top_big = -INFINITY;
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        const float by = row_scale * sh.key_scale[st][half * 2 + g];
+        by[g] = row_scale * sh.key_scale[st][half * 2 + g];                    // (not negative)
         e[g] = sh.exponent[st][half * 2 + g];
         f[g] = sh.fraction[st][half * 2 + g];
-#pragma unroll
-        for (int c = g * 16; c < g * 16 + 16; c++) s[c] *= by;
         if (!whole) {
 #pragma unroll
           for (int c = g * 16; c < g * 16 + 16; c++)
@@ -324,6 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         float top = -INFINITY;
 #pragma unroll
         for (int c = g * 16; c < g * 16 + 16; c++) top = fmaxf(top, s[c]);
+        top = top == -INFINITY ? top : top * by[g];
         top_s = fmaxf(top_s, top);
         top_big = fmaxf(top_big, top + e[g]);
       }
@@ -343,19 +342,19 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
       const uint32_t to = lane_base + (uint32_t)(T::P + (j & 1) * BK + half * 16);   // (chunk j - 2's values are done: o_full)
 #pragma unroll
       for (int g = 0; g < 2; g++) {
-        const float by = f[g] * exp2_of(fminf(m_ref + e[g] - big_ref + WEIGHT_BITS, 126.f));
+        const float weigh = f[g] * exp2_of(fminf(m_ref + e[g] - big_ref + WEIGHT_BITS, 126.f));
         float sum = 0.f;
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
           const float s0 = s[g * 16 + c], s1 = s[g * 16 + c + 1];
-          const float p0 = exp2_of(s0 - m_ref), p1 = exp2_of(s1 - m_ref);
-          sum += p0 + p1;
-          float w0 = p0 * by, w1 = p1 * by;
-          if (!whole) {                            // (a scale that is no number is for the rows that see it)
-            w0 = s0 == -INFINITY ? 0.f : w0;
-            w1 = s1 == -INFINITY ? 0.f : w1;
+          float p0 = exp2_of(fmaf(s0, by[g], -m_ref)), p1 = exp2_of(fmaf(s1, by[g], -m_ref));
+          float w0 = p0 * weigh, w1 = p1 * weigh;
+          if (!whole) {                            // (nothing of what the row does not see, not even a scale that is no number)
+            if (s0 == -INFINITY) p0 = w0 = 0.f;
+            if (s1 == -INFINITY) p1 = w1 = 0.f;
           }
+          sum += p0 + p1;
           split_halves(w0, w1, hi[c / 2], lo[c / 2]);
         }
         l += sum;
@@ -438,20 +437,24 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
             w[r][i] = from ? pdl_ld(reinterpret_cast<const uint32_t*>(from + side_bytes + r * DH + column * VN) + i) : 0u;
       };
       int pages = page_of(entry_of(0), 0), next_entry = entry_of(1);
+      float key_scale = 0.f, value_scale = 0.f;      // of group `id` of the chunk, for the first four threads
+      const auto load_scales = [&]() {
+        key_scale = value_scale = 0.f;
+        if (id < 4 && pages >= 0) {
+          const float* scales = pdl_after(a.scales) + (int64_t)pages * 2 * a.kv_heads + kvh;
+          key_scale = pdl_ld(scales);
+          value_scale = pdl_ld(scales + a.kv_heads);
+        }
+      };
+      load_scales();
       load(codes_at(pages, 0, octet * 8));
       for (int j = 0; j < chunks; j++) {
         const int st = j % STAGES;
         ok = stage_free(j);
         if (!ok) break;
-        const int these = pages;
+        const bool there_now = pages >= 0;
         pages = page_of(next_entry, j + 1);
         next_entry = entry_of(j + 2);
-        float key_scale = 0.f, value_scale = 0.f;
-        if (id < 4 && these >= 0) {
-          const float* scales = pdl_after(a.scales) + (int64_t)these * 2 * a.kv_heads + kvh;
-          key_scale = pdl_ld(scales);
-          value_scale = pdl_ld(scales + a.kv_heads);
-        }
         unsigned char* to = stages + st * T::STAGE + T::VALUES;
 #pragma unroll
         for (int i = 0; i < WORDS; i++) {
@@ -475,9 +478,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         if (id < 4) {
           exponent_of(value_scale, sh.exponent[st][id], sh.fraction[st][id]);
           sh.key_scale[st][id] = key_scale;
-          const unsigned there = __ballot_sync(15u, these >= 0);
+          const unsigned there = __ballot_sync(15u, there_now);
           if (id == 0) sh.there[st] = (int)there;
         }
+        load_scales();
         filled(st);
       }
     } else if (warp < ISSUER) {
