@@ -602,35 +602,36 @@ class WebDNNCudaContext:
         for each row (without: logprob is None); ``top`` up to 32 best alternatives, ties by the lower index (0: the last two
         are None).  Results have the leading dims of ``logits``; they are written to ``out`` where that is given, in which an
         entry of None leaves that result out."""
-        self.asserts_cuda_tensor(logits)
-        if logits.ndim < 1 or logits.data_type != "float32" or logits.layout != "nchw":
-            raise TypeError("token_logprobs: logits are float32 rows")
+        for t, kind in ((logits, "float32"), (tokens, "int32")):
+            if t is not None:
+                if t.__class__ is not CudaTensor or t.context is not self:
+                    self.asserts_cuda_tensor(t)
+                if t.data_type != kind or t.layout != "nchw":
+                    raise TypeError("token_logprobs: logits are float32 rows, tokens int32")
+        if logits.ndim < 1:
+            raise ValueError("token_logprobs: logits have rows")
         width = logits.dims[-1]
-        lead, vocab = logits.dims[:-1], width if vocab is None else int(vocab)
+        vocab = width if vocab is None else vocab
         rows = logits.length // width if width else 0
         if not 0 < vocab <= width:
             raise ValueError(f"token_logprobs: vocab {vocab} of rows of {width}")
         if not 0 <= top <= min(32, vocab):
             raise ValueError(f"token_logprobs: top {top} is not 0 .. {min(32, vocab)}")
-        if tokens is not None:
-            self.asserts_cuda_tensor(tokens)
-            if tokens.data_type != "int32" or tokens.length != rows:
-                raise TypeError(f"token_logprobs: tokens are one int32 for each of {rows} rows")
+        if tokens is not None and tokens.length != rows:
+            raise ValueError(f"token_logprobs: tokens are one for each of {rows} rows")
         if out is None:
+            lead = logits.dims[:-1]
             out = (self.empty_tensor(lead) if tokens is not None else None, self.empty_tensor(lead),
                    self.empty_tensor(lead + [top], "int32") if top else None, self.empty_tensor(lead + [top]) if top else None)
         else:
             if len(out) != 4 or (tokens is None and out[0] is not None):
                 raise ValueError("token_logprobs: out is (logprob, entropy, top_ids, top_logprobs)")
             for t, n, kind in zip(out, (rows, rows, rows * top, rows * top), ("float32", "float32", "int32", "float32")):
-                if t is not None:
-                    self.asserts_cuda_tensor(t)
-                    if t.length != n or t.data_type != kind:
-                        raise ValueError(f"token_logprobs: a result has {n} values of {kind}")
+                if t is not None and (t.__class__ is not CudaTensor or t.context is not self or t.length != n or t.data_type != kind):
+                    raise ValueError(f"token_logprobs: a result has {n} values of {kind}, in this context")
         if rows:
-            at = [c_void_p(t.ptr) if t is not None and t.length else None for t in out]
-            self._call("wdc_token_logprobs", byref(LogprobsDesc(rows, vocab, width, top)), c_void_p(logits.ptr),
-                       c_void_p(tokens.ptr) if tokens is not None else None, *at)
+            self._call("wdc_token_logprobs", byref(LogprobsDesc(rows, vocab, width, top)), logits.ptr,
+                       tokens.ptr if tokens is not None else None, *[t.ptr if t is not None and t.length else None for t in out])
         return tuple(out)
 
     def conv2d(self, desc: ConvDesc, x, w, scale, shift, residual, y) -> None:

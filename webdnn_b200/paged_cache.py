@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
-from ctypes import byref, c_void_p
+from ctypes import byref
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -48,8 +48,8 @@ class PagedCache:
         self.codes = codes if codes is not None else context.empty_tensor(shape, "int32")
         self.scales = scales if scales is not None else context.empty_tensor(shape[:4])
         self._layer_bytes, self._layer_scale_bytes = self.codes.length // self.layers * 4, self.scales.length // self.layers * 4
-        self._descs: Dict[tuple, ctypes.Structure] = {}      # of the shapes seen
-        self._pages_desc = CachePagesDesc(self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_size)
+        self._descs: Dict[tuple, tuple] = {}                 # of the shapes seen
+        self._pages_desc = byref(CachePagesDesc(self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_size))
         self.registered = False                              # by WebDNNCudaContext.add_cache
         self._sequences: Dict[int, List[int]] = {}           # pages of each sequence
         self._lengths: Dict[int, int] = {}
@@ -66,54 +66,62 @@ class PagedCache:
     # ---------------------------------------------------------------------------------- on the device
     MAX_SHAPES = 1024
 
-    def _desc(self, key, make):
-        d = self._descs.get(key)
-        if d is None:
-            if len(self._descs) >= self.MAX_SHAPES:
-                self._descs.clear()
-            d = self._descs[key] = make()
-        return d
+    def _keep(self, key, desc):
+        """The description of a call of these shapes, checked once and kept by its shapes alone."""
+        if len(self._descs) >= self.MAX_SHAPES:
+            self._descs.clear()
+        self._descs[key] = kept = (byref(desc), desc)
+        return kept
 
     def _at(self, layer: int):
         if not 0 <= layer < self.layers:
             raise ValueError(f"PagedCache: layer {layer} of {self.layers}")
-        return c_void_p(self.codes.ptr + layer * self._layer_bytes), c_void_p(self.scales.ptr + layer * self._layer_scale_bytes)
+        return self.codes.ptr + layer * self._layer_bytes, self.scales.ptr + layer * self._layer_scale_bytes
 
-    def _batch(self, who: str, rows: Sequence[CudaTensor], page_table: CudaTensor, lengths: CudaTensor,
-               counts: Optional[CudaTensor]):
+    def _operands(self, who: str, rows: Sequence[CudaTensor], page_table: CudaTensor, lengths: CudaTensor,
+                  counts: Optional[CudaTensor]) -> None:
+        """Tensors of this context, of the types and in the order of memory that a call takes."""
+        for tensors, kind in ((rows, "float32"), ((page_table, lengths) if counts is None else (page_table, lengths, counts), "int32")):
+            for t in tensors:
+                if t.__class__ is not CudaTensor or t.context is not self.context:
+                    self.context.asserts_cuda_tensor(t)
+                if t.data_type != kind or t.layout != "nchw":
+                    raise TypeError(f"{who}: operands are float32, page_table, lengths and counts int32, all row-major")
+
+    @staticmethod
+    def _batch(who: str, rows: Sequence[CudaTensor], page_table: CudaTensor, lengths: CudaTensor, counts: Optional[CudaTensor]):
         """(batch, tokens) of a call: of its [batch, tokens, width] tensors and the int32 ones beside them."""
         for t in rows:
-            self.context.asserts_cuda_tensor(t)
-            if t.ndim != 3 or t.data_type != "float32" or t.dims[:2] != rows[0].dims[:2]:
-                raise ValueError(f"{who}: operands are float32 [batch, tokens, width]")
+            if t.ndim != 3 or t.dims[:2] != rows[0].dims[:2]:
+                raise ValueError(f"{who}: operands are [batch, tokens, width]")
         batch = rows[0].dims[0]
-        for t, dims in ((page_table, None), (lengths, [batch]), (counts, [batch])):
-            if t is None:
-                continue
-            self.context.asserts_cuda_tensor(t)
-            if t.data_type != "int32" or (t.dims != dims if dims else t.ndim != 2 or t.dims[0] != batch):
-                raise ValueError(f"{who}: page_table is int32 [{batch}, pages], lengths and counts are int32 [{batch}]")
+        if page_table.ndim != 2 or page_table.dims[0] != batch or lengths.dims != [batch] or (
+                counts is not None and counts.dims != [batch]):
+            raise ValueError(f"{who}: page_table is [{batch}, pages], lengths and counts are [{batch}]")
         return batch, rows[0].dims[1]
 
     def append(self, layer: int, k: CudaTensor, v: CudaTensor, page_table: CudaTensor, lengths: CudaTensor,
                counts: Optional[CudaTensor] = None, k_column: int = 0, v_column: int = 0) -> None:
         """Writes new tokens to one layer (``wdc_cache_append``).  k, v: [batch, tokens, width], of which kv_heads *
         head_size columns from ``k_column`` / ``v_column`` on are the heads side by side; ``lengths`` counts the tokens of each
-        sequence with the new ones, ``counts`` the new ones (without: all are)."""
+        sequence with the new ones, ``counts`` the new ones (without: all are).  The same call again changes nothing."""
+        self._operands("PagedCache.append", (k, v), page_table, lengths, counts)
+        key = ("append", *map(tuple, (k.dims, v.dims, page_table.dims, lengths.dims)), counts is not None and tuple(counts.dims), k_column,
+               v_column)
+        kept = self._descs.get(key) or self._append_desc(key, k, v, page_table, lengths, counts, k_column, v_column)
+        if k.length and v.length:
+            self.context._call("wdc_cache_append", kept[0], k.ptr + 4 * k_column, v.ptr + 4 * v_column, *self._at(layer),
+                               page_table.ptr, lengths.ptr, counts.ptr if counts is not None else None)
+
+    def _append_desc(self, key, k, v, page_table, lengths, counts, k_column, v_column):
         batch, tokens = self._batch("PagedCache.append", (k, v), page_table, lengths, counts)
         width = self.kv_heads * self.head_size
         for t, c in ((k, k_column), (v, v_column)):
             if c < 0 or c % 4 or c + width > t.dims[2] or t.dims[2] % 4:
                 raise ValueError(f"PagedCache.append: {width} columns from {c} on, of {t.dims[2]} (multiples of 4)")
-        if not batch or not tokens:
-            return
         kw, vw, c = k.dims[2], v.dims[2], self.head_size
-        d = self._desc((batch, tokens, page_table.dims[1], kw, vw), lambda: CacheAppendDesc(
-            self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1], tokens * kw, c, kw,
-            tokens * vw, c, vw))
-        self.context._call("wdc_cache_append", byref(d), c_void_p(k.ptr + 4 * k_column), c_void_p(v.ptr + 4 * v_column),
-                           *self._at(layer), c_void_p(page_table.ptr), c_void_p(lengths.ptr),
-                           c_void_p(counts.ptr) if counts is not None else None)
+        return self._keep(key, CacheAppendDesc(self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1],
+                                               tokens * kw, c, kw, tokens * vw, c, vw))
 
     def attention(self, layer: int, q: CudaTensor, page_table: CudaTensor, lengths: CudaTensor,
                   counts: Optional[CudaTensor] = None, heads: Optional[int] = None, q_column: int = 0,
@@ -122,39 +130,42 @@ class PagedCache:
         ``append``.  q: [batch, tokens, width], of which ``heads`` * head_size columns from ``q_column`` on count (without
         ``heads``: all from there on); the result is [batch, tokens, heads * head_size], rows of padding 0.  ``scale``:
         1 / sqrt(head_size) unless given."""
+        self._operands("PagedCache.attention", (q,), page_table, lengths, counts)
+        key = (*map(tuple, (q.dims, page_table.dims, lengths.dims)), counts is not None and tuple(counts.dims), heads, q_column, scale)
+        kept = self._descs.get(key) or self._attention_desc(key, q, page_table, lengths, counts, heads, q_column, scale)
+        d = kept[1]
+        dims = [d.batch, d.tokens, d.heads * d.head_size]
+        if out is None:
+            out = self.context.empty_tensor(dims)
+        elif out.__class__ is not CudaTensor or out.context is not self.context or out.dims != dims or out.data_type != "float32":
+            raise ValueError(f"PagedCache.attention: the result is float32 {dims} of this context")
+        if out.length:
+            self.context._call("wdc_cache_attention", kept[0], q.ptr + 4 * q_column, *self._at(layer), page_table.ptr, lengths.ptr,
+                               counts.ptr if counts is not None else None, out.ptr)
+        return out
+
+    def _attention_desc(self, key, q, page_table, lengths, counts, heads, q_column, scale):
         batch, tokens = self._batch("PagedCache.attention", (q,), page_table, lengths, counts)
         c, width = self.head_size, q.dims[2]
         heads = (width - q_column) // c if heads is None else heads
         if heads < 1 or heads % self.kv_heads or q_column < 0 or q_column % 4 or q_column + heads * c > width or width % 4:
             raise ValueError(f"PagedCache.attention: {heads} heads of {c} from column {q_column} on, of {width}; "
                              f"{self.kv_heads} key heads")
-        if out is None:
-            out = self.context.empty_tensor([batch, tokens, heads * c])
-        else:
-            self.context.asserts_cuda_tensor(out)
-            if out.dims != [batch, tokens, heads * c] or out.data_type != "float32":
-                raise ValueError(f"PagedCache.attention: the result is float32 {[batch, tokens, heads * c]}")
-        if not out.length:
-            return out
         row = heads * c
-        scale = c ** -0.5 if scale is None else float(scale)
-        d = self._desc((batch, tokens, page_table.dims[1], width, heads, scale), lambda: CacheAttentionDesc(
-            self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1], heads, tokens * width, c, width,
-            tokens * row, c, row, scale))
-        self.context._call("wdc_cache_attention", byref(d), c_void_p(q.ptr + 4 * q_column), *self._at(layer),
-                           c_void_p(page_table.ptr), c_void_p(lengths.ptr),
-                           c_void_p(counts.ptr) if counts is not None else None, c_void_p(out.ptr))
-        return out
+        return self._keep(key, CacheAttentionDesc(self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1],
+                                                  heads, tokens * width, c, width, tokens * row, c, row,
+                                                  c ** -0.5 if scale is None else scale))
 
     def copy_pages(self, sources: Sequence[int], targets: Sequence[int]) -> None:
         """Page sources[i] to page targets[i], in every layer (``wdc_cache_copy_pages``)."""
-        pairs = np.array((sources, targets), np.int64)
-        if pairs.ndim != 2 or (pairs.size and not 0 <= pairs.min() <= pairs.max() < self.pages):
-            raise ValueError(f"PagedCache.copy_pages: as many sources as targets, pages of 0 .. {self.pages - 1}")
-        pairs = pairs.astype(np.int32)
-        n, at = pairs.shape[1], pairs.ctypes.data
-        self.context._call("wdc_cache_copy_pages", byref(self._pages_desc), c_void_p(self.codes.ptr),
-                           c_void_p(self.scales.ptr), n, c_void_p(at), c_void_p(at + 4 * n))
+        n = len(sources)
+        if n != len(targets):
+            raise ValueError("PagedCache.copy_pages: as many sources as targets")
+        if n and (min(min(sources), min(targets)) < 0 or max(max(sources), max(targets)) >= self.pages):
+            raise ValueError(f"PagedCache.copy_pages: pages are 0 .. {self.pages - 1}")
+        array = ctypes.c_int32 * n                       # (in range: nothing is cut off)
+        self.context._call("wdc_cache_copy_pages", self._pages_desc, self.codes.ptr, self.scales.ptr, n, array(*sources),
+                           array(*targets))
 
     # ---------------------------------------------------------------------------------- on the host
     @property
