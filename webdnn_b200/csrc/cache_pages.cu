@@ -7,7 +7,6 @@
 
 namespace {
 
-constexpr int APPEND_THREADS = 256;
 
 struct AppendArgs {
   const float *k, *v;
@@ -47,7 +46,7 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
 // Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.  The new numbers are read
 // once and wait in registers for their scale, HELD float4 a thread (a whole page).
-template <int HELD>
+template <int APPEND_THREADS, int HELD>
 __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
   pdl_wait();
   const int part = (int)(blockIdx.x % (unsigned)(2 * a.kv_heads));
@@ -59,16 +58,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Appe
   const int start = span.length - span.count, index = (start >> a.page_shift) + slot;
   const int first = index << a.page_shift;                       // the page's first token
   if (first >= span.length) return;
-  const int page = cache_page(a.page_table + (int64_t)b * a.table_pages, index, a.pages, a.status);
-  if (page < 0) return;
+  const int page = pdl_ld(a.page_table + (int64_t)b * a.table_pages + index);   // (looked at when the new numbers are on their way)
   const int lo = max(start, first), hi = min(span.length, first + (1 << a.page_shift));
   const float* x = is_v ? pdl_after(a.v) + b * a.v_sb + head * a.v_sh + (lo - start) * a.v_st
                         : pdl_after(a.k) + b * a.k_sb + head * a.k_sh + (lo - start) * a.k_st;
   const int64_t row = is_v ? a.v_st : a.k_st;
   const int n = (hi - lo) << a.quad_shift, quad = (1 << a.quad_shift) - 1;      // float4 of the new tokens
-  const int64_t block = ((int64_t)page * 2 + is_v) * a.kv_heads + head;
-  uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes) + (block << (a.page_shift + a.quad_shift));
-
   __shared__ uint32_t peaks[APPEND_THREADS / 32];
   uint32_t peak = 0;
   float4 f[HELD];
@@ -77,6 +72,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Appe
     const int i = threadIdx.x + j * APPEND_THREADS;
     f[j] = i < n ? pdl_ld(reinterpret_cast<const float4*>(x + (i >> a.quad_shift) * row) + (i & quad)) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  if (page < 0 || page >= a.pages) {
+    a.status[WDC_STATUS_CACHE] = 1;
+    return;
+  }
+  const int64_t block = ((int64_t)page * 2 + is_v) * a.kv_heads + head;
+  uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes) + (block << (a.page_shift + a.quad_shift));
   const float before = lo > first ? pdl_ld(a.scales + block) : 0.f;
 #pragma unroll
   for (int j = 0; j < HELD; j++)
@@ -172,11 +173,13 @@ extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d
   WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_cache_append: batch exceeds the grid");
   // float4 of a page's new tokens a thread: of all its tokens, or of as many as the call can bring
   const int64_t most = (d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * d->head_size / 4;
-  auto kernel = most <= APPEND_THREADS       ? cache_append_kernel<1>
-                : most <= 4 * APPEND_THREADS ? cache_append_kernel<4>
-                : most <= 8 * APPEND_THREADS ? cache_append_kernel<8> : cache_append_kernel<16>;
   DeviceGuard g(ctx->device);
-  wdc_launch_pdl(ctx, kernel, dim3((unsigned)ctas), dim3(APPEND_THREADS), 0, a);
+  const auto launch = [&](auto kernel, int threads) { wdc_launch_pdl(ctx, kernel, dim3((unsigned)ctas), dim3((unsigned)threads), 0, a); };
+  if (most <= 64) launch(cache_append_kernel<64, 1>, 64);
+  else if (most <= 256) launch(cache_append_kernel<128, 2>, 128);
+  else if (most <= 1024) launch(cache_append_kernel<256, 4>, 256);
+  else if (most <= 2048) launch(cache_append_kernel<256, 8>, 256);
+  else launch(cache_append_kernel<256, 16>, 256);
   return wdc_check_launch(ctx, "cache_append_kernel");
 }
 

@@ -6,7 +6,8 @@
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS, EACH = 4;      // float4 a thread and round
+constexpr int EACH = 4;                                        // float4 a thread and round
+constexpr int WARPS_MOST = 8, SM_WARPS = 24;                   // of a CTA; of an SM (80 registers a thread)
 constexpr int TOP_MOST = 32, PARTS_MOST = 8;
 constexpr int KEPT = 192;                                      // keys that a warp's list of candidates holds
 constexpr int PART_LEAST = 4096;                               // logits of a part, where a row is cut into several
@@ -36,29 +37,38 @@ __device__ __forceinline__ float exp_of(float x) {
   return y;
 }
 
-// s = sum e^(x - m), t = sum (x - m) e^(x - m).  A difference below -200, whose exponential is 0, counts as -200 in t: it may be
-// infinite, and infinity times 0 is NaN.  A NaN or +inf makes s NaN.
+// s + c = sum e^(x - m), t = sum (x - m) e^(x - m).  c has what the additions to s rounded off: a sum is often 1 and many terms too
+// small for it.  A difference below -200, whose exponential is 0, counts as -200 in t: it may be infinite, and infinity times 0 is
+// NaN.  A NaN or +inf makes s NaN.
 struct Sums {
-  float m, s, t;
+  float m, s, c, t;
 };
 __device__ __forceinline__ void raise_to(Sums& a, float m) {
   if (m > a.m) {
     const float d = a.m - m, f = exp_of(d);
     a.t = f * fmaf(a.s, fmaxf(d, -200.f), a.t);
     a.s *= f;
+    a.c *= f;
     a.m = m;
   }
+}
+__device__ __forceinline__ void add_to(Sums& a, float s, float c, float t) {
+  const float sum = a.s + s, of_s = sum - a.s;
+  a.c += c + ((a.s - (sum - of_s)) + (s - of_s));
+  a.s = sum;
+  a.t += t;
 }
 __device__ __forceinline__ void add(Sums& a, Sums b) {
   raise_to(a, b.m);
   raise_to(b, a.m);
-  a.s += b.s;
-  a.t += b.t;
+  add_to(a, b.s, b.c, b.t);
 }
-__device__ __forceinline__ void take(Sums& a, float x, float ref) {
-  const float d = x - ref, e = exp_of(d);
-  a.s += e;
-  a.t = fmaf(fmaxf(d, -200.f), e, a.t);
+// Four logits: their exponentials' sum, and that of their products.
+__device__ __forceinline__ float2 four_terms(float4 x, float ref) {
+  const float4 d = make_float4(x.x - ref, x.y - ref, x.z - ref, x.w - ref);
+  const float4 e = make_float4(exp_of(d.x), exp_of(d.y), exp_of(d.z), exp_of(d.w));
+  return make_float2((e.x + e.y) + (e.z + e.w), fmaf(fmaxf(d.x, -200.f), e.x, fmaxf(d.y, -200.f) * e.y) +
+                                                    fmaf(fmaxf(d.z, -200.f), e.z, fmaxf(d.w, -200.f) * e.w));
 }
 
 // Keys of a warp, one a lane: sorted, largest in lane 0; and the 32 largest of two sorted lists, `b` given backwards.
@@ -82,6 +92,7 @@ __device__ __forceinline__ uint64_t warp_joined(uint64_t a, uint64_t b_backwards
   return key;
 }
 
+template <int WARPS>
 struct Shared {
   uint64_t kept[WARPS][KEPT];          // a warp's candidates, in no order
   uint64_t lists[WARPS][32];
@@ -121,14 +132,17 @@ __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// One CTA per row, or a cluster of `parts` where rows are few, each on a range of the row.  A round is EACH float4 a thread.
+// One CTA per row, of as few warps as still fill the GPU with the rows there are (one where rows are many: then nothing waits for
+// another warp); where rows are fewer than that with eight warps, a cluster of `parts` CTAs, each on a range of the row.  A round is EACH
+// float4 a thread, and the next round's are on their way.
 //
 // Candidates for the best `top`: the floor is a key that `top` logits of the range are known to be above.  After the first round it
 // is just below the `top`-th largest of the threads' largest keys; from then on every warp keeps what is above it in a list of its
 // own, without a barrier.  A list that might overflow is cut to its `top` largest, which raises the floor for all.
-template <bool kTop, bool kCluster>
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobArgs a) {
-  __shared__ Shared sh;
+template <int WARPS, bool kTop, bool kCluster>
+__global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_kernel(const LogprobArgs a) {
+  constexpr int THREADS = 32 * WARPS;
+  __shared__ Shared<WARPS> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kCluster ? (int)(blockIdx.x % (unsigned)a.parts) : 0;
   const int64_t row = kCluster ? blockIdx.x / (unsigned)a.parts : blockIdx.x;
@@ -142,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
   const int end = kCluster ? (int)((int64_t)(rank + 1) * quads / a.parts) : quads;
   const float4* x4 = reinterpret_cast<const float4*>(x + before);
 
-  Sums sums = {-INFINITY, 0.f, 0.f};
+  Sums sums = {-INFINITY, 0.f, 0.f, 0.f};
   uint64_t floor_key = 0;
   uint64_t* kept = sh.kept[warp];
   int have = 0;                                    // candidates of this warp
@@ -152,31 +166,36 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
       const int i = lane < before ? lane : quads * 4 + lane;
       const float v = pdl_ld(x + i);
       raise_to(sums, v);
-      take(sums, v, sums.m == -INFINITY ? 0.f : sums.m);
+      const float2 terms = four_terms(make_float4(v, -INFINITY, -INFINITY, -INFINITY), sums.m == -INFINITY ? 0.f : sums.m);
+      add_to(sums, terms.x, 0.f, terms.y);
       if (kTop) kept[lane] = order_key(v, i);
     }
     have = singles;
   }
-  for (int base = begin; base < end; base += THREADS * EACH) {
-    float4 f[EACH];
+  float4 ahead[EACH];                              // of the next round
+  const auto load = [&](int base) {
 #pragma unroll
     for (int j = 0; j < EACH; j++) {
       const int at = base + j * THREADS + (int)threadIdx.x;
-      f[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      ahead[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
+  };
+  load(begin);
+  for (int base = begin; base < end; base += THREADS * EACH) {
+    float4 f[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; j++) f[j] = ahead[j];
+    load(base + THREADS * EACH);
     float peaks[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; j++) peaks[j] = fmaxf(fmaxf(f[j].x, f[j].y), fmaxf(f[j].z, f[j].w));
     const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
     raise_to(sums, peak);
     const float ref = sums.m == -INFINITY ? 0.f : sums.m;
+    float2 terms[EACH];
 #pragma unroll
-    for (int j = 0; j < EACH; j++) {
-      take(sums, f[j].x, ref);
-      take(sums, f[j].y, ref);
-      take(sums, f[j].z, ref);
-      take(sums, f[j].w, ref);
-    }
+    for (int j = 0; j < EACH; j++) terms[j] = four_terms(f[j], ref);
+    add_to(sums, (terms[0].x + terms[1].x) + (terms[2].x + terms[3].x), 0.f, (terms[0].y + terms[1].y) + (terms[2].y + terms[3].y));
     if (kTop) {
       const int first = before + 4 * (base + (int)threadIdx.x);
       if (base == begin) {
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1)
     add(sums, {__shfl_xor_sync(0xffffffffu, sums.m, w), __shfl_xor_sync(0xffffffffu, sums.s, w),
-               __shfl_xor_sync(0xffffffffu, sums.t, w)});
+               __shfl_xor_sync(0xffffffffu, sums.c, w), __shfl_xor_sync(0xffffffffu, sums.t, w)});
   if (lane == 0) sh.sums[warp] = sums;
   if (kTop) {
     sh.lists[warp][lane] = warp_best(kept, have);
@@ -248,9 +267,9 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
     if (warp == 0) {
       if (kTop)
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at(&sh.part_lists[rank][lane], 0)), "l"(sh.lists[0][lane]) : "memory");
-      if (lane < 3)
+      if (lane < 4)
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_at(&sh.part_sums[rank].m + lane, 0)),
-                     "f"(lane == 0 ? sums.m : lane == 1 ? sums.s : sums.t) : "memory");
+                     "f"(lane == 0 ? sums.m : lane == 1 ? sums.s : lane == 2 ? sums.c : sums.t) : "memory");
     }
     cluster_arrive();
     cluster_wait();
@@ -259,7 +278,8 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
     if (kTop) join_lists(sh.part_lists, a.parts);
   }
   const bool none = sums.m == -INFINITY;
-  const float log_s = none ? NAN : logf(sums.s);
+  // log(s + c): a sum just above 1 by its small part
+  const float above = (sums.s - 1.f) + sums.c, log_s = none ? NAN : above < 0.5f ? log1pf(above) : logf(sums.s + sums.c);
   if (threadIdx.x == 0) {
     if (a.logprob) {
       const int token = pdl_ld(a.tokens + row);
@@ -302,15 +322,15 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
   }
 }
 
-template <bool kTop>
+template <int WARPS, bool kCluster>
 cudaError_t launch(wdc_context* ctx, const LogprobArgs& a, int64_t rows) {
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * a.parts));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(32 * WARPS);
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
-  if (a.parts > 1) {
+  if (kCluster) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
     attr[cfg.numAttrs].val.clusterDim.x = (unsigned)a.parts;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
@@ -321,8 +341,8 @@ cudaError_t launch(wdc_context* ctx, const LogprobArgs& a, int64_t rows) {
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs++;
   }
-  return a.parts > 1 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kTop, true>, a)
-                     : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<kTop, false>, a);
+  return a.top ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, true, kCluster>, a)
+               : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, false, kCluster>, a);
 }
 
 }  // namespace
@@ -348,9 +368,15 @@ extern "C" int wdc_token_logprobs(wdc_context* ctx, const wdc_logprobs_desc* d, 
   DeviceGuard g(ctx->device);
   LogprobArgs a = {logits, tokens, logprob, entropy, top_logprobs, top_ids, d->row_stride, (int)d->vocab,
                    top_ids ? (int)d->top : 0, 1};
-  while (a.parts < PARTS_MOST && d->rows * a.parts < 2 * ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
+  int warps = 1;
+  while (warps < WARPS_MOST && d->rows * 2 * warps <= (int64_t)SM_WARPS * ctx->sm_count && d->vocab >= 2 * warps * 32 * EACH * 4) warps *= 2;
+  if (warps == WARPS_MOST)
+    while (a.parts < PARTS_MOST && d->rows * a.parts < 2 * ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
   WDC_REQUIRE(ctx, d->rows * a.parts < (1ll << 31), "wdc_token_logprobs: rows exceed the grid");
-  const cudaError_t e = a.top ? launch<true>(ctx, a, d->rows) : launch<false>(ctx, a, d->rows);
+  const cudaError_t e = a.parts > 1  ? launch<8, true>(ctx, a, d->rows)
+                        : warps == 8 ? launch<8, false>(ctx, a, d->rows)
+                        : warps == 4 ? launch<4, false>(ctx, a, d->rows)
+                        : warps == 2 ? launch<2, false>(ctx, a, d->rows) : launch<1, false>(ctx, a, d->rows);
   WDC_CUDA(ctx, e);
   return wdc_check_launch(ctx, "token_logprobs_kernel");
 }
