@@ -16,7 +16,7 @@ struct AppendArgs {
   int* status;
   int64_t pages, table_pages;
   int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
-  int tokens, slots, kv_heads, page_shift, quad_shift;   // 2^page_shift tokens a page, 2^quad_shift float4 a head
+  int tokens, kv_heads, page_shift, quad_shift;   // 2^page_shift tokens a page, 2^quad_shift float4 a head
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -49,9 +49,7 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
 template <int APPEND_THREADS, int HELD>
 __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
   pdl_wait();
-  const int part = (int)(blockIdx.x % (unsigned)(2 * a.kv_heads));
-  const int rest = (int)(blockIdx.x / (unsigned)(2 * a.kv_heads));
-  const int slot = rest % a.slots, b = rest / a.slots;
+  const int part = (int)blockIdx.x, slot = (int)blockIdx.y, b = (int)blockIdx.z;
   const int is_v = part >= a.kv_heads, head = part - is_v * a.kv_heads;
   const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
   if (span.count == 0) return;
@@ -165,16 +163,17 @@ extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d
               cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4),
               "wdc_cache_append: buffers are not aligned");
   AppendArgs a = {k, v, (int8_t*)codes, scales, page_table, lengths, counts, ctx->status_word, d->pages, d->table_pages,
-                  d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st, (int)d->tokens,
-                  (int)((d->tokens + d->page_tokens - 2) / d->page_tokens + 1), (int)d->kv_heads, 4, 3};
+                  d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st, (int)d->tokens, (int)d->kv_heads, 4, 3};
   while (1 << a.page_shift < d->page_tokens) a.page_shift++;
   while (4 << a.quad_shift < d->head_size) a.quad_shift++;
-  const int64_t ctas = d->batch * a.slots * 2 * d->kv_heads;
-  WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_cache_append: batch exceeds the grid");
+  const int64_t slots = (d->tokens + d->page_tokens - 2) / d->page_tokens + 1;   // pages that a sequence may touch
+  WDC_REQUIRE(ctx, slots <= 65535 && d->batch <= 65535, "wdc_cache_append: batch exceeds the grid");
   // float4 of a page's new tokens a thread: of all its tokens, or of as many as the call can bring
   const int64_t most = (d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * d->head_size / 4;
   DeviceGuard g(ctx->device);
-  const auto launch = [&](auto kernel, int threads) { wdc_launch_pdl(ctx, kernel, dim3((unsigned)ctas), dim3((unsigned)threads), 0, a); };
+  const auto launch = [&](auto kernel, int threads) {
+    wdc_launch_pdl(ctx, kernel, dim3((unsigned)(2 * d->kv_heads), (unsigned)slots, (unsigned)d->batch), dim3((unsigned)threads), 0, a);
+  };
   if (most <= 64) launch(cache_append_kernel<64, 1>, 64);
   else if (most <= 256) launch(cache_append_kernel<128, 2>, 128);
   else if (most <= 1024) launch(cache_append_kernel<256, 4>, 256);

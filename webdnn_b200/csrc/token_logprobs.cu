@@ -9,7 +9,11 @@ namespace {
 constexpr int EACH = 4;                                        // float4 a thread and round
 constexpr int WARPS_MOST = 8, SM_WARPS = 24;                   // of a CTA; of an SM (80 registers a thread)
 constexpr int TOP_MOST = 32, PARTS_MOST = 8;
-constexpr int KEPT = 192;                                      // keys that a warp's list of candidates holds
+// Which best are wanted: none, some, or many of a row of few rounds.  In the first round then most threads have candidates, and the
+// kernel looks at all of them at once (3 x 384 with 32: 5.8 against 8.4 us); its code is too long for the other kernel to have it as
+// well (3000 x 50001 with 1: 116 against 106).
+enum { NONE = 0, SOME = 1, MANY = 2 };
+constexpr int MANY_TOP = 9, MANY_ROUNDS = 2;
 constexpr int PART_LEAST = 4096;                               // logits of a part, where a row is cut into several
 
 struct LogprobArgs {
@@ -92,12 +96,13 @@ __device__ __forceinline__ uint64_t warp_joined(uint64_t a, uint64_t b_backwards
   return key;
 }
 
-template <int WARPS>
+template <int WARPS, int KEPT, bool kCluster>
 struct Shared {
   uint64_t kept[WARPS][KEPT];          // a warp's candidates, in no order
+  float4 looked_at[WARPS][2][EACH];    // a round of the two threads that a warp looks at
   uint64_t lists[WARPS][32];
-  uint64_t part_lists[PARTS_MOST][32]; // of the parts of a row, in the first CTA of its cluster
-  Sums part_sums[PARTS_MOST];
+  uint64_t part_lists[kCluster ? PARTS_MOST : 1][32];   // of the parts of a row, in the first CTA of its cluster
+  Sums part_sums[kCluster ? PARTS_MOST : 1];
   Sums sums[WARPS];
   uint64_t best[WARPS];
   unsigned long long floor_key;
@@ -139,10 +144,11 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Candidates for the best `top`: the floor is a key that `top` logits of the range are known to be above.  After the first round it
 // is just below the `top`-th largest of the threads' largest keys; from then on every warp keeps what is above it in a list of its
 // own, without a barrier.  A list that might overflow is cut to its `top` largest, which raises the floor for all.
-template <int WARPS, bool kTop, bool kCluster>
+template <int WARPS, int kTop, bool kCluster>
 __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_kernel(const LogprobArgs a) {
   constexpr int THREADS = 32 * WARPS;
-  __shared__ Shared<WARPS> sh;
+  constexpr int KEPT = kTop == MANY ? 192 : 128;   // keys that a warp's list of candidates holds
+  __shared__ Shared<WARPS, KEPT, kCluster> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = kCluster ? (int)(blockIdx.x % (unsigned)a.parts) : 0;
   const int64_t row = kCluster ? blockIdx.x / (unsigned)a.parts : blockIdx.x;
@@ -172,21 +178,21 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
     }
     have = singles;
   }
-  float4 ahead[EACH];                              // of the next round
-  const auto load = [&](int base) {
+  constexpr int ROUND = THREADS * EACH;
+  const auto load = [&](float4 (&f)[EACH], int base) {
+    if (base + ROUND <= end) {
 #pragma unroll
-    for (int j = 0; j < EACH; j++) {
-      const int at = base + j * THREADS + (int)threadIdx.x;
-      ahead[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      for (int j = 0; j < EACH; j++) f[j] = pdl_ld(x4 + base + j * THREADS + (int)threadIdx.x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < EACH; j++) {
+        const int at = base + j * THREADS + (int)threadIdx.x;
+        f[j] = at < end ? pdl_ld(x4 + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      }
     }
   };
-  load(begin);
-  for (int base = begin; base < end; base += THREADS * EACH) {
-    float4 f[EACH];
-#pragma unroll
-    for (int j = 0; j < EACH; j++) f[j] = ahead[j];
-    load(base + THREADS * EACH);
-    float peaks[EACH];
+  // adds a round to the sums; the largest of each float4
+  const auto sum_up = [&](const float4 (&f)[EACH], float (&peaks)[EACH]) {
 #pragma unroll
     for (int j = 0; j < EACH; j++) peaks[j] = fmaxf(fmaxf(f[j].x, f[j].y), fmaxf(f[j].z, f[j].w));
     const float peak = fmaxf(fmaxf(peaks[0], peaks[1]), fmaxf(peaks[2], peaks[3]));
@@ -196,55 +202,101 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
 #pragma unroll
     for (int j = 0; j < EACH; j++) terms[j] = four_terms(f[j], ref);
     add_to(sums, (terms[0].x + terms[1].x) + (terms[2].x + terms[3].x), 0.f, (terms[0].y + terms[1].y) + (terms[2].y + terms[3].y));
-    if (kTop) {
-      const int first = before + 4 * (base + (int)threadIdx.x);
-      if (base == begin) {
-        uint64_t mine = 0;
+    return peak;
+  };
+  // cuts the list to its `top` largest, where there are more
+  const auto cut = [&]() {
+    const uint64_t key = warp_best(kept, have), least = __shfl_sync(0xffffffffu, key, a.top - 1) - 1;
+    __syncwarp();
+    kept[lane] = key;
+    have = a.top;
+    if (least > floor_key) {
+      floor_key = least;
+      if (lane == 0) atomicMax(&sh.floor_key, least);
+    }
+    __syncwarp();
+  };
+  // keeps what a round has above the floor: the first one, of which many threads have some
+  const auto keep_first = [&](const float4 (&f)[EACH]) {
 #pragma unroll
-        for (int j = 0; j < EACH; j++) {
-          if (base + j * THREADS + (int)threadIdx.x >= end) break;
-          // the largest of the four, and the first of those
-          const int i = first + 4 * j * THREADS + (f[j].x == peaks[j] ? 0 : f[j].y == peaks[j] ? 1 : f[j].z == peaks[j] ? 2 : 3);
-          const uint64_t key = order_key(peaks[j], i);
-          mine = key > mine ? key : mine;
-        }
-        sh.lists[warp][lane] = warp_sorted(mine);
-        join_lists(sh.lists, WARPS);
-        floor_key = sh.lists[0][a.top - 1];
-        if (floor_key) floor_key--;                // (fewer than `top` threads have any)
-        __syncthreads();                           // (the lists are used again)
-      } else {
-        const uint64_t raised = *(volatile unsigned long long*)&sh.floor_key;
-        floor_key = raised > floor_key ? raised : floor_key;
+    for (int j = 0; j < EACH; j++) {
+      const int at = begin + j * THREADS + (int)threadIdx.x;
+      const float v[4] = {f[j].x, f[j].y, f[j].z, f[j].w};
+      if (!__any_sync(0xffffffffu, at < end)) break;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const uint64_t key = order_key(v[c], before + 4 * at + c);
+        const bool above = at < end && key > floor_key && v[c] == v[c];
+        const unsigned who = __ballot_sync(0xffffffffu, above);
+        if (above) kept[have + __popc(who & ((1u << lane) - 1))] = key;
+        have += __popc(who);
       }
-      const float floor_value = floor_key ? key_value(floor_key) : -INFINITY;
-      if (!__any_sync(0xffffffffu, peak >= floor_value)) continue;
+      if (have > KEPT - 128) cut();                // (64 or more)
+    }
+  };
+  // and the others
+  const auto keep = [&](const float4 (&f)[EACH], float peak, int base) {
+    const uint64_t raised = *(volatile unsigned long long*)&sh.floor_key;
+    floor_key = raised > floor_key ? raised : floor_key;
+    const float floor_value = floor_key ? key_value(floor_key) : -INFINITY;
+    // two threads at a time, their 16 logits by as many lanes each: there are few such threads after the first rounds
+    static_assert(EACH == 4, "16 lanes a thread");
+    unsigned who = __ballot_sync(0xffffffffu, peak >= floor_value);
+    while (who) {
+      const int first = __ffs((int)who) - 1;
+      who &= who - 1;
+      const int second = __ffs((int)who) - 1;      // (-1: there is no second)
+      who &= who - 1;
+      if (have > KEPT - 32) cut();
+      if (lane == first || lane == second) {
+#pragma unroll
+        for (int j = 0; j < EACH; j++) sh.looked_at[warp][lane == second][j] = f[j];
+      }
+      __syncwarp();
+      const int of = lane < 16 ? first : second, at = base + lane % 16 / 4 * THREADS + warp * 32 + of;
+      const float v = reinterpret_cast<const float*>(sh.looked_at[warp])[lane];
+      const uint64_t key = order_key(v, before + 4 * at + lane % 4);
+      const bool above = of >= 0 && at < end && key > floor_key && v == v;
+      const unsigned new_ones = __ballot_sync(0xffffffffu, above);
+      if (above) kept[have + __popc(new_ones & ((1u << lane) - 1))] = key;
+      have += __popc(new_ones);
+      __syncwarp();
+    }
+  };
+  // (two buffers in turn, so that nothing is moved from one to the other)
+  float4 even[EACH], odd[EACH];
+  float peaks[EACH], peak;
+  if (begin < end) {
+    load(even, begin);
+    load(odd, begin + ROUND);
+    peak = sum_up(even, peaks);
+    if (kTop) {
+      // the floor: below the `top`-th largest of the threads' largest keys
+      uint64_t mine = 0;
 #pragma unroll
       for (int j = 0; j < EACH; j++) {
-        const bool inside = base + j * THREADS + (int)threadIdx.x < end;
-        if (!__any_sync(0xffffffffu, inside && peaks[j] >= floor_value)) continue;
-        const int i = first + 4 * j * THREADS;
-        const float v[4] = {f[j].x, f[j].y, f[j].z, f[j].w};
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const uint64_t key = order_key(v[c], i + c);
-          const bool above = inside && key > floor_key && v[c] == v[c];
-          const unsigned who = __ballot_sync(0xffffffffu, above);
-          if (above) kept[have + __popc(who & ((1u << lane) - 1))] = key;
-          have += __popc(who);
-        }
-        if (have > KEPT - 128) {
-          const uint64_t key = warp_best(kept, have), least = __shfl_sync(0xffffffffu, key, a.top - 1) - 1;
-          __syncwarp();
-          kept[lane] = key;
-          have = a.top;                            // (there were more than that)
-          if (least > floor_key) {
-            floor_key = least;
-            if (lane == 0) atomicMax(&sh.floor_key, least);
-          }
-          __syncwarp();
-        }
+        const int at = begin + j * THREADS + (int)threadIdx.x;
+        if (at >= end) break;
+        // the largest of the four, and the first of those
+        const uint64_t key = order_key(peaks[j], before + 4 * at + (even[j].x == peaks[j] ? 0 : even[j].y == peaks[j] ? 1 : even[j].z == peaks[j] ? 2 : 3));
+        mine = key > mine ? key : mine;
       }
+      sh.lists[warp][lane] = warp_sorted(mine);
+      join_lists(sh.lists, WARPS);
+      floor_key = sh.lists[0][a.top - 1];
+      if (floor_key) floor_key--;                  // (fewer than `top` threads have any)
+      __syncthreads();                             // (the lists are used again)
+      if (kTop == MANY) keep_first(even);
+      else keep(even, peak, begin);
+    }
+    for (int base = begin + ROUND; base < end; base += 2 * ROUND) {
+      load(even, base + ROUND);
+      peak = sum_up(odd, peaks);
+      if (kTop) keep(odd, peak, base);
+      if (base + ROUND >= end) break;
+      load(odd, base + 2 * ROUND);
+      peak = sum_up(even, peaks);
+      if (kTop) keep(even, peak, base + ROUND);
     }
   }
 
@@ -341,8 +393,10 @@ cudaError_t launch(wdc_context* ctx, const LogprobArgs& a, int64_t rows) {
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs++;
   }
-  return a.top ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, true, kCluster>, a)
-               : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, false, kCluster>, a);
+  if (!a.top) return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, NONE, kCluster>, a);
+  if (a.top >= MANY_TOP && a.vocab <= MANY_ROUNDS * a.parts * WARPS * 32 * EACH * 4)
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, MANY, kCluster>, a);
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<WARPS, SOME, kCluster>, a);
 }
 
 }  // namespace
