@@ -325,6 +325,20 @@ def test_sharp_and_tiny_scores(cuda_context, tokens):
     cache.dispose()
 
 
+@pytest.mark.parametrize("tokens", [2, 130])
+@pytest.mark.parametrize("scale", [-0.4, 0.0])
+def test_scales_that_are_negative_or_zero(cuda_context, scale, tokens):
+    rng = np.random.default_rng(21)
+    cache = PagedCache(cuda_context, 1, 30, 20, 64, 32)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, [300, 140])
+    q = rng.standard_normal((2, tokens, 20, 64)).astype(f32)
+    got = run_attention(cuda_context, cache, q, table, [300, 140], [tokens] * 2, scale=scale)
+    want, tol = reference_attention(q, codes[0], scales[0], table, [300, 140], [tokens] * 2, 32, float(f32(scale)))
+    assert np.abs(got - want).max() <= tol
+    cache.dispose()
+
+
 def test_value_scales_that_differ_by_orders_of_magnitude(cuda_context):
     """The page with the large scale gets a small weight, so that both matter: errors are relative to what is in the sum."""
     rng = np.random.default_rng(9)

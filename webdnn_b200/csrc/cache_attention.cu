@@ -578,12 +578,14 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
   }
   const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = Layout<DH>::CTAS * ctx->sm_count;
   const int64_t tiles = ceil_div64(a.table_pages << a.page_shift, TILE);
-  // Measured, us with equal parts / shared out: 3 sequences of 12000 to 40001 tokens and 16 key heads (48 units, 142 tiles a CTA)
-  // 73.5 / 65.3; 48 of 1 to 4100 and 8 (384, 118) 48.0 / 51.3; 1 of 700 and 4 (4, 1) 6.0 / 7.0.
-  a.splits = (int)ceil_div64(slots, units);
+  // As many parts as make one wave of CTAs (two, where that would leave a third of it empty or more); shared out where a CTA has 32
+  // tiles and more.  Measured, us with equal parts / shared out: 3 sequences of 12000 to 40001 tokens and 16 key heads (48 units, 142
+  // tiles a CTA) 82.2 / 70.2; 16 of 1959 to 2979 and 16 (256, 57) 52.4 / 44.7; 48 of 1 to 4100 and 8 (384, 118) 49.9 / 52.8; 20 of 100 to
+  // 1500 and 8, two row tiles (320, 27) 17.0 / 20.2; 16 of 2243 to 11554 and 2, heads of 32 (32, 20) 13.5 / 16.3.
+  a.splits = (int)(2 * units <= slots ? slots / units : units < slots ? 2 : 1);
   if (a.splits > ceil_div64(tiles, WARPS)) a.splits = (int)ceil_div64(tiles, WARPS);
   if (a.splits < 1) a.splits = 1;
-  if (a.batch <= PLAN_MOST && 2 * units <= slots && units * tiles >= 16 * slots &&
+  if (a.batch <= PLAN_MOST && units < 2 * slots && units * tiles >= 32 * slots &&
       units * (tiles + BEGIN) < (1ll << 31) - slots * WARPS)
     a.splits = 0;
   const int64_t ctas = a.splits ? units * a.splits : slots, parts = a.splits == 1 ? 0 : a.splits ? ctas : 2 * ctas;
