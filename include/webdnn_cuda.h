@@ -357,7 +357,8 @@ typedef struct wdc_cache_append_desc {
 /* Writes the new tokens.  The scale of a page and head is max |x| / 127 over its tokens: where the page holds older tokens it
  * only grows, and their codes are then rounded again, rint(code * old scale / new scale).  A new code is rint(x / scale), ties
  * to even.  A page and head that is given an infinity or a NaN stands for NaN until its first token is written again.
- * No page may be that of two sequences of the call, other than pages that the call does not write. */
+ * No page may be that of two sequences of the call, other than pages that the call does not write.  batch is at most 65535 (else
+ * WDC_ERR_INVALID). */
 int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d, const float* k, const float* v, void* codes,
                      float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts);
 typedef struct wdc_cache_attention_desc {

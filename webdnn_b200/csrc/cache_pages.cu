@@ -45,7 +45,8 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
 
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
 // Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.  The new numbers are read
-// once and wait in registers for their scale, HELD float4 a thread (a whole page).
+// once and wait in registers for their scale, HELD float4 a thread (a whole page).  Bound: issue for prompts (9131 tokens of 8 heads
+// of 128: 23.4 us, 3.9 TB/s), three dependent loads for single tokens (64 x 1: 2.2 us).
 template <int APPEND_THREADS, int HELD>
 __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
   pdl_wait();
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Appe
 }
 
 // ------------------------------------------------------------------------------------------- copies
+// Bound: memory (150 pages of 24 layers, 944 MB read and written: 143.5 us, 6.6 TB/s); the launch for a few (1.7 us).
 constexpr int COPY_THREADS = 256, COPY_EACH = 4, COPY_PIECE = COPY_THREADS * COPY_EACH;   // uint4 a CTA
 constexpr int COPY_PAIRS = 480;            // that fit a launch's arguments (4 KB)
 
