@@ -267,6 +267,29 @@ def test_attention_of_prompts(cuda_context, size, c, heads, kv_heads, lengths, c
     cache.dispose()
 
 
+@pytest.mark.parametrize("batch,c,group", [(50, 64, 2), (8, 128, 7), (5, 64, 12), (70, 64, 1)])
+def test_prompts_of_many_uneven_sequences(cuda_context, batch, c, group):
+    """More tiles than SMs, of sequences whose order says nothing about their lengths; some are empty, some have nothing new."""
+    rng = np.random.default_rng(batch)
+    ctx, size, kv_heads = cuda_context, 32, 4
+    lengths = [int(n) for n in rng.integers(1, 260, batch)]
+    counts = [int(min(n, m)) for n, m in zip(lengths, rng.integers(0, 151, batch))]
+    lengths[2] = counts[2] = counts[1] = 0
+    lengths[batch - 2], counts[batch - 2] = 1100, 150
+    cache = PagedCache(ctx, 1, sum(-(-n // size) for n in lengths) + 1, kv_heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, lengths)
+    q = rng.standard_normal((batch, 150, group * kv_heads, c)).astype(f32)
+    before = ctx.stats()["tensor_core_launches"]
+    got = run_attention(ctx, cache, q, table, lengths, counts)
+    assert ctx.stats()["tensor_core_launches"] == before + 1
+    want, tol = reference_attention(q, codes[0], scales[0], table, lengths, counts, size, c ** -0.5)
+    assert np.abs(got - want).max() <= tol
+    for b, n in enumerate(counts):
+        assert not got[b, n:].any()
+    cache.dispose()
+
+
 def test_prompts_with_sharp_scores_missing_pages_and_scales_that_are_no_numbers(cuda_context):
     rng = np.random.default_rng(20)
     ctx, size, c, heads = cuda_context, 16, 64, 20
