@@ -29,10 +29,10 @@ namespace {
 // less: it starts HEADROOM above what the first tile has, and rises only when a term would pass it, so that O is rarely scaled
 // again.  A tile's tokens of one page are a group: 32 of them, or 16 where pages hold no more (GROUPS).
 //
-// Bound: instruction issue, about 770 instructions for a tile of heads of 128 (8 KB): 160 and 230 of them widen keys and values and
-// multiply, the rest are scores, weights, copies.  12 warps an SM reach half of the issue slots.  Measured: 48 sequences of 1 to 4100
-// tokens, 32 query and 8 key heads of 128, 52.8 us (3.9 TB/s); 3 of 12000 to 40001, 16 heads, 70.2 us (4.6 TB/s); one of 700, 16 and 4
-// heads of 64, 6.3 us.
+// Bound: 370 cycles of an SM a tile of heads of 128 (8 KB; 6.1 TB/s over all), of which issue takes 200 (about 770 instructions: 160 and
+// 230 of them widen keys and values and multiply, the rest are scores, weights, copies) and the ALUs, shared memory and tensor core half
+// each; 16 warps an SM need as long.  Around that, beginnings and ends of units.  Measured: 48 sequences of 1 to 4100 tokens, 32 query and
+// 8 key heads of 128, 52.8 us (3.9 TB/s); 3 of 12000 to 40001, 16 heads, 70.2 us (4.6 TB/s); one of 700, 16 and 4 heads of 64, 6.3 us.
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, ROWS = 8;
 constexpr int PLAN_MOST = 512;             // sequences whose tiles are shared out
 constexpr int BEGIN = 8;

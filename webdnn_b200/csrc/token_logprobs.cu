@@ -142,7 +142,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // float4 a thread, and the next round's are on their way.
 //
 // Bound: memory where rows are many (3000 x 50001: 104.7 us, 5.7 TB/s, 87% of a copy's rate); launch, first round and joins where
-// they are few (1 x 32000: 7.0 us, 36 x 100003: 13.2 us).
+// they are few (1 x 32000: 6.7 us, 36 x 100003: 12.7 us).
 //
 // Candidates for the best `top`: the floor is a key that `top` logits of the range are known to be above.  After the first round it
 // is just below the `top`-th largest of the threads' largest keys; from then on every warp keeps what is above it in a list of its
@@ -164,6 +164,14 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
   const int begin = kCluster ? (int)((int64_t)rank * quads / a.parts) : 0;
   const int end = kCluster ? (int)((int64_t)(rank + 1) * quads / a.parts) : quads;
   const float4* x4 = reinterpret_cast<const float4*>(x + before);
+
+  // the given token's logit, asked for early and behind the first round's: two loads that nothing waits for until the end
+  const bool asks = a.logprob && rank == 0 && warp == 0;
+  const int token = asks ? pdl_ld(a.tokens + row) : -1;
+  float chosen = NAN;
+  const auto ask = [&]() {
+    if (token >= 0 && token < a.vocab) chosen = pdl_ld(x + token);
+  };
 
   Sums sums = {-INFINITY, 0.f, 0.f, 0.f};
   uint64_t floor_key = 0;
@@ -272,6 +280,7 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
   if (begin < end) {
     load(even, begin);
     load(odd, begin + ROUND);
+    ask();
     peak = sum_up(even, peaks);
     if (kTop) {
       // the floor: below the `top`-th largest of the threads' largest keys
@@ -301,6 +310,8 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
       peak = sum_up(even, peaks);
       if (kTop) keep(even, peak, base + ROUND);
     }
+  } else {
+    ask();
   }
 
 #pragma unroll
@@ -336,10 +347,7 @@ __global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_logprobs_k
   // log(s + c): a sum just above 1 by its small part
   const float above = (sums.s - 1.f) + sums.c, log_s = none ? NAN : above < 0.5f ? log1pf(above) : logf(sums.s + sums.c);
   if (threadIdx.x == 0) {
-    if (a.logprob) {
-      const int token = pdl_ld(a.tokens + row);
-      a.logprob[row] = token < 0 || token >= a.vocab ? NAN : pdl_ld(x + token) - sums.m - log_s;
-    }
+    if (a.logprob) a.logprob[row] = chosen - sums.m - log_s;
     if (a.entropy) a.entropy[row] = log_s - sums.t / sums.s;
   }
   if (!kTop) return;
