@@ -45,8 +45,8 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
 
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
 // Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.  The new numbers are read
-// once and wait in registers for their scale, HELD float4 a thread (a whole page).  Bound: issue for prompts (9131 tokens of 8 heads
-// of 128: 23.4 us, 3.9 TB/s), three dependent loads for single tokens (64 x 1: 2.2 us).
+// once and wait in registers for their scale, HELD float4 a thread (a whole page).  Bound: for prompts the length of a CTA's
+// dependent loads (9131 tokens of 8 heads of 128: 18.6 us, 4.9 TB/s), as for single tokens (64 x 1: 2.2 us).
 template <int APPEND_THREADS, int HELD>
 __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
   pdl_wait();
@@ -176,11 +176,13 @@ extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d
   const auto launch = [&](auto kernel, int threads) {
     wdc_launch_pdl(ctx, kernel, dim3((unsigned)(2 * d->kv_heads), (unsigned)slots, (unsigned)d->batch), dim3((unsigned)threads), 0, a);
   };
+  // (few threads with many loads each on their way, where a page has them: 1024 by 128 threads 16.7 us, by 256 22.0, by 64 18.1; 4096 by
+  // 512 19.9, by 256 21.4; 256 by 64 11.5, by 128 12.0)
   if (most <= 64) launch(cache_append_kernel<64, 1>, 64);
-  else if (most <= 256) launch(cache_append_kernel<128, 2>, 128);
-  else if (most <= 1024) launch(cache_append_kernel<256, 4>, 256);
+  else if (most <= 256) launch(cache_append_kernel<64, 4>, 64);
+  else if (most <= 1024) launch(cache_append_kernel<128, 8>, 128);
   else if (most <= 2048) launch(cache_append_kernel<256, 8>, 256);
-  else launch(cache_append_kernel<256, 16>, 256);
+  else launch(cache_append_kernel<512, 8>, 512);
   return wdc_check_launch(ctx, "cache_append_kernel");
 }
 
