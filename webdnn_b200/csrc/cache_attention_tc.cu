@@ -17,7 +17,7 @@
 // one's scores.
 //
 // Bound: the chain of a row's weights (scores out of tensor memory, the maximum with the other thread, exponentials, halves), about 2600
-// cycles a chunk, of which the tensor pipe needs 1000; 54% of the issue slots are used.  A tile's beginning and end are 10 us.  Measured:
+// cycles a chunk, of which the tensor pipe needs 1000; 51% of the issue slots are used.  A tile's beginning and end are 10 us.  Measured:
 // prompts of up to 900 tokens, three sequences of 450 to 1800, 16 query and 4 key heads of 128: 66 us (234 TFLOP/s).
 // Every mbarrier wait is bounded (2 s): on expiry the CTA records a status code, raises its abort flag, frees its TMEM and returns.
 #include <cuda_fp16.h>
