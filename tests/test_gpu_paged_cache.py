@@ -144,6 +144,12 @@ def test_append(cuda_context, size, c, heads, lengths, counts):
     cache.dispose()
 
 
+@pytest.mark.parametrize("size,c,heads,lengths,counts", [
+    (64, 128, 3, [130, 64, 190], [130, 1, 77]), (128, 64, 2, [128, 300], [127, 129]), (128, 32, 2, [255, 40, 129], [35, 40, 33])])
+def test_append_with_many_numbers_a_thread(cuda_context, size, c, heads, lengths, counts):
+    test_append(cuda_context, size, c, heads, lengths, counts)
+
+
 def test_append_token_by_token_keeps_the_scale_growing(cuda_context):
     """A page filled one token at a time, each larger than those before it: every step rounds the older codes again."""
     rng = np.random.default_rng(3)
