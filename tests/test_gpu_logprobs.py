@@ -160,3 +160,17 @@ def test_refusals(cuda_context):
             ctx._call("wdc_token_logprobs", byref(d), *args)
         assert e.value.status == 1
     ctx.sync()
+
+
+@pytest.mark.parametrize("vocab,top", [(1, 1), (5, 5), (32, 32), (40, 10), (5000, 32), (70001, 7)])
+def test_nan_at_the_first_logit(cuda_context, vocab, top):
+    """The first logit can be the one that is no number, alone or among others; every place of the order is somebody's."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((6, vocab)).astype(f32)
+    x[:5, 0] = np.nan
+    x[1] = np.nan
+    x[2, -1] = np.nan
+    x[3, 1:2] = np.inf
+    x[4, 1:] = -np.inf
+    x[5, 0] = -np.float32(np.nan)
+    check(cuda_context, x, rng.integers(0, vocab, 6), top)

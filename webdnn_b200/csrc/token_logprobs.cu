@@ -25,9 +25,10 @@ struct LogprobArgs {
   int vocab, top, parts;
 };
 
-// A key that orders by value, NaN above everything and -0 as 0, then by the lower index.  No key is 0.
+// A key that orders by value, NaN above everything and -0 as 0, then by the lower index.  No key is 0 or ~0, which stand below and
+// above all of them.
 __device__ __forceinline__ uint64_t order_key(float x, int index) {
-  uint32_t bits = x == x ? __float_as_uint(x + 0.f) : 0x7fffffffu;
+  uint32_t bits = x == x ? __float_as_uint(x + 0.f) : 0x7fc00000u;
   bits = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
   return (uint64_t)bits << 32 | (uint32_t)~index;
 }
