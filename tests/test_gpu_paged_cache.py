@@ -618,3 +618,42 @@ def test_refusals_of_the_library(cuda_context):
     for t in (x, i):
         t.dispose()
     cache.dispose()
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("size,c", [(16, 32), (64, 64), (32, 128)])
+def test_a_key_that_is_not_finite_makes_every_row_that_sees_its_page_nan(cuda_context, size, c, bad):
+    rng = np.random.default_rng(c)
+    heads, length = 8, 3 * size
+    cache = PagedCache(cuda_context, 1, 4, 2, c, size)
+    set_pool(cache, np.zeros(pool_codes(cache).shape, np.int8), np.zeros((1, 4, 2, 2), f32))
+    k, v = (rng.standard_normal((1, length, 2, c)).astype(f32) for _ in range(2))
+    k[0, size + 3, 1, 7] = bad
+    table = [[2, 0, 3]]
+    run_append(cuda_context, cache, k, v, table, [length], None)
+    q = rng.standard_normal((1, length, heads, c)).astype(f32)
+    y = run_attention(cuda_context, cache, q, table, [length], None)
+    assert np.isfinite(y[0, :, :4]).all() and np.isfinite(y[0, :size]).all()
+    assert np.isnan(y[0, size:, 4:]).all()
+    cache.dispose()
+
+
+@pytest.mark.parametrize("tokens", [5, 150])
+def test_key_scales_that_are_no_numbers(cuda_context, tokens):
+    """Whatever the codes beside such a scale are, and however few of them a row sees."""
+    rng = np.random.default_rng(23)
+    size, c, heads = 64, 64, 20
+    cache = PagedCache(cuda_context, 1, 4, heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    scales[0, 1, 0, ::2] = np.inf
+    scales[0, 2, 0, 1::4] = np.nan
+    set_pool(cache, codes, scales)
+    table, lengths = [[1, 0, 0], [2, 3, 3]], [tokens, tokens]
+    q = rng.standard_normal((2, tokens, heads, c)).astype(f32)
+    before = cuda_context.stats()["tensor_core_launches"]
+    y = run_attention(cuda_context, cache, q, table, lengths, None)
+    assert cuda_context.stats()["tensor_core_launches"] == before + (tokens == 150)
+    nan = np.zeros((2, heads), bool)
+    nan[0, ::2] = nan[1, 1::4] = True
+    assert (np.isnan(y) == nan[:, None, :, None]).all()
+    cache.dispose()

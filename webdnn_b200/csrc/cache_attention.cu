@@ -328,7 +328,7 @@ next_segment:
 #pragma unroll
     for (int group = 0; group < GROUPS; group++) {
       const float2 sc = *reinterpret_cast<const float2*>(tile_at + L::SCALES + group * 8);
-      key_scale[group] = sc.x;
+      key_scale[group] = key_scale_of(sc.x);
       value_scale[group] = sc.y;
     }
     const int there = *reinterpret_cast<const int*>(tile_at + L::THERE);

@@ -47,6 +47,8 @@ __device__ __forceinline__ float exp2_of(float x) {      // results below 2^-126
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A key scale; one that is no number or infinite makes every score NaN, whatever the codes beside it are.
+__device__ __forceinline__ float key_scale_of(float scale) { return fabsf(scale) < INFINITY ? scale : NAN; }
 // A value scale as 2^e * f, 1 <= f < 2 (0: e = -infinity; no number: f is NaN).
 __device__ __forceinline__ void exponent_of(float scale, float& e, float& f) {
   const bool small = scale < 1.2e-38f;                       // (below the normal range)

@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         load(codes_at(pages, j + 1, octet * 8));
         if (id < 4) {
           exponent_of(value_scale, sh.exponent[st][id], sh.fraction[st][id]);
-          sh.key_scale[st][id] = key_scale;
+          sh.key_scale[st][id] = key_scale_of(key_scale);
           const unsigned there = __ballot_sync(15u, there_now);
           if (id == 0) sh.there[st] = (int)there;
         }
