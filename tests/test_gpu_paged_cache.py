@@ -657,3 +657,30 @@ def test_key_scales_that_are_no_numbers(cuda_context, tokens):
     nan[0, ::2] = nan[1, 1::4] = True
     assert (np.isnan(y) == nan[:, None, :, None]).all()
     cache.dispose()
+
+
+@pytest.mark.parametrize("mean", [0.0, 5.0])
+@pytest.mark.parametrize("size,c,heads,kv_heads,tokens", [(16, 32, 6, 2, 1), (32, 64, 4, 4, 3), (64, 128, 16, 2, 1), (16, 128, 24, 3, 2),
+                                                          (32, 128, 48, 8, 70)])
+def test_small_codes_and_queries_of_one_sign(cuda_context, size, c, heads, kv_heads, tokens, mean):
+    """One key channel that is far larger than the others sets a page's scale, so that the codes of all others are small; and queries
+    whose channels do not cancel: a score's error is relative to sum |q k|, which is then far below 127 times the sum of the queries."""
+    rng = np.random.default_rng(size + c + heads)
+    lengths = [max(tokens, n) for n in (2, 3, 33, 5, 90, 2, 4)]
+    counts = [tokens] * len(lengths)
+    cache = PagedCache(cuda_context, 1, sum(-(-n // size) for n in lengths), kv_heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    codes[:, :, 0] = np.rint(rng.standard_normal(codes[:, :, 0].shape) * 3)
+    codes[:, :, 0, :, size - 1, 9] = 127
+    scales[:, :, 0] = 0.1
+    set_pool(cache, codes, scales)
+    table = tables(rng, cache, lengths)
+    q = (rng.standard_normal((len(lengths), tokens, heads, c)) + mean).astype(f32)
+    got = run_attention(cuda_context, cache, q, table, lengths, counts)
+    for b, n in enumerate(lengths):                  # each with the tolerance of its own scores
+        for h in range(heads):
+            of = slice(h * kv_heads // heads, h * kv_heads // heads + 1)
+            want, tol = reference_attention(q[b:b + 1, :, h:h + 1], codes[0][:, :, of], scales[0][:, :, of], table[b:b + 1], [n], [tokens],
+                                            size, c ** -0.5)
+            assert np.abs(got[b:b + 1, :, h:h + 1] - want).max() <= tol
+    cache.dispose()

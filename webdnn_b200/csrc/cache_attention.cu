@@ -21,6 +21,9 @@ namespace {
 // Both products run on mma.m16n8k16 with float16 operands and 32-bit sums.  A code (-127 .. 127) is exact in float16; a
 // query is split into a high and a low half, 22 bits together, and so is a weight.  The halves are the two halves of the
 // instruction's 16 rows: eight rows with both halves are one instruction, and their sums meet in one thread's registers.
+// (Codes + 128 would be exact as well, and two instructions a word less.  But the scores' sums would be of that size, and cancel
+// when the 128 is taken off: with codes of about 3 two scores' difference was up to 9 x 2^-21 of sum |q k| off, 26 x with queries of a
+// mean of 5, against 1 x.)
 //
 // Weights carry the value scale of their page.  With s the scores (base 2) and lv = log2(value scale) of a group of 16 tokens,
 //   m = max s,  l = sum 2^(s - m);      M = max (s + [lv]),  O = sum 2^(s + lv - M) code,      y = O 2^(M - m) / l,
@@ -29,10 +32,10 @@ namespace {
 // less: it starts HEADROOM above what the first tile has, and rises only when a term would pass it, so that O is rarely scaled
 // again.  A tile's tokens of one page are a group: 32 of them, or 16 where pages hold no more (GROUPS).
 //
-// Bound: 370 cycles of an SM a tile of heads of 128 (8 KB; 6.1 TB/s over all), of which issue takes 200 (about 770 instructions: 160 and
-// 230 of them widen keys and values and multiply, the rest are scores, weights, copies) and the ALUs, shared memory and tensor core half
+// Bound: 380 cycles of an SM a tile of heads of 128 (8 KB; 6.0 TB/s over all), of which issue takes 190 (about 760 instructions, of
+// which 225 and 230 are the widening of keys and values and the products with them) and the ALUs, shared memory and tensor core half
 // each; 16 warps an SM need as long.  Around that, beginnings and ends of units.  Measured: 48 sequences of 1 to 4100 tokens, 32 query and
-// 8 key heads of 128, 52.8 us (3.9 TB/s); 3 of 12000 to 40001, 16 heads, 70.2 us (4.6 TB/s); one of 700, 16 and 4 heads of 64, 6.3 us.
+// 8 key heads of 128, 52.7 us (3.9 TB/s); 3 of 12000 to 40001, 16 heads, 71.5 us (4.5 TB/s); one of 700, 16 and 4 heads of 64, 6.4 us.
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32, ROWS = 8;
 constexpr int PLAN_MOST = 512;             // sequences whose tiles are shared out
 constexpr int BEGIN = 8;
@@ -69,11 +72,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two bytes of a word of codes + 128 as float16.  A byte alone is a number below float16's normal range, byte * 2^-24, which the
-// product takes exactly: a key's score is then 2^24 of that sum, less 128 times the sum of the query's channels.  (Sums of weighted
-// values cancel, so that the 128 has to go before them: 0x6400 + byte is 1024 + byte.)
-template <int SELECT>
-__device__ __forceinline__ uint32_t two_bytes(uint32_t w) { return __byte_perm(w, 0, SELECT); }
 // Where the 16-byte chunk `c` of token `t` lies in a tile of keys or values: as in memory, chunks of a 128-byte line exchanged
 // so that the eight (16-byte loads), sixteen (8) or 32 (4) threads that load at a time meet different banks.
 template <int DH>
@@ -261,7 +259,7 @@ next_segment:
 
   // this row's queries, scaled by a power of two, in halves: step j of the sum covers channels at(j) .. + 3 of thread t
   uint32_t q[STEPS][4];
-  float row_scale, offset;
+  float row_scale;
   {
     const float* qp = pdl_after(a.q) + b * a.q_sb + head * a.q_sh + token * a.q_st;
     float4 x[STEPS];
@@ -273,21 +271,12 @@ next_segment:
       peak = fmaxf(fmaxf(fmaxf(peak, fabsf(x[j].x)), fmaxf(fabsf(x[j].y), fabsf(x[j].z))), fabsf(x[j].w));
     }
     peak = quad_max(peak);
-    const float up = query_scale(peak, a.scale_log2 * 16777216.f, row_scale);
-    float sum = 0.f;
+    const float up = query_scale(peak, a.scale_log2, row_scale);
 #pragma unroll
     for (int j = 0; j < STEPS; j++) {
       split_halves(x[j].x * up, x[j].y * up, q[j][0], q[j][1]);
       split_halves(x[j].z * up, x[j].w * up, q[j][2], q[j][3]);
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float2 both = __half22float2(*reinterpret_cast<const __half2*>(&q[j][k]));
-        sum += both.x + both.y;
-      }
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    offset = sum * 0x1p-17f;                       // 128 * 2^-24 of it
   }
 
   float o[DH / 8][4], m = -INFINITY, big = -INFINITY, l = 0.f;
@@ -342,11 +331,11 @@ next_segment:
         uint32_t w[KB / 4];
         load_words<KB>(tile_at + (DH == 32 ? key_at<DH>(n * 8 + g, t >> 1) + (t & 1) * 8 : key_at<DH>(n * 8 + g, j + t)), w);
 #pragma unroll
-        for (int k = 0; k < KB / 4; k++) mma(c, q[j + k], two_bytes<0x4140>(w[k]), two_bytes<0x4342>(w[k]));
+        for (int k = 0; k < KB / 4; k++) mma(c, q[j + k], two_codes<0x4140>(w[k]), two_codes<0x4342>(w[k]));
       }
       const float by = row_scale * key_scale[n / PER];
-      s[n][0] = (c[0] + c[2] - offset) * by;
-      s[n][1] = (c[1] + c[3] - offset) * by;
+      s[n][0] = (c[0] + c[2]) * by;
+      s[n][1] = (c[1] + c[3]) * by;
     }
     // what this row does not see
     const bool whole = (i + 1) * TILE <= seen_by_all && there == (1 << GROUPS) - 1;
