@@ -41,27 +41,35 @@ class Decoder:
     def step(self, sequences: Sequence[int], new_tokens: Sequence[Sequence[int]], wanted: Sequence[Tuple[int, int]],
              targets: Sequence[int]):
         """Appends new_tokens[i] to sequences[i]; (logprob of targets[j], entropy, top ids, top logprobs) behind the new token
-        wanted[j] = (which sequence of the call, which of its new tokens)."""
+        wanted[j] = (which sequence of the call, which of its new tokens).  A step that fails leaves the sequences as long as they were."""
         counts = [len(t) for t in new_tokens]
+        before = [self.cache.length(s) for s in sequences]
         self.cache.extend(dict(zip(sequences, counts)))
-        width = max(counts)
-        ids, places = np.zeros((len(sequences), width), np.int32), np.zeros((len(sequences), width), np.int32)
-        for i, (s, t) in enumerate(zip(sequences, new_tokens)):
-            ids[i, :len(t)] = t
-            places[i, :len(t)] = np.arange(self.cache.length(s) - len(t), self.cache.length(s))
-        rows = np.array([i * width + j for i, j in wanted], np.int32)
-        inputs = [CPUTensor.from_array(ids), CPUTensor.from_array(places),
-                  *self.cache.batch(sequences, counts, self.table_pages),
-                  CPUTensor.from_array(rows), CPUTensor.from_array(np.array(targets, np.int32))]
-        return tuple(t.numpy().copy() for t in self.runner.run(inputs))
+        try:
+            width = max(counts)
+            ids, places = np.zeros((len(sequences), width), np.int32), np.zeros((len(sequences), width), np.int32)
+            for i, (s, t) in enumerate(zip(sequences, new_tokens)):
+                ids[i, :len(t)] = t
+                places[i, :len(t)] = np.arange(self.cache.length(s) - len(t), self.cache.length(s))
+            rows = np.array([i * width + j for i, j in wanted], np.int32)
+            inputs = [CPUTensor.from_array(ids), CPUTensor.from_array(places),
+                      *self.cache.batch(sequences, counts, self.table_pages),
+                      CPUTensor.from_array(rows), CPUTensor.from_array(np.array(targets, np.int32))]
+            return tuple(t.numpy().copy() for t in self.runner.run(inputs))
+        except BaseException:
+            for s, length in zip(sequences, before):         # (what was written behind that is written again)
+                self.cache.truncate(s, length)
+            raise
 
     def score(self, texts: Sequence[Sequence[int]]) -> List[np.ndarray]:
         """Log probability of every token of each text but its first, given those before it."""
         sequences = [self.cache.add_sequence() for _ in texts]
         wanted = [(i, j) for i, t in enumerate(texts) for j in range(len(t) - 1)]
-        logprob = self.step(sequences, texts, wanted, [texts[i][j + 1] for i, j in wanted])[0]
-        for s in sequences:
-            self.cache.release(s)
+        try:
+            logprob = self.step(sequences, texts, wanted, [texts[i][j + 1] for i, j in wanted])[0]
+        finally:
+            for s in sequences:
+                self.cache.release(s)
         ends = np.cumsum([len(t) - 1 for t in texts])
         return np.split(logprob, ends[:-1])
 
@@ -69,27 +77,34 @@ class Decoder:
         """The ``beams`` continuations with the highest log probability that the search finds: (log probability, tokens), best
         first.  A beam that has several successors forks; one that has none gives its pages back."""
         first = self.cache.add_sequence()
-        *_, ids, logs = self.step([first], [prompt], [(0, len(prompt) - 1)], [0])
-        alive = [(0.0, [], first)]
-        for step in range(new_tokens):
-            found = sorted(((score + float(logs[i, j]), i, int(ids[i, j])) for i, (score, _, _) in enumerate(alive)
-                            for j in range(self.top)), reverse=True)[:beams]
-            heirs = {}
-            following = []
-            for score, i, token in found:
-                _, text, sequence = alive[i]
-                heirs[i] = heirs.get(i, 0) + 1
-                following.append((score, text + [token], sequence if heirs[i] == 1 else self.cache.fork(sequence)))
-            for i, (_, _, sequence) in enumerate(alive):
-                if i not in heirs:
-                    self.cache.release(sequence)
-            alive = following
-            if step + 1 < new_tokens:
-                n = len(alive)
-                *_, ids, logs = self.step([s for _, _, s in alive], [t[-1:] for _, t, _ in alive], [(i, 0) for i in range(n)],
-                                          [0] * n)
-        for _, _, sequence in alive:
-            self.cache.release(sequence)
+        held = {first}
+        try:
+            *_, ids, logs = self.step([first], [prompt], [(0, len(prompt) - 1)], [0])
+            alive = [(0.0, [], first)]
+            for step in range(new_tokens):
+                found = sorted(((score + float(logs[i, j]), i, int(ids[i, j])) for i, (score, _, _) in enumerate(alive)
+                                for j in range(self.top)), reverse=True)[:beams]
+                heirs = {}
+                following = []
+                for score, i, token in found:
+                    _, text, sequence = alive[i]
+                    heirs[i] = heirs.get(i, 0) + 1
+                    if heirs[i] > 1:
+                        sequence = self.cache.fork(sequence)
+                        held.add(sequence)
+                    following.append((score, text + [token], sequence))
+                for i, (_, _, sequence) in enumerate(alive):
+                    if i not in heirs:
+                        held.remove(sequence)
+                        self.cache.release(sequence)
+                alive = following
+                if step + 1 < new_tokens:
+                    n = len(alive)
+                    *_, ids, logs = self.step([s for _, _, s in alive], [t[-1:] for _, t, _ in alive], [(i, 0) for i in range(n)],
+                                              [0] * n)
+        finally:
+            for sequence in held:
+                self.cache.release(sequence)
         return [(score, text) for score, text, _ in alive]
 
 
