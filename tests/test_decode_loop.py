@@ -104,3 +104,20 @@ def test_a_search_that_fills_the_pool_gives_its_pages_back(decoder):
     assert nothing_is_held(decoder)
     found = decoder.beam_search([1] * 20, 6, beams=3)
     assert nothing_is_held(decoder) and len(found) == 3 and [len(t) for _, t in found] == [6] * 3
+
+
+def test_texts_beyond_the_places_are_refused(decoder):
+    """70 places in pages of 16: the table has room for 80 tokens."""
+    cache = decoder.cache
+    with pytest.raises(ValueError, match="places"):
+        decoder.score([[1] * 71])
+    with pytest.raises(ValueError, match="places"):
+        decoder.beam_search([1] * 68, 4, beams=1)    # (three tokens are appended)
+    assert nothing_is_held(decoder) and len(decoder.runner.calls) == 3
+    decoder.beam_search([1] * 68, 3, beams=1)
+    a = cache.add_sequence()
+    decoder.step([a], [[1] * 70], [(0, 0)], [0])
+    calls = len(decoder.runner.calls)
+    with pytest.raises(ValueError, match="places"):
+        decoder.step([a], [[1]], [(0, 0)], [0])
+    assert cache.length(a) == 70 and len(decoder.runner.calls) == calls

@@ -26,7 +26,7 @@ class Decoder:
         if context is None:
             context = WebDNNCudaContext()
             context.initialize()
-        self.context, self.top = context, top
+        self.context, self.top, self.positions = context, top, positions
         self.cache = PagedCache(context, layers, pages, kv_heads, d // heads, page_tokens)
         context.add_cache(name, self.cache)
         self.table_pages = -(-positions // page_tokens)      # the same for every call, so that calls repeat
@@ -44,6 +44,8 @@ class Decoder:
         wanted[j] = (which sequence of the call, which of its new tokens).  A step that fails leaves the sequences as long as they were."""
         counts = [len(t) for t in new_tokens]
         before = [self.cache.length(s) for s in sequences]
+        if max((n + c for n, c in zip(before, counts)), default=0) > self.positions:      # (Gather would take the last place)
+            raise ValueError(f"Decoder.step: there are places for {self.positions} tokens")
         self.cache.extend(dict(zip(sequences, counts)))
         try:
             width = max(counts)
