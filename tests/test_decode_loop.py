@@ -68,9 +68,12 @@ def test_a_step_that_fails_leaves_the_sequences_as_long_as_they_were(decoder):
         decoder.step([a, b], [[1] * 20, [2]], [(0, 0), (1, 0)], [0, 0])
     assert cache.length(a) == cache.length(b) == 20 and cache.used_pages <= 3
     assert cache.sequence_pages(a)[0] == cache.sequence_pages(b)[0] == pages[0]
+    rest = cache.add_sequence()
+    cache.extend({rest: 16 * cache.free_pages})
     with pytest.raises(MemoryError):
-        decoder.step([a], [[1] * 130], [(0, 0)], [0])
+        decoder.step([a], [[1] * 30], [(0, 0)], [0])
     assert cache.length(a) == 20
+    cache.release(rest)
     cache.release(a)
     cache.release(b)
     assert nothing_is_held(decoder)
