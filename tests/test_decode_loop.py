@@ -124,3 +124,15 @@ def test_texts_beyond_the_places_are_refused(decoder):
     with pytest.raises(ValueError, match="places"):
         decoder.step([a], [[1]], [(0, 0)], [0])
     assert cache.length(a) == 70 and len(decoder.runner.calls) == calls
+
+
+def test_texts_without_a_second_token_have_no_scores(decoder):
+    decoder.runner.run = lambda inputs, run=decoder.runner.run: [FakeTensor(np.arange(inputs[5].length))] + run(inputs)[1:]
+    got = decoder.score([[], [1, 2, 3], [4], [5, 6], []])
+    assert [s.tolist() for s in got] == [[], [0, 1], [], [2], []]
+    assert decoder.runner.calls[0][4].tolist() == [3, 2]          # (the graph sees the others only)
+    assert [s.tolist() for s in decoder.score([[7], []])] == [[], []] and decoder.score([]) == []
+    assert len(decoder.runner.calls) == 1 and nothing_is_held(decoder)
+    with pytest.raises(ValueError):
+        decoder.beam_search([], 3)
+    assert nothing_is_held(decoder)

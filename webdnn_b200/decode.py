@@ -65,19 +65,24 @@ class Decoder:
 
     def score(self, texts: Sequence[Sequence[int]]) -> List[np.ndarray]:
         """Log probability of every token of each text but its first, given those before it."""
-        sequences = [self.cache.add_sequence() for _ in texts]
-        wanted = [(i, j) for i, t in enumerate(texts) for j in range(len(t) - 1)]
+        scored = [t for t in texts if len(t) > 1]
+        if not scored:
+            return [np.zeros(0, np.float32) for _ in texts]
+        sequences = [self.cache.add_sequence() for _ in scored]
+        wanted = [(i, j) for i, t in enumerate(scored) for j in range(len(t) - 1)]
         try:
-            logprob = self.step(sequences, texts, wanted, [texts[i][j + 1] for i, j in wanted])[0]
+            logprob = self.step(sequences, scored, wanted, [scored[i][j + 1] for i, j in wanted])[0]
         finally:
             for s in sequences:
                 self.cache.release(s)
-        ends = np.cumsum([len(t) - 1 for t in texts])
+        ends = np.cumsum([max(len(t) - 1, 0) for t in texts])
         return np.split(logprob, ends[:-1])
 
     def beam_search(self, prompt: Sequence[int], new_tokens: int, beams: int = 4) -> List[Tuple[float, List[int]]]:
         """The ``beams`` continuations with the highest log probability that the search finds: (log probability, tokens), best
         first.  A beam that has several successors forks; one that has none gives its pages back."""
+        if not len(prompt):
+            raise ValueError("Decoder.beam_search: a prompt has a token")
         first = self.cache.add_sequence()
         held = {first}
         try:
