@@ -136,3 +136,18 @@ def test_texts_without_a_second_token_have_no_scores(decoder):
     with pytest.raises(ValueError):
         decoder.beam_search([], 3)
     assert nothing_is_held(decoder)
+
+
+def test_steps_that_do_not_fit_together_are_refused(decoder):
+    cache = decoder.cache
+    a, b = cache.add_sequence(), cache.add_sequence()
+    good = [a, b], [[1, 2], [3]], [(0, 1), (1, 0)], [0, 0]
+    for change in ({0: [a, a]}, {0: [a]}, {0: [], 1: [], 2: [], 3: []}, {1: [[1, 2]]}, {1: [[], []], 2: [], 3: []},  # one sequence twice ...
+                   {1: [[1, VOCAB], [3]]}, {1: [[1, -1], [3]]},                    # (Gather would take the last token's embedding)
+                   {2: [(0, 1)]}, {3: [0]}, {2: [(0, 2), (1, 0)]}, {2: [(0, 1), (1, 1)]}, {2: [(2, 0), (1, 0)]}, {2: [(0, -1), (1, 0)]}):
+        with pytest.raises(ValueError):
+            decoder.step(*[change.get(i, v) for i, v in enumerate(good)])
+        assert cache.length(a) == cache.length(b) == cache.used_pages == 0 and not decoder.runner.calls, change
+    decoder.step(*good)
+    decoder.step([a, b], [[], [VOCAB - 1]], [], [])
+    assert cache.length(a) == 2 and cache.length(b) == 2

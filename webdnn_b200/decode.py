@@ -26,7 +26,7 @@ class Decoder:
         if context is None:
             context = WebDNNCudaContext()
             context.initialize()
-        self.context, self.top, self.positions = context, top, positions
+        self.context, self.vocab, self.top, self.positions = context, vocab, top, positions
         self.cache = PagedCache(context, layers, pages, kv_heads, d // heads, page_tokens)
         context.add_cache(name, self.cache)
         self.table_pages = -(-positions // page_tokens)      # the same for every call, so that calls repeat
@@ -43,17 +43,25 @@ class Decoder:
         """Appends new_tokens[i] to sequences[i]; (logprob of targets[j], entropy, top ids, top logprobs) behind the new token
         wanted[j] = (which sequence of the call, which of its new tokens).  A step that fails leaves the sequences as long as they were."""
         counts = [len(t) for t in new_tokens]
+        width = max(counts, default=0)
+        # (two rows of one sequence would write to the same page at a time)
+        if width == 0 or len(counts) != len(sequences) or len(set(sequences)) != len(sequences):
+            raise ValueError("Decoder.step: some new tokens, one list for each of different sequences")
+        if len(wanted) != len(targets) or not all(0 <= i < len(counts) and 0 <= j < counts[i] for i, j in wanted):
+            raise ValueError("Decoder.step: one target for each wanted token, which is a new one")
         before = [self.cache.length(s) for s in sequences]
-        if max((n + c for n, c in zip(before, counts)), default=0) > self.positions:      # (Gather would take the last place)
+        ids, places = np.zeros((len(sequences), width), np.int32), np.zeros((len(sequences), width), np.int32)
+        for i, (n, t) in enumerate(zip(before, new_tokens)):
+            ids[i, :len(t)] = t
+            places[i, :len(t)] = np.arange(n, n + len(t))
+        # (Gather would take the first or the last)
+        if places.max() >= self.positions:
             raise ValueError(f"Decoder.step: there are places for {self.positions} tokens")
+        if ids.min() < 0 or ids.max() >= self.vocab:
+            raise ValueError(f"Decoder.step: tokens are 0 .. {self.vocab - 1}")
+        rows = np.array([i * width + j for i, j in wanted], np.int32)
         self.cache.extend(dict(zip(sequences, counts)))
         try:
-            width = max(counts)
-            ids, places = np.zeros((len(sequences), width), np.int32), np.zeros((len(sequences), width), np.int32)
-            for i, (s, t) in enumerate(zip(sequences, new_tokens)):
-                ids[i, :len(t)] = t
-                places[i, :len(t)] = np.arange(self.cache.length(s) - len(t), self.cache.length(s))
-            rows = np.array([i * width + j for i, j in wanted], np.int32)
             inputs = [CPUTensor.from_array(ids), CPUTensor.from_array(places),
                       *self.cache.batch(sequences, counts, self.table_pages),
                       CPUTensor.from_array(rows), CPUTensor.from_array(np.array(targets, np.int32))]
