@@ -195,3 +195,23 @@ def test_beam_search(decoder):
         assert abs(total - score) <= 0.02 * len(tokens)
     ((greedy, _),) = decoder.beam_search(prompt, 9, beams=1)
     assert found[0][0] >= greedy - 0.02 * 9
+
+
+def test_steps_that_want_nothing_and_texts_without_scores(decoder):
+    """A prompt may be appended without asking for anything; the next step sees it."""
+    rng = np.random.default_rng(6)
+    cache, reference = decoder.cache, reference_of(decoder)
+    a = cache.add_sequence()
+    prompt = rng.integers(0, SHAPE["vocab"], 21).tolist()
+    for _ in range(3):                               # (node by node, recorded, replayed)
+        got = decoder.step([a], [prompt], [], [])
+        assert [o.shape for o in got] == [(0,), (0,), (0, 6), (0, 6)]
+    logs = [reference.step(t)[-1] for t in (prompt, prompt, prompt, [7])][-1]
+    logprob, *_ = decoder.step([a], [[7]], [(0, 0)], [5])
+    np.testing.assert_allclose(logprob[0], logs[5], atol=0.02)
+    cache.release(a)
+    got = decoder.score([[], prompt, [3]])
+    want = reference_of(decoder).step(prompt)
+    assert [len(s) for s in got] == [0, 20, 0]
+    np.testing.assert_allclose(got[1], want[np.arange(20), prompt[1:]], atol=0.02)
+    assert cache.used_pages == 0
