@@ -270,3 +270,24 @@ def test_the_decoder_graph_keeps_its_operators():
     types = [n.op_type for n in model.graph.node]
     assert types.count("CudaCacheAttention") == 2 and types.count("CudaTokenLogProbs") == 1
     assert types.count("CudaLayerNorm") == 4 and "ReduceMean" not in types
+
+
+def test_a_copy_that_fails_gives_no_room():
+    context, cache = make()
+    a = cache.add_sequence()
+    cache.extend({a: 20})
+    b, c = cache.fork(a), cache.fork(a)
+    state = lambda: ([cache.sequence_pages(s) for s in (a, b, c)], [cache.length(s) for s in (a, b, c)], sorted(cache._free), cache._users[:])  # noqa: E731
+    before = state()
+
+    def fails(name, *args):
+        raise RuntimeError(name)
+
+    context._call, call = fails, context._call
+    with pytest.raises(RuntimeError, match="copy_pages"):
+        cache.extend({a: 1, b: 30, c: 0})
+    assert state() == before
+    context._call = call
+    cache.extend({a: 1, b: 30, c: 0})
+    assert cache.sequence_pages(c) == [0, 1] and context.copies() == [(1, 2), (1, 3)]
+    assert cache.sequence_pages(a) == [0, 2] and cache.sequence_pages(b) == [0, 3, 4, 5] and cache.used_pages == 6

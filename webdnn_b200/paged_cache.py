@@ -216,7 +216,7 @@ class PagedCache:
         wanted += sum(w if self._users[p] > w else w - 1 for p, w in shared.items())
         if wanted > len(self._free):
             raise MemoryError(f"PagedCache: {wanted} pages are needed, {len(self._free)} are free")
-        sources, targets = [], []
+        sources, targets, copied = [], [], []
         for (s, n), more in zip(new_tokens.items(), need):
             pages, length = self._sequences[s], self._lengths[s]
             at = length // self.page_tokens
@@ -225,10 +225,20 @@ class PagedCache:
                 self._users[pages[at]] -= 1
                 pages[at] = self._take()
                 targets.append(pages[at])
+                copied.append((pages, at))
             pages.extend(self._take() for _ in range(more))
             self._lengths[s] = length + n
         if sources:
-            self.copy_pages(sources, targets)
+            try:
+                self.copy_pages(sources, targets)
+            except BaseException:
+                for s, n in new_tokens.items():
+                    self.truncate(s, self._lengths[s] - n)
+                for (pages, at), page in zip(copied, sources):
+                    self._drop(pages[at])
+                    pages[at] = page
+                    self._users[page] += 1
+                raise
 
     def fork(self, sequence: int) -> int:
         """A new sequence with the same tokens, on the same pages."""
