@@ -291,3 +291,17 @@ def test_a_copy_that_fails_gives_no_room():
     cache.extend({a: 1, b: 30, c: 0})
     assert cache.sequence_pages(c) == [0, 1] and context.copies() == [(1, 2), (1, 3)]
     assert cache.sequence_pages(a) == [0, 2] and cache.sequence_pages(b) == [0, 3, 4, 5] and cache.used_pages == 6
+
+
+def test_results_are_row_major():
+    """A result in another order of memory would be read as something else."""
+    context, cache = make()
+    logits, tokens = context.empty_tensor([2, 3, 4, 5, 9]), context.empty_tensor([2, 3, 4, 5], "int32")
+    good = [context.empty_tensor([2, 3, 4, 5]), context.empty_tensor([2, 3, 4, 5]), None, None]
+    context.token_logprobs(logits, tokens, out=good)
+    for i in (0, 1):
+        out = list(good)
+        out[i] = context.empty_tensor([2, 3, 4, 5], layout="nhwc")
+        with pytest.raises(ValueError):
+            context.token_logprobs(logits, tokens, out=out)
+    assert [name for name, _ in context.calls] == ["wdc_token_logprobs"]

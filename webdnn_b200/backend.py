@@ -627,8 +627,9 @@ class WebDNNCudaContext:
             if len(out) != 4 or (tokens is None and out[0] is not None):
                 raise ValueError("token_logprobs: out is (logprob, entropy, top_ids, top_logprobs)")
             for t, n, kind in zip(out, (rows, rows, rows * top, rows * top), ("float32", "float32", "int32", "float32")):
-                if t is not None and (t.__class__ is not CudaTensor or t.context is not self or t.length != n or t.data_type != kind):
-                    raise ValueError(f"token_logprobs: a result has {n} values of {kind}, in this context")
+                if t is not None and (t.__class__ is not CudaTensor or t.context is not self or t.length != n or t.data_type != kind
+                                      or t.layout != "nchw"):
+                    raise ValueError(f"token_logprobs: a result has {n} values of {kind}, row-major, in this context")
         if rows:
             self._call("wdc_token_logprobs", byref(LogprobsDesc(rows, vocab, width, top)), logits.ptr,
                        tokens.ptr if tokens is not None else None, *[t.ptr if t is not None and t.length else None for t in out])
