@@ -174,3 +174,32 @@ def test_nan_at_the_first_logit(cuda_context, vocab, top):
     x[4, 1:] = -np.inf
     x[5, 0] = -np.float32(np.nan)
     check(cuda_context, x, rng.integers(0, vocab, 6), top)
+
+
+@pytest.mark.parametrize("top", [0, 5, 32])
+@pytest.mark.parametrize("rows", [300, 450, 900, 1800])
+def test_long_rows_of_one_cta_each(cuda_context, rows, top):
+    """Rows of many rounds with eight, four, two and one warp: rising (every logit is a candidate), falling, random, mostly masked,
+    and with few different logits."""
+    rng = np.random.default_rng(rows)
+    vocab = 20001                                    # (rows begin at every place between two 16-byte boundaries)
+    x = rng.standard_normal((10, vocab)).astype(f32) * 3
+    x[0] = np.linspace(-20, 20, vocab, dtype=f32)
+    x[1] = x[0, ::-1]
+    x[2] = np.arange(vocab) // 7 * f32(1e-3)
+    x[3, rng.random(vocab) < 0.999] = -np.inf
+    x[4, 100:] = -np.inf
+    x[5] = rng.integers(-3, 3, vocab)
+    x[6, :vocab // 2] -= 50                          # the best are behind all that the first rounds kept
+    of = np.arange(rows) % len(x)
+    tokens = rng.integers(0, vocab, len(x))
+    logprob, entropy, ids, best, _ = reference(x, tokens, top)
+    ts = [dev(cuda_context, x[of]), dev(cuda_context, tokens[of].astype(np.int32))]
+    got = cuda_context.token_logprobs(*ts, top)
+    near(got[0].get_data(), logprob[of], 1)
+    near(got[1].get_data(), entropy[of], (1 + np.log(vocab) + entropy)[of])
+    if top:
+        assert np.array_equal(got[2].get_data().reshape(rows, top), ids[of])
+        near(got[3].get_data().reshape(rows, top), best[of], 1)
+    for t in ts + [t for t in got if t is not None]:
+        t.dispose()

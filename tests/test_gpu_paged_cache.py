@@ -684,3 +684,86 @@ def test_small_codes_and_queries_of_one_sign(cuda_context, size, c, heads, kv_he
                                             size, c ** -0.5)
             assert np.abs(got[b:b + 1, :, h:h + 1] - want).max() <= tol
     cache.dispose()
+
+
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_sharp_and_tiny_scores_head_by_head(cuda_context, tokens):
+    """Queries of very different magnitudes beside one another, each head within the tolerance of its own scores."""
+    rng = np.random.default_rng(8)
+    magnitudes = np.array([30, 1, 1e-6, 1e-30, 1e-37], f32)
+    cache = PagedCache(cuda_context, 1, 24, 10, 64, 16)
+    codes, scales = random_pool(rng, cache)
+    lengths, counts = [300, 71], [tokens, tokens]
+    table = tables(rng, cache, lengths)
+    scales[0, table[0, :19], 0] *= np.linspace(0.2, 8, 19, dtype=f32)[:, None]
+    set_pool(cache, codes, scales)
+    q = rng.standard_normal((2, tokens, 20, 64)).astype(f32) * np.repeat(magnitudes, 4)[:, None]
+    got = run_attention(cuda_context, cache, q, table, lengths, counts, scale=0.7)
+    for h in range(20):
+        of = slice(h // 2, h // 2 + 1)
+        want, tol = reference_attention(q[:, :, h:h + 1], codes[0][:, :, of], scales[0][:, :, of], table, lengths, counts, 16, float(f32(0.7)))
+        assert np.abs(got[:, :, h:h + 1] - want).max() <= tol
+    cache.dispose()
+
+
+def short_sequences_of_a_wide_table(ctx, batch, c, heads, kv_heads, size, tokens, wide, lengths, counts, seed):
+    """Compares them with the reference; numbers of the sequences in `counts` that do not fit the call give rows of zeros."""
+    rng = np.random.default_rng(seed)
+    fits = [0 <= n <= m and n <= tokens and m <= wide * size for n, m in zip(counts, lengths)]
+    held = [m if f else 0 for m, f in zip(lengths, fits)]
+    cache = PagedCache(ctx, 1, sum(-(-m // size) for m in held) + 1, kv_heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, held)
+    table = np.concatenate([table, np.full((batch, wide - table.shape[1]), -1, np.int32)], 1)
+    q = rng.standard_normal((batch, tokens, heads, c)).astype(f32)
+    ts = [dev(ctx, a) for a in (q.reshape(batch, tokens, -1), table, np.array(lengths, np.int32), np.array(counts, np.int32))]
+    y = cache.attention(0, *ts)
+    if all(fits):
+        ctx.sync()
+    else:
+        with pytest.raises(CudaBackendError, match="out of range"):
+            ctx.sync()
+    got = y.get_data().reshape(q.shape)
+    want, tol = reference_attention(q, codes[0], scales[0], table, held, [n if f else 0 for n, f in zip(counts, fits)], size, c ** -0.5)
+    assert np.abs(got - want).max() <= tol
+    for b, (n, f) in enumerate(zip(counts, fits)):
+        assert not got[b, n if f else 0:].any()
+    for t in ts + [y]:
+        t.dispose()
+    cache.dispose()
+
+
+# (Such a call's tiles are shared out between three or four CTAs an SM where the table has room for 32 and more of them a CTA.)
+@pytest.mark.parametrize("batch,c,heads,kv_heads,size,tokens,wide", [
+    (1, 128, 2, 1, 128, 1, 3600), (3, 64, 8, 2, 64, 9, 400), (5, 64, 4, 2, 32, 1, 2000), (20, 32, 6, 2, 16, 3, 1000),
+    (37, 128, 8, 4, 64, 2, 100), (200, 128, 4, 4, 128, 1, 40), (512, 64, 1, 1, 64, 1, 24), (511, 32, 4, 1, 32, 2, 40),
+    (512, 128, 3, 1, 16, 2, 80), (2, 128, 24, 2, 32, 30, 700)])
+def test_tiles_that_are_shared_out(cuda_context, batch, c, heads, kv_heads, size, tokens, wide):
+    """Sequences of any length, some empty, some without new tokens."""
+    rng = np.random.default_rng(batch + c)
+    longest = min(wide * size, 40_000 // batch + 2 * tokens)
+    lengths = [int(n) for n in rng.integers(1, longest + 1, batch)]
+    counts = [int(rng.integers(0, min(n, tokens) + 1)) for n in lengths]
+    lengths[0], counts[0] = longest, tokens
+    if batch > 2:
+        lengths[1] = counts[1] = counts[2] = 0
+    short_sequences_of_a_wide_table(cuda_context, batch, c, heads, kv_heads, size, tokens, wide, lengths, counts, batch)
+
+
+def test_tiles_that_are_shared_out_beside_numbers_out_of_range(cuda_context):
+    lengths = [500, -1, 90, 3000 * 32 + 1, 70, 5, 41, 1000]
+    counts = [2, 1, 3, 1, -1, 6, 2, 1]
+    short_sequences_of_a_wide_table(cuda_context, 8, 64, 8, 2, 32, 2, 3000, lengths, counts, 1)
+
+
+@pytest.mark.parametrize("batch,length", [(444, 250), (222, 768), (222, 250), (148, 500), (111, 500), (300, 1), (148, 32)])
+def test_units_that_end_where_a_ctas_tiles_end(cuda_context, batch, length):
+    """Equal units, of which whole ones, halves, thirds or quarters are a CTA's (or only a beginning, without a tile)."""
+    short_sequences_of_a_wide_table(cuda_context, batch, 128, 2, 1, 128, 1, 140, [length] * batch, [1] * batch, batch)
+
+
+@pytest.mark.parametrize("size,c,heads,kv_heads,tokens", [(16, 64, 8, 2, 1), (64, 128, 4, 4, 2), (32, 32, 9, 3, 12)])
+def test_parts_without_a_tile(cuda_context, size, c, heads, kv_heads, tokens):
+    """Sequences that are much shorter than the table has room for, cut into equal parts of which most have nothing."""
+    lengths, counts = [1, 90, 0, 40, 700], [1, min(tokens, 9), 0, tokens, tokens]
+    short_sequences_of_a_wide_table(cuda_context, 5, c, heads, kv_heads, size, tokens, 4096 // size, lengths, counts, c)
