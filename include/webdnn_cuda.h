@@ -338,8 +338,9 @@ int wdc_decode_eightbit(wdc_context* ctx, const void* codes, float* out, int64_t
  * keep nothing between runs).  A page holds page_tokens tokens of one sequence:
  *   codes  int8    [2 (keys, values)][kv_heads][page_tokens][head_size]
  *   scales float32 [2][kv_heads]
- * and a number is code * scale.  A pool of several layers is [layers][pages] of these: a page has the same index in every
- * layer, and the calls of one layer take the address of that layer's first page.
+ * and a number is code * scale.  No scale is negative; one that is not finite counts as NaN.  A pool of several layers is
+ * [layers][pages] of these: a page has the same index in every layer, and the calls of one layer take the address of that layer's
+ * first page.
  * page_table is int32 [batch][table_pages]: the pages of each sequence in order.  lengths is int32 [batch]: the tokens of
  * each sequence, those of this call included; counts is int32 [batch] or NULL: how many of them are new, the last ones (NULL:
  * `tokens` of each).  Row i of k, v, q and y is a sequence's i-th new token; rows from its count on are padding.

@@ -573,9 +573,12 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
   const int64_t units = (int64_t)a.batch * a.kv_heads * a.row_tiles, slots = Layout<DH>::CTAS * ctx->sm_count;
   const int64_t tiles = ceil_div64(a.table_pages << a.page_shift, TILE);
   // As many parts as make one wave of CTAs (two, where that would leave a third of it empty or more); shared out where a CTA has 32
-  // tiles and more.  Measured, us with equal parts / shared out: 3 sequences of 12000 to 40001 tokens and 16 key heads (48 units, 142
-  // tiles a CTA) 82.2 / 70.2; 16 of 1959 to 2979 and 16 (256, 57) 52.4 / 44.7; 48 of 1 to 4100 and 8 (384, 118) 49.9 / 52.8; 20 of 100 to
-  // 1500 and 8, two row tiles (320, 27) 17.0 / 20.2; 16 of 2243 to 11554 and 2, heads of 32 (32, 20) 13.5 / 16.3.
+  // tiles and more, as far as the table's width tells.  Measured, us with equal parts / shared out, heads of 128 (units, tiles a CTA): 3
+  // sequences of 12000 to 40001 tokens and 16 key heads (48, 142) 84.2 / 70.7; 16 of 1959 to 2979 and 16 (256, 57) 53.8 / 44.3; of 1 to 4100
+  // and 8 key heads, 32 sequences (256, 78) 46.0 / 40.4, 64 (512, 157) 78.6 / 66.6; 20 of 100 to 1500 and 8, two row tiles (320, 27) 17.0 /
+  // 20.2; 16 of 2243 to 11554 and 2, heads of 32 (32, 20) 13.5 / 16.3.  Two and more equal parts or whole units for each place can be the
+  // better ones when uneven units happen to fill their waves: 48 of 1 to 4100 (384, 118) 49.7 / 52.6, 96 (768, 235) 81.1 / 92.5; but 48 of
+  // 3000 to 4100 (384, 118) 79.3 / 77.5.  The host does not know the lengths that decide it.
   a.splits = (int)(2 * units <= slots ? slots / units : units < slots ? 2 : 1);
   if (a.splits > ceil_div64(tiles, WARPS)) a.splits = (int)ceil_div64(tiles, WARPS);
   if (a.splits < 1) a.splits = 1;

@@ -185,6 +185,8 @@ struct WholeRows {
 // of chunks and more.  It costs a CTA 1 us, and is done where more than one wave of CTAs and tiles of 16 chunks and more make it worth
 // that, and sequences are at most ORDERED.  Measured, us without / with: three prompts of 900, 750 and 450 tokens behind 900, 375
 // and 0, heads of 128 80.6 / 65.9 and of 64 60.1 / 50.7; four of 1000 to 500 behind none 123.5 / 125.4; six of 153 to 83 18.3 / 21.2.
+// With more sequences the waves are many, and less is gained than taking a tile costs: up to 900 new tokens of 100 to 1000, 12 sequences
+// 139.5 / 151.8 and 24 269 / 324; 300 of 100 to 2000, 12 sequences 113.2 / 104.2 and 24 201 / 216.
 constexpr int ORDERED = 8;
 __device__ __forceinline__ int4 take_tile(const CacheAttArgs& a, int place, int lane) {
   const int64_t capacity = a.table_pages << a.page_shift;
@@ -642,7 +644,11 @@ int launch(wdc_context* ctx, const CacheAttArgs& a, int64_t ctas) {
 
 }  // namespace
 
-// WDC_ERR_UNSUPPORTED (nothing written): the caller runs the kernel for few rows.
+// WDC_ERR_UNSUPPORTED (nothing written): the caller runs the kernel for few rows, which is as fast at 64 rows of a key head, and at a tile
+// of 128 for every fourth SM.  Measured, us here / by the other kernel, heads of 128: 8 sequences and 8 key heads of 500 tokens, 48 rows
+// 20.5 / 24.8, 64 rows 20.6 / 18.1, 96 rows 21.0 / 39.6; of 4000 tokens 99.2 / 83.2, 99.2 / 105.7 and 99.6 / 151; 19 sequences 192 / 155,
+// 193 / 193 and 193 / 274.  One sequence, tiles of all its key heads: of 600 tokens 32 tiles 23.8 / 26.4, 40 tiles 23.9 / 38.5; of 4000 98.3 /
+// 103 and 98.3 / 126; of 20000 455 / 427 and 452 / 531.
 int wdc_cache_attention_tc(wdc_context* ctx, CacheAttArgs a, int head_size) {
   if (head_size != 64 && head_size != 128) return WDC_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)a.tokens * a.group;

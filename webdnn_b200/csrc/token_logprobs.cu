@@ -142,8 +142,8 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // another warp); where rows are fewer than that with eight warps, a cluster of `parts` CTAs, each on a range of the row.  A round is EACH
 // float4 a thread, and the next round's are on their way.
 //
-// Bound: memory where rows are many (3000 x 50001: 104.2 us, 5.8 TB/s, 87% of a copy's rate); launch, first round and joins where
-// they are few (1 x 32000: 6.7 us, 36 x 100003: 12.7 us).
+// Bound: memory where rows are many (3000 x 50001: 105 to 115 us by machine and inputs, 5.2 to 5.7 TB/s, 80 to 87% of a copy's rate);
+// launch, first round and joins where they are few (1 x 32000: 6.9 us, 36 x 100003: 12.7 us).
 //
 // Candidates for the best `top`: the floor is a key that `top` logits of the range are known to be above.  After the first round it
 // is just below the `top`-th largest of the threads' largest keys; from then on every warp keeps what is above it in a list of its

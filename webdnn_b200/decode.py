@@ -19,6 +19,9 @@ from .runner import load
 
 
 class Decoder:
+    """A decoder with random weights (``zoo.decoder``) and its cache, which the context knows as ``name`` and keeps for its own life: a
+    second decoder of one context needs another name."""
+
     def __init__(self, context: Optional[WebDNNCudaContext] = None, vocab: int = 1000, d: int = 256, heads: int = 8,
                  kv_heads: int = 2, layers: int = 4, ffn: int = 1024, positions: int = 4096, top: int = 8, pages: int = 512,
                  page_tokens: int = 32, name: str = "cache"):
