@@ -383,6 +383,90 @@ typedef struct wdc_cache_pages_desc {
 int wdc_cache_copy_pages(wdc_context* ctx, const wdc_cache_pages_desc* d, void* codes, float* scales, int64_t n,
                          const int32_t* from, const int32_t* to);
 
+/* ---- a decoder that drafts --------------------------------------------------------------------
+ * What a decoder with rotary positions needs, and one whose drafted tokens are checked several at a time (no counterpart in the
+ * reference).  A position, parent, path or number of kept tokens that comes from the device and is out of range does no harm beyond
+ * what each call says, and the next waiting call returns WDC_ERR_INVALID once.
+ *
+ * wdc_rotate_heads: heads normalised and rotated, y[row][head] from x[row][head], both rows of head_size floats at their strides
+ * (non-negative multiples of 4 floats; buffers 16-byte, positions 4-byte aligned):
+ *   n = x * weight / sqrt(mean(x^2) + epsilon)   (weight [head_size]; NULL: n = x)
+ *   pairs (a, b) of the first `rotary` channels become a cos - b sin, b cos + a sin; they are channels i and i + rotary / 2, or
+ *   with `interleaved` 2 i and 2 i + 1; cos and sin are [places][rotary / 2], of which the row's position names one (positions
+ *   NULL: the row's number).  A position out of range counts as the nearest one.
+ * Computed in 64 bits and rounded once.  y may be x (with the same strides); otherwise they do not overlap.
+ * head_size is a multiple of 4 up to 256, rotary a multiple of 8 up to head_size, 0: none (else WDC_ERR_UNSUPPORTED). */
+typedef struct wdc_rotate_desc {
+  int64_t rows, heads, head_size, rotary, places;
+  int64_t x_st, x_sh, y_st, y_sh; /* strides: row, head */
+  float epsilon;
+  int32_t interleaved;
+} wdc_rotate_desc;
+int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, const float* x, const float* weight, const float* cos,
+                     const float* sin, const int32_t* positions, float* y);
+
+/* wdc_cache_append of keys that are normalised and rotated like wdc_rotate_heads' on the way; where q is given, its heads are as well,
+ * into q_out (rows of padding become zero).  Nothing of q is written unless q_out is q (with the same strides); otherwise they do not
+ * overlap.  positions is int32 [batch][tokens] or NULL (a token's place in its sequence); one out of range counts as the nearest one. */
+typedef struct wdc_cache_append_rotary_desc {
+  wdc_cache_append_desc append;
+  int64_t heads; /* of q */
+  int64_t q_sb, q_sh, q_st;
+  int64_t y_sb, y_sh, y_st; /* strides of q_out */
+  int64_t rotary, places;
+  float epsilon;
+  int32_t interleaved;
+} wdc_cache_append_rotary_desc;
+int wdc_cache_append_rotary(wdc_context* ctx, const wdc_cache_append_rotary_desc* d, const float* q, const float* k, const float* v,
+                            const float* q_weight, const float* k_weight, const float* cos, const float* sin,
+                            const int32_t* positions, void* codes, float* scales, const int32_t* page_table,
+                            const int32_t* lengths, const int32_t* counts, float* q_out);
+
+/* wdc_cache_attention of new tokens that are a tree: parents is int32 [batch][tokens], the new token that each continues, always one
+ * before it, -1: the text before the new ones.  A token sees that text, its ancestors and itself.  A parent that is not before its
+ * token counts as -1.  At most 1024 tokens (else WDC_ERR_UNSUPPORTED). */
+int wdc_cache_attention_tree(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
+                             const float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts,
+                             const int32_t* parents, float* y);
+
+/* Which of a tree's drafted tokens stand, and the token that follows them.  New token 0 of each sequence is decided already; the others
+ * are drafts, tokens int32 [batch][tokens], in a tree (parents as above, NULL: each continues the one before) of which counts
+ * int32 [batch] (NULL: `tokens`) are there.  logits [batch][tokens][vocab] (sequences logits_sb floats apart, tokens logits_st) has
+ * the target's logits behind each new token; its distribution is softmax(logits / temperature), at temperature 0 the first of the largest.
+ * The walk begins at token 0.  Standing at token i, with p the distribution behind it:
+ *   without draft_logits, a token is drawn from p with uniforms[i]; the first child that has this token stands and the walk goes on
+ *   there; if none has, the drawn token is `next`.
+ *   With draft_logits (strides draft_sb, draft_st; q = softmax(draft_logits / draft_temperature), from which the children of token i
+ *   were drawn, each by itself), the children c are tried in order: c stands where uniforms[c] q(token) < p(token), else p becomes
+ *   max(p - q, 0) over its sum (p stays where that is 0).  If none stands, `next` is drawn from p with uniforms[0].
+ * A token drawn from p with u is the first whose running sum of p passes u times all of it.  uniforms is float32 [batch][tokens], 0
+ * <= u < 1 (what is below counts as 0, what is not below 1 as 1 - 2^-24, NaN as 0); it may be NULL at temperature 0 without drafts.
+ * All of it is in 64 bits.  Results: path int32 [batch][tokens], the tokens that stand, 0 first, -1 behind them; accepted [batch], how
+ * many; next [batch].  A distribution that does not exist (a NaN, +inf, or nothing above -inf) ends the walk with next = -1; a
+ * drafted token outside 0 .. vocab - 1 never stands; a sequence whose count is 0 has accepted 0 and next -1, and so has one whose
+ * count is out of range.  batch is at most 65535, tokens at most 1024, vocab less than 2^30 (else WDC_ERR_UNSUPPORTED). */
+typedef struct wdc_verify_desc {
+  int64_t batch, tokens, vocab;
+  int64_t logits_sb, logits_st, draft_sb, draft_st;
+  float temperature, draft_temperature;
+} wdc_verify_desc;
+int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, const float* logits, const float* draft_logits,
+                      const int32_t* tokens, const int32_t* parents, const int32_t* counts, const float* uniforms,
+                      int32_t* path, int32_t* accepted, int32_t* next);
+
+/* Moves the tokens that stand to the front of a sequence's new ones, in all layers: new token path[i] to the place of new token i, for i
+ * < accepted (path int32 [batch][tokens], rising from 0 or more, accepted int32 [batch], as wdc_verify_drafts gives them; lengths, counts
+ * and page_table as above).  A token that comes from another page is rounded again by the scale of its new page, which grows where
+ * that token needs it, rint(code * its scale / the page's), and with it all codes of the page up to there; the others keep their codes.  What lies behind
+ * the kept tokens is left as it is: the caller counts them as gone.  A path that does not rise within the count, or is longer,
+ * leaves its sequence alone.  Calling it again moves again: a tape that it is part of is not repeated. */
+typedef struct wdc_cache_keep_desc {
+  int64_t layers, pages, kv_heads, page_tokens, head_size;
+  int64_t batch, tokens, table_pages;
+} wdc_cache_keep_desc;
+int wdc_cache_keep_paths(wdc_context* ctx, const wdc_cache_keep_desc* d, void* codes, float* scales, const int32_t* page_table,
+                         const int32_t* lengths, const int32_t* counts, const int32_t* path, const int32_t* accepted);
+
 /* Log probabilities under softmax(logits), logits [rows][vocab] with rows row_stride floats apart (no counterpart in the
  * reference, which ends at Softmax).  Any of the results may be NULL (top_ids and top_logprobs together):
  *   logprob [rows]             of the tokens int32 [rows] (NULL: no logprob); NaN for a token outside 0 .. vocab - 1

@@ -25,7 +25,7 @@ from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 
-from .lib import (DTYPE_CODE, ConvDesc, CudaBackendError, GemmDesc, Library, LogprobsDesc, PoolDesc, i64_array)
+from .lib import (DTYPE_CODE, ConvDesc, CudaBackendError, GemmDesc, Library, LogprobsDesc, PoolDesc, RotateDesc, VerifyDesc, i64_array)
 
 NP_DTYPE = {"float32": np.float32, "int32": np.int32, "bool": np.uint8}
 
@@ -633,6 +633,120 @@ class WebDNNCudaContext:
         if rows:
             self._call("wdc_token_logprobs", byref(LogprobsDesc(rows, vocab, width, top)), logits.ptr,
                        tokens.ptr if tokens is not None else None, *[t.ptr if t is not None and t.length else None for t in out])
+        return tuple(out)
+
+    def asserts_int_rows(self, who: str, what: str, t: CudaTensor, dims: Sequence[int]) -> None:
+        """``t`` is int32 of these dims, row-major, in this context."""
+        self.asserts_cuda_tensor(t)
+        if t.data_type != "int32" or t.layout != "nchw":
+            raise TypeError(f"{who}: {what} is int32, row-major")
+        if t.dims != list(dims):
+            raise ValueError(f"{who}: {what} is {list(dims)}, not {t.dims}")
+
+    def asserts_rotation(self, who: str, head_size: int, cos: Optional[CudaTensor], sin: Optional[CudaTensor],
+                         positions: Optional[CudaTensor], weights: Sequence[Optional[CudaTensor]]) -> None:
+        """The tables, positions and weights of ``rotate_heads`` fit together."""
+        for t, kind in ((cos, "float32"), (sin, "float32"), (positions, "int32"), *((w, "float32") for w in weights)):
+            if t is not None:
+                self.asserts_cuda_tensor(t)
+                if t.data_type != kind or t.layout != "nchw":
+                    raise TypeError(f"{who}: cos, sin and weights are float32, positions int32, all row-major")
+        if (cos is None) != (sin is None) or (cos is None and positions is not None):
+            raise ValueError(f"{who}: cos and sin come together, and positions with them")
+        if cos is not None and (cos.ndim != 2 or cos.dims != sin.dims or cos.dims[0] < 1 or cos.dims[1] % 4 or not 0 < 2 * cos.dims[1] <= head_size):
+            raise ValueError(f"{who}: cos and sin are [places, pairs], pairs a multiple of 4 up to {head_size // 2}, not {cos.dims} and {sin.dims}")
+        for w in weights:
+            if w is not None and w.dims != [head_size]:
+                raise ValueError(f"{who}: a weight is [{head_size}], not {w.dims}")
+
+    def rotate_heads(self, x: CudaTensor, heads: int, head_size: int, cos: Optional[CudaTensor] = None, sin: Optional[CudaTensor] = None,
+                     positions: Optional[CudaTensor] = None, weight: Optional[CudaTensor] = None, epsilon: float = 1e-6,
+                     interleaved: bool = False, column: int = 0, out: Optional[CudaTensor] = None) -> CudaTensor:
+        """Heads normalised by the root of their mean square and rotated by their position (``wdc_rotate_heads``).
+
+        ``x`` float32 [..., n], of which ``heads`` * ``head_size`` columns from ``column`` on are the heads side by side; the result
+        is [..., heads * head_size].  ``weight`` float32 [head_size] (without: no norm); ``cos`` and ``sin`` float32 [places, pairs]
+        (without: no rotation): the first 2 * pairs channels of a head are rotated, channels i and i + pairs together or, with
+        ``interleaved``, 2 i and 2 i + 1.  ``positions`` int32, one for each row of ``x`` (without: the row's number).  ``out`` may be
+        ``x``, where that has its shape."""
+        who = "rotate_heads"
+        self.asserts_cuda_tensor(x)
+        if x.data_type != "float32" or x.layout != "nchw":
+            raise TypeError(f"{who}: x is float32, row-major")
+        if heads < 1 or head_size < 1 or head_size % 4 or head_size > 256:
+            raise ValueError(f"{who}: {heads} heads of {head_size} (a multiple of 4 up to 256)")
+        self.asserts_rotation(who, head_size, cos, sin, positions, (weight,))
+        n = x.dims[-1] if x.ndim else 0
+        if column < 0 or column % 4 or n % 4 or column + heads * head_size > n:
+            raise ValueError(f"{who}: {heads} heads of {head_size} from column {column} on, of {x.dims} (multiples of 4)")
+        rows, dims = x.length // n, x.dims[:-1] + [heads * head_size]
+        if positions is not None and positions.length != rows:
+            raise ValueError(f"{who}: positions are one for each of {rows} rows")
+        if out is None:
+            out = self.empty_tensor(dims)
+        elif out.__class__ is not CudaTensor or out.context is not self or out.dims != dims or out.data_type != "float32" or out.layout != "nchw" or (
+                out.ptr == x.ptr and (column or out.dims != x.dims)):
+            raise ValueError(f"{who}: the result is float32 {dims}, row-major, in this context, and x only where that has its shape")
+        if rows:
+            pointers = [t.ptr if t is not None else None for t in (weight, cos, sin, positions)]
+            desc = RotateDesc(rows, heads, head_size, 2 * cos.dims[1] if cos is not None else 0, cos.dims[0] if cos is not None else 0, n, head_size,
+                              heads * head_size, head_size, epsilon, interleaved)
+            self._call("wdc_rotate_heads", byref(desc), x.ptr + 4 * column, *pointers, out.ptr)
+        return out
+
+    def verify_drafts(self, logits: CudaTensor, tokens: CudaTensor, parents: Optional[CudaTensor] = None,
+                      counts: Optional[CudaTensor] = None, uniforms: Optional[CudaTensor] = None,
+                      draft_logits: Optional[CudaTensor] = None, temperature: float = 1.0, draft_temperature: Optional[float] = None,
+                      vocab: Optional[int] = None, out: Optional[Sequence[CudaTensor]] = None):
+        """Which drafted tokens of a tree stand, and the token that follows (``wdc_verify_drafts``): (path, accepted, next), int32
+        [batch, tokens], [batch] and [batch].
+
+        ``tokens`` int32 [batch, tokens]: of each sequence token 0 is decided, the others are drafts; ``parents`` int32 [batch, tokens]
+        which one each continues (without: the one before), ``counts`` int32 [batch] how many there are.  ``logits`` float32
+        [batch, tokens, n], behind each token, of which the first ``vocab`` columns count (all, if not given); ``draft_logits`` the
+        distribution that a token's children were drawn from, where they were (by ``draft_temperature``: ``temperature`` unless given).
+        ``uniforms`` float32 [batch, tokens] in [0, 1): random numbers.  ``temperature`` 0: the largest logit, no random numbers."""
+        who = "verify_drafts"
+        for t, what in ((logits, "logits"), (uniforms, "uniforms"), (draft_logits, "draft_logits")):
+            if t is not None:
+                self.asserts_cuda_tensor(t)
+                if t.data_type != "float32" or t.layout != "nchw":
+                    raise TypeError(f"{who}: {what} are float32, row-major")
+        if logits.ndim != 3:
+            raise ValueError(f"{who}: logits are [batch, tokens, vocab]")
+        batch, n, width = logits.dims
+        self.asserts_int_rows(who, "tokens", tokens, [batch, n])
+        if parents is not None:
+            self.asserts_int_rows(who, "parents", parents, [batch, n])
+        if counts is not None:
+            self.asserts_int_rows(who, "counts", counts, [batch])
+        vocab = width if vocab is None else vocab
+        if not 0 < vocab <= width:
+            raise ValueError(f"{who}: vocab {vocab} of rows of {width}")
+        draft_width = width if draft_logits is None else draft_logits.dims[-1] if draft_logits.ndim == 3 else -1
+        if draft_logits is not None and (draft_logits.dims[:-1] != [batch, n] or draft_width < vocab):
+            raise ValueError(f"{who}: draft_logits are [{batch}, {n}, {vocab} or more]")
+        draft_temperature = temperature if draft_temperature is None else draft_temperature
+        for t in (temperature, draft_temperature):
+            if not (t == 0 or 1e-6 <= t <= 1e6):
+                raise ValueError(f"{who}: a temperature is 0, or 1e-6 to 1e6")
+        if uniforms is None:
+            if temperature != 0 or draft_logits is not None:
+                raise ValueError(f"{who}: a temperature, or drafts with a distribution, need uniforms")
+        elif uniforms.dims != [batch, n]:
+            raise ValueError(f"{who}: uniforms are [{batch}, {n}]")
+        shapes = ([batch, n], [batch], [batch])
+        if out is None:
+            out = tuple(self.empty_tensor(s, "int32") for s in shapes)
+        elif len(out) != 3:
+            raise ValueError(f"{who}: out is (path, accepted, next)")
+        for t, what, s in zip(out, ("path", "accepted", "next"), shapes):
+            self.asserts_int_rows(who, what, t, s)
+        if batch:
+            def at(t):
+                return t.ptr if t is not None and t.length else None
+            desc = VerifyDesc(batch, n, vocab, n * width, width, n * draft_width, draft_width, temperature, draft_temperature)
+            self._call("wdc_verify_drafts", byref(desc), *map(at, (logits, draft_logits, tokens, parents, counts, uniforms, *out)))
         return tuple(out)
 
     def conv2d(self, desc: ConvDesc, x, w, scale, shift, residual, y) -> None:

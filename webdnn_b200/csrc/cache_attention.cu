@@ -122,7 +122,7 @@ __device__ __forceinline__ void copy_half(uint32_t to_k, uint32_t to_v, const in
   }
 }
 
-template <int DH, int GROUPS>
+template <int DH, int GROUPS, bool TREE>
 __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_kernel(const CacheAttArgs a) {
   constexpr int STEPS = DH / 16;                  // of the score product's sum; also columns of O a thread and key row
   constexpr int KB = DH == 32 ? 8 : 16;           // bytes of a key a thread loads at a time
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(THREADS, Layout<DH>::CTAS) cache_attention_ker
   using L = Layout<DH>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int plan[PLAN_MOST + 1], plan_sums[WARPS];
+  __shared__ uint32_t tree[TREE ? ROWS : 1][TREE ? TREE_WORDS : 1];
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int units = a.kv_heads * a.row_tiles;     // of a sequence
@@ -205,7 +206,7 @@ next_segment:
   // the last token that this row sees (rows of padding see all: nobody reads theirs), and those of the tile's first and last row
   const int first_token = tile * ROWS / a.group, top_token = min((tile * ROWS + ROWS - 1) / a.group, span.count - 1);
   const int last = token < span.count ? before + token : 0x7fffffff;
-  const int seen_by_all = before + first_token + 1;
+  const int seen_by_all = TREE ? before : before + first_token + 1;
   const int seen = first_token < span.count ? before + top_token + 1 : 0;
   {
     const int tiles = (seen + TILE - 1) / TILE, part = (int)(blockIdx.x % (unsigned)max(a.splits, 1));
@@ -279,6 +280,13 @@ next_segment:
     }
   }
 
+  if (TREE && end * TILE > before) {               // (the copies of the first tiles are on their way)
+    if (threadIdx.x < ROWS)
+      tree_row(tree[threadIdx.x], pdl_after(a.parents) + (int64_t)b * a.tokens, (tile * ROWS + (int)threadIdx.x) / a.group, span.count, before, seen,
+               a.status);
+    __syncthreads();
+  }
+
   float o[DH / 8][4], m = -INFINITY, big = -INFINITY, l = 0.f;
 #pragma unroll
   for (int d = 0; d < DH / 8; d++)
@@ -341,11 +349,15 @@ next_segment:
     const bool whole = (i + 1) * TILE <= seen_by_all && there == (1 << GROUPS) - 1;
     if (!whole) {
       const int t0 = i * TILE + 2 * t;
+      // (the last tile may be wider than what any row sees)
+      const uint32_t bits = TREE ? (i < before / TILE ? 0xffffffffu : tree[g][i - before / TILE]) >> (2 * t) : 0;
 #pragma unroll
       for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-          if (t0 + n * 8 + k > last || !(there >> (n / PER) & 1)) s[n][k] = -INFINITY;
+        for (int k = 0; k < 2; k++) {
+          const bool hidden = TREE ? !(bits >> (n * 8 + k) & 1) : t0 + n * 8 + k > last;
+          if (hidden || !(there >> (n / PER) & 1)) s[n][k] = -INFINITY;
+        }
     }
     float e[GROUPS], f[GROUPS], m_new = m, big_new = -INFINITY;
 #pragma unroll
@@ -561,12 +573,12 @@ __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const Cac
   a.y[b * a.y_sb + (kvh * a.group + row % a.group) * a.y_sh + token * a.y_st + threadIdx.x] = sum * by;
 }
 
-template <int DH, int GROUPS>
+template <int DH, int GROUPS, bool TREE>
 int launch(wdc_context* ctx, CacheAttArgs& a) {
   static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
   WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "wdc_cache_attention: device index out of range");
   if (!opted_in[ctx->device]) {
-    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_kernel<DH, GROUPS, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Layout<DH>::SMEM));
     opted_in[ctx->device] = true;
   }
@@ -594,7 +606,7 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
     a.part_plan = (int*)(a.part_stats + parts * ROWS * 3);
   }
   WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_cache_attention: batch exceeds the grid");
-  wdc_launch_pdl(ctx, cache_attention_kernel<DH, GROUPS>, dim3((unsigned)ctas), dim3(THREADS), Layout<DH>::SMEM, a);
+  wdc_launch_pdl(ctx, cache_attention_kernel<DH, GROUPS, TREE>, dim3((unsigned)ctas), dim3(THREADS), Layout<DH>::SMEM, a);
   int s = wdc_check_launch(ctx, "cache_attention_kernel");
   if (s == WDC_OK && parts) {
     wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)((int64_t)a.batch * a.heads * a.tokens)), dim3(THREADS), 0, a);
@@ -604,15 +616,13 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
   return s;
 }
 
-}  // namespace
+template <int DH, int GROUPS>
+int launch(wdc_context* ctx, CacheAttArgs& a) {
+  return a.parents ? launch<DH, GROUPS, true>(ctx, a) : launch<DH, GROUPS, false>(ctx, a);
+}
 
-extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
-                                   const float* scales, const int32_t* page_table, const int32_t* lengths,
-                                   const int32_t* counts, float* y) {
-  if (!ctx) return wdc_fail(ctx, WDC_ERR_INVALID, "wdc_cache_attention: null context");
-  WDC_TAPE(ctx, wdc_cache_attention, tape_desc(d), q, codes, scales, page_table, lengths, counts, y);
-  wdc_note_write(ctx, y);
-  WDC_REQUIRE(ctx, d, "wdc_cache_attention: null argument");
+int attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes, const float* scales,
+              const int32_t* page_table, const int32_t* lengths, const int32_t* counts, const int32_t* parents, float* y) {
   CACHE_TRY(cache_check_pool(ctx, "wdc_cache_attention", d->pages, d->kv_heads, d->page_tokens, d->head_size));
   CACHE_TRY(cache_check_batch(ctx, "wdc_cache_attention", d->batch, d->tokens, d->table_pages, d->page_tokens));
   WDC_REQUIRE(ctx, d->heads > 0 && d->heads <= 65535 && d->heads % d->kv_heads == 0,
@@ -623,11 +633,11 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   WDC_REQUIRE(ctx, q && codes && scales && lengths && y && (page_table || d->table_pages == 0),
               "wdc_cache_attention: null argument");
   WDC_REQUIRE(ctx, cache_aligned(q, 16) && cache_aligned(codes, 16) && cache_aligned(y, 16) && cache_aligned(scales, 4) &&
-              cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4),
+              cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4) && cache_aligned(parents, 4),
               "wdc_cache_attention: buffers are not aligned");
   CacheAttArgs a = {};
   a.q = q; a.codes = (const int8_t*)codes; a.scales = scales;
-  a.page_table = page_table; a.lengths = lengths; a.counts = counts;
+  a.page_table = page_table; a.lengths = lengths; a.counts = counts; a.parents = parents;
   a.y = y; a.status = ctx->status_word;
   a.pages = d->pages; a.table_pages = d->table_pages;
   a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
@@ -648,4 +658,28 @@ extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_d
   if (d->head_size == 32) return small ? launch<32, 2>(ctx, a) : launch<32, 1>(ctx, a);
   if (d->head_size == 64) return small ? launch<64, 2>(ctx, a) : launch<64, 1>(ctx, a);
   return small ? launch<128, 2>(ctx, a) : launch<128, 1>(ctx, a);
+}
+
+}  // namespace
+
+extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
+                                   const float* scales, const int32_t* page_table, const int32_t* lengths,
+                                   const int32_t* counts, float* y) {
+  if (!ctx) return wdc_fail(ctx, WDC_ERR_INVALID, "wdc_cache_attention: null context");
+  WDC_TAPE(ctx, wdc_cache_attention, tape_desc(d), q, codes, scales, page_table, lengths, counts, y);
+  wdc_note_write(ctx, y);
+  WDC_REQUIRE(ctx, d, "wdc_cache_attention: null argument");
+  return attention(ctx, d, q, codes, scales, page_table, lengths, counts, nullptr, y);
+}
+
+extern "C" int wdc_cache_attention_tree(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
+                                        const float* scales, const int32_t* page_table, const int32_t* lengths,
+                                        const int32_t* counts, const int32_t* parents, float* y) {
+  if (!ctx) return wdc_fail(ctx, WDC_ERR_INVALID, "wdc_cache_attention_tree: null context");
+  WDC_TAPE(ctx, wdc_cache_attention_tree, tape_desc(d), q, codes, scales, page_table, lengths, counts, parents, y);
+  wdc_note_write(ctx, y);
+  WDC_REQUIRE(ctx, d && (parents || d->batch == 0 || d->tokens == 0), "wdc_cache_attention_tree: null argument");
+  if (d->tokens > TREE_MOST)
+    return wdc_fail(ctx, WDC_ERR_UNSUPPORTED, "wdc_cache_attention_tree: %lld tokens of a tree (up to %d)", (long long)d->tokens, TREE_MOST);
+  return attention(ctx, d, q, codes, scales, page_table, lengths, counts, parents, y);
 }

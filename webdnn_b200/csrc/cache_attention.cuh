@@ -11,6 +11,7 @@ struct CacheAttArgs {
   const int8_t* codes;
   const float* scales;
   const int32_t *page_table, *lengths, *counts;
+  const int32_t* parents;          // of new tokens that are a tree, or null
   float* y;
   int* status;
   int64_t pages, table_pages;
@@ -25,6 +26,22 @@ struct CacheAttArgs {
 
 constexpr float WEIGHT_BITS = 14.f;        // weights are less than 2^15: both halves stay in float16's normal range
 constexpr int QUERY_BITS = 13;             // a row's queries are scaled to less than 2^14
+
+// New tokens that are a tree: token i sees what is before the new ones, its ancestors and itself, as a bit for each place from the last
+// multiple of 32 on that is not behind the first new one.  At most TREE_MOST new tokens.
+constexpr int TREE_MOST = 1024, TREE_WORDS = TREE_MOST / 32 + 1;
+// The row of new token `token` (behind the count: all bits, nobody reads its row), of words up to that of place `end` - 1.
+__device__ __forceinline__ void tree_row(uint32_t* words, const int32_t* parents, int token, int count, int before, int end, int* status) {
+  const int first = before & ~31, n = min((end - first + 31) >> 5, TREE_WORDS);
+  for (int w = 0; w < n; w++) words[w] = token >= count ? 0xffffffffu : w == 0 ? (1u << (before & 31)) - 1 : 0u;
+  for (int i = token; i >= 0 && token < count;) {
+    const int at = (before & 31) + i;
+    words[at >> 5] |= 1u << (at & 31);
+    const int parent = pdl_ld(parents + i);
+    if (parent < -1 || parent >= i) status[WDC_STATUS_DRAFT] = 1;
+    i = parent < i ? parent : -1;
+  }
+}
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // Two halves of a pair: h = x in float16, l = what is missing.

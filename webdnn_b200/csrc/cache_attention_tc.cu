@@ -153,7 +153,9 @@ struct Tile {
   static constexpr int KEYS = 0, VALUES = DH / 64 * K_BLOCK, STAGE = 2 * VALUES;
   static constexpr int Q = STAGES * STAGE, Q_STRIDE = 4 * DH + 16;   // queries on their way: a row's high halves, then the low ones
   static constexpr int OUT_STRIDE = DH + 4;                // floats of a row of the result, over all of this at the end
-  static constexpr int SMEM = Q + BQ * Q_STRIDE + 1024;
+  static constexpr int TREE = Q + BQ * Q_STRIDE;           // the rows' bits, where new tokens are a tree
+  static constexpr int SMEM = TREE + 1024;
+  static constexpr int TREE_SMEM = SMEM + BQ * TREE_WORDS * 4;
   // tensor-memory columns; S and P of two chunks
   static constexpr int Q_HI = 0, Q_LO = DH / 2, S = DH, P = S + 2 * BK, O = P + 2 * BK, COLS = 512;
   static_assert(BQ * OUT_STRIDE * 4 <= SMEM - 1024, "the result's place");
@@ -226,7 +228,7 @@ __device__ __forceinline__ int4 take_tile(const CacheAttArgs& a, int place, int 
   return make_int4(b, __shfl_sync(0xffffffffu, tile, b), __shfl_sync(0xffffffffu, span.length, b), __shfl_sync(0xffffffffu, span.count, b));
 }
 
-template <int DH, bool IN_ORDER>
+template <int DH, bool IN_ORDER, bool TREE>
 __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const CacheAttArgs a) {
   using T = Tile<DH>;
   using Rows = WholeRows<DH>;
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   const int before = span.length - span.count;
   const int first_token = tile * BQ / a.group, top_token = min((tile * BQ + BQ - 1) / a.group, span.count - 1);
   const int seen = first_token < span.count ? before + top_token + 1 : 0;
-  const int seen_by_all = before + first_token + 1;
+  const int seen_by_all = TREE ? before : before + first_token + 1;
   const int chunks = (seen + BK - 1) / BK;
 
   bool ok = true;
@@ -284,6 +286,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     const int in_tile = (int)threadIdx.x % BQ, half = (int)threadIdx.x / BQ;
     const int token = (tile * BQ + in_tile) / a.group;
     const int last = token < span.count ? before + token : 0x7fffffff;
+    uint32_t* const tree = reinterpret_cast<uint32_t*>(stages + T::TREE) + in_tile * TREE_WORDS;   // (33 words: rows meet different banks)
+    if (TREE && !half && chunks > 0) tree_row(tree, pdl_after(a.parents) + (int64_t)b * a.tokens, token, span.count, before, seen, a.status);
     {
       // The tile's queries, whole rows by a warp: scaled by a power of two, in halves, through shared memory to tensor memory.  (A
       // loop that is short in code: what runs once waits for its instructions, about as long as they are.)
@@ -366,6 +370,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
       tmem_loaded();
       const int there = sh.there[st] >> (half * 2), t0 = j * BK + half * 32;
       const bool whole = (j + 1) * BK <= seen_by_all && sh.there[st] == 15;
+      const int word = (t0 >> 5) - (before >> 5);
+      const uint32_t bits = !TREE || whole ? 0 : word < 0 ? 0xffffffffu : word <= (seen - 1 >> 5) - (before >> 5) ? tree[word] : 0;
       float by[2], e[2], f[2], top_s = -INFINITY, top_big = -INFINITY;
 #pragma unroll
       for (int g = 0; g < 2; g++) {
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
         if (!whole) {
 #pragma unroll
           for (int c = g * 16; c < g * 16 + 16; c++)
-            if (t0 + c > last || !(there >> g & 1)) s[c] = -INFINITY;
+            if ((TREE ? !(bits >> c & 1) : t0 + c > last) || !(there >> g & 1)) s[c] = -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
@@ -629,17 +635,22 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   }
 }
 
-template <int DH, bool IN_ORDER>
+template <int DH, bool IN_ORDER, bool TREE>
 int launch(wdc_context* ctx, const CacheAttArgs& a, int64_t ctas) {
+  constexpr int SMEM = TREE ? Tile<DH>::TREE_SMEM : Tile<DH>::SMEM;
   static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
   WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "wdc_cache_attention: device index out of range");
   if (!opted_in[ctx->device]) {
-    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_tc_kernel<DH, IN_ORDER>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<DH>::SMEM));
+    WDC_CUDA(ctx, cudaFuncSetAttribute(cache_attention_tc_kernel<DH, IN_ORDER, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     opted_in[ctx->device] = true;
   }
-  wdc_launch_pdl(ctx, cache_attention_tc_kernel<DH, IN_ORDER>, dim3((unsigned)ctas), dim3(THREADS), Tile<DH>::SMEM, a);
+  wdc_launch_pdl(ctx, cache_attention_tc_kernel<DH, IN_ORDER, TREE>, dim3((unsigned)ctas), dim3(THREADS), SMEM, a);
   ctx->n_tc_launch++;
   return wdc_check_launch(ctx, "cache_attention_tc_kernel");
+}
+template <int DH, bool IN_ORDER>
+int launch(wdc_context* ctx, const CacheAttArgs& a, int64_t ctas) {
+  return a.parents ? launch<DH, IN_ORDER, true>(ctx, a, ctas) : launch<DH, IN_ORDER, false>(ctx, a, ctas);
 }
 
 }  // namespace

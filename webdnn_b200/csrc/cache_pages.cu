@@ -1,9 +1,10 @@
-// Writing to a paged cache in 8 bits: the new tokens' keys and values (wdc_cache_append), and copies of pages
-// (wdc_cache_copy_pages).  Neither has a counterpart in the reference.
+// Writing to a paged cache in 8 bits: the new tokens' keys and values (wdc_cache_append), with the keys' norms and rotations on the way
+// (wdc_cache_append_rotary), and copies of pages (wdc_cache_copy_pages).  None has a counterpart in the reference.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
-#include "paged_cache.cuh"
+#include "head_rotation.cuh"
 
 namespace {
 
@@ -17,6 +18,13 @@ struct AppendArgs {
   int64_t pages, table_pages;
   int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
   int tokens, kv_heads, page_shift, quad_shift;   // 2^page_shift tokens a page, 2^quad_shift float4 a head
+};
+struct RotaryAppendArgs : AppendArgs {
+  HeadRotation rotation;
+  const float *q, *q_weight, *k_weight;
+  float* y;
+  int64_t q_sb, q_sh, q_st, y_sb, y_sh, y_st;
+  int heads, heads_shift;          // of q; 2^heads_shift of them a CTA
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -43,14 +51,70 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
   return pack4(quantise(x.x, scale), quantise(x.y, scale), quantise(x.z, scale), quantise(x.w, scale));
 }
 
+// Normalises and rotates a thread's float4 of `n`: number i is quad i % 2^quad_shift of a head of row row0 + (i >> (quad_shift +
+// heads_shift)) of the call, whose place in its sequence is `start` further on.
+template <int APPEND_THREADS, int HELD>
+__device__ __forceinline__ void rotate_held(const RotaryAppendArgs& a, float4 (&f)[HELD], const float* weights, int n, int row0, int start, int b,
+                                            int quad_shift, int heads_shift) {
+  const HeadRotation& r = a.rotation;
+  const int quad = threadIdx.x & ((1 << quad_shift) - 1);
+  int64_t place[HELD];
+#pragma unroll
+  for (int j = 0; j < HELD; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS, row = row0 + (i >> (quad_shift + heads_shift));
+    place[j] = i >= n || r.half == 0 ? 0 : rotation_place(r, r.positions ? (int64_t)pdl_ld(r.positions + (int64_t)b * a.tokens + row) : start + row, a.status);
+  }
+  const float4 weight = weights ? pdl_ld(reinterpret_cast<const float4*>(weights) + quad) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < HELD; j++)
+    f[j] = rotated_head(r, f[j], quad, 1 << quad_shift, 4 << quad_shift, weights != nullptr, weight, rotation_angles(r, place[j], quad));
+}
+
+// The queries of 2^page_shift rows of the call and 2^heads_shift heads; rows of padding become zero.
+template <int APPEND_THREADS, int HELD>
+__device__ __forceinline__ void append_queries(const RotaryAppendArgs& a, int part, int slot, int b) {
+  const int row0 = slot << a.page_shift, head0 = part << a.heads_shift;
+  if (row0 >= a.tokens) return;
+  const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
+  const int rows = min(a.tokens - row0, 1 << a.page_shift), n = rows << (a.quad_shift + a.heads_shift);
+  const int mine = min(max(span.count - row0, 0), rows) << (a.quad_shift + a.heads_shift);        // that are no padding
+  const int quad = (1 << a.quad_shift) - 1, heads = (1 << a.heads_shift) - 1;
+  const float* q = pdl_after(a.q) + b * a.q_sb + row0 * a.q_st + head0 * a.q_sh;
+  float* y = a.y + b * a.y_sb + row0 * a.y_st + head0 * a.y_sh;
+  float4 f[HELD];
+#pragma unroll
+  for (int j = 0; j < HELD; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS, head = i >> a.quad_shift & heads, row = i >> (a.quad_shift + a.heads_shift);
+    f[j] = i < mine && head0 + head < a.heads ? pdl_ld(reinterpret_cast<const float4*>(q + row * a.q_st + head * a.q_sh) + (i & quad))
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  rotate_held<APPEND_THREADS, HELD>(a, f, a.q_weight, mine, row0, span.length - span.count, b, a.quad_shift, a.heads_shift);
+#pragma unroll
+  for (int j = 0; j < HELD; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS, head = i >> a.quad_shift & heads, row = i >> (a.quad_shift + a.heads_shift);
+    if (i < n && head0 + head < a.heads)
+      *(reinterpret_cast<float4*>(y + row * a.y_st + head * a.y_sh) + (i & quad)) = i < mine ? f[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
 // Absolute values are compared as bits, in which a NaN is above infinity: either one becomes the scale.  The new numbers are read
 // once and wait in registers for their scale, HELD float4 a thread (a whole page).  Bound: for prompts the length of a CTA's
 // dependent loads (9131 tokens of 8 heads of 128: 18.6 us, 4.9 TB/s), as for single tokens (64 x 1: 2.2 us).
-template <int APPEND_THREADS, int HELD>
-__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const AppendArgs a) {
+//
+// With rotations, a head's float4 are those of neighbouring lanes, so that its norm and the other channels of its pairs are a few
+// exchanges away; and further CTAs take the queries of as many tokens as a page has.
+template <int APPEND_THREADS, int HELD, class Args>
+__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Args a) {
+  constexpr bool ROTARY = std::is_same<Args, RotaryAppendArgs>::value;
   pdl_wait();
   const int part = (int)blockIdx.x, slot = (int)blockIdx.y, b = (int)blockIdx.z;
+  if constexpr (ROTARY) {
+    if (part >= 2 * a.kv_heads) {
+      append_queries<APPEND_THREADS, HELD>(a, part - 2 * a.kv_heads, slot, b);
+      return;
+    }
+  }
   const int is_v = part >= a.kv_heads, head = part - is_v * a.kv_heads;
   const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
   if (span.count == 0) return;
@@ -74,6 +138,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Appe
   if (page < 0 || page >= a.pages) {
     a.status[WDC_STATUS_CACHE] = 1;
     return;
+  }
+  if constexpr (ROTARY) {
+    if (!is_v) rotate_held<APPEND_THREADS, HELD>(a, f, a.k_weight, n, lo - start, start, b, a.quad_shift, 0);
   }
   const int64_t block = ((int64_t)page * 2 + is_v) * a.kv_heads + head;
   uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes) + (block << (a.page_shift + a.quad_shift));
@@ -148,6 +215,52 @@ __global__ void __launch_bounds__(COPY_THREADS) cache_copy_kernel(const __grid_c
 
 }  // namespace
 
+// What both kinds of append check and fill in; *slots: pages that a sequence may touch.
+static int append_args(wdc_context* ctx, const char* who, const wdc_cache_append_desc* d, AppendArgs& a, const float* k, const float* v, void* codes,
+                       float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts, int64_t* slots) {
+  CACHE_TRY(cache_check_pool(ctx, who, d->pages, d->kv_heads, d->page_tokens, d->head_size));
+  CACHE_TRY(cache_check_batch(ctx, who, d->batch, d->tokens, d->table_pages, d->page_tokens));
+  const int64_t strides[6] = {d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st};
+  CACHE_TRY(cache_check_strides(ctx, who, strides, 6));
+  *slots = 0;
+  if (d->batch == 0 || d->tokens == 0) return WDC_OK;
+  WDC_REQUIRE(ctx, k && v && codes && scales && lengths && (page_table || d->table_pages == 0), "%s: null argument", who);
+  WDC_REQUIRE(ctx, cache_aligned(k, 16) && cache_aligned(v, 16) && cache_aligned(codes, 16) && cache_aligned(scales, 4) &&
+              cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4),
+              "%s: buffers are not aligned", who);
+  a = {k, v, (int8_t*)codes, scales, page_table, lengths, counts, ctx->status_word, d->pages, d->table_pages,
+       d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st, (int)d->tokens, (int)d->kv_heads, 4, 3};
+  while (1 << a.page_shift < d->page_tokens) a.page_shift++;
+  while (4 << a.quad_shift < d->head_size) a.quad_shift++;
+  *slots = (d->tokens + d->page_tokens - 2) / d->page_tokens + 1;
+  WDC_REQUIRE(ctx, *slots <= 65535 && d->batch <= 65535, "%s: batch exceeds the grid", who);
+  return WDC_OK;
+}
+
+template <class Args>
+static int append_launch(wdc_context* ctx, const wdc_cache_append_desc* d, const Args& args, int64_t slots) {
+  // float4 of a page's new tokens a thread: of all its tokens, or of as many as the call can bring
+  const int64_t most = (d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * d->head_size / 4;
+  DeviceGuard g(ctx->device);
+  const auto launch = [&](auto kernel, int threads, int held) {
+    Args a = args;
+    int64_t parts = 2 * d->kv_heads;
+    if constexpr (std::is_same<Args, RotaryAppendArgs>::value) {
+      while (most << (a.heads_shift + 1) <= threads * held && 1 << a.heads_shift < a.heads) a.heads_shift++;
+      parts += ceil_div64(a.heads, 1 << a.heads_shift);
+    }
+    wdc_launch_pdl(ctx, kernel, dim3((unsigned)parts, (unsigned)slots, (unsigned)d->batch), dim3((unsigned)threads), 0, a);
+  };
+  // (few threads with many loads each on their way, where a page has them: 1024 by 128 threads 16.7 us, by 256 22.0, by 64 18.1; 4096 by
+  // 512 19.9, by 256 21.4; 256 by 64 11.5, by 128 12.0)
+  if (most <= 64) launch(cache_append_kernel<64, 1, Args>, 64, 1);
+  else if (most <= 256) launch(cache_append_kernel<64, 4, Args>, 64, 4);
+  else if (most <= 1024) launch(cache_append_kernel<128, 8, Args>, 128, 8);
+  else if (most <= 2048) launch(cache_append_kernel<256, 8, Args>, 256, 8);
+  else launch(cache_append_kernel<512, 8, Args>, 512, 8);
+  return wdc_check_launch(ctx, "cache_append_kernel");
+}
+
 extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d, const float* k, const float* v, void* codes,
                                 float* scales, const int32_t* page_table, const int32_t* lengths, const int32_t* counts) {
   if (!ctx) return wdc_fail(ctx, WDC_ERR_INVALID, "wdc_cache_append: null context");
@@ -155,35 +268,38 @@ extern "C" int wdc_cache_append(wdc_context* ctx, const wdc_cache_append_desc* d
   wdc_note_write(ctx, codes);
   wdc_note_write(ctx, scales);
   WDC_REQUIRE(ctx, d, "wdc_cache_append: null argument");
-  CACHE_TRY(cache_check_pool(ctx, "wdc_cache_append", d->pages, d->kv_heads, d->page_tokens, d->head_size));
-  CACHE_TRY(cache_check_batch(ctx, "wdc_cache_append", d->batch, d->tokens, d->table_pages, d->page_tokens));
-  const int64_t strides[6] = {d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st};
-  CACHE_TRY(cache_check_strides(ctx, "wdc_cache_append", strides, 6));
-  if (d->batch == 0 || d->tokens == 0) return WDC_OK;
-  WDC_REQUIRE(ctx, k && v && codes && scales && lengths && (page_table || d->table_pages == 0), "wdc_cache_append: null argument");
-  WDC_REQUIRE(ctx, cache_aligned(k, 16) && cache_aligned(v, 16) && cache_aligned(codes, 16) && cache_aligned(scales, 4) &&
-              cache_aligned(page_table, 4) && cache_aligned(lengths, 4) && cache_aligned(counts, 4),
-              "wdc_cache_append: buffers are not aligned");
-  AppendArgs a = {k, v, (int8_t*)codes, scales, page_table, lengths, counts, ctx->status_word, d->pages, d->table_pages,
-                  d->k_sb, d->k_sh, d->k_st, d->v_sb, d->v_sh, d->v_st, (int)d->tokens, (int)d->kv_heads, 4, 3};
-  while (1 << a.page_shift < d->page_tokens) a.page_shift++;
-  while (4 << a.quad_shift < d->head_size) a.quad_shift++;
-  const int64_t slots = (d->tokens + d->page_tokens - 2) / d->page_tokens + 1;   // pages that a sequence may touch
-  WDC_REQUIRE(ctx, slots <= 65535 && d->batch <= 65535, "wdc_cache_append: batch exceeds the grid");
-  // float4 of a page's new tokens a thread: of all its tokens, or of as many as the call can bring
-  const int64_t most = (d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * d->head_size / 4;
-  DeviceGuard g(ctx->device);
-  const auto launch = [&](auto kernel, int threads) {
-    wdc_launch_pdl(ctx, kernel, dim3((unsigned)(2 * d->kv_heads), (unsigned)slots, (unsigned)d->batch), dim3((unsigned)threads), 0, a);
-  };
-  // (few threads with many loads each on their way, where a page has them: 1024 by 128 threads 16.7 us, by 256 22.0, by 64 18.1; 4096 by
-  // 512 19.9, by 256 21.4; 256 by 64 11.5, by 128 12.0)
-  if (most <= 64) launch(cache_append_kernel<64, 1>, 64);
-  else if (most <= 256) launch(cache_append_kernel<64, 4>, 64);
-  else if (most <= 1024) launch(cache_append_kernel<128, 8>, 128);
-  else if (most <= 2048) launch(cache_append_kernel<256, 8>, 256);
-  else launch(cache_append_kernel<512, 8>, 512);
-  return wdc_check_launch(ctx, "cache_append_kernel");
+  AppendArgs a;
+  int64_t slots = 0;
+  CACHE_TRY(append_args(ctx, "wdc_cache_append", d, a, k, v, codes, scales, page_table, lengths, counts, &slots));
+  return slots ? append_launch(ctx, d, a, slots) : WDC_OK;
+}
+
+extern "C" int wdc_cache_append_rotary(wdc_context* ctx, const wdc_cache_append_rotary_desc* d, const float* q, const float* k,
+                                       const float* v, const float* q_weight, const float* k_weight, const float* cos,
+                                       const float* sin, const int32_t* positions, void* codes, float* scales,
+                                       const int32_t* page_table, const int32_t* lengths, const int32_t* counts, float* q_out) {
+  if (!ctx) return wdc_fail(ctx, WDC_ERR_INVALID, "wdc_cache_append_rotary: null context");
+  WDC_TAPE(ctx, wdc_cache_append_rotary, tape_desc(d), q, k, v, q_weight, k_weight, cos, sin, positions, codes, scales, page_table,
+           lengths, counts, q_out);
+  wdc_note_write(ctx, codes);
+  wdc_note_write(ctx, scales);
+  wdc_note_write(ctx, q_out);
+  const char* who = "wdc_cache_append_rotary";
+  WDC_REQUIRE(ctx, d, "%s: null argument", who);
+  RotaryAppendArgs a = {};
+  int64_t slots = 0;
+  CACHE_TRY(append_args(ctx, who, &d->append, a, k, v, codes, scales, page_table, lengths, counts, &slots));
+  CACHE_TRY(rotation_check(ctx, who, a.rotation, d->append.head_size, d->rotary, d->places, cos, sin, positions, d->epsilon, d->interleaved));
+  const int64_t strides[6] = {d->q_sb, d->q_sh, d->q_st, d->y_sb, d->y_sh, d->y_st};
+  CACHE_TRY(cache_check_strides(ctx, who, strides, 6));
+  WDC_REQUIRE(ctx, d->heads >= 0 && d->heads <= 65535 && !q == !q_out && (q || d->heads == 0 || !slots), "%s: bad queries", who);
+  WDC_REQUIRE(ctx, cache_aligned(q, 16) && cache_aligned(q_out, 16) && cache_aligned(q_weight, 16) && cache_aligned(k_weight, 16),
+              "%s: buffers are not aligned", who);
+  a.q = q; a.y = q_out; a.q_weight = q_weight; a.k_weight = k_weight;
+  a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
+  a.y_sb = d->y_sb; a.y_sh = d->y_sh; a.y_st = d->y_st;
+  a.heads = q ? (int)d->heads : 0;
+  return slots ? append_launch(ctx, &d->append, a, slots) : WDC_OK;
 }
 
 extern "C" int wdc_cache_copy_pages(wdc_context* ctx, const wdc_cache_pages_desc* d, void* codes, float* scales, int64_t n,

@@ -84,6 +84,8 @@ struct wdc_context {
 
 // The word behind status_word's first that the kernels over a paged cache set when they leave something out.
 constexpr int WDC_STATUS_CACHE = 1;
+// The one behind it: positions, parents and paths of drafted tokens.
+constexpr int WDC_STATUS_DRAFT = 2;
 
 int wdc_fail(wdc_context* ctx, int code, const char* fmt, ...);
 int wdc_check_cuda(wdc_context* ctx, cudaError_t e, const char* what);

@@ -484,6 +484,10 @@ static int report_device_status(wdc_context* ctx) {
     word[WDC_STATUS_CACHE] = 0;
     return wdc_fail(ctx, WDC_ERR_INVALID, "a cache call was given a length, count or page out of range; that part was left out");
   }
+  if (word[WDC_STATUS_DRAFT] != 0) {
+    word[WDC_STATUS_DRAFT] = 0;
+    return wdc_fail(ctx, WDC_ERR_INVALID, "a call on drafted tokens was given a position, parent, path or count out of range");
+  }
   return WDC_OK;
 }
 

@@ -76,6 +76,25 @@ class CachePagesDesc(Structure):
     _fields_ = [(n, c_int64) for n in ("layers", "pages", "kv_heads", "page_tokens", "head_size")]
 
 
+class CacheAppendRotaryDesc(Structure):
+    _fields_ = ([("append", CacheAppendDesc)] + [(n, c_int64) for n in ("heads", "q_sb", "q_sh", "q_st", "y_sb", "y_sh", "y_st", "rotary", "places")]
+                + [("epsilon", c_float), ("interleaved", c_int32)])
+
+
+class CacheKeepDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("layers", "pages", "kv_heads", "page_tokens", "head_size", "batch", "tokens", "table_pages")]
+
+
+class RotateDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("rows", "heads", "head_size", "rotary", "places", "x_st", "x_sh", "y_st", "y_sh")] + [
+        ("epsilon", c_float), ("interleaved", c_int32)]
+
+
+class VerifyDesc(Structure):
+    _fields_ = [(n, c_int64) for n in ("batch", "tokens", "vocab", "logits_sb", "logits_st", "draft_sb", "draft_st")] + [
+        ("temperature", c_float), ("draft_temperature", c_float)]
+
+
 class LogprobsDesc(Structure):
     _fields_ = [(n, c_int64) for n in ("rows", "vocab", "row_stride", "top")]
 
@@ -108,6 +127,11 @@ SIGNATURES = {
     "wdc_cache_append": (c_int, [c_void_p, POINTER(CacheAppendDesc)] + [c_void_p] * 7),
     "wdc_cache_attention": (c_int, [c_void_p, POINTER(CacheAttentionDesc)] + [c_void_p] * 7),
     "wdc_cache_copy_pages": (c_int, [c_void_p, POINTER(CachePagesDesc), c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "wdc_rotate_heads": (c_int, [c_void_p, POINTER(RotateDesc)] + [c_void_p] * 6),
+    "wdc_cache_append_rotary": (c_int, [c_void_p, POINTER(CacheAppendRotaryDesc)] + [c_void_p] * 14),
+    "wdc_cache_attention_tree": (c_int, [c_void_p, POINTER(CacheAttentionDesc)] + [c_void_p] * 8),
+    "wdc_cache_keep_paths": (c_int, [c_void_p, POINTER(CacheKeepDesc)] + [c_void_p] * 7),
+    "wdc_verify_drafts": (c_int, [c_void_p, POINTER(VerifyDesc)] + [c_void_p] * 9),
     "wdc_token_logprobs": (c_int, [c_void_p, POINTER(LogprobsDesc)] + [c_void_p] * 6),
     "wdc_decode_eightbit": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_float]),
     "wdc_capture_begin": (c_int, [c_void_p]),

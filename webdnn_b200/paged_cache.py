@@ -5,7 +5,8 @@ its inputs bring along.  ``PagedCache`` is the state that such a graph needs: th
 to an int32 word, and a float32 scale for each page, head and side), and on the host which pages belong to which
 sequence.
 
-* device: ``append`` writes new tokens, ``attention`` lets them attend to their sequences, ``copy_pages`` moves pages.  They
+* device: ``append`` writes new tokens (``append_rotary`` with their keys and queries normalised and rotated), ``attention`` lets
+  them attend to their sequences, ``keep_paths`` moves those of a tree that stand to its front, ``copy_pages`` moves pages.  They
   take the page table, lengths and counts as int32 tensors, so a recorded run (tape or graph) repeats with new ones; the pool
   stays where it is.
 * host: sequences are numbers.  ``extend`` gives one room for new tokens, ``fork`` shares its pages with a new one, ``release``
@@ -24,7 +25,7 @@ from typing import Dict, List, Optional, Sequence
 import numpy as np
 
 from .backend import CPUTensor, CudaTensor, WebDNNCudaContext
-from .lib import CacheAppendDesc, CacheAttentionDesc, CachePagesDesc
+from .lib import CacheAppendDesc, CacheAppendRotaryDesc, CacheAttentionDesc, CacheKeepDesc, CachePagesDesc
 
 
 class PagedCache:
@@ -95,10 +96,14 @@ class PagedCache:
             if t.ndim != 3 or t.dims[:2] != rows[0].dims[:2]:
                 raise ValueError(f"{who}: operands are [batch, tokens, width]")
         batch = rows[0].dims[0]
+        PagedCache._batch_ints(who, batch, page_table, lengths, counts)
+        return batch, rows[0].dims[1]
+
+    @staticmethod
+    def _batch_ints(who: str, batch: int, page_table: CudaTensor, lengths: CudaTensor, counts: Optional[CudaTensor]) -> None:
         if page_table.ndim != 2 or page_table.dims[0] != batch or lengths.dims != [batch] or (
                 counts is not None and counts.dims != [batch]):
             raise ValueError(f"{who}: page_table is [{batch}, pages], lengths and counts are [{batch}]")
-        return batch, rows[0].dims[1]
 
     def append(self, layer: int, k: CudaTensor, v: CudaTensor, page_table: CudaTensor, lengths: CudaTensor,
                counts: Optional[CudaTensor] = None, k_column: int = 0, v_column: int = 0) -> None:
@@ -114,23 +119,84 @@ class PagedCache:
                                page_table.ptr, lengths.ptr, counts.ptr if counts is not None else None)
 
     def _append_desc(self, key, k, v, page_table, lengths, counts, k_column, v_column):
-        batch, tokens = self._batch("PagedCache.append", (k, v), page_table, lengths, counts)
+        return self._keep(key, self._append_fields("PagedCache.append", k, v, page_table, lengths, counts, k_column, v_column))
+
+    def _append_fields(self, who, k, v, page_table, lengths, counts, k_column, v_column):
+        batch, tokens = self._batch(who, (k, v), page_table, lengths, counts)
         width = self.kv_heads * self.head_size
         for t, c in ((k, k_column), (v, v_column)):
             if c < 0 or c % 4 or c + width > t.dims[2] or t.dims[2] % 4:
-                raise ValueError(f"PagedCache.append: {width} columns from {c} on, of {t.dims[2]} (multiples of 4)")
+                raise ValueError(f"{who}: {width} columns from {c} on, of {t.dims[2]} (multiples of 4)")
         kw, vw, c = k.dims[2], v.dims[2], self.head_size
-        return self._keep(key, CacheAppendDesc(self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1],
-                                               tokens * kw, c, kw, tokens * vw, c, vw))
+        return CacheAppendDesc(self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1],
+                               tokens * kw, c, kw, tokens * vw, c, vw)
+
+    def append_rotary(self, layer: int, k: CudaTensor, v: CudaTensor, page_table: CudaTensor, lengths: CudaTensor,
+                      counts: Optional[CudaTensor] = None, cos: Optional[CudaTensor] = None, sin: Optional[CudaTensor] = None,
+                      positions: Optional[CudaTensor] = None, q: Optional[CudaTensor] = None, heads: Optional[int] = None,
+                      q_weight: Optional[CudaTensor] = None, k_weight: Optional[CudaTensor] = None, epsilon: float = 1e-6,
+                      interleaved: bool = False, q_column: int = 0, k_column: int = 0, v_column: int = 0,
+                      out: Optional[CudaTensor] = None) -> Optional[CudaTensor]:
+        """``append`` of keys whose heads are normalised (``k_weight``) and rotated (``cos``, ``sin``) on the way, like
+        ``WebDNNCudaContext.rotate_heads`` (``wdc_cache_append_rotary``).  ``positions``: int32 [batch, tokens], without: a token's
+        place in its sequence.  With ``q``, whose ``heads`` * head_size columns from ``q_column`` on count, its heads are too
+        (``q_weight``); the result is [batch, tokens, heads * head_size], rows of padding 0."""
+        who = "PagedCache.append_rotary"
+        rows = (k, v) if q is None else (k, v, q)
+        self._operands(who, rows, page_table, lengths, counts)
+        extra = (cos, sin, positions, q_weight, k_weight)
+        dims = tuple(tuple(t.dims) if t is not None else None for t in (k, v, q, page_table, lengths, counts, *extra))
+        key = ("append_rotary", dims, heads, epsilon, bool(interleaved), q_column, k_column, v_column)
+        self.context.asserts_rotation(who, self.head_size, cos, sin, positions, (q_weight, k_weight))
+        kept = self._descs.get(key) or self._append_rotary_desc(who, key, k, v, page_table, lengths, counts, cos, positions, q, heads,
+                                                                q_weight, epsilon, interleaved, q_column, k_column, v_column, out)
+        d = kept[1]
+        if q is not None:
+            shape = [d.append.batch, d.append.tokens, d.heads * self.head_size]
+            if out is None:
+                out = self.context.empty_tensor(shape)
+            elif out.__class__ is not CudaTensor or out.context is not self.context or out.dims != shape or out.data_type != "float32" or (
+                    out.layout != "nchw" or (out.ptr == q.ptr and (q_column or out.dims != q.dims))):
+                raise ValueError(f"{who}: the result is float32 {shape}, row-major, in this context, and q only where that has its shape")
+        if k.length and v.length:
+            at = lambda t, column=0: t.ptr + 4 * column if t is not None else None  # noqa: E731
+            self.context._call("wdc_cache_append_rotary", kept[0], at(q, q_column), at(k, k_column), at(v, v_column), at(q_weight), at(k_weight),
+                               at(cos), at(sin), at(positions), *self._at(layer), page_table.ptr, lengths.ptr, at(counts), at(out))
+        return out
+
+    def _append_rotary_desc(self, who, key, k, v, page_table, lengths, counts, cos, positions, q, heads, q_weight, epsilon,
+                            interleaved, q_column, k_column, v_column, out):
+        fields = self._append_fields(who, k, v, page_table, lengths, counts, k_column, v_column)
+        c, batch, tokens = self.head_size, fields.batch, fields.tokens
+        if positions is not None and positions.dims != [batch, tokens]:
+            raise ValueError(f"{who}: positions are [{batch}, {tokens}]")
+        if q is None:
+            if heads or q_column or out is not None or q_weight is not None:
+                raise ValueError(f"{who}: heads, q_column, q_weight and out are of queries")
+            heads = width = 0
+        else:
+            width = q.dims[2] if q.ndim == 3 else 0
+            heads = (width - q_column) // c if heads is None else heads
+            if q.ndim != 3 or q.dims[:2] != [batch, tokens] or heads < 1 or q_column < 0 or q_column % 4 or q_column + heads * c > width or width % 4:
+                raise ValueError(f"{who}: {heads} heads of {c} from column {q_column} on, of {q.dims}")
+        row = heads * c
+        return self._keep(key, CacheAppendRotaryDesc(fields, heads, tokens * width, c, width, tokens * row, c, row,
+                                                     2 * cos.dims[1] if cos is not None else 0, cos.dims[0] if cos is not None else 0,
+                                                     epsilon, interleaved))
 
     def attention(self, layer: int, q: CudaTensor, page_table: CudaTensor, lengths: CudaTensor,
                   counts: Optional[CudaTensor] = None, heads: Optional[int] = None, q_column: int = 0,
-                  scale: Optional[float] = None, out: Optional[CudaTensor] = None) -> CudaTensor:
+                  scale: Optional[float] = None, out: Optional[CudaTensor] = None,
+                  parents: Optional[CudaTensor] = None) -> CudaTensor:
         """Attention of the new tokens over their sequences, themselves and what is before them (``wdc_cache_attention``), after
         ``append``.  q: [batch, tokens, width], of which ``heads`` * head_size columns from ``q_column`` on count (without
         ``heads``: all from there on); the result is [batch, tokens, heads * head_size], rows of padding 0.  ``scale``:
-        1 / sqrt(head_size) unless given."""
+        1 / sqrt(head_size) unless given.  ``parents``: int32 [batch, tokens], the new tokens are a tree
+        (``wdc_cache_attention_tree``): which of the new ones, before it, each continues, -1: the text before them; a token then
+        sees that text, its ancestors and itself."""
         self._operands("PagedCache.attention", (q,), page_table, lengths, counts)
+        if parents is not None:
+            self.context.asserts_int_rows("PagedCache.attention", "parents", parents, q.dims[:2])
         key = (*map(tuple, (q.dims, page_table.dims, lengths.dims)), counts is not None and tuple(counts.dims), heads, q_column, scale)
         kept = self._descs.get(key) or self._attention_desc(key, q, page_table, lengths, counts, heads, q_column, scale)
         d = kept[1]
@@ -140,8 +206,9 @@ class PagedCache:
         elif out.__class__ is not CudaTensor or out.context is not self.context or out.dims != dims or out.data_type != "float32":
             raise ValueError(f"PagedCache.attention: the result is float32 {dims} of this context")
         if out.length:
-            self.context._call("wdc_cache_attention", kept[0], q.ptr + 4 * q_column, *self._at(layer), page_table.ptr, lengths.ptr,
-                               counts.ptr if counts is not None else None, out.ptr)
+            tree = () if parents is None else (parents.ptr,)
+            self.context._call("wdc_cache_attention_tree" if tree else "wdc_cache_attention", kept[0], q.ptr + 4 * q_column, *self._at(layer),
+                               page_table.ptr, lengths.ptr, counts.ptr if counts is not None else None, *tree, out.ptr)
         return out
 
     def _attention_desc(self, key, q, page_table, lengths, counts, heads, q_column, scale):
@@ -155,6 +222,25 @@ class PagedCache:
         return self._keep(key, CacheAttentionDesc(self.pages, self.kv_heads, self.page_tokens, c, batch, tokens, page_table.dims[1],
                                                   heads, tokens * width, c, width, tokens * row, c, row,
                                                   c ** -0.5 if scale is None else scale))
+
+    def keep_paths(self, page_table: CudaTensor, lengths: CudaTensor, counts: Optional[CudaTensor], path: CudaTensor,
+                   accepted: CudaTensor) -> None:
+        """Moves the new tokens that stand to the front of their sequences' new ones, in every layer (``wdc_cache_keep_paths``): ``path``
+        int32 [batch, tokens] and ``accepted`` int32 [batch] as ``WebDNNCudaContext.verify_drafts`` gives them; the other operands are
+        those of the step.  ``truncate`` then takes the sequences to length - count + accepted."""
+        self._operands("PagedCache.keep_paths", (), page_table, lengths, counts)
+        if path.ndim != 2:
+            raise ValueError("PagedCache.keep_paths: path is [batch, tokens]")
+        batch, tokens = path.dims
+        self.context.asserts_int_rows("PagedCache.keep_paths", "path", path, [batch, tokens])
+        self.context.asserts_int_rows("PagedCache.keep_paths", "accepted", accepted, [batch])
+        self._batch_ints("PagedCache.keep_paths", batch, page_table, lengths, counts)
+        key = ("keep", batch, tokens, page_table.dims[1])
+        kept = self._descs.get(key) or self._keep(key, CacheKeepDesc(self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_size,
+                                                                     batch, tokens, page_table.dims[1]))
+        if path.length:
+            self.context._call("wdc_cache_keep_paths", kept[0], self.codes.ptr, self.scales.ptr, page_table.ptr, lengths.ptr,
+                               counts.ptr if counts is not None else None, path.ptr, accepted.ptr)
 
     def copy_pages(self, sources: Sequence[int], targets: Sequence[int]) -> None:
         """Page sources[i] to page targets[i], in every layer (``wdc_cache_copy_pages``)."""
