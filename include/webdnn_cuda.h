@@ -394,7 +394,8 @@ int wdc_cache_copy_pages(wdc_context* ctx, const wdc_cache_pages_desc* d, void* 
  *   pairs (a, b) of the first `rotary` channels become a cos - b sin, b cos + a sin; they are channels i and i + rotary / 2, or
  *   with `interleaved` 2 i and 2 i + 1; cos and sin are [places][rotary / 2], of which the row's position names one (positions
  *   NULL: the row's number).  A position out of range counts as the nearest one.
- * Computed in 64 bits and rounded once.  y may be x (with the same strides); otherwise they do not overlap.
+ * Computed in 32 bits: a result is within 2^-20 (|a| + |b|) of it, or 2^-20 |n|; the squares of large or tiny numbers neither
+ * overflow nor vanish.  y may be x (with the same strides); otherwise they do not overlap.
  * head_size is a multiple of 4 up to 256, rotary a multiple of 8 up to head_size, 0: none (else WDC_ERR_UNSUPPORTED). */
 typedef struct wdc_rotate_desc {
   int64_t rows, heads, head_size, rotary, places;
@@ -405,8 +406,8 @@ typedef struct wdc_rotate_desc {
 int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, const float* x, const float* weight, const float* cos,
                      const float* sin, const int32_t* positions, float* y);
 
-/* wdc_cache_append of keys that are normalised and rotated like wdc_rotate_heads' on the way; where q is given, its heads are as well,
- * into q_out (rows of padding become zero).  Nothing of q is written unless q_out is q (with the same strides); otherwise they do not
+/* wdc_cache_append of keys that are normalised and rotated like wdc_rotate_heads' on the way, but in 64 bits and rounded once (their codes
+ * hang on the last bit); where q is given, its heads are as wdc_rotate_heads' are, into q_out (rows of padding become zero).  Nothing of q is written unless q_out is q (with the same strides); otherwise they do not
  * overlap.  positions is int32 [batch][tokens] or NULL (a token's place in its sequence); one out of range counts as the nearest one. */
 typedef struct wdc_cache_append_rotary_desc {
   wdc_cache_append_desc append;

@@ -1,9 +1,10 @@
 """The operators of a decoder that drafts on the GPU, against their definitions in 64 bits.
 
 Tolerances, from the arithmetic that the operators promise:
-* heads are computed in 64 bits and rounded once: half a step of float32, 2^-24 of the value, and 2^-48 of the head's largest number
-  for the roundings of 64 bits;
-* codes of rotated keys and kept paths are whole numbers, verdicts are decisions: equal;
+* heads: a mean of at most 256 squares, 13 additions one after the other and a product, is (14 + 1) * 2^-24 off, its root half of that;
+  rsqrtf 3 * 2^-24, two products with it and the weight 2, a rotation's products and sum 2 more: less than 15 * 2^-24 of |n1| + |n2|,
+  which is less than 2^-20 of it;
+* rotated keys are computed in 64 bits and rounded once, so codes of rotated keys and kept paths are whole numbers, verdicts are decisions: equal;
 * attention of a tree: as that of a text (test_gpu_paged_cache).
 """
 import numpy as np
@@ -35,8 +36,12 @@ def rotated(x, weight, cos, sin, epsilon, interleaved):
     return y
 
 
-def assert_rounded_once(got, want):
-    room = 2.0 ** -24 * (1 + 2.0 ** -20) * np.abs(want) + 2.0 ** -48 * np.abs(want).max(-1, keepdims=True) + 2.0 ** -149
+def assert_heads(got, x, weight, cos, sin, epsilon, interleaved):
+    """``got`` is rotated(...), within 2^-20 of the magnitudes that a number is the sum of."""
+    want = rotated(x, weight, cos, sin, epsilon, interleaved)
+    parts = rotated(np.abs(x), None if weight is None else np.abs(weight), np.abs(cos), -np.abs(sin), epsilon, interleaved)
+    other = rotated(np.abs(x), None if weight is None else np.abs(weight), np.abs(cos), np.abs(sin), epsilon, interleaved)
+    room = 2.0 ** -20 * np.maximum(np.abs(parts), np.abs(other)) + 2.0 ** -148
     assert (np.abs(got.astype(np.float64) - want) <= room).all()
 
 
@@ -64,8 +69,7 @@ def test_heads(cuda_context, rows, heads, c, pairs, interleaved, norm):
     ts = [dev(ctx, a) if a is not None else None for a in (x, weight, cos if pairs else None, sin if pairs else None, positions if pairs else None)]
     y = ctx.rotate_heads(ts[0], heads, c, cos=ts[2], sin=ts[3], positions=ts[4], weight=ts[1], epsilon=1e-5, interleaved=interleaved, column=column)
     got = y.get_data().reshape(rows, heads, c)
-    want = rotated(x[:, column:column + heads * c].reshape(rows, heads, c), weight, cos[positions], sin[positions], 1e-5, interleaved)
-    assert_rounded_once(got, want)
+    assert_heads(got, x[:, column:column + heads * c].reshape(rows, heads, c), weight, cos[positions], sin[positions], 1e-5, interleaved)
     ctx.sync()
     dispose(y, *ts)
 
@@ -78,13 +82,12 @@ def test_heads_in_place_and_rows_numbered(cuda_context):
         t, tc, ts, w = dev(ctx, x), dev(ctx, cos), dev(ctx, sin), dev(ctx, np.ones(c, f32))
         y = ctx.rotate_heads(t, 3, c, cos=tc, sin=ts, weight=w, epsilon=0.0, out=t)
         assert y is t and y.dims == [2, 50, 3 * c]
-        want = rotated(x.reshape(100, 3, c), np.ones(c, f32), cos, sin, 0.0, False)
-        assert_rounded_once(y.get_data().reshape(100, 3, c), want)
+        assert_heads(y.get_data().reshape(100, 3, c), x.reshape(100, 3, c), np.ones(c, f32), cos, sin, 0.0, False)
         dispose(t, tc, ts, w)
 
 
 def test_heads_of_any_magnitude(cuda_context):
-    """The square of a float32 number does not overflow 64 bits; a head of zeros stays zero; a NaN is its head's alone."""
+    """Squares of large or tiny numbers neither overflow nor vanish; a head of zeros stays zero; a NaN is its head's alone."""
     ctx = cuda_context
     x = np.ones((5, 2, 32), f32)
     x[0] *= f32(3e38)
@@ -95,7 +98,10 @@ def test_heads_of_any_magnitude(cuda_context):
     y = ctx.rotate_heads(t, 2, 32, weight=w, epsilon=1e-6)
     got = y.get_data().reshape(x.shape)
     assert np.allclose(got[0], 2, rtol=2.0 ** -22) and np.array_equal(got[2], np.zeros((2, 32), f32))
-    assert_rounded_once(got[1], rotated(x[1], np.full(32, 2, f32), np.zeros(0), np.zeros(0), 1e-6, False))
+    assert_heads(got[1], x[1], np.full(32, 2, f32), np.zeros(0), np.zeros(0), 1e-6, False)
+    y.dispose()
+    y = ctx.rotate_heads(t, 2, 32, weight=w, epsilon=0.0)
+    assert np.allclose(y.get_data().reshape(x.shape)[:2], 2, rtol=2.0 ** -20)
     assert np.isnan(got[3, 1]).all() and not np.isnan(got[3, 0]).any() and not np.isnan(got[4]).any()
     dispose(t, w, y)
 
@@ -110,7 +116,7 @@ def test_positions_out_of_range_count_as_the_nearest_and_are_reported(cuda_conte
         ctx.sync()
     ctx.sync()
     at = [0, 9, 3]
-    assert_rounded_once(y.get_data().reshape(3, 1, 64), rotated(x.reshape(3, 1, 64), None, cos[at], sin[at], 0, False))
+    assert_heads(y.get_data().reshape(3, 1, 64), x.reshape(3, 1, 64), None, cos[at], sin[at], 0, False)
     dispose(t, tc, ts, p, y)
 
 
@@ -141,9 +147,9 @@ def test_append_of_rotated_keys(cuda_context, size, c, heads, kv_heads, lengths,
                                 epsilon=1e-6, interleaved=interleaved, k_column=4, q_column=8 if heads else 0)
         if heads:
             there = np.arange(tokens) < np.array(counts)[:, None]
-            want = rotated(q, qw if norm else None, cos[positions], sin[positions], 1e-6, interleaved) * there[..., None, None]
             got = y.get_data().reshape(q.shape)
-            assert_rounded_once(got, want)
+            assert not got[~there].any()
+            assert_heads(got[there], q[there], qw if norm else None, cos[positions][there], sin[positions][there], 1e-6, interleaved)
             y.dispose()
         else:
             assert y is None

@@ -24,7 +24,7 @@ struct RotaryAppendArgs : AppendArgs {
   const float *q, *q_weight, *k_weight;
   float* y;
   int64_t q_sb, q_sh, q_st, y_sb, y_sh, y_st;
-  int heads, heads_shift;          // of q; 2^heads_shift of them a CTA
+  int heads, chunks;               // of q, and groups that take a row of them
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -51,50 +51,54 @@ __device__ __forceinline__ uint32_t quantise4(float4 x, float scale, float inver
   return pack4(quantise(x.x, scale), quantise(x.y, scale), quantise(x.z, scale), quantise(x.w, scale));
 }
 
-// Normalises and rotates a thread's float4 of `n`: number i is quad i % 2^quad_shift of a head of row row0 + (i >> (quad_shift +
-// heads_shift)) of the call, whose place in its sequence is `start` further on.
+// Normalises and rotates the keys that a thread holds, in 64 bits: f[j] and f[j + 1] are the two float4 of a slot of a head.  Slot number
+// i = threadIdx.x + j / 2 * APPEND_THREADS of `n` is slot i % 2^(quad_shift - 1) of the head of new token row0 + (i >> (quad_shift - 1)),
+// whose place in its sequence is `start` further on.
 template <int APPEND_THREADS, int HELD>
-__device__ __forceinline__ void rotate_held(const RotaryAppendArgs& a, float4 (&f)[HELD], const float* weights, int n, int row0, int start, int b,
-                                            int quad_shift, int heads_shift) {
+__device__ __forceinline__ void rotate_keys(const RotaryAppendArgs& a, float4 (&f)[HELD], int n, int row0, int start, int b) {
   const HeadRotation& r = a.rotation;
-  const int quad = threadIdx.x & ((1 << quad_shift) - 1);
-  int64_t place[HELD];
+  const int shift = a.quad_shift - 1, p = threadIdx.x & ((1 << shift) - 1);
+  const Slot slot(r, p);
+  int64_t position[HELD / 2];
 #pragma unroll
-  for (int j = 0; j < HELD; j++) {
-    const int i = threadIdx.x + j * APPEND_THREADS, row = row0 + (i >> (quad_shift + heads_shift));
-    place[j] = i >= n || r.half == 0 ? 0 : rotation_place(r, r.positions ? (int64_t)pdl_ld(r.positions + (int64_t)b * a.tokens + row) : start + row, a.status);
+  for (int j = 0; j < HELD / 2; j++) {
+    const int i = threadIdx.x + j * APPEND_THREADS, row = row0 + (i >> shift);
+    position[j] = i >= n || r.half == 0 ? 0 : r.positions ? (int64_t)pdl_ld(r.positions + (int64_t)b * a.tokens + row) : start + row;
   }
-  const float4 weight = weights ? pdl_ld(reinterpret_cast<const float4*>(weights) + quad) : make_float4(0.f, 0.f, 0.f, 0.f);
+  Quad<double> wa[1] = {}, wb[1] = {};
+  if (a.k_weight) {
+    wa[0] = quad_of<double>(pdl_ld(reinterpret_cast<const float4*>(a.k_weight) + slot.a));
+    wb[0] = quad_of<double>(pdl_ld(reinterpret_cast<const float4*>(a.k_weight) + slot.b));
+  }
 #pragma unroll
-  for (int j = 0; j < HELD; j++)
-    f[j] = rotated_head(r, f[j], quad, 1 << quad_shift, 4 << quad_shift, weights != nullptr, weight, rotation_angles(r, place[j], quad));
+  for (int j = 0; j < HELD / 2; j++) {
+    if (j * APPEND_THREADS >= n) break;            // (nobody has any)
+    Quad<double> na[1] = {quad_of<double>(f[2 * j])}, nb[1] = {quad_of<double>(f[2 * j + 1])};
+    if (a.k_weight) normalise(r, na, nb, 1 << shift, wa, wb);
+    if (slot.turns) rotate_slot(r, na[0], nb[0], rotation_angles<double>(r, rotation_place(r, position[j], a.status), p));
+    f[2 * j] = rounded(na[0]);
+    f[2 * j + 1] = rounded(nb[0]);
+  }
 }
 
-// The queries of 2^page_shift rows of the call and 2^heads_shift heads; rows of padding become zero.
-template <int APPEND_THREADS, int HELD>
+// Queries: a group of 2^(quad_shift - 1) lanes takes EACH heads of a row, of the call's rows with number slot * 2^page_shift and up; rows
+// of padding become zero.
+template <int EACH>
 __device__ __forceinline__ void append_queries(const RotaryAppendArgs& a, int part, int slot, int b) {
-  const int row0 = slot << a.page_shift, head0 = part << a.heads_shift;
-  if (row0 >= a.tokens) return;
+  const int shift = a.quad_shift - 1, lanes = 1 << shift;
+  const int row0 = slot << a.page_shift, rows = min(a.tokens - row0, 1 << a.page_shift);
+  const int item = (part * (int)blockDim.x + (int)threadIdx.x) >> shift, in_slot = item / a.chunks;
+  const bool there = in_slot < rows;
+  if (!__any_sync(0xffffffffu, there)) return;
   const CacheSpan span = cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
-  const int rows = min(a.tokens - row0, 1 << a.page_shift), n = rows << (a.quad_shift + a.heads_shift);
-  const int mine = min(max(span.count - row0, 0), rows) << (a.quad_shift + a.heads_shift);        // that are no padding
-  const int quad = (1 << a.quad_shift) - 1, heads = (1 << a.heads_shift) - 1;
-  const float* q = pdl_after(a.q) + b * a.q_sb + row0 * a.q_st + head0 * a.q_sh;
-  float* y = a.y + b * a.y_sb + row0 * a.y_st + head0 * a.y_sh;
-  float4 f[HELD];
-#pragma unroll
-  for (int j = 0; j < HELD; j++) {
-    const int i = threadIdx.x + j * APPEND_THREADS, head = i >> a.quad_shift & heads, row = i >> (a.quad_shift + a.heads_shift);
-    f[j] = i < mine && head0 + head < a.heads ? pdl_ld(reinterpret_cast<const float4*>(q + row * a.q_st + head * a.q_sh) + (i & quad))
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  rotate_held<APPEND_THREADS, HELD>(a, f, a.q_weight, mine, row0, span.length - span.count, b, a.quad_shift, a.heads_shift);
-#pragma unroll
-  for (int j = 0; j < HELD; j++) {
-    const int i = threadIdx.x + j * APPEND_THREADS, head = i >> a.quad_shift & heads, row = i >> (a.quad_shift + a.heads_shift);
-    if (i < n && head0 + head < a.heads)
-      *(reinterpret_cast<float4*>(y + row * a.y_st + head * a.y_sh) + (i & quad)) = i < mine ? f[j] : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  const int row = there ? row0 + in_slot : row0, head0 = there ? (item - in_slot * a.chunks) * EACH : 0;
+  const int heads = there ? min(EACH, a.heads - head0) : 0;
+  const bool padding = row >= span.count;
+  const HeadRotation& r = a.rotation;
+  const int64_t position = padding || r.half == 0 ? 0 : r.positions ? (int64_t)pdl_ld(r.positions + (int64_t)b * a.tokens + row)
+                                                                    : span.length - span.count + row;
+  rotate_heads_of<1, EACH>(r, pdl_after(a.q) + b * a.q_sb + row * a.q_st + head0 * a.q_sh, a.q_sh, a.y + b * a.y_sb + row * a.y_st + head0 * a.y_sh, a.y_sh,
+                           padding ? 0 : heads, heads, threadIdx.x & (lanes - 1), lanes, 2 * lanes, a.q_weight, position, a.status);
 }
 
 // One CTA per (sequence, touched page, head, keys or values): max |x| of the page's new tokens, the page's scale, the codes.
@@ -102,16 +106,18 @@ __device__ __forceinline__ void append_queries(const RotaryAppendArgs& a, int pa
 // once and wait in registers for their scale, HELD float4 a thread (a whole page).  Bound: for prompts the length of a CTA's
 // dependent loads (9131 tokens of 8 heads of 128: 18.6 us, 4.9 TB/s), as for single tokens (64 x 1: 2.2 us).
 //
-// With rotations, a head's float4 are those of neighbouring lanes, so that its norm and the other channels of its pairs are a few
-// exchanges away; and further CTAs take the queries of as many tokens as a page has.
+// With rotations a thread has float4 in twos, the slots of a head, whose channels are rotated together; and further CTAs take the
+// queries of as many tokens as a page has.  Bound: the CTAs' chains and their instructions (five prompts of up to 2001 tokens, 24 query, 8
+// key heads of 64: 33.2 us, 4.0 TB/s; 64 new tokens, 32 query, 8 key heads of 128: 3.9), so that 1024 threads an SM are worth the few
+// registers that they leave in local memory (33.2 against 34.6 of 768 and 42.8 of 512; heads of 128 in pages of 64 42.3, 44.1, 55.0).
 template <int APPEND_THREADS, int HELD, class Args>
-__global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Args a) {
+__global__ void __launch_bounds__(APPEND_THREADS, std::is_same<Args, RotaryAppendArgs>::value ? 1024 / APPEND_THREADS : 0) cache_append_kernel(const Args a) {
   constexpr bool ROTARY = std::is_same<Args, RotaryAppendArgs>::value;
   pdl_wait();
   const int part = (int)blockIdx.x, slot = (int)blockIdx.y, b = (int)blockIdx.z;
   if constexpr (ROTARY) {
     if (part >= 2 * a.kv_heads) {
-      append_queries<APPEND_THREADS, HELD>(a, part - 2 * a.kv_heads, slot, b);
+      append_queries<HELD / 2>(a, part - 2 * a.kv_heads, slot, b);
       return;
     }
   }
@@ -129,10 +135,19 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Args
   const int n = (hi - lo) << a.quad_shift, quad = (1 << a.quad_shift) - 1;      // float4 of the new tokens
   __shared__ uint32_t peaks[APPEND_THREADS / 32];
   uint32_t peak = 0;
+  // where float4 number j of this thread is: which of the new tokens' float4, at or behind n: none
+  const auto held = [&](int j) {
+    const int i = threadIdx.x + (ROTARY ? j / 2 : j) * APPEND_THREADS;
+    if constexpr (ROTARY) {
+      const Slot slot(a.rotation, i & (quad >> 1));
+      return (i >> (a.quad_shift - 1) << a.quad_shift) + (j & 1 ? slot.b : slot.a);
+    }
+    return i;
+  };
   float4 f[HELD];
 #pragma unroll
   for (int j = 0; j < HELD; j++) {
-    const int i = threadIdx.x + j * APPEND_THREADS;
+    const int i = held(j);
     f[j] = i < n ? pdl_ld(reinterpret_cast<const float4*>(x + (i >> a.quad_shift) * row) + (i & quad)) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
   if (page < 0 || page >= a.pages) {
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Args
     return;
   }
   if constexpr (ROTARY) {
-    if (!is_v) rotate_held<APPEND_THREADS, HELD>(a, f, a.k_weight, n, lo - start, start, b, a.quad_shift, 0);
+    if (!is_v && (a.k_weight || a.rotation.half)) rotate_keys<APPEND_THREADS, HELD>(a, f, n >> 1, lo - start, start, b);
   }
   const int64_t block = ((int64_t)page * 2 + is_v) * a.kv_heads + head;
   uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes) + (block << (a.page_shift + a.quad_shift));
@@ -171,7 +186,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) cache_append_kernel(const Args
   uint32_t* to = codes + ((lo - first) << a.quad_shift);
 #pragma unroll
   for (int j = 0; j < HELD; j++) {
-    const int i = threadIdx.x + j * APPEND_THREADS;
+    const int i = held(j);
     if (i < n) to[i] = usable ? quantise4(f[j], scale, inverse) : 0u;
   }
   if (threadIdx.x == 0) a.scales[block] = scale;
@@ -246,14 +261,15 @@ static int append_launch(wdc_context* ctx, const wdc_cache_append_desc* d, const
     Args a = args;
     int64_t parts = 2 * d->kv_heads;
     if constexpr (std::is_same<Args, RotaryAppendArgs>::value) {
-      while (most << (a.heads_shift + 1) <= threads * held && 1 << a.heads_shift < a.heads) a.heads_shift++;
-      parts += ceil_div64(a.heads, 1 << a.heads_shift);
+      a.chunks = (a.heads + held / 2 - 1) / (held / 2);
+      parts += ceil_div64((d->tokens < d->page_tokens ? d->tokens : d->page_tokens) * a.chunks << (a.quad_shift - 1), threads);
     }
     wdc_launch_pdl(ctx, kernel, dim3((unsigned)parts, (unsigned)slots, (unsigned)d->batch), dim3((unsigned)threads), 0, a);
   };
   // (few threads with many loads each on their way, where a page has them: 1024 by 128 threads 16.7 us, by 256 22.0, by 64 18.1; 4096 by
   // 512 19.9, by 256 21.4; 256 by 64 11.5, by 128 12.0)
-  if (most <= 64) launch(cache_append_kernel<64, 1, Args>, 64, 1);
+  constexpr bool ROTARY = std::is_same<Args, RotaryAppendArgs>::value;
+  if (most <= 64) launch(cache_append_kernel<ROTARY ? 32 : 64, ROTARY ? 2 : 1, Args>, ROTARY ? 32 : 64, ROTARY ? 2 : 1);
   else if (most <= 256) launch(cache_append_kernel<64, 4, Args>, 64, 4);
   else if (most <= 1024) launch(cache_append_kernel<128, 8, Args>, 128, 8);
   else if (most <= 2048) launch(cache_append_kernel<256, 8, Args>, 256, 8);

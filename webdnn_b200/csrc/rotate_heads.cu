@@ -13,89 +13,37 @@ struct RotateArgs {
   float* y;
   int* status;
   HeadRotation rotation;
-  int64_t rows, x_st, x_sh, y_st, y_sh;
-  int heads, head_size, chunks;      // chunks of EACH heads a row
+  int64_t x_st, x_sh, y_st, y_sh;
+  int heads, head_size;
+  uint32_t chunks, items;            // chunks of EACH heads a row, and in all
 };
 
-// A group of LANES lanes takes EACH heads of a row, QUADS float4 a lane, all of them loaded before the first is used.  Nothing of a
-// head is written before all of it has been read: y may be x.
-template <int LANES, int QUADS, int EACH>
-__global__ void __launch_bounds__(THREADS) rotate_heads_kernel(const RotateArgs a) {
+// A group of LANES lanes takes EACH heads of a row, SLOTS slots a lane.  y may be x: no two groups have a head.
+//
+// Bound: memory (9001 rows of 24 heads of 80, 139 MB: 29 us, 4.8 TB/s; of 16 heads of 128 25.8, 5.7 TB/s); the launch for few (1.7 us).
+template <int LANES, int SLOTS, int EACH, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) rotate_heads_kernel(const RotateArgs a) {
   pdl_wait();
-  constexpr int GROUPS = THREADS / LANES;
-  const int lane = threadIdx.x % LANES, quads = a.head_size >> 2;
-  const int64_t item = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
-  const bool there = item < a.rows * a.chunks;
-  const int64_t row = there ? item / a.chunks : 0;
-  const int head0 = there ? (int)(item - row * a.chunks) * EACH : 0;
-  const int heads = there ? min(EACH, a.heads - head0) : 0;
-  const float* x = pdl_after(a.x) + row * a.x_st + head0 * a.x_sh;
-  float4 v[EACH][QUADS];
-#pragma unroll
-  for (int e = 0; e < EACH; e++)
-#pragma unroll
-    for (int k = 0; k < QUADS; k++) {
-      const int quad = lane + k * LANES;
-      v[e][k] = e < heads && quad < quads ? pdl_ld(reinterpret_cast<const float4*>(x + e * a.x_sh) + quad) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  QuadAngles angles[QUADS];
-  float4 weight[QUADS];
-  const int64_t position = a.rotation.half == 0 ? 0 : a.rotation.positions ? (int64_t)pdl_ld(a.rotation.positions + row) : row;
-  const int64_t place = a.rotation.half == 0 ? 0 : rotation_place(a.rotation, position, a.status);
-#pragma unroll
-  for (int k = 0; k < QUADS; k++) {
-    const int quad = lane + k * LANES;
-    angles[k] = rotation_angles(a.rotation, place, quad);
-    weight[k] = a.weight && quad < quads ? pdl_ld(reinterpret_cast<const float4*>(a.weight) + quad) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  float* y = a.y + row * a.y_st + head0 * a.y_sh;
-#pragma unroll
-  for (int e = 0; e < EACH; e++) {
-    if (QUADS == 1) {
-      const float4 out = rotated_head(a.rotation, v[e][0], lane, LANES, a.head_size, a.weight != nullptr, weight[0], angles[0]);
-      if (e < heads && lane < quads) *(reinterpret_cast<float4*>(y + e * a.y_sh) + lane) = out;
-    } else {
-      Quad64 n[QUADS];
-      double sum = 0.0;
-#pragma unroll
-      for (int k = 0; k < QUADS; k++) sum += square_sum(v[e][k]);
-      const double by = a.weight ? rsqrt(group_sum(sum, LANES) / a.head_size + a.rotation.epsilon) : 1.0;
-#pragma unroll
-      for (int k = 0; k < QUADS; k++)
-        n[k] = a.weight ? scaled(v[e][k], by, weight[k]) : Quad64{v[e][k].x, v[e][k].y, v[e][k].z, v[e][k].w};
-#pragma unroll
-      for (int k = 0; k < QUADS; k++) {
-        const int quad = lane + k * LANES;
-        const bool turns = quad * 2 < a.rotation.half;
-        float4 out;
-        if (a.rotation.interleaved) {
-          out = turns ? rotated_neighbours(n[k], angles[k]) : rounded(n[k]);
-        } else {
-          // the other channels are in any lane, in any of its float4
-          const int other = other_quad(a.rotation, quad);
-          Quad64 o = from_lane(n[0], other % LANES);
-#pragma unroll
-          for (int m = 1; m < QUADS; m++) {
-            const Quad64 p = from_lane(n[m], other % LANES);
-            if (other / LANES == m) o = p;
-          }
-          out = turns ? rotated_halves(n[k], o, angles[k], quad * 4 >= a.rotation.half) : rounded(n[k]);
-        }
-        if (e < heads && quad < quads) *(reinterpret_cast<float4*>(y + e * a.y_sh) + quad) = out;
-      }
-    }
-  }
+  const uint32_t item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
+  const bool there = item < a.items;
+  const uint32_t at = there ? item / a.chunks : 0;
+  const int head0 = there ? (int)(item - at * a.chunks) * EACH : 0, heads = there ? min(EACH, a.heads - head0) : 0;
+  const int64_t row = at, position = a.rotation.half && a.rotation.positions ? (int64_t)pdl_ld(a.rotation.positions + row) : row;
+  rotate_heads_of<SLOTS, EACH>(a.rotation, pdl_after(a.x) + row * a.x_st + head0 * a.x_sh, a.x_sh, a.y + row * a.y_st + head0 * a.y_sh, a.y_sh, heads, 0,
+                               threadIdx.x % LANES, LANES, a.head_size >> 2, a.weight, position, a.status);
 }
 
-template <int LANES, int QUADS>
-int launch(wdc_context* ctx, RotateArgs& a) {
+template <int LANES, int SLOTS, int MOST, int CTAS>
+int launch(wdc_context* ctx, RotateArgs& a, int64_t rows) {
   constexpr int GROUPS = THREADS / LANES;
-  // four heads a group where that still gives every SM work
-  const bool many = a.rows * a.heads >= 4 * GROUPS * (int64_t)ctx->sm_count;
-  a.chunks = many ? (a.heads + 3) / 4 : a.heads;
-  const int64_t ctas = ceil_div64(a.rows * a.chunks, GROUPS);
-  WDC_REQUIRE(ctx, ctas < (1ll << 31), "wdc_rotate_heads: rows exceed the grid");
-  wdc_launch_pdl(ctx, many ? rotate_heads_kernel<LANES, QUADS, 4> : rotate_heads_kernel<LANES, QUADS, 1>, dim3((unsigned)ctas), dim3(THREADS),
+  // several heads a group where that still gives every SM work
+  const bool many = rows * a.heads >= 2 * MOST * GROUPS * (int64_t)ctx->sm_count;
+  const int each = many ? MOST : 1;
+  a.chunks = (uint32_t)((a.heads + each - 1) / each);
+  WDC_REQUIRE(ctx, rows * a.chunks < (1ll << 32) - THREADS, "wdc_rotate_heads: rows exceed the grid");
+  a.items = (uint32_t)(rows * a.chunks);
+  const int64_t ctas = ceil_div64(a.items, GROUPS);
+  wdc_launch_pdl(ctx, many ? rotate_heads_kernel<LANES, SLOTS, MOST, CTAS> : rotate_heads_kernel<LANES, SLOTS, 1, CTAS>, dim3((unsigned)ctas), dim3(THREADS),
                  0, a);
   return wdc_check_launch(ctx, "rotate_heads_kernel");
 }
@@ -113,12 +61,19 @@ extern "C" int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, cons
     return wdc_fail(ctx, WDC_ERR_UNSUPPORTED, "wdc_rotate_heads: heads of %lld (multiples of 4 up to 256)", (long long)d->head_size);
   const int64_t strides[4] = {d->x_st, d->x_sh, d->y_st, d->y_sh};
   CACHE_TRY(cache_check_strides(ctx, "wdc_rotate_heads", strides, 4));
-  RotateArgs a = {x, weight, y, ctx->status_word, {}, d->rows, d->x_st, d->x_sh, d->y_st, d->y_sh, (int)d->heads, (int)d->head_size, 0};
+  RotateArgs a = {x, weight, y, ctx->status_word, {}, d->x_st, d->x_sh, d->y_st, d->y_sh, (int)d->heads, (int)d->head_size, 0, 0};
   if (d->rows == 0 || d->heads == 0) return WDC_OK;
   CACHE_TRY(rotation_check(ctx, "wdc_rotate_heads", a.rotation, d->head_size, d->rotary, d->places, cos, sin, positions, d->epsilon, d->interleaved));
   WDC_REQUIRE(ctx, x && y, "wdc_rotate_heads: null argument");
   WDC_REQUIRE(ctx, cache_aligned(x, 16) && cache_aligned(y, 16) && cache_aligned(weight, 16), "wdc_rotate_heads: buffers are not aligned");
   DeviceGuard g(ctx->device);
-  const int quads = a.head_size / 4;
-  return quads <= 8 ? launch<8, 1>(ctx, a) : quads <= 16 ? launch<16, 1>(ctx, a) : quads <= 32 ? launch<32, 1>(ctx, a) : launch<32, 2>(ctx, a);
+  const int slots = (a.head_size / 4 + 1) / 2;
+  // Lanes, slots and heads a group by what was measured, us of 173 million numbers (floor 22): heads of 32 26.2 (two slots a lane 34.1), of
+  // 64 25.7 (two slots 26.5, two heads 27.1), of 128 25.8 (one slot 25.7, one head 27.5), of 80 29.2 (8 lanes of two slots 31.0, 16 of one 31.4).
+  return slots <= 4    ? launch<4, 1, 4, 3>(ctx, a, d->rows)
+         : slots <= 8  ? launch<8, 1, 4, 3>(ctx, a, d->rows)
+         : slots <= 12 ? launch<4, 3, 2, 2>(ctx, a, d->rows)
+         : slots <= 16 ? launch<8, 2, 2, 3>(ctx, a, d->rows)
+         : slots <= 24 ? launch<8, 3, 2, 2>(ctx, a, d->rows)
+                       : launch<16, 2, 2, 3>(ctx, a, d->rows);
 }
