@@ -2,8 +2,8 @@
 // graphs end at Softmax (operators/cpu/operators/standard/softmax.ts:15-59).
 //
 // The walk from token to token is serial, and only the rows of logits that it comes by are needed.  A cluster of CTAs takes a
-// sequence: each warp of it has a range of the vocabulary, whose maximum and sum of exponentials it finds in one pass; the first CTA
-// (the leader) joins them, tests or draws, and tells the others what to do next.
+// sequence: each warp of it has a range of the vocabulary, whose maximum and sum of exponentials it finds; the first CTA (the leader)
+// joins them, tests or draws, and tells the others what to do next.
 //
 // A drawn token is the one in whose range of the running sum a number falls, and with 100000 tokens there are borders everywhere: sums that
 // are 2^-22 of the whole off would name another token in several of a hundred draws.  So weights and sums are in 64 bits.  Their
@@ -16,9 +16,9 @@
 namespace {
 
 constexpr int WARPS = 16, THREADS = 32 * WARPS, PARTS_MOST = 8, RANGES_MOST = WARPS * PARTS_MOST;
-constexpr int EACH = 4;                            // float4 a lane that are on their way
 constexpr int TOKENS_MOST = 1024;
 constexpr int PART_LEAST = 2048;                   // logits of a CTA, where a row is cut into several
+constexpr int SLICE_BYTES = 96 * 1024;             // shared memory for a CTA's logits, two CTAs an SM
 
 struct VerifyArgs {
   const float *logits, *draft, *uniforms;
@@ -27,34 +27,41 @@ struct VerifyArgs {
   int* status;
   int64_t logits_sb, logits_st, draft_sb, draft_st;
   int n_tokens, vocab, parts;
+  int chunk, chunks;                               // float4 of a warp's range that are in shared memory at a time, and how many times
   double scale, draft_scale;                       // 16 log2(e) / temperature; 0: temperature 0
 };
 
-// What a range of a row (or all of it) has: the largest logit, the sum of 2^((x - top) scale / 16), or where the first of the largest
-// is; whether there is a NaN or +inf.
+// What a range of a row has, or all of a CTA's, or the row: the largest logit, the sum of 2^((x - top) scale / 16), or where the first of
+// the largest is; whether there is a NaN or +inf.
 struct Range {
   double sum;
   float top;
-  int first, bad;
+  int first, bad, unused;
 };
+__device__ __forceinline__ Range nothing() { return {0.0, -INFINITY, 0x7fffffff, 0, 0}; }
 enum Todo { STOP = 0, ROW = 1, RESIDUAL = 2 };
 struct Command {
   int todo, token;                                 // the token that the walk stands at
-  int with_draft, first, draft_first;
+  int with_draft;                                  // ROW: whether the draft's row is wanted; RESIDUAL: rejections, this one included
+  int first, draft_first;
   float top, draft_top;
+  int unused;
   double draft_inverse, step;                      // 1 / sum of the draft's weights, of those before the last rejection
 };
 struct Shared {
   double table[16];
   double steps[TOKENS_MOST];                       // 1 / the sums that a rejection divided by
   Command command;
+  Range mine[2][WARPS];                            // of this CTA's ranges: target and draft
   // of the leader
-  Range ranges[2][RANGES_MOST];                    // target and draft
-  double run[RANGES_MOST], fresh[RANGES_MOST];     // sums of the ranges, all relative to one maximum; after the last rejection
+  Range parts[2][PARTS_MOST];
+  double run[RANGES_MOST], fresh[RANGES_MOST];     // sums of all ranges, relative to their CTA's largest; after the last rejection
+  double part_factors[PARTS_MOST];                 // what relates that to the row's
   double warp_sums[WARPS];
+  int draw;                                        // which uniform a token is to be drawn with, or -1
+  int found;
   float uniforms[TOKENS_MOST];
   int tokens[TOKENS_MOST], parents[TOKENS_MOST], path[TOKENS_MOST];
-  int found, child;
 };
 
 __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
@@ -72,49 +79,68 @@ __device__ __forceinline__ void cluster_put(T* to, int rank, const T& value) {
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(T) / 4); i++) cluster_put(at + 4 * i, w[i]);
 }
+// All threads of the cluster wait for one another.  What a CTA has written by then is seen by the others: its warp 0, behind a barrier of the
+// CTA's, says so for all.
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  if (threadIdx.x < 32) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  else asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// 2^(d scale / 16) for d <= 0, within 2^-42 of it; 0 where that is below 2^-1000 (d is -inf or NaN).  n is the nearest whole number
-// to d scale, which adding 1.5 * 2^52 leaves in the last bits; 2^(g / 16), |g| <= 1/2, by five terms of its series.
-__device__ __forceinline__ double power(float x, float top, double scale, const double* table) {
-  const double magic = 6755399441055744.0, u = 0.043321698784996582;           // ln(2) / 16
-  const double d = (double)x - (double)top, shifted = fma(d, scale, magic), g = fma(d, scale, magic - shifted);
-  const int n = __double2loint(shifted);
-  double p = u * u * u * u * u / 120;
-  p = fma(p, g, u * u * u * u / 24);
-  p = fma(p, g, u * u * u / 6);
-  p = fma(p, g, u * u / 2);
-  p = fma(p, g, u);
-  const double t = table[n & 15], y = fma(t, p * g, t);
-  const double out = __hiloint2double(__double2hiint(y) + ((n >> 4) << 20), __double2loint(y));
-  return (x - top) * (float)scale > -16000.f ? out : 0.0;
-}
-
-__device__ __forceinline__ Range joined(Range a, const Range& b, double scale, const double* table) {
-  const float top = fmaxf(a.top, b.top);
-  if (scale == 0.0) {
-    if (b.top > a.top || (b.top == a.top && b.first < a.first)) a.first = b.first;
-  } else {
-    a.sum = a.sum * (a.top < top ? power(a.top, top, scale, table) : 1.0) + b.sum * (b.top < top ? power(b.top, top, scale, table) : 1.0);
-  }
-  a.top = top;
-  a.bad |= b.bad;
-  return a;
-}
-__device__ __forceinline__ Range warp_joined(Range a, double scale, const double* table) {
+// 2^(d scale / 16), d = x - top <= 0, within 2^-42 of it; 0 where that is below 2^-1000 (d is -inf or NaN).  n is the nearest whole
+// number to d scale, which adding 1.5 * 2^52 leaves in the last bits; 2^(g / 16), |g| <= 1/2, by five terms of its series.  N of
+// them side by side, step by step: one waits for 14 operations in a row.
+template <int N>
+__device__ __forceinline__ void powers(const float (&x)[N], float top, double scale, const double* table, double (&out)[N]) {
+  const double magic = 6755399441055744.0, u = 0.043321698784996582, high = top;           // ln(2) / 16
+  const float near_scale = (float)scale;
+  double d[N], shifted[N], g[N], p[N], t[N];
 #pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    Range b;
-    b.sum = __shfl_xor_sync(0xffffffffu, a.sum, w);
-    b.top = __shfl_xor_sync(0xffffffffu, a.top, w);
-    b.first = __shfl_xor_sync(0xffffffffu, a.first, w);
-    b.bad = __shfl_xor_sync(0xffffffffu, a.bad, w);
-    a = joined(a, b, scale, table);
+  for (int i = 0; i < N; i++) d[i] = (double)x[i] - high;
+#pragma unroll
+  for (int i = 0; i < N; i++) shifted[i] = fma(d[i], scale, magic);
+#pragma unroll
+  for (int i = 0; i < N; i++) t[i] = table[__double2loint(shifted[i]) & 15];
+#pragma unroll
+  for (int i = 0; i < N; i++) g[i] = fma(d[i], scale, magic - shifted[i]);
+#pragma unroll
+  for (int i = 0; i < N; i++) p[i] = fma(u * u * u * u * u / 120, g[i], u * u * u * u / 24);
+#pragma unroll
+  for (int i = 0; i < N; i++) p[i] = fma(p[i], g[i], u * u * u / 6);
+#pragma unroll
+  for (int i = 0; i < N; i++) p[i] = fma(p[i], g[i], u * u / 2);
+#pragma unroll
+  for (int i = 0; i < N; i++) p[i] = fma(p[i], g[i], u) * g[i];
+#pragma unroll
+  for (int i = 0; i < N; i++) p[i] = fma(t[i], p[i], t[i]);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const double y = __hiloint2double(__double2hiint(p[i]) + ((__double2loint(shifted[i]) >> 4) << 20), __double2loint(p[i]));
+    out[i] = (x[i] - top) * near_scale > -16000.f ? y : 0.0;
   }
-  return a;
+}
+__device__ __forceinline__ double power(float x, float top, double scale, const double* table) {
+  const float one[1] = {x};
+  double out[1];
+  powers(one, top, scale, table, out);
+  return out[0];
+}
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+  return x;
+}
+template <int LANES>
+__device__ __forceinline__ float group_max(float x) {
+#pragma unroll
+  for (int w = 1; w < LANES; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+  return x;
+}
+template <int LANES>
+__device__ __forceinline__ int group_min(int x) {
+#pragma unroll
+  for (int w = 1; w < LANES; w <<= 1) x = min(x, __shfl_xor_sync(0xffffffffu, x, w));
+  return x;
 }
 
 // How a row is cut: float4 number j has logits 4 j - before .. + 3 (`before`: how far the row is behind a 16-byte boundary), and a
@@ -130,93 +156,169 @@ struct Cut {
   __device__ int logit(int quad) const { return max(4 * quad - before, 0); }
 };
 
-__device__ Range row_range(const float* row, int vocab, int range, int ranges, double scale, const double* table) {
-  const Cut cut(row, vocab, ranges);
-  const int lane = threadIdx.x & 31, end = cut.first(range + 1);
-  Range r = {0.0, -INFINITY, 0x7fffffff, 0};
-  for (int j0 = cut.first(range) + lane; j0 < end; j0 += 32 * EACH) {
-    float x[EACH][4];
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-      const int j = j0 + e * 32, i = 4 * j - cut.before;
-      if (j < end && i >= 0 && i + 3 < vocab) {
-        const float4 v = pdl_ld(reinterpret_cast<const float4*>(row + i));
-        x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w;
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; c++) x[e][c] = j < end && i + c >= 0 && i + c < vocab ? pdl_ld(row + i + c) : -INFINITY;
-      }
+// `quads` float4 of a row, from logit i0 on, to shared memory, by asynchronous copies of a warp; -inf where the row has none, which is in the
+// first and the last.  whole: as they are in memory.
+__device__ __forceinline__ void fetch_quads(float4* to, const float* row, int vocab, int i0, int quads, bool whole) {
+  const int lane = threadIdx.x & 31;
+  const bool cut_off = quads > 0 && (i0 < 0 || i0 + 4 * quads > vocab);
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(to);
+  if (whole) {
+    const int inside = i0 < 0 ? 1 : 0, end = i0 + 4 * quads > vocab ? quads - 1 : quads;
+    const float* from = row + i0 + 4 * lane;
+    for (int j = lane; j < end; j += 32, from += 128)
+      if (j >= inside) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + 16 * j), "l"(from) : "memory");
+    if (!cut_off) return;
+  }
+  // number by number: all of them, or the first and the last float4
+  for (int k = lane; k < 4 * quads; k += 32) {
+    if (whole && k >= 4 && k < 4 * quads - 4) continue;
+    const int i = i0 + k;
+    if (i >= 0 && i < vocab) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + 4 * k), "l"(row + i) : "memory");
+    else reinterpret_cast<float*>(to)[k] = -INFINITY;
+  }
+}
+// What a warp's range has: its float4, `quads` from logit i0 on, which are in `mine`, or are brought there a chunk at a time where they
+// are several chunks.  (A function of its own, which has the registers to itself.)
+__device__ __noinline__ Range row_range(float4* mine, const float* row, int vocab, int i0, int quads, int chunk, int chunks, bool whole, double scale,
+                                        const double* table) {
+  const int lane = threadIdx.x & 31;
+  Range r = nothing();
+#pragma unroll 1
+  for (; quads > 0; quads -= chunk, i0 += 4 * chunk) {
+    const int n = min(quads, chunk);
+    if (chunks > 1) {
+      __syncwarp();
+      fetch_quads(mine, row, vocab, i0, n, whole);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
     }
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-      const float top = fmaxf(fmaxf(x[e][0], x[e][1]), fmaxf(x[e][2], x[e][3]));
-#pragma unroll
-      for (int c = 0; c < 4; c++) r.bad |= !(x[e][c] < INFINITY);
-      if (top > r.top) {
-        if (scale == 0.0)
-          r.first = 4 * (j0 + e * 32) - cut.before + (x[e][0] == top ? 0 : x[e][1] == top ? 1 : x[e][2] == top ? 2 : 3);
-        else
-          r.sum *= power(r.top, top, scale, table);
-        r.top = top;
+    float its_top = -INFINITY;
+    int bad = 0;
+#pragma unroll 2
+    for (int j = lane; j < n; j += 32) {
+      const float4 v = mine[j];
+      const float most = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+      if (most > its_top) {
+        its_top = most;
+        if (scale == 0.0 && most > r.top) r.first = i0 + 4 * j + (v.x == most ? 0 : v.y == most ? 1 : v.z == most ? 2 : 3);
       }
-      if (scale != 0.0) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) r.sum += power(x[e][c], r.top, scale, table);
-      }
+      bad |= !(v.x < INFINITY) | !(v.y < INFINITY) | !(v.z < INFINITY) | !(v.w < INFINITY);
+    }
+    r.bad |= bad;
+    if (scale == 0.0) {                            // (lanes have their own largest, and the first of it)
+      r.top = fmaxf(r.top, its_top);
+      continue;
+    }
+    const float top = fmaxf(r.top, group_max<32>(its_top));
+    if (top > r.top) {
+      r.sum *= power(r.top, top, scale, table);
+      r.top = top;
+    }
+#pragma unroll 1
+    for (int j = lane; j < n; j += 32) {
+      const float4 v = mine[j];
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      double w[4];
+      powers(x, r.top, scale, table, w);
+      r.sum += (w[0] + w[1]) + (w[2] + w[3]);
     }
   }
-  return warp_joined(r, scale, table);
+  r.bad = __any_sync(0xffffffffu, r.bad);
+  if (scale == 0.0) {
+    const float top = group_max<32>(r.top);
+    r.first = __reduce_min_sync(0xffffffffu, r.top == top ? r.first : 0x7fffffff);
+    r.top = top;
+  } else {
+    r.sum = warp_sum(r.sum);
+  }
+  return r;
 }
 
-// The weight of one token under the target's distribution after `n` rejections, not normalised.
+// The weight of tokens under the target's distribution after `n` rejections, not normalised.
 struct Weights {
-  const float *row, *draft;
+  const Command& c;
+  const double *table, *steps;
   double scale, draft_scale;
-  const Shared* sh;
   int n;
-  __device__ double draft_at(int i) const {
-    const Command& c = sh->command;
-    return draft_scale == 0.0 ? (double)(i == c.draft_first) : power(pdl_ld(draft + i), c.draft_top, draft_scale, sh->table) * c.draft_inverse;
+  template <int N>
+  __device__ __forceinline__ void drafted(int i, int step, const float (&y)[N], double (&q)[N]) const {
+    if (draft_scale != 0.0) powers(y, c.draft_top, draft_scale, table, q);
+#pragma unroll
+    for (int e = 0; e < N; e++) q[e] = draft_scale == 0.0 ? (double)(i + e * step == c.draft_first) : q[e] * c.draft_inverse;
   }
-  __device__ double at(int i) const {
-    const Command& c = sh->command;
-    double p = scale == 0.0 ? (double)(i == c.first) : power(pdl_ld(row + i), c.top, scale, sh->table);
-    if (n) {
-      const double q = draft_at(i);
-      for (int k = 0; k < n; k++) p = fmax(fma(p, sh->steps[k], -q), 0.0);
+  // of N tokens i, i + step, .. with logits x and y
+  template <int N>
+  __device__ __forceinline__ void of(int i, int step, const float (&x)[N], const float (&y)[N], double (&p)[N]) const {
+    if (scale != 0.0) powers(x, c.top, scale, table, p);
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (scale == 0.0) p[e] = (double)(i + e * step == c.first);
+    if (n == 0) return;
+    double q[N];
+    drafted(i, step, y, q);
+#pragma unroll 1
+    for (int k = 0; k < n; k++) {
+      const double by = steps[k];
+#pragma unroll
+      for (int e = 0; e < N; e++) p[e] = fmax(fma(p[e], by, -q[e]), 0.0);
     }
-    return p;
   }
 };
 
-__device__ __forceinline__ double warp_sum(double x) {
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-  return x;
+// The sum of a warp's range after `n` rejections; its float4 of both sides are in shared memory, `apart` float4 from one another, or are
+// brought there again where they are several chunks.
+__device__ __noinline__ double residual(float4* mine, int apart, const float* row, const float* draft, int vocab, int i0, int quads, int chunk, int chunks,
+                                        bool same, const Weights& weights) {
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+#pragma unroll 1
+  for (; quads > 0; quads -= chunk, i0 += 4 * chunk) {
+    const int n = min(quads, chunk);
+    if (chunks > 1) {
+      __syncwarp();
+      fetch_quads(mine, row, vocab, i0, n, true);
+      fetch_quads(mine + apart, draft, vocab, i0, n, same);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+    }
+#pragma unroll 1
+    for (int j = lane; j < n; j += 32) {
+      const float4 v = mine[j], u = mine[apart + j];
+      const float x[4] = {v.x, v.y, v.z, v.w}, y[4] = {u.x, u.y, u.z, u.w};
+      double w[4];
+      weights.of(i0 + 4 * j, 1, x, y, w);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+  }
+  return warp_sum(sum);
 }
 
-// The first token whose running sum passes u times all of it; the ranges' sums are in `run`.  All threads of the leader.
-__device__ int drawn(Shared& sh, const Weights& weights, const Cut& cut, int vocab, int ranges, float uniform) {
+// Sums of the lanes up to this one.
+__device__ __forceinline__ double warp_scan(double x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, x, w);
+    if (lane >= w) x += other;
+  }
+  return x;
+}
+// The first token whose running sum passes u times all of it, or -1 where nothing weighs anything; the ranges' sums are in `run`.  All threads of
+// the leader: every warp finds the range, then each has neighbours of it.
+__device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const float* row, const float* draft, const Cut& cut, int vocab, int ranges,
+                                  float uniform) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double u = (double)fminf(fmaxf(uniform, 0.f), 0.999999940395355f);      // (NaN: 0)
-  if (threadIdx.x == 0) sh.found = -1;
-  // every warp finds the range: lane l has ranges l * per .. of it
-  constexpr int PER = RANGES_MOST / 32;
+  constexpr int PER = RANGES_MOST / 32, N = 2;     // ranges of a lane, all of one CTA; tokens of a thread
   double mine[PER], sum = 0.0;
 #pragma unroll
   for (int k = 0; k < PER; k++) {
-    mine[k] = lane * PER + k < ranges ? sh.run[lane * PER + k] : 0.0;
+    const int r = lane * PER + k;
+    mine[k] = r < ranges ? sh.run[r] * (weights.n ? 1.0 : sh.part_factors[r / WARPS]) : 0.0;
     sum += mine[k];
   }
-  double up = sum;
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    const double other = __shfl_up_sync(0xffffffffu, up, w);
-    if (lane >= w) up += other;
-  }
+  double up = warp_scan(sum), before = up - sum;
   const double goal = u * __shfl_sync(0xffffffffu, up, 31);
-  double before = __shfl_up_sync(0xffffffffu, up, 1);
-  if (lane == 0) before = 0.0;
   int range = -1;
   double base = 0.0;
 #pragma unroll
@@ -228,69 +330,92 @@ __device__ int drawn(Shared& sh, const Weights& weights, const Cut& cut, int voc
     before += mine[k];
   }
   const unsigned have = __ballot_sync(0xffffffffu, range >= 0);
-  const int who = have ? __ffs((int)have) - 1 : 0;
+  if (!have) return -1;
+  const int who = __ffs((int)have) - 1;
   range = __shfl_sync(0xffffffffu, range, who);
   base = __shfl_sync(0xffffffffu, base, who);
-  __syncthreads();
-  if (range < 0) return -1;                        // (nothing weighs anything)
-  // its tokens, a few neighbours each thread
   const int lo = cut.logit(cut.first(range)), hi = min(cut.logit(cut.first(range + 1)), vocab);
-  const int per = (hi - lo + THREADS - 1) / THREADS, from = lo + (int)threadIdx.x * per, to = min(from + per, hi);
-  double own = 0.0;
-  for (int i = from; i < to; i++) own += weights.at(i);
-  double scan = own;
+  // (found: tokens that pass, the first the largest, are above all that do not: the last that weighs anything, where roundings of 2^-53
+  // keep the goal from all)
+#pragma unroll 1
+  for (int i0 = lo; i0 < hi; i0 += THREADS * N) {
+    const int from = i0 + (int)threadIdx.x * N;
+    float x[N], y[N];
 #pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    const double other = __shfl_up_sync(0xffffffffu, scan, w);
-    if (lane >= w) scan += other;
-  }
-  if (lane == 31) sh.warp_sums[warp] = scan;
-  __syncthreads();
-  double running = base;
-  for (int w = 0; w < warp; w++) running += sh.warp_sums[w];
-  const double shifted = __shfl_up_sync(0xffffffffu, scan, 1);
-  running += lane ? shifted : 0.0;
-  // the token that passes; where roundings of 2^-53 keep all from it, the last that weighs anything
-  int token = -1, last = -1;
-  for (int i = from; i < to; i++) {
-    const double w = weights.at(i);
-    running += w;
-    if (w > 0.0) {
-      last = i;
-      if (token < 0 && running > goal) token = i;
+    for (int e = 0; e < N; e++) {
+      x[e] = from + e < hi ? pdl_ld(row + from + e) : -INFINITY;
+      y[e] = from + e < hi && weights.n ? pdl_ld(draft + from + e) : -INFINITY;
     }
+    double w[N];
+    weights.of(from, 1, x, y, w);
+#pragma unroll
+    for (int e = 0; e < N; e++) w[e] = from + e < hi ? w[e] : 0.0;
+    const double scan = warp_scan(w[0] + w[1]);
+    if (lane == 31) sh.warp_sums[warp] = scan;
+    __syncthreads();
+    double running = base + (scan - (w[0] + w[1]));
+#pragma unroll 1
+    for (int k = 0; k < WARPS; k++) {
+      const double of_warp = sh.warp_sums[k];
+      if (k < warp) running += of_warp;
+      base += of_warp;
+    }
+    int best = -1;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      running += w[e];
+      if (w[e] > 0.0 && best < 1 << 30) best = running > goal ? (1 << 30) + ((1 << 30) - 1 - (from + e)) : from + e;
+    }
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (lane == 0 && best >= 0) atomicMax(&sh.found, best);
+    __syncthreads();
+    if (sh.found >= 1 << 30) break;
   }
-  const unsigned passes = __ballot_sync(0xffffffffu, token >= 0);
-  // (found: tokens that pass count down from 2^30, so that the first is the largest, and are above all that do not)
-  if (passes && lane == __ffs((int)passes) - 1) atomicMax(&sh.found, (1 << 30) + ((1 << 30) - 1 - token));
-  else if (!passes) {
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0 && last >= 0) atomicMax(&sh.found, last);
-  }
-  __syncthreads();
   const int found = sh.found;
-  __syncthreads();
   return found >= 1 << 30 ? (1 << 30) - 1 - (found - (1 << 30)) : found;
 }
 
-// The next child of new token `of` behind new token `after`, which has token `want` where `only` is set, or -1.  All threads of the
-// leader.
-__device__ int child_of(Shared& sh, int of, int after, int count, bool only = false, int want = 0) {
-  __syncthreads();
-  if (threadIdx.x == 0) sh.child = 0x7fffffff;
-  __syncthreads();
-  for (int i = after + 1 + (int)threadIdx.x; i < count; i += THREADS)
-    if (sh.parents[i] == of && (!only || sh.tokens[i] == want)) {
-      atomicMin(&sh.child, i);
-      break;
-    }
-  __syncthreads();
-  const int child = sh.child;
-  return child == 0x7fffffff ? -1 : child;
+// The next child of new token `of` behind new token `after`, which has token `want` where `only` is set, or -1.  Every warp finds it.
+__device__ __forceinline__ int child_of(const Shared& sh, int of, int after, int count, bool only = false, int want = 0) {
+  for (int i0 = after + 1; i0 < count; i0 += 32) {
+    const int i = i0 + (int)(threadIdx.x & 31);
+    const unsigned is = __ballot_sync(0xffffffffu, i < count && sh.parents[i] == of && (!only || sh.tokens[i] == want));
+    if (is) return i0 + __ffs((int)is) - 1;
+  }
+  return -1;
 }
+
+// A CTA's ranges, both sides at once, to the leader.  Warp 0.
+__device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int rank, bool row, bool with_draft) {
+  const int lane = threadIdx.x & 31, side = lane / WARPS, r = lane % WARPS;
+  Range its = nothing();
+  if (side == 0 || with_draft) its = sh.mine[side][r];
+  const double scale = side ? a.draft_scale : a.scale;
+  // (the sides' scales may differ: exchanges between lanes are outside of what depends on them)
+  const float top = group_max<WARPS>(its.top);
+  const int first = group_min<WARPS>(its.top == top ? its.first : 0x7fffffff);
+  if (row && scale == 0.0) its.sum = its.first == first && its.top > -INFINITY ? 1.0 : 0.0;
+  else if (row) its.sum *= power(its.top, top, scale, sh.table);
+  its.first = first;
+  its.top = top;
+  if (side == 0) cluster_put((row ? sh.run : sh.fresh) + rank * WARPS + r, 0, its.sum);
+#pragma unroll
+  for (int w = 1; w < WARPS; w <<= 1) {
+    its.sum += __shfl_xor_sync(0xffffffffu, its.sum, w);
+    its.bad |= __shfl_xor_sync(0xffffffffu, its.bad, w);
+  }
+  if (r == 0) cluster_put(&sh.parts[side][rank], 0, its);
+}
+
+// Warp 0 of the leader: where the walk stands, and what the last pass has to say about it.
+struct Walk {
+  int at = 0, length = 1, child = 0, rejections = 0, next = -1;
+  double total = 0.0;
+};
 
 __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
+  extern __shared__ float4 slices[];               // logits: each warp's of the target, then of the draft
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)a.parts), b = (int)(blockIdx.x / (unsigned)a.parts), ranges = a.parts * WARPS;
   if (threadIdx.x < 16) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 16);
@@ -305,6 +430,7 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
     c.todo = ROW;
     c.with_draft = a.draft && count > 1;
     sh.command = c;
+    sh.path[0] = 0;
   }
   if (rank == 0) {
     for (int i = threadIdx.x; i < count; i += THREADS) {
@@ -319,132 +445,161 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
       sh.uniforms[i] = a.uniforms ? pdl_ld(a.uniforms + at) : 0.f;
     }
   }
+  __syncthreads();
   cluster_sync();                                  // all CTAs of the cluster have begun
 
-  // of the leader
-  int at = 0, length = 1, child = 0, rejections = 0, next = -1;
-  double total = 0.0;
-  if (rank == 0 && threadIdx.x == 0) sh.path[0] = 0;
+  float4* const mine = slices + warp * a.chunk;
+  const int apart = WARPS * a.chunk;
+  Walk walk;
+#pragma unroll 1
   for (;;) {
-    const Command now = sh.command;
-    if (now.todo == STOP) break;
-    const float* row = a.logits + b * a.logits_sb + now.token * a.logits_st;
-    const float* draft = a.draft ? a.draft + b * a.draft_sb + now.token * a.draft_st : nullptr;
-    const int range = rank * WARPS + warp;
-    if (now.todo == ROW) {
-      if (count > 0) {
-        const Range r = row_range(row, a.vocab, range, ranges, a.scale, sh.table);
-        if (lane == 0) cluster_put(&sh.ranges[0][range], 0, r);
-        if (now.with_draft) {
-          const Range q = row_range(draft, a.vocab, range, ranges, a.draft_scale, sh.table);
-          if (lane == 0) cluster_put(&sh.ranges[1][range], 0, q);
-        }
+    const int todo = sh.command.todo, standing = sh.command.token, with_draft = sh.command.with_draft;
+    if (todo == STOP) break;
+    const float* row = a.logits + b * a.logits_sb + standing * a.logits_st;
+    const float* draft = a.draft ? a.draft + b * a.draft_sb + standing * a.draft_st : nullptr;
+    const Cut cut(row, a.vocab, ranges);
+    const int first = cut.first(rank * WARPS + warp), quads = cut.first(rank * WARPS + warp + 1) - first, i0 = 4 * first - cut.before;
+    const bool same = (reinterpret_cast<uintptr_t>(row) >> 2 & 3) == (reinterpret_cast<uintptr_t>(draft) >> 2 & 3);
+    if (count == 0) {
+    } else if (todo == ROW) {
+      if (a.chunks == 1) {
+#pragma unroll 1
+        for (int side = 0; side <= (with_draft != 0); side++) fetch_quads(mine + side * apart, side ? draft : row, a.vocab, i0, quads, side == 0 || same);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+      }
+#pragma unroll 1
+      for (int side = 0; side <= (with_draft != 0); side++) {
+        const Range r = row_range(mine + side * apart, side ? draft : row, a.vocab, i0, quads, a.chunk, a.chunks, side == 0 || same,
+                                  side ? a.draft_scale : a.scale, sh.table);
+        if (lane == 0) sh.mine[side][warp] = r;
       }
     } else {
       // the rejection that has just been: its step is the last
-      if (threadIdx.x == 0) sh.steps[now.with_draft - 1] = now.step;
+      if (threadIdx.x == 0) sh.steps[with_draft - 1] = sh.command.step;
       __syncthreads();
-      const Weights weights = {row, draft, a.scale, a.draft_scale, &sh, now.with_draft};
-      const Cut cut(row, a.vocab, ranges);
-      const int hi = min(cut.logit(cut.first(range + 1)), a.vocab);
-      double sum = 0.0;
-#pragma unroll 4
-      for (int i = cut.logit(cut.first(range)) + lane; i < hi; i += 32) sum += weights.at(i);
-      sum = warp_sum(sum);
-      if (lane == 0) cluster_put(&sh.fresh[range], 0, sum);
+      const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, with_draft};
+      const double sum = residual(mine, apart, row, draft, a.vocab, i0, quads, a.chunk, a.chunks, same, weights);
+      if (lane == 0) sh.mine[0][warp] = {sum, 0.f, 0, 0, 0};
     }
+    __syncthreads();
+    if (warp == 0 && count > 0) to_leader(sh, a, rank, todo == ROW, todo == ROW && with_draft);
     cluster_sync();
     if (rank == 0) {
-      Command c = now;
-      c.todo = STOP;
-      const Cut cut(row, a.vocab, ranges);
-      bool test = false;                           // whether drafts of `at` are to be tried
-      if (now.todo == ROW && count > 0) {
-        // every warp joins the ranges
-        Range p = {0.0, -INFINITY, 0x7fffffff, 0}, q = p;
-        for (int r = lane; r < ranges; r += 32) {
-          p = joined(p, sh.ranges[0][r], a.scale, sh.table);
-          if (now.with_draft) q = joined(q, sh.ranges[1][r], a.draft_scale, sh.table);
-        }
-        p = warp_joined(p, a.scale, sh.table);
-        q = warp_joined(q, a.draft_scale, sh.table);
-        const bool none = p.bad || p.top == -INFINITY || (now.with_draft && (q.bad || q.top == -INFINITY));
-        __syncthreads();
-        for (int r = threadIdx.x; r < ranges; r += THREADS) {
-          const Range mine = sh.ranges[0][r];
-          sh.run[r] = a.scale == 0.0 ? (mine.top == p.top && mine.first == p.first ? 1.0 : 0.0) : mine.top == -INFINITY ? 0.0
-                                     : mine.sum * (mine.top < p.top ? power(mine.top, p.top, a.scale, sh.table) : 1.0);
-        }
-        total = a.scale == 0.0 ? 1.0 : p.sum;
-        c.first = p.first; c.top = p.top;
-        c.draft_first = q.first; c.draft_top = q.top;
-        c.draft_inverse = a.draft_scale == 0.0 ? 1.0 : 1.0 / q.sum;
-        c.with_draft = rejections = 0;
-        __syncthreads();
-        if (threadIdx.x == 0) sh.command = c;      // (for the weights below; told to the others at the end)
-        __syncthreads();
-        if (!none && a.draft) {
-          child = child_of(sh, at, at, count);
-          test = true;
-        } else if (!none) {
-          const Weights weights = {row, draft, a.scale, a.draft_scale, &sh, 0};
-          const int token = a.scale == 0.0 ? p.first : drawn(sh, weights, cut, a.vocab, ranges, sh.uniforms[at]);
-          child = child_of(sh, at, at, count, true, token);
-          if (child < 0) {
-            next = token;
+      Command c = {};                              // (of warp 0, which decides; all threads draw)
+      bool test = false;
+      if (warp == 0) {
+        c = sh.command;
+        c.todo = STOP;
+        int draw = -1;
+        if (count > 0) {
+          // the CTAs' parts, both sides at once
+          const int side = lane / PARTS_MOST & 1, part = lane % PARTS_MOST;
+          const bool there = lane < 2 * PARTS_MOST && part < a.parts && (side == 0 || (todo == ROW && with_draft));
+          Range its = nothing();
+          if (there) its = sh.parts[side][part];
+          const double scale = side ? a.draft_scale : a.scale;
+          const float top = group_max<PARTS_MOST>(its.top);
+          const int first_of_all = group_min<PARTS_MOST>(its.top == top ? its.first : 0x7fffffff);
+          double f = 1.0;
+          if (todo == ROW) {
+            f = scale == 0.0 ? (double)(its.first == first_of_all && its.top > -INFINITY) : power(its.top, top, scale, sh.table);
+            if (there && side == 0) sh.part_factors[part] = f;
+          }
+          its.sum *= f;
+#pragma unroll
+          for (int w = 1; w < PARTS_MOST; w <<= 1) {
+            its.sum += __shfl_xor_sync(0xffffffffu, its.sum, w);
+            its.bad |= __shfl_xor_sync(0xffffffffu, its.bad, w);
+          }
+          const double total = __shfl_sync(0xffffffffu, its.sum, 0), draft_total = __shfl_sync(0xffffffffu, its.sum, PARTS_MOST);
+          if (todo == ROW) {
+            const bool none = __any_sync(0xffffffffu, lane < (with_draft ? 2 : 1) * PARTS_MOST && (its.bad || top == -INFINITY));
+            c.first = __shfl_sync(0xffffffffu, first_of_all, 0);
+            c.top = __shfl_sync(0xffffffffu, top, 0);
+            c.draft_first = __shfl_sync(0xffffffffu, first_of_all, PARTS_MOST);
+            c.draft_top = __shfl_sync(0xffffffffu, top, PARTS_MOST);
+            c.draft_inverse = with_draft ? 1.0 / draft_total : 1.0;
+            walk.total = total;
+            walk.rejections = 0;
+            walk.child = standing;
+            test = !none && a.draft;
+            if (!none && !a.draft) draw = standing;
           } else {
-            at = child;
-            c.todo = ROW;
+            if (total > 0.0) {
+              for (int r = lane; r < ranges; r += 32) sh.run[r] = sh.fresh[r];
+              walk.total = total;
+              walk.rejections = with_draft;
+            }
+            test = true;
+          }
+          if (test) {
+            walk.child = child_of(sh, standing, walk.child, count);
+            if (walk.child < 0) draw = 0;
           }
         }
-      } else if (now.todo == RESIDUAL) {
-        double sum = 0.0;
-        for (int r = lane; r < ranges; r += 32) sum += sh.fresh[r];
-        sum = warp_sum(sum);
-        __syncthreads();
-        if (sum > 0.0) {
-          for (int r = threadIdx.x; r < ranges; r += THREADS) sh.run[r] = sh.fresh[r];
-          total = sum;
-          rejections = now.with_draft;
+        __syncwarp();
+        if (lane == 0) {
+          sh.command = c;                          // (for the weights below; told to the others at the end)
+          sh.command.with_draft = walk.rejections;
+          sh.draw = draw;
+          sh.found = -1;
         }
-        child = child_of(sh, at, child, count);
-        test = true;
-      }
-      if (test) {
-        const Weights weights = {row, draft, a.scale, a.draft_scale, &sh, rejections};
-        if (child < 0) {
-          next = drawn(sh, weights, cut, a.vocab, ranges, sh.uniforms[0]);
-        } else {
-          const int token = sh.tokens[child];
-          const bool there = token >= 0 && token < a.vocab;
-          const double u = (double)fminf(fmaxf(sh.uniforms[child], 0.f), 0.999999940395355f);
-          if (there && u * weights.draft_at(token) * total < weights.at(token)) {
-            at = child;
-            c.todo = ROW;
-          } else {
-            c.todo = RESIDUAL;
-            c.with_draft = rejections + 1;
-            c.step = 1.0 / total;
-          }
-        }
-      }
-      if (c.todo == ROW) {
-        c.token = at;
-        if (threadIdx.x == 0) sh.path[length] = at;
-        length++;
-        c.with_draft = a.draft && child_of(sh, at, at, count) >= 0;
+        __syncwarp();
       }
       __syncthreads();
-      if (threadIdx.x < a.parts) cluster_put(&sh.command, (int)threadIdx.x, c);
+      if (sh.draw >= 0) {
+        const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, sh.command.with_draft};
+        const int token = drawn(sh, weights, row, draft, cut, a.vocab, ranges, sh.uniforms[sh.draw]);
+        if (warp == 0) {
+          walk.child = token < 0 || a.draft ? -1 : child_of(sh, standing, standing, count, true, token);
+          if (walk.child < 0) {
+            walk.next = token;
+          } else {
+            walk.at = walk.child;
+            c.todo = ROW;
+          }
+        }
+      } else if (test) {
+        const int token = sh.tokens[walk.child];
+        const double u = (double)fminf(fmaxf(sh.uniforms[walk.child], 0.f), 0.999999940395355f);
+        bool stands = false;
+        if (token >= 0 && token < a.vocab) {
+          const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, walk.rejections};
+          const float x[1] = {pdl_ld(row + token)}, y[1] = {pdl_ld(draft + token)};
+          double p[1], q[1];
+          weights.of(token, 1, x, y, p);
+          weights.drafted(token, 1, y, q);
+          stands = u * q[0] * walk.total < p[0];
+        }
+        if (stands) {
+          walk.at = walk.child;
+          c.todo = ROW;
+        } else {
+          c.todo = RESIDUAL;
+          c.with_draft = walk.rejections + 1;
+          c.step = 1.0 / walk.total;
+        }
+      }
+      if (warp == 0) {
+        if (c.todo == ROW) {
+          c.token = walk.at;
+          c.with_draft = a.draft && child_of(sh, walk.at, walk.at, count) >= 0;
+          if (lane == 0) sh.path[walk.length] = walk.at;
+          walk.length++;
+        }
+        __syncwarp();
+        if (lane < a.parts) cluster_put(&sh.command, lane, c);
+      }
     }
     cluster_sync();
   }
-  if (rank != 0) return;
-  for (int i = threadIdx.x; i < a.n_tokens; i += THREADS)
-    a.path[(int64_t)b * a.n_tokens + i] = count > 0 && i < length ? sh.path[i] : -1;
-  if (threadIdx.x == 0) {
-    a.accepted[b] = count > 0 ? length : 0;
-    a.next[b] = next;
+  if (rank != 0 || warp != 0) return;
+  __syncwarp();
+  for (int i = lane; i < a.n_tokens; i += 32) a.path[(int64_t)b * a.n_tokens + i] = count > 0 && i < walk.length ? sh.path[i] : -1;
+  if (lane == 0) {
+    a.accepted[b] = count > 0 ? walk.length : 0;
+    a.next[b] = walk.next;
   }
 }
 
@@ -474,16 +629,28 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
                         (const void*)uniforms, (const void*)path, (const void*)accepted, (const void*)next})
     WDC_REQUIRE(ctx, (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: buffers are not aligned", who);
   VerifyArgs a = {logits, draft_logits, uniforms, tokens, parents, counts, path, accepted, next, ctx->status_word,
-                  d->logits_sb, d->logits_st, d->draft_sb, d->draft_st, (int)d->tokens, (int)d->vocab, 1, 0.0, 0.0};
+                  d->logits_sb, d->logits_st, d->draft_sb, d->draft_st, (int)d->tokens, (int)d->vocab, 1, 1, 1, 0.0, 0.0};
   const double to16 = 16 * 1.4426950408889634;     // 16 log2(e)
   if (d->temperature > 0.f) a.scale = to16 / d->temperature;
   if (d->draft_temperature > 0.f) a.draft_scale = to16 / d->draft_temperature;
   while (a.parts < PARTS_MOST && d->batch * a.parts < ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
+  // Shared memory for the logits of a warp's range, or for as many of them as there is room for.
+  const int sides = draft_logits ? 2 : 1;
+  const int64_t each = ceil_div64((d->vocab + 6) / 4, a.parts * WARPS), most = SLICE_BYTES / (16 * WARPS * sides);
+  a.chunk = (int)(each < most ? each : most);
+  a.chunks = (int)ceil_div64(each, a.chunk);
   DeviceGuard g(ctx->device);
+  static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
+  WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "%s: device index out of range", who);
+  if (!opted_in[ctx->device]) {
+    WDC_CUDA(ctx, cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SLICE_BYTES));
+    opted_in[ctx->device] = true;
+  }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(d->batch * a.parts));
   cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)(16 * WARPS * sides) * a.chunk;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
