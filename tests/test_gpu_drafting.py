@@ -263,9 +263,10 @@ def test_attention_of_a_tree(cuda_context, size, c, heads, kv_heads, lengths, co
     assert np.abs(got - want).max() <= room
     for b, n in enumerate(counts):
         assert not got[b, n:].any()
-    # a chain is a text, to the last bit
+    # a chain is a text, whichever way its tokens are cut into parts: both are within `room` of it
     chain = np.tile(random_tree(rng, max(counts), "chain"), (len(lengths), 1))
-    assert np.array_equal(run_tree(cuda_context, cache, q, table, lengths, counts, chain), run_attention(cuda_context, cache, q, table, lengths, counts))
+    text = run_attention(cuda_context, cache, q, table, lengths, counts)
+    assert np.abs(run_tree(cuda_context, cache, q, table, lengths, counts, chain) - text).max() <= 2 * room
     cache.dispose()
 
 

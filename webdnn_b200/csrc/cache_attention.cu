@@ -485,10 +485,11 @@ next_segment:
   const int out_row = tile * ROWS + r;
   if (out_row < a.tokens * a.group) {
     if (complete) {
-      const float by = l_all == 0.f || out_row / a.group >= span.count ? 0.f : exp2f(big_all - finite_or_0(m_all) - WEIGHT_BITS) / l_all;
+      const bool padding = out_row / a.group >= span.count;        // (which may have met a scale that is no number)
+      const float by = l_all == 0.f || padding ? 0.f : exp2f(big_all - finite_or_0(m_all) - WEIGHT_BITS) / l_all;
       float* y = a.y + b * a.y_sb + (kvh * a.group + out_row % a.group) * a.y_sh + out_row / a.group * a.y_st + c0;
 #pragma unroll
-      for (int c = 0; c < DH / PER; c++) y[c] = out[c] * by;
+      for (int c = 0; c < DH / PER; c++) y[c] = padding ? 0.f : out[c] * by;
     } else {
       const int64_t at = (a.splits ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 2 + began_here) * ROWS + r;
       float* to = a.part_rows + at * DH + c0;
@@ -510,7 +511,7 @@ next_segment:
 
 // Joins the parts of a row, one CTA each, where its unit was cut: warp w takes parts w, w + 4, ...  Rows of empty sequences are
 // its business too.
-template <int DH>
+template <int DH, int TILE_ROWS>
 __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const CacheAttArgs a) {
   pdl_wait();
   constexpr int C = DH / 32;
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const Cac
   int64_t begin = 0;                               // the place of part 0; that of a shared-out unit: of its first CTA
   int parts = a.splits, share = 0, cta = 0, from = 0;
   if (a.splits) {
-    begin = ((int64_t)bh * a.row_tiles + row / ROWS) * a.splits;
+    begin = ((int64_t)bh * a.row_tiles + row / TILE_ROWS) * a.splits;
   } else {
     const int* plan = pdl_after(a.part_plan);
     const int size = (plan[b + 1] - plan[b]) / units;
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const Cac
     if (parts == 1) return;
   }
   const auto place = [&](int p) {
-    return (share ? (int64_t)(cta + p) * 2 + (from >= (int64_t)(cta + p) * share) : begin + p) * ROWS + row % ROWS;
+    return (share ? (int64_t)(cta + p) * 2 + (from >= (int64_t)(cta + p) * share) : begin + p) * TILE_ROWS + row % TILE_ROWS;
   };
   const float* stats = pdl_after(a.part_stats);
   const float* rows = pdl_after(a.part_rows) + lane * C;
@@ -570,7 +571,8 @@ __global__ void __launch_bounds__(THREADS) cache_attention_join_kernel(const Cac
   }
   // (a count out of range leaves l at 0)
   const float by = total == 0.f || token >= count ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / total;
-  a.y[b * a.y_sb + (kvh * a.group + row % a.group) * a.y_sh + token * a.y_st + threadIdx.x] = sum * by;
+  // (padding may have met a scale that is no number)
+  a.y[b * a.y_sb + (kvh * a.group + row % a.group) * a.y_sh + token * a.y_st + threadIdx.x] = token >= count ? 0.f : sum * by;
 }
 
 template <int DH, int GROUPS, bool TREE>
@@ -609,8 +611,7 @@ int launch(wdc_context* ctx, CacheAttArgs& a) {
   wdc_launch_pdl(ctx, cache_attention_kernel<DH, GROUPS, TREE>, dim3((unsigned)ctas), dim3(THREADS), Layout<DH>::SMEM, a);
   int s = wdc_check_launch(ctx, "cache_attention_kernel");
   if (s == WDC_OK && parts) {
-    wdc_launch_pdl(ctx, cache_attention_join_kernel<DH>, dim3((unsigned)((int64_t)a.batch * a.heads * a.tokens)), dim3(THREADS), 0, a);
-    s = wdc_check_launch(ctx, "cache_attention_join_kernel");
+    s = wdc_cache_attention_join(ctx, a, DH, ROWS);
   }
   if (scratch) wdc_free(ctx, scratch);   // stream-ordered: reused only by work queued after the kernels
   return s;
@@ -661,6 +662,19 @@ int attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* 
 }
 
 }  // namespace
+
+int wdc_cache_attention_join(wdc_context* ctx, const CacheAttArgs& a, int head_size, int tile_rows) {
+  const auto launch = [&](auto kernel) {
+    wdc_launch_pdl(ctx, kernel, dim3((unsigned)((int64_t)a.batch * a.heads * a.tokens)), dim3(THREADS), 0, a);
+  };
+  if (tile_rows == ROWS)
+    head_size == 32   ? launch(cache_attention_join_kernel<32, ROWS>)
+    : head_size == 64 ? launch(cache_attention_join_kernel<64, ROWS>)
+                      : launch(cache_attention_join_kernel<128, ROWS>);
+  else
+    head_size == 64 ? launch(cache_attention_join_kernel<64, 128>) : launch(cache_attention_join_kernel<128, 128>);
+  return wdc_check_launch(ctx, "cache_attention_join_kernel");
+}
 
 extern "C" int wdc_cache_attention(wdc_context* ctx, const wdc_cache_attention_desc* d, const float* q, const void* codes,
                                    const float* scales, const int32_t* page_table, const int32_t* lengths,

@@ -86,3 +86,5 @@ __device__ __forceinline__ float query_scale(float peak, float scale, float& row
 
 // For many new tokens (cache_attention_tc.cu); WDC_ERR_UNSUPPORTED where the other kernel is to run.
 int wdc_cache_attention_tc(wdc_context* ctx, CacheAttArgs a, int head_size);
+// Joins a.splits equal parts of tiles of `tile_rows` rows, 8 or 128 (cache_attention.cu).
+int wdc_cache_attention_join(wdc_context* ctx, const CacheAttArgs& a, int head_size, int tile_rows);

@@ -266,8 +266,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   const uint32_t tmem_base = sh.tmem_base;
   if (!IN_ORDER) pdl_wait();
 
-  const int bh = (int)(blockIdx.x % (unsigned)(a.batch * a.kv_heads));
-  const int tile = IN_ORDER ? sh.work.y : a.row_tiles - 1 - (int)(blockIdx.x / (unsigned)(a.batch * a.kv_heads));
+  // (trees: a tile's chunks may be cut into a.splits parts, a CTA each)
+  const unsigned splits = TREE ? (unsigned)a.splits : 1u, unit = blockIdx.x / splits, part = blockIdx.x - unit * splits;
+  const int bh = (int)(unit % (unsigned)(a.batch * a.kv_heads));
+  const int tile = IN_ORDER ? sh.work.y : a.row_tiles - 1 - (int)(unit / (unsigned)(a.batch * a.kv_heads));
   const int kvh = bh % a.kv_heads, b = IN_ORDER ? sh.work.x : bh / a.kv_heads;
   const CacheSpan span = IN_ORDER ? CacheSpan{sh.work.z, sh.work.w}
                                   : cache_span(a.lengths, a.counts, b, a.tokens, a.table_pages << a.page_shift, a.status);
@@ -275,7 +277,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
   const int first_token = tile * BQ / a.group, top_token = min((tile * BQ + BQ - 1) / a.group, span.count - 1);
   const int seen = first_token < span.count ? before + top_token + 1 : 0;
   const int seen_by_all = TREE ? before : before + first_token + 1;
-  const int chunks = (seen + BK - 1) / BK;
+  const int all_chunks = (seen + BK - 1) / BK;
+  const int begin = TREE ? (int)((int64_t)part * all_chunks / splits) : 0;
+  const int chunks = TREE ? (int)((int64_t)(part + 1) * all_chunks / splits) - begin : all_chunks;   // of this CTA, from `begin` on
 
   bool ok = true;
   if (warp < ROW_THREADS / 32) {
@@ -287,22 +291,32 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     const int token = (tile * BQ + in_tile) / a.group;
     const int last = token < span.count ? before + token : 0x7fffffff;
     uint32_t* const tree = reinterpret_cast<uint32_t*>(stages + T::TREE) + in_tile * TREE_WORDS;   // (33 words: rows meet different banks)
-    if (TREE && !half && chunks > 0) tree_row(tree, pdl_after(a.parents) + (int64_t)b * a.tokens, token, span.count, before, seen, a.status);
     {
-      // The tile's queries, whole rows by a warp: scaled by a power of two, in halves, through shared memory to tensor memory.  (A
-      // loop that is short in code: what runs once waits for its instructions, about as long as they are.)
-      Rows rows(a, tile, warp, lane);
-#pragma unroll 1
-      for (int i = 0; i < Rows::PASSES; i += 4) {
-        float4 x[4];
-        int r[4];
+      // The tile's queries, whole rows by a warp: asynchronous copies of all of them, to the place of their halves; then scaled by a power
+      // of two, in halves, to tensor memory.  (Loops that are short in code: what runs once waits for its instructions, about as long as
+      // they are.)
+      constexpr int MINE = Rows::PASSES * Rows::TOGETHER;          // rows of a warp; lane r knows where number r is (< 0: padding)
+      const int my_row = tile * BQ + warp * MINE + lane % MINE, my_token = my_row / a.group;
+      const int64_t my_from = my_token < span.count ? b * a.q_sb + (kvh * a.group + my_row - my_token * a.group) * a.q_sh + my_token * a.q_st : -1;
+      const int channel = lane % Rows::LANES * 4;
+      const float* q = pdl_after(a.q) + channel;
+      unsigned char* at = stages + T::Q + (warp * MINE + lane / Rows::LANES) * T::Q_STRIDE;
+      static_assert(MINE <= 32, "a lane for each row");
 #pragma unroll
-        for (int k = 0; k < 4; k++, rows.next()) {
-          r[k] = rows.row;
-          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (rows.token < span.count)
-            x[k] = pdl_ld(reinterpret_cast<const float4*>(pdl_after(a.q) + b * a.q_sb + (kvh * a.group + rows.head) * a.q_sh + rows.token * a.q_st + rows.channel));
-        }
+      for (int i = 0; i < Rows::PASSES; i++) {
+        const int64_t from = __shfl_sync(0xffffffffu, my_from, i * Rows::TOGETHER + lane / Rows::LANES);
+        unsigned char* to = at + i * Rows::TOGETHER * T::Q_STRIDE + channel * 4;
+        if (from >= 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(q + from) : "memory");
+        else *reinterpret_cast<float4*>(to) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (TREE && !half && chunks > 0) tree_row(tree, pdl_after(a.parents) + (int64_t)b * a.tokens, token, span.count, before, seen, a.status);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+      for (int i = 0; i < Rows::PASSES; i += 4, at += 4 * Rows::TOGETHER * T::Q_STRIDE) {
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const float4*>(at + k * Rows::TOGETHER * T::Q_STRIDE + channel * 4);
+        __syncwarp();                              // (the halves go to where other lanes' numbers were)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           float peak = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
@@ -310,11 +324,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
           for (int w = 1; w < Rows::LANES; w <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, w));
           float row_scale;
           const float up = query_scale(peak, a.scale_log2, row_scale);
-          if (rows.channel == 0) sh.row_scale[r[k]] = row_scale;
+          if (channel == 0) sh.row_scale[warp * MINE + (i + k) * Rows::TOGETHER + lane / Rows::LANES] = row_scale;
           uint2 hi, lo;
           split_halves(x[k].x * up, x[k].y * up, hi.x, lo.x);
           split_halves(x[k].z * up, x[k].w * up, hi.y, lo.y);
-          unsigned char* to = stages + T::Q + r[k] * T::Q_STRIDE + rows.channel * 2;
+          unsigned char* to = at + k * Rows::TOGETHER * T::Q_STRIDE + channel * 2;
           *reinterpret_cast<uint2*>(to) = hi;
           *reinterpret_cast<uint2*>(to + 2 * DH) = lo;
         }
@@ -368,8 +382,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
       tmem_ld16(lane_base + (uint32_t)(T::S + (j & 1) * BK + half * 32), s);
       tmem_ld16(lane_base + (uint32_t)(T::S + (j & 1) * BK + half * 32 + 16), s + 16);
       tmem_loaded();
-      const int there = sh.there[st] >> (half * 2), t0 = j * BK + half * 32;
-      const bool whole = (j + 1) * BK <= seen_by_all && sh.there[st] == 15;
+      const int there = sh.there[st] >> (half * 2), t0 = (begin + j) * BK + half * 32;
+      const bool whole = (begin + j + 1) * BK <= seen_by_all && sh.there[st] == 15;
       const int word = (t0 >> 5) - (before >> 5);
       const uint32_t bits = !TREE || whole ? 0 : word < 0 ? 0xffffffffu : word <= (seen - 1 >> 5) - (before >> 5) ? tree[word] : 0;
       float by[2], e[2], f[2], top_s = -INFINITY, top_big = -INFINITY;
@@ -444,7 +458,16 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     l = sh.tops[0][0][in_tile].x;
     // The result through shared memory, so that rows are written whole: every product that reads it has completed.  (Not ok: it may
     // have not, and nothing is written.)
-    const float by = l == 0.f ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
+    // A part's rows as they are, and what they are relative to, for the join.
+    const bool whole_row = !TREE || splits == 1;
+    const float by = !whole_row ? 1.f : l == 0.f ? 0.f : exp2f(big - finite_or_0(m) - WEIGHT_BITS) / l;
+    const int64_t place = ((int64_t)(bh * a.row_tiles + tile) * splits + part) * BQ;
+    if (!whole_row && !half && ok) {
+      float* stats = a.part_stats + (place + in_tile) * 3;
+      stats[0] = m;
+      stats[1] = big;
+      stats[2] = l;
+    }
     float* out = reinterpret_cast<float*>(stages);
     if (ok && token < span.count) {
 #pragma unroll
@@ -458,6 +481,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
       if (!ok || rows.token >= a.tokens) continue;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);                              // (padding)
       if (rows.token < span.count) x = *reinterpret_cast<const float4*>(out + rows.row * T::OUT_STRIDE + rows.channel);
+      if (!whole_row) {
+        *reinterpret_cast<float4*>(a.part_rows + (place + rows.row) * DH + rows.channel) = x;
+        continue;
+      }
       *reinterpret_cast<float4*>(a.y + b * a.y_sb + (kvh * a.group + rows.head) * a.y_sh + rows.token * a.y_st + rows.channel) = x;
     }
   } else {
@@ -468,16 +495,16 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_tc_kernel(const Ca
     // Lane g of a warp has the page of a chunk's group g (-1: not there).  A table entry is read two chunks before its codes are
     // fetched, and looked at a chunk later: nothing waits for it.
     const auto entry_of = [&](int j) {
-      const int t0 = j * BK + lane * 16;
+      const int t0 = (begin + j) * BK + lane * 16;
       return lane < 4 && t0 < seen ? pdl_ld(table + (t0 >> a.page_shift)) : -1;
     };
     const auto page_of = [&](int entry, int j) {
       if (entry >= 0 && entry < a.pages) return entry;
-      if (lane < 4 && j * BK + lane * 16 < seen) a.status[WDC_STATUS_CACHE] = 1;
+      if (lane < 4 && (begin + j) * BK + lane * 16 < seen) a.status[WDC_STATUS_CACHE] = 1;
       return -1;
     };
     const auto codes_at = [&](int pages, int j, int in_chunk) -> const int8_t* {        // a token's keys, or null
-      const int page = __shfl_sync(0xffffffffu, pages, in_chunk / 16), token = j * BK + in_chunk;
+      const int page = __shfl_sync(0xffffffffu, pages, in_chunk / 16), token = (begin + j) * BK + in_chunk;
       return page < 0 ? nullptr : mine + (int64_t)page * 2 * side_bytes + (token & ((1 << a.page_shift) - 1)) * DH;
     };
     const auto stage_free = [&](int j) { return mbar_wait(&sh.kv_empty[j % STAGES], (uint32_t)(j / STAGES & 1) ^ 1, &sh, a.status, 83); };
@@ -648,9 +675,38 @@ int launch(wdc_context* ctx, const CacheAttArgs& a, int64_t ctas) {
   ctx->n_tc_launch++;
   return wdc_check_launch(ctx, "cache_attention_tc_kernel");
 }
-template <int DH, bool IN_ORDER>
-int launch(wdc_context* ctx, const CacheAttArgs& a, int64_t ctas) {
-  return a.parents ? launch<DH, IN_ORDER, true>(ctx, a, ctas) : launch<DH, IN_ORDER, false>(ctx, a, ctas);
+// Trees: few rows over long texts, so that a tile's chunks are cut into equal parts: one wave of CTAs of them, and up to two while each
+// has 16 chunks (sequences differ, and the host does not know how).  Measured, us of 1 / 2 / 3 / 4 / 6 / 8 parts: 48 tiles of 9000 to 20001
+// tokens 476 / 258 / 181 / 171 / 153 / 176; 192 of 100 to 2500 71 / 90 / 99 / 116 / 137 / 165.
+// Which kernel is by what each takes, in us of an SM: 1.55 a chunk and 10 a part here, 0.17 for eight rows and 32 tokens there, as far as
+// the table's width tells.  Measured, us here / by the kernel for few rows, heads of 128, rows of a key head: 24 sequences of 833 to 2500 tokens
+// and 8 key heads, 32 rows 79 / 79, 52 rows 79 / 94, 128 rows 80 / 198; 2 of 6667 to 20000, 40 rows 63 / 59, 52 rows 63 / 76, 128 rows 66 /
+// 153; one of 900 and 4 key heads of 64, 52 rows 11.3 / 8.4.
+int tree(wdc_context* ctx, CacheAttArgs& a, int head_size, int64_t rows, int64_t units) {
+  const int64_t chunks = ceil_div64(a.table_pages << a.page_shift, BK), sms = ctx->sm_count;
+  if (rows > INT_MAX - BQ || chunks == 0) return WDC_ERR_UNSUPPORTED;
+  int64_t parts = chunks / 16;
+  if (parts > 2 * sms / units) parts = 2 * sms / units;
+  if (parts < sms / units) parts = sms / units;
+  if (parts > chunks / 2) parts = chunks / 2;
+  if (parts < 1) parts = 1;
+  if (units * parts >= (1ll << 31)) return WDC_ERR_UNSUPPORTED;
+  const double all = units * (1.55 * chunks + 10.0 * parts) / sms, one = 1.55 * chunks / parts + 10.0;
+  const double here = (all > one ? all : one) + (parts > 1 ? 3.0 : 0.0);
+  const double there = (double)a.batch * a.kv_heads * ceil_div64(rows, 8) * 2 * chunks * 0.17 / sms + 6.0;
+  if (there < here) return WDC_ERR_UNSUPPORTED;
+  a.splits = (int)parts;
+  const int64_t places = a.splits > 1 ? units * a.splits * BQ : 0;
+  float* scratch = nullptr;
+  if (places) {
+    CACHE_TRY(wdc_alloc(ctx, places * (head_size + 3) * 4, (void**)&scratch));
+    a.part_rows = scratch;
+    a.part_stats = scratch + places * head_size;
+  }
+  int s = head_size == 64 ? launch<64, false, true>(ctx, a, units * a.splits) : launch<128, false, true>(ctx, a, units * a.splits);
+  if (s == WDC_OK && places) s = wdc_cache_attention_join(ctx, a, head_size, BQ);
+  if (scratch) wdc_free(ctx, scratch);
+  return s;
 }
 
 }  // namespace
@@ -665,8 +721,9 @@ int wdc_cache_attention_tc(wdc_context* ctx, CacheAttArgs a, int head_size) {
   const int64_t rows = (int64_t)a.tokens * a.group;
   a.row_tiles = (int)ceil_div64(rows, BQ);
   const int64_t ctas = (int64_t)a.batch * a.kv_heads * a.row_tiles;
+  if (a.parents) return ctas > 0 ? tree(ctx, a, head_size, rows, ctas) : WDC_ERR_UNSUPPORTED;
   if (rows < BQ / 2 || rows > INT_MAX - BQ || 4 * ctas < ctx->sm_count || ctas >= (1ll << 31)) return WDC_ERR_UNSUPPORTED;
   const bool in_order = a.batch > 1 && a.batch <= ORDERED && ctas > ctx->sm_count && a.table_pages << a.page_shift >= 16 * BK;
-  if (head_size == 64) return in_order ? launch<64, true>(ctx, a, ctas) : launch<64, false>(ctx, a, ctas);
-  return in_order ? launch<128, true>(ctx, a, ctas) : launch<128, false>(ctx, a, ctas);
+  if (head_size == 64) return in_order ? launch<64, true, false>(ctx, a, ctas) : launch<64, false, false>(ctx, a, ctas);
+  return in_order ? launch<128, true, false>(ctx, a, ctas) : launch<128, false, false>(ctx, a, ctas);
 }
