@@ -20,7 +20,7 @@ from typing import List
 import numpy as np
 
 from ..backend import NP_DTYPE, CPUTensor, CudaTensor, WebDNNCudaContext
-from ..lib import BINARY_OPS, REDUCE_KINDS, UNARY_OPS, AttentionDesc, ConvDesc, ConvTransposeDesc, GemmDesc, PoolDesc
+from ..lib import BINARY_OPS, REDUCE_KINDS, UNARY_OPS, AttentionDesc, ConvDesc, ConvTransposeDesc, GemmDesc, PoolDesc, RotateDesc
 from ..operator_table import OperatorEntry
 from . import base
 from .base import (OperatorImpl, array_prod, broadcast_multi, broadcast_uni, get_attr_float, get_attr_int,
@@ -357,6 +357,14 @@ class CudaAttention(OperatorImpl):
         return [y]
 
 
+def _extras(attribute, who: str, known) -> List[str]:
+    """The names in the attribute ``extras``, with commas between."""
+    names = [n for n in get_attr_string(attribute, "extras", "").split(",") if n]
+    if len(set(names)) != len(names) or not set(names) <= set(known):
+        raise ValueError(f"{who}: extras are some of {', '.join(known)}, not {names}")
+    return names
+
+
 class CudaCacheAttention(OperatorImpl):
     """A decoder layer's self-attention over a paged 8-bit cache: the new tokens' keys and values are appended, then the
     new tokens attend to their sequences.  No operator of the reference, whose graphs keep nothing between runs.
@@ -364,12 +372,21 @@ class CudaCacheAttention(OperatorImpl):
     Inputs q, k, v [batch, tokens, width], page_table [batch, pages], lengths [batch] and, optionally, counts [batch] (int32, as
     ``PagedCache.batch`` gives them); the result is [batch, tokens, heads * head_size].  Attributes: ``cache``, the name the
     cache was given (``WebDNNCudaContext.add_cache``); ``layer``; ``scale`` (1 / sqrt(head_size) unless given); ``heads``
-    and ``q_column``, ``k_column``, ``v_column`` where an operand is some columns of its tensor."""
+    and ``q_column``, ``k_column``, ``v_column`` where an operand is some columns of its tensor.
+
+    ``extras`` names, with commas between, the inputs that follow counts (which is there then): ``positions``, ``cos``, ``sin``, ``q_weight``,
+    ``k_weight`` (queries and keys are normalised and rotated on the way, ``PagedCache.append_rotary``; attributes ``epsilon`` and
+    ``interleaved``) and ``parents`` (the new tokens are a tree)."""
+
+    EXTRAS = ("positions", "cos", "sin", "q_weight", "k_weight", "parents")
 
     def __init__(self):
         super().__init__("cuda")
 
     def initialize(self, attribute):
+        self.extras = _extras(attribute, "CudaCacheAttention", self.EXTRAS)
+        self.epsilon = get_attr_float(attribute, "epsilon", 1e-6)
+        self.interleaved = bool(get_attr_int(attribute, "interleaved", 0))
         self.cache = get_attr_string(attribute, "cache", "")
         self.layer = get_attr_int(attribute, "layer", 0)
         self.heads = get_attr_int(attribute, "heads", 0) or None
@@ -379,14 +396,139 @@ class CudaCacheAttention(OperatorImpl):
 
     def run(self, context, inputs, n_outputs):
         context.asserts_cuda_tensor_array(inputs)
-        if len(inputs) not in (5, 6):
-            raise ValueError("CudaCacheAttention: inputs are q, k, v, page_table, lengths and, optionally, counts")
+        if len(inputs) not in ((6 + len(self.extras),) if self.extras else (5, 6)):
+            raise ValueError("CudaCacheAttention: inputs are q, k, v, page_table, lengths and, optionally, counts"
+                             + "".join(f", {name}" for name in self.extras))
         cache = context.caches.get(self.cache)
         if cache is None:
             raise ValueError(f"CudaCacheAttention: the context has no cache {self.cache!r}")
-        q, k, v, *where = inputs
-        cache.append(self.layer, k, v, *where, k_column=self.columns[1], v_column=self.columns[2])
-        return [cache.attention(self.layer, q, *where, heads=self.heads, q_column=self.columns[0], scale=self.scale)]
+        q, k, v, *where = inputs[:6]
+        given = dict(zip(self.extras, inputs[6:]))
+        parents = given.pop("parents", None)
+        columns = dict(k_column=self.columns[1], v_column=self.columns[2])
+        if not given:
+            cache.append(self.layer, k, v, *where, **columns)
+            return [cache.attention(self.layer, q, *where, heads=self.heads, q_column=self.columns[0], scale=self.scale, parents=parents)]
+        q = cache.append_rotary(self.layer, k, v, *where, q=q, heads=self.heads, epsilon=self.epsilon, interleaved=self.interleaved,
+                                q_column=self.columns[0], **columns, **given)
+        y = cache.attention(self.layer, q, *where, scale=self.scale, parents=parents)
+        q.dispose()
+        return [y]
+
+
+class CudaRotateHeads(OperatorImpl):
+    """Heads normalised and rotated by their position (``WebDNNCudaContext.rotate_heads``).  No operator of the reference.
+
+    Input x [..., n]; ``extras`` names the inputs that follow: ``positions``, ``cos``, ``sin``, ``weight``.  Attributes: ``heads``,
+    ``head_size``, ``epsilon``, ``interleaved``, ``column``."""
+
+    EXTRAS = ("positions", "cos", "sin", "weight")
+
+    def __init__(self):
+        super().__init__("cuda")
+
+    def initialize(self, attribute):
+        self.extras = _extras(attribute, "CudaRotateHeads", self.EXTRAS)
+        self.heads, self.head_size = get_attr_int(attribute, "heads", 1), get_attr_int(attribute, "head_size", 0)
+        self.epsilon = get_attr_float(attribute, "epsilon", 1e-6)
+        self.interleaved = bool(get_attr_int(attribute, "interleaved", 0))
+        self.column = get_attr_int(attribute, "column", 0)
+
+    def run(self, context, inputs, n_outputs):
+        context.asserts_cuda_tensor_array(inputs)
+        if len(inputs) != 1 + len(self.extras):
+            raise ValueError("CudaRotateHeads: inputs are x" + "".join(f", {name}" for name in self.extras))
+        x = context.canonical(inputs[0])
+        y = context.rotate_heads(x, self.heads, self.head_size, epsilon=self.epsilon, interleaved=self.interleaved, column=self.column,
+                                 **dict(zip(self.extras, inputs[1:])))
+        if x is not inputs[0]:
+            x.dispose()
+        return [y]
+
+
+class CudaRotaryEmbedding(OperatorImpl):
+    """ONNX RotaryEmbedding (opset 23; not in the reference): X [batch, tokens, heads * head_size] (attribute ``num_heads``) or [batch, heads,
+    tokens, head_size], cos_cache and sin_cache [places, pairs] with position_ids [batch, tokens], or [batch, tokens, pairs] without.
+    Pairs are a multiple of 4, head_size a multiple of 4 up to 256."""
+
+    def __init__(self):
+        super().__init__("cuda")
+
+    def initialize(self, attribute):
+        self.interleaved = bool(get_attr_int(attribute, "interleaved", 0))
+        self.num_heads = get_attr_int(attribute, "num_heads", 0)
+        self.rotary = get_attr_int(attribute, "rotary_embedding_dim", 0)
+
+    def run(self, context, inputs, n_outputs):
+        context.asserts_cuda_tensor_array(inputs)
+        if len(inputs) not in (3, 4):
+            raise ValueError("RotaryEmbedding: inputs are X, cos_cache, sin_cache and, optionally, position_ids")
+        x, cos, sin = (context.canonical(t) for t in inputs[:3])
+        positions = inputs[3] if len(inputs) == 4 else None
+        try:
+            if x.ndim == 4:
+                batch, heads, tokens, size = x.dims
+            elif x.ndim == 3 and self.num_heads > 0 and x.dims[2] % self.num_heads == 0:
+                batch, tokens, heads, size = *x.dims[:2], self.num_heads, x.dims[2] // self.num_heads
+            else:
+                raise ValueError("RotaryEmbedding: X is [batch, heads, tokens, head_size], or [batch, tokens, n] with num_heads")
+            pairs = (self.rotary or size) // 2
+            want = [batch, tokens, pairs] if positions is None else [cos.dims[0] if cos.ndim else 0, pairs]
+            if cos.dims != want or sin.dims != want:
+                raise ValueError(f"RotaryEmbedding: cos_cache and sin_cache are {want}, not {cos.dims} and {sin.dims}")
+            if positions is not None:
+                context.asserts_int_rows("RotaryEmbedding", "position_ids", positions, [batch, tokens])
+            # (a table that has a row for each token is a table of batch * tokens places)
+            cos, sin = (t if positions is not None else t.alias([batch * tokens, pairs]) for t in (cos, sin))
+            if x.ndim == 3:
+                return [context.rotate_heads(x, heads, size, cos=cos, sin=sin, positions=positions, interleaved=self.interleaved)]
+            context.asserts_rotation("RotaryEmbedding", size, cos, sin, positions, ())
+            if size % 4 or size > 256:
+                raise ValueError(f"RotaryEmbedding: heads of {size} (a multiple of 4 up to 256)")
+            y = context.empty_tensor(x.dims)
+            for b in range(batch if x.length else 0):
+                first, at = b * heads * tokens * size * 4, b * tokens * 4
+                skip = 0 if positions is not None else at * pairs
+                desc = RotateDesc(tokens, heads, size, 2 * pairs, cos.dims[0] if positions is not None else tokens, size, tokens * size, size,
+                                  tokens * size, 0.0, self.interleaved)
+                context._call("wdc_rotate_heads", byref(desc), x.ptr + first, None, cos.ptr + skip, sin.ptr + skip,
+                              positions.ptr + at if positions is not None else None, y.ptr + first)
+            return [y]
+        finally:
+            for made, given in zip((x, cos, sin), inputs):
+                if made is not given:
+                    made.dispose()
+
+
+class CudaVerifyDrafts(OperatorImpl):
+    """Which drafted tokens of a tree stand, and the token that follows (``WebDNNCudaContext.verify_drafts``).  No operator of the reference.
+
+    Inputs logits [batch, tokens, vocab] and tokens [batch, tokens]; ``extras`` names the inputs that follow: ``parents``, ``counts``,
+    ``uniforms``, ``draft_logits``.  Attributes: ``temperature`` (1), ``draft_temperature`` (the same).  Results path [batch, tokens],
+    accepted [batch] and next [batch], int32."""
+
+    EXTRAS = ("parents", "counts", "uniforms", "draft_logits")
+
+    def __init__(self):
+        super().__init__("cuda")
+
+    def initialize(self, attribute):
+        self.extras = _extras(attribute, "CudaVerifyDrafts", self.EXTRAS)
+        self.temperature = get_attr_float(attribute, "temperature", 1.0)
+        self.draft_temperature = get_attr_float(attribute, "draft_temperature", self.temperature)
+
+    def run(self, context, inputs, n_outputs):
+        context.asserts_cuda_tensor_array(inputs)
+        if len(inputs) != 2 + len(self.extras):
+            raise ValueError("CudaVerifyDrafts: inputs are logits, tokens" + "".join(f", {name}" for name in self.extras))
+        logits = context.canonical(inputs[0])
+        outs = context.verify_drafts(logits, inputs[1], temperature=self.temperature, draft_temperature=self.draft_temperature,
+                                     **dict(zip(self.extras, inputs[2:])))
+        if logits is not inputs[0]:
+            logits.dispose()
+        for t in outs[n_outputs:]:
+            t.dispose()
+        return list(outs[:n_outputs])
 
 
 class CudaTokenLogProbs(OperatorImpl):
@@ -1193,6 +1335,9 @@ def get_op_entries() -> List[OperatorEntry]:
         E("CudaAttention", 1, None, "cuda", CudaAttention),
         E("CudaCacheAttention", 1, None, "cuda", CudaCacheAttention),
         E("CudaTokenLogProbs", 1, None, "cuda", CudaTokenLogProbs),
+        E("CudaRotateHeads", 1, None, "cuda", CudaRotateHeads),
+        E("RotaryEmbedding", 23, None, "cuda", CudaRotaryEmbedding),
+        E("CudaVerifyDrafts", 1, None, "cuda", CudaVerifyDrafts),
         E("MatMul", 1, None, "cuda", CudaMatMul),
         E("Conv", 1, None, "cuda", CudaConv),
         E("CudaConvFused", 1, None, "cuda", lambda: CudaConv(fused=True)),

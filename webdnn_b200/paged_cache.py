@@ -142,6 +142,8 @@ class PagedCache:
         place in its sequence.  With ``q``, whose ``heads`` * head_size columns from ``q_column`` on count, its heads are too
         (``q_weight``); the result is [batch, tokens, heads * head_size], rows of padding 0."""
         who = "PagedCache.append_rotary"
+        if q is None and (heads or q_column or out is not None or q_weight is not None):
+            raise ValueError(f"{who}: heads, q_column, q_weight and out are of queries")
         rows = (k, v) if q is None else (k, v, q)
         self._operands(who, rows, page_table, lengths, counts)
         extra = (cos, sin, positions, q_weight, k_weight)
@@ -149,7 +151,7 @@ class PagedCache:
         key = ("append_rotary", dims, heads, epsilon, bool(interleaved), q_column, k_column, v_column)
         self.context.asserts_rotation(who, self.head_size, cos, sin, positions, (q_weight, k_weight))
         kept = self._descs.get(key) or self._append_rotary_desc(who, key, k, v, page_table, lengths, counts, cos, positions, q, heads,
-                                                                q_weight, epsilon, interleaved, q_column, k_column, v_column, out)
+                                                                epsilon, interleaved, q_column, k_column, v_column)
         d = kept[1]
         if q is not None:
             shape = [d.append.batch, d.append.tokens, d.heads * self.head_size]
@@ -164,15 +166,13 @@ class PagedCache:
                                at(cos), at(sin), at(positions), *self._at(layer), page_table.ptr, lengths.ptr, at(counts), at(out))
         return out
 
-    def _append_rotary_desc(self, who, key, k, v, page_table, lengths, counts, cos, positions, q, heads, q_weight, epsilon,
-                            interleaved, q_column, k_column, v_column, out):
+    def _append_rotary_desc(self, who, key, k, v, page_table, lengths, counts, cos, positions, q, heads, epsilon, interleaved,
+                            q_column, k_column, v_column):
         fields = self._append_fields(who, k, v, page_table, lengths, counts, k_column, v_column)
         c, batch, tokens = self.head_size, fields.batch, fields.tokens
         if positions is not None and positions.dims != [batch, tokens]:
             raise ValueError(f"{who}: positions are [{batch}, {tokens}]")
         if q is None:
-            if heads or q_column or out is not None or q_weight is not None:
-                raise ValueError(f"{who}: heads, q_column, q_weight and out are of queries")
             heads = width = 0
         else:
             width = q.dims[2] if q.ndim == 3 else 0

@@ -246,27 +246,51 @@ def lstm(seq: int = 128, batch: int = 64, input_size: int = 256, hidden: int = 5
 
 
 def decoder(vocab: int = 1000, d: int = 256, heads: int = 8, kv_heads: int = 2, layers: int = 4, ffn: int = 1024,
-            positions: int = 4096, top: int = 8, cache: str = "cache") -> Model:
+            positions: int = 4096, top: int = 8, cache: str = "cache", rotary: bool = False, drafts: bool = False, temperature: float = 1.0) -> Model:
     """Post-norm decoder whose layers attend over a paged 8-bit cache (``PagedCache``, known to the context as ``cache``), any
     number of sequences and new tokens.  Inputs, all int32: token_ids and places [batch, tokens] (of rows behind a
     sequence's count: anything), page_table, lengths and counts as ``PagedCache.batch`` gives them, rows [n]: which of the
     batch * tokens rows have their logits computed, and tokens [n]: whose log probabilities are wanted.  Outputs of those
-    rows: logprob, entropy [n], top_ids and top_logprobs [n, top]."""
+    rows: logprob, entropy [n], top_ids and top_logprobs [n, top].
+
+    ``rotary``: the heads of queries and keys are normalised and rotated by their places, instead of an embedding of the places.
+    ``drafts``: the new tokens of each sequence are a tree of drafts behind its first, and the outputs say which stand (path
+    [batch, tokens], accepted and next [batch]); instead of rows and tokens, the inputs are parents (int32) and uniforms (float32)
+    [batch, tokens], and ``temperature`` is that of the decision.  Weights are the same with drafts and without."""
     b = _Builder(0)
     t = _Transformer(b, 0, d, heads, ffn)
     table = b.init("embedding", b.rng.standard_normal((vocab, d)).astype(np.float32))
-    place = b.init("place_embedding", b.rng.standard_normal((positions, d)).astype(np.float32))
-    h = b.node("Add", [b.node("Gather", [table, "token_ids"], axis=0)[0], b.node("Gather", [place, "places"], axis=0)[0]])[0]
+    h = b.node("Gather", [table, "token_ids"], axis=0)[0]
+    extras, attributes = [], {}
+    if rotary:
+        angle = np.arange(positions)[:, None] * 10000.0 ** (-np.arange(t.dh // 2) / (t.dh // 2))
+        tables = [b.init("cos", np.cos(angle).astype(np.float32)), b.init("sin", np.sin(angle).astype(np.float32))]
+    else:
+        place = b.init("place_embedding", b.rng.standard_normal((positions, d)).astype(np.float32))
+        h = b.node("Add", [h, b.node("Gather", [place, "places"], axis=0)[0]])[0]
     for layer in range(layers):
         q, k, v = t.linear(h, d, d), t.linear(h, d, kv_heads * t.dh), t.linear(h, d, kv_heads * t.dh)
-        a = b.node("CudaCacheAttention", [q, k, v, "page_table", "lengths", "counts"], cache=cache, layer=layer)[0]
+        if rotary:
+            weights = [b.init(b.name("norm"), b.rng.uniform(0.8, 1.2, t.dh).astype(np.float32)) for _ in range(2)]
+            extras, attributes = ["places", *tables, *weights], dict(extras="positions,cos,sin,q_weight,k_weight")
+        if drafts:
+            extras, attributes = [*extras, "parents"], dict(extras=",".join(filter(None, [attributes.get("extras"), "parents"])))
+        a = b.node("CudaCacheAttention", [q, k, v, "page_table", "lengths", "counts", *extras], cache=cache, layer=layer, **attributes)[0]
+        extras, attributes = [], {}
         h = t.add_norm(h, t.linear(a, d, d))
         h = t.add_norm(h, t.feed_forward(h))
-    h = b.node("Gather", [b.node("Reshape", [h, t.shape([-1, d])])[0], "rows"], axis=0)[0]
-    outs = b.node("CudaTokenLogProbs", [t.linear(h, d, vocab), "tokens"], n_out=4, top=top)
-    ints = [("token_ids", 2), ("places", 2), ("page_table", 2), ("lengths", 1), ("counts", 1), ("rows", 1), ("tokens", 1)]
-    g = Graph("decoder", b.nodes, b.inits, [ValueInfo(n, INT32, [0] * rank) for n, rank in ints],
-              [ValueInfo(o, kind, []) for o, kind in zip(outs, (FLOAT, FLOAT, INT32, FLOAT))])
+    kinds = {"uniforms": FLOAT}
+    ints = [("token_ids", 2), ("places", 2), ("page_table", 2), ("lengths", 1), ("counts", 1)]
+    if drafts:
+        outs = b.node("CudaVerifyDrafts", [t.linear(h, d, vocab), "token_ids", "parents", "counts", "uniforms"], n_out=3,
+                      extras="parents,counts,uniforms", temperature=float(temperature))
+        ints, out_kinds = ints + [("parents", 2), ("uniforms", 2)], (INT32, INT32, INT32)
+    else:
+        h = b.node("Gather", [b.node("Reshape", [h, t.shape([-1, d])])[0], "rows"], axis=0)[0]
+        outs = b.node("CudaTokenLogProbs", [t.linear(h, d, vocab), "tokens"], n_out=4, top=top)
+        ints, out_kinds = ints + [("rows", 1), ("tokens", 1)], (FLOAT, FLOAT, INT32, FLOAT)
+    g = Graph("decoder", b.nodes, b.inits, [ValueInfo(n, kinds.get(n, INT32), [0] * rank) for n, rank in ints],
+              [ValueInfo(o, kind, []) for o, kind in zip(outs, out_kinds)])
     return Model(g, ir_version=7, opset_import=[("", 13)], producer_name="webdnn_b200.zoo")
 
 
