@@ -288,6 +288,7 @@ class WebDNNCudaContext:
         self.precision = "tf32x3"
         self.profile = False      # backendOptions.cuda.profile: NVTX range "name(opType)" around every node
         self.caches: Dict[str, object] = {}   # add_cache
+        self._kept: Dict[tuple, tuple] = {}   # descriptions of calls, by the shapes that they were checked with
 
     # --- lifecycle
     def initialize(self) -> None:
@@ -643,14 +644,29 @@ class WebDNNCudaContext:
         if t.dims != list(dims):
             raise ValueError(f"{who}: {what} is {list(dims)}, not {t.dims}")
 
+    MAX_KEPT = 1024
+
+    def _keep(self, key: tuple, desc, *more) -> tuple:
+        """A description, checked once and kept by the shapes alone."""
+        if len(self._kept) >= self.MAX_KEPT:
+            self._kept.clear()
+        self._kept[key] = kept = (byref(desc), desc, *more)
+        return kept
+
+    def asserts_rows(self, who: str, floats: Sequence[Optional[CudaTensor]], ints: Sequence[Optional[CudaTensor]]) -> None:
+        """Tensors of this context, row-major, of these types; None is left out."""
+        for tensors, kind in ((floats, "float32"), (ints, "int32")):
+            for t in tensors:
+                if t is None:
+                    continue
+                if t.__class__ is not CudaTensor or t.context is not self:
+                    self.asserts_cuda_tensor(t)
+                if t.data_type != kind or t.layout != "nchw":
+                    raise TypeError(f"{who}: an operand is {t.data_type}, {t.layout}, not {kind}, row-major")
+
     def asserts_rotation(self, who: str, head_size: int, cos: Optional[CudaTensor], sin: Optional[CudaTensor],
                          positions: Optional[CudaTensor], weights: Sequence[Optional[CudaTensor]]) -> None:
         """The tables, positions and weights of ``rotate_heads`` fit together."""
-        for t, kind in ((cos, "float32"), (sin, "float32"), (positions, "int32"), *((w, "float32") for w in weights)):
-            if t is not None:
-                self.asserts_cuda_tensor(t)
-                if t.data_type != kind or t.layout != "nchw":
-                    raise TypeError(f"{who}: cos, sin and weights are float32, positions int32, all row-major")
         if (cos is None) != (sin is None) or (cos is None and positions is not None):
             raise ValueError(f"{who}: cos and sin come together, and positions with them")
         if cos is not None and (cos.ndim != 2 or cos.dims != sin.dims or cos.dims[0] < 1 or cos.dims[1] % 4 or not 0 < 2 * cos.dims[1] <= head_size):
@@ -669,30 +685,35 @@ class WebDNNCudaContext:
         (without: no rotation): the first 2 * pairs channels of a head are rotated, channels i and i + pairs together or, with
         ``interleaved``, 2 i and 2 i + 1.  ``positions`` int32, one for each row of ``x`` (without: the row's number).  ``out`` may be
         ``x``, where that has its shape."""
+        self.asserts_rows("rotate_heads", (x, cos, sin, weight), (positions,))
+        key = ("rotate_heads", *(t is not None and tuple(t.dims) for t in (x, cos, sin, positions, weight)), heads, head_size, epsilon, bool(interleaved),
+               column)
+        kept = self._kept.get(key) or self._rotate_desc(key, x, heads, head_size, cos, sin, positions, weight, epsilon, interleaved, column)
+        dims = kept[2]
+        if out is None:
+            out = self.empty_tensor(dims)
+        elif out.__class__ is not CudaTensor or out.context is not self or out.dims != dims or out.data_type != "float32" or out.layout != "nchw" or (
+                out.ptr == x.ptr and (column or out.dims != x.dims)):
+            raise ValueError(f"rotate_heads: the result is float32 {dims}, row-major, in this context, and x only where that has its shape")
+        if out.length:
+            self._call("wdc_rotate_heads", kept[0], x.ptr + 4 * column, weight.ptr if weight is not None else None, cos.ptr if cos is not None else None,
+                       sin.ptr if sin is not None else None, positions.ptr if positions is not None else None, out.ptr)
+        return out
+
+    def _rotate_desc(self, key, x, heads, head_size, cos, sin, positions, weight, epsilon, interleaved, column):
         who = "rotate_heads"
-        self.asserts_cuda_tensor(x)
-        if x.data_type != "float32" or x.layout != "nchw":
-            raise TypeError(f"{who}: x is float32, row-major")
         if heads < 1 or head_size < 1 or head_size % 4 or head_size > 256:
             raise ValueError(f"{who}: {heads} heads of {head_size} (a multiple of 4 up to 256)")
         self.asserts_rotation(who, head_size, cos, sin, positions, (weight,))
         n = x.dims[-1] if x.ndim else 0
         if column < 0 or column % 4 or n % 4 or column + heads * head_size > n:
             raise ValueError(f"{who}: {heads} heads of {head_size} from column {column} on, of {x.dims} (multiples of 4)")
-        rows, dims = x.length // n, x.dims[:-1] + [heads * head_size]
+        rows = x.length // n
         if positions is not None and positions.length != rows:
             raise ValueError(f"{who}: positions are one for each of {rows} rows")
-        if out is None:
-            out = self.empty_tensor(dims)
-        elif out.__class__ is not CudaTensor or out.context is not self or out.dims != dims or out.data_type != "float32" or out.layout != "nchw" or (
-                out.ptr == x.ptr and (column or out.dims != x.dims)):
-            raise ValueError(f"{who}: the result is float32 {dims}, row-major, in this context, and x only where that has its shape")
-        if rows:
-            pointers = [t.ptr if t is not None else None for t in (weight, cos, sin, positions)]
-            desc = RotateDesc(rows, heads, head_size, 2 * cos.dims[1] if cos is not None else 0, cos.dims[0] if cos is not None else 0, n, head_size,
-                              heads * head_size, head_size, epsilon, interleaved)
-            self._call("wdc_rotate_heads", byref(desc), x.ptr + 4 * column, *pointers, out.ptr)
-        return out
+        desc = RotateDesc(rows, heads, head_size, 2 * cos.dims[1] if cos is not None else 0, cos.dims[0] if cos is not None else 0, n, head_size,
+                          heads * head_size, head_size, epsilon, interleaved)
+        return self._keep(key, desc, x.dims[:-1] + [heads * head_size])
 
     def verify_drafts(self, logits: CudaTensor, tokens: CudaTensor, parents: Optional[CudaTensor] = None,
                       counts: Optional[CudaTensor] = None, uniforms: Optional[CudaTensor] = None,
@@ -706,20 +727,36 @@ class WebDNNCudaContext:
         [batch, tokens, n], behind each token, of which the first ``vocab`` columns count (all, if not given); ``draft_logits`` the
         distribution that a token's children were drawn from, where they were (by ``draft_temperature``: ``temperature`` unless given).
         ``uniforms`` float32 [batch, tokens] in [0, 1): random numbers.  ``temperature`` 0: the largest logit, no random numbers."""
+        self.asserts_rows("verify_drafts", (logits, uniforms, draft_logits), (tokens, parents, counts))
+        key = ("verify_drafts", *(t is not None and tuple(t.dims) for t in (logits, tokens, parents, counts, uniforms, draft_logits)), temperature,
+               draft_temperature, vocab)
+        kept = self._kept.get(key) or self._verify_desc(key, logits, tokens, parents, counts, uniforms, draft_logits, temperature, draft_temperature, vocab)
+        shapes = kept[2]
+        if out is None:
+            out = tuple(self.empty_tensor(s, "int32") for s in shapes)
+        elif len(out) != 3:
+            raise ValueError("verify_drafts: out is (path, accepted, next)")
+        else:
+            self.asserts_rows("verify_drafts", (), out)
+            for t, s in zip(out, shapes):
+                if t.dims != s:
+                    raise ValueError(f"verify_drafts: a result is {s}, not {t.dims}")
+        path, accepted, following = out
+        if accepted.length:
+            self._call("wdc_verify_drafts", kept[0], logits.ptr if logits.length else None,
+                       draft_logits.ptr if draft_logits is not None and draft_logits.length else None, tokens.ptr if tokens.length else None,
+                       parents.ptr if parents is not None and parents.length else None, counts.ptr if counts is not None else None,
+                       uniforms.ptr if uniforms is not None and uniforms.length else None, path.ptr if path.length else None, accepted.ptr, following.ptr)
+        return tuple(out)
+
+    def _verify_desc(self, key, logits, tokens, parents, counts, uniforms, draft_logits, temperature, draft_temperature, vocab):
         who = "verify_drafts"
-        for t, what in ((logits, "logits"), (uniforms, "uniforms"), (draft_logits, "draft_logits")):
-            if t is not None:
-                self.asserts_cuda_tensor(t)
-                if t.data_type != "float32" or t.layout != "nchw":
-                    raise TypeError(f"{who}: {what} are float32, row-major")
         if logits.ndim != 3:
             raise ValueError(f"{who}: logits are [batch, tokens, vocab]")
         batch, n, width = logits.dims
-        self.asserts_int_rows(who, "tokens", tokens, [batch, n])
-        if parents is not None:
-            self.asserts_int_rows(who, "parents", parents, [batch, n])
-        if counts is not None:
-            self.asserts_int_rows(who, "counts", counts, [batch])
+        for t, what, dims in ((tokens, "tokens", [batch, n]), (parents, "parents", [batch, n]), (counts, "counts", [batch]), (uniforms, "uniforms", [batch, n])):
+            if t is not None and t.dims != dims:
+                raise ValueError(f"{who}: {what} are {dims}, not {t.dims}")
         vocab = width if vocab is None else vocab
         if not 0 < vocab <= width:
             raise ValueError(f"{who}: vocab {vocab} of rows of {width}")
@@ -730,24 +767,10 @@ class WebDNNCudaContext:
         for t in (temperature, draft_temperature):
             if not (t == 0 or 1e-6 <= t <= 1e6):
                 raise ValueError(f"{who}: a temperature is 0, or 1e-6 to 1e6")
-        if uniforms is None:
-            if temperature != 0 or draft_logits is not None:
-                raise ValueError(f"{who}: a temperature, or drafts with a distribution, need uniforms")
-        elif uniforms.dims != [batch, n]:
-            raise ValueError(f"{who}: uniforms are [{batch}, {n}]")
-        shapes = ([batch, n], [batch], [batch])
-        if out is None:
-            out = tuple(self.empty_tensor(s, "int32") for s in shapes)
-        elif len(out) != 3:
-            raise ValueError(f"{who}: out is (path, accepted, next)")
-        for t, what, s in zip(out, ("path", "accepted", "next"), shapes):
-            self.asserts_int_rows(who, what, t, s)
-        if batch:
-            def at(t):
-                return t.ptr if t is not None and t.length else None
-            desc = VerifyDesc(batch, n, vocab, n * width, width, n * draft_width, draft_width, temperature, draft_temperature)
-            self._call("wdc_verify_drafts", byref(desc), *map(at, (logits, draft_logits, tokens, parents, counts, uniforms, *out)))
-        return tuple(out)
+        if uniforms is None and (temperature != 0 or draft_logits is not None):
+            raise ValueError(f"{who}: a temperature, or drafts with a distribution, need uniforms")
+        desc = VerifyDesc(batch, n, vocab, n * width, width, n * draft_width, draft_width, temperature, draft_temperature)
+        return self._keep(key, desc, ([batch, n], [batch], [batch]))
 
     def conv2d(self, desc: ConvDesc, x, w, scale, shift, residual, y) -> None:
         def p(t):

@@ -482,6 +482,7 @@ class CudaRotaryEmbedding(OperatorImpl):
             cos, sin = (t if positions is not None else t.alias([batch * tokens, pairs]) for t in (cos, sin))
             if x.ndim == 3:
                 return [context.rotate_heads(x, heads, size, cos=cos, sin=sin, positions=positions, interleaved=self.interleaved)]
+            context.asserts_rows("RotaryEmbedding", (x, cos, sin), ())
             context.asserts_rotation("RotaryEmbedding", size, cos, sin, positions, ())
             if size % 4 or size > 256:
                 raise ValueError(f"RotaryEmbedding: heads of {size} (a multiple of 4 up to 256)")

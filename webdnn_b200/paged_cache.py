@@ -144,16 +144,14 @@ class PagedCache:
         who = "PagedCache.append_rotary"
         if q is None and (heads or q_column or out is not None or q_weight is not None):
             raise ValueError(f"{who}: heads, q_column, q_weight and out are of queries")
-        rows = (k, v) if q is None else (k, v, q)
-        self._operands(who, rows, page_table, lengths, counts)
-        extra = (cos, sin, positions, q_weight, k_weight)
-        dims = tuple(tuple(t.dims) if t is not None else None for t in (k, v, q, page_table, lengths, counts, *extra))
-        key = ("append_rotary", dims, heads, epsilon, bool(interleaved), q_column, k_column, v_column)
-        self.context.asserts_rotation(who, self.head_size, cos, sin, positions, (q_weight, k_weight))
-        kept = self._descs.get(key) or self._append_rotary_desc(who, key, k, v, page_table, lengths, counts, cos, positions, q, heads,
-                                                                epsilon, interleaved, q_column, k_column, v_column)
-        d = kept[1]
+        self.context.asserts_rows(who, (k, v, q, cos, sin, q_weight, k_weight), (page_table, lengths, counts, positions))
+        key = ("append_rotary", *(t is not None and tuple(t.dims) for t in (k, v, q, page_table, lengths, counts, cos, sin, positions, q_weight, k_weight)),
+               heads, epsilon, bool(interleaved), q_column, k_column, v_column)
+        kept = self._descs.get(key) or self._append_rotary_desc(who, key, k, v, page_table, lengths, counts, cos, sin, positions, q, heads,
+                                                                (q_weight, k_weight), epsilon, interleaved, q_column, k_column, v_column)
+        codes, scales = self._at(layer)
         if q is not None:
+            d = kept[1]
             shape = [d.append.batch, d.append.tokens, d.heads * self.head_size]
             if out is None:
                 out = self.context.empty_tensor(shape)
@@ -161,13 +159,16 @@ class PagedCache:
                     out.layout != "nchw" or (out.ptr == q.ptr and (q_column or out.dims != q.dims))):
                 raise ValueError(f"{who}: the result is float32 {shape}, row-major, in this context, and q only where that has its shape")
         if k.length and v.length:
-            at = lambda t, column=0: t.ptr + 4 * column if t is not None else None  # noqa: E731
-            self.context._call("wdc_cache_append_rotary", kept[0], at(q, q_column), at(k, k_column), at(v, v_column), at(q_weight), at(k_weight),
-                               at(cos), at(sin), at(positions), *self._at(layer), page_table.ptr, lengths.ptr, at(counts), at(out))
+            self.context._call("wdc_cache_append_rotary", kept[0], q.ptr + 4 * q_column if q is not None else None, k.ptr + 4 * k_column, v.ptr + 4 * v_column,
+                               q_weight.ptr if q_weight is not None else None, k_weight.ptr if k_weight is not None else None,
+                               cos.ptr if cos is not None else None, sin.ptr if sin is not None else None,
+                               positions.ptr if positions is not None else None, codes, scales, page_table.ptr, lengths.ptr,
+                               counts.ptr if counts is not None else None, out.ptr if q is not None else None)
         return out
 
-    def _append_rotary_desc(self, who, key, k, v, page_table, lengths, counts, cos, positions, q, heads, epsilon, interleaved,
+    def _append_rotary_desc(self, who, key, k, v, page_table, lengths, counts, cos, sin, positions, q, heads, weights, epsilon, interleaved,
                             q_column, k_column, v_column):
+        self.context.asserts_rotation(who, self.head_size, cos, sin, positions, weights)
         fields = self._append_fields(who, k, v, page_table, lengths, counts, k_column, v_column)
         c, batch, tokens = self.head_size, fields.batch, fields.tokens
         if positions is not None and positions.dims != [batch, tokens]:
