@@ -6,9 +6,18 @@
 // joins them, tests or draws, and tells the others what to do next.
 //
 // A drawn token is the one in whose range of the running sum a number falls, and with 100000 tokens there are borders everywhere: sums that
-// are 2^-22 of the whole off would name another token in several of a hundred draws.  So weights and sums are in 64 bits.  Their
-// exponential is 2^(n / 16) from a table times a polynomial in what is left, 11 operations in all.  At an SM's 64 lanes that is 0.17
-// cycles a logit, what reading it takes (0.17 at 24 bytes a cycle and SM).
+// are 2^-22 of the whole off would name another token in several of a hundred draws.  In 64 bits a weight takes 25 instructions, four
+// times as many as in 32.  So a walk is made in 32 bits, together with a bound of what that leaves out; a test or a draw that is nearer
+// to a border than the bound stops it, and a second kernel, in 64 bits, goes on from the token that it stands at.
+//
+// In 32 bits the weights stay in shared memory, where a rejection makes p into max(p - q, 0).  The bound E is one of the sum of all weights'
+// errors (so of any running sum's, too):
+//   a weight 2^t, t = (x - top) c:  2^-22 of it for the exponential, 3 * 2^-24 |t| ln 2 for t's three roundings, and the sum of four
+//   weights in 32 bits two more of 2^-24; so E = 1.6 * 2^-22 S + 2.2 * 2^-24 sum w |t|, S = sum w.  The last sum is that of -w log2 w,
+//   which is concave: over n weights it is at most S log2(n / S);
+//   a rejection, p / S - q with q of sum 1:  E' = 2 E / S + Eq + 8 * 2^-24  (S is off by E itself; four roundings, and the sum's two).
+// In 64 bits the exponential is 2^(n / 16) from a table times a polynomial in what is left, 11 operations in all.
+#include <limits.h>
 #include <math.h>
 
 #include "paged_cache.cuh"
@@ -18,7 +27,7 @@ namespace {
 constexpr int WARPS = 16, THREADS = 32 * WARPS, PARTS_MOST = 8, RANGES_MOST = WARPS * PARTS_MOST;
 constexpr int TOKENS_MOST = 1024;
 constexpr int PART_LEAST = 2048;                   // logits of a CTA, where a row is cut into several
-constexpr int SLICE_BYTES = 96 * 1024;             // shared memory for a CTA's logits, two CTAs an SM
+constexpr int SLICE_BYTES = 106 * 1024;            // shared memory for a CTA's logits and what it has of tokens, two CTAs an SM
 
 struct VerifyArgs {
   const float *logits, *draft, *uniforms;
@@ -27,6 +36,7 @@ struct VerifyArgs {
   int* status;
   int64_t logits_sb, logits_st, draft_sb, draft_st;
   int n_tokens, vocab, parts;
+  int goes_on;
   int chunk, chunks;                               // float4 of a warp's range that are in shared memory at a time, and how many times
   double scale, draft_scale;                       // 16 log2(e) / temperature; 0: temperature 0
 };
@@ -34,35 +44,40 @@ struct VerifyArgs {
 // What a range of a row has, or all of a CTA's, or the row: the largest logit, the sum of 2^((x - top) scale / 16), or where the first of
 // the largest is; whether there is a NaN or +inf.
 struct Range {
-  double sum;
+  double sum, off;                                 // off: E
   float top;
   int first, bad, unused;
 };
-__device__ __forceinline__ Range nothing() { return {0.0, -INFINITY, 0x7fffffff, 0, 0}; }
+__device__ __forceinline__ Range nothing() { return {0.0, 0.0, -INFINITY, 0x7fffffff, 0, 0}; }
 enum Todo { STOP = 0, ROW = 1, RESIDUAL = 2 };
 struct Command {
   int todo, token;                                 // the token that the walk stands at
   int with_draft;                                  // ROW: whether the draft's row is wanted; RESIDUAL: rejections, this one included
   int first, draft_first;
   float top, draft_top;
-  int unused;
+  int guess;                                       // the token that the walk may come to next, or -1
   double draft_inverse, step;                      // 1 / sum of the draft's weights, of those before the last rejection
 };
 struct Shared {
   double table[16];
-  double steps[TOKENS_MOST];                       // 1 / the sums that a rejection divided by
+  // as many as there are tokens, behind the logits
+  double* steps;                                   // 1 / the sums that a rejection divided by
+  float* uniforms;                                 // of the leader
+  int *tokens, *parents, *path;
   Command command;
   Range mine[2][WARPS];                            // of this CTA's ranges: target and draft
+  float tops[2][WARPS];                            // their largest logits
   // of the leader
   Range parts[2][PARTS_MOST];
   double run[RANGES_MOST], fresh[RANGES_MOST];     // sums of all ranges, relative to their CTA's largest; after the last rejection
   double part_factors[PARTS_MOST];                 // what relates that to the row's
   double warp_sums[WARPS];
+  float all_tops[2][RANGES_MOST];                  // the largest logits of all ranges
+  double draw_error;                               // E, for a draw
   int draw;                                        // which uniform a token is to be drawn with, or -1
-  int found;
-  float uniforms[TOKENS_MOST];
-  int tokens[TOKENS_MOST], parents[TOKENS_MOST], path[TOKENS_MOST];
+  uint32_t found, last;
 };
+constexpr int TOKEN_BYTES = 24;
 
 __device__ __forceinline__ uint32_t cluster_at(const void* p, int rank) {
   uint32_t at;
@@ -236,6 +251,7 @@ __device__ __noinline__ Range row_range(float4* mine, const float* row, int voca
 
 // The weight of tokens under the target's distribution after `n` rejections, not normalised.
 struct Weights {
+  __device__ __forceinline__ const Weights& in(int) const { return *this; }
   const Command& c;
   const double *table, *steps;
   double scale, draft_scale;
@@ -293,6 +309,92 @@ __device__ __noinline__ double residual(float4* mine, int apart, const float* ro
   return warp_sum(sum);
 }
 
+// ------------------------------------------------------------------------------------------- in 32 bits
+__device__ __forceinline__ float exp2_of(float x) {      // results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float near_weight(float x, float top, float c) { return exp2_of((x - (top == -INFINITY ? 0.f : top)) * c); }
+// A warp's logits in shared memory become weights relative to the largest of them.  (A NaN or +inf makes the sum NaN.)
+__device__ __noinline__ Range near_range(float4* mine, int quads, double scale, int most) {
+  const int lane = threadIdx.x & 31;
+  float its_top = -INFINITY;
+#pragma unroll 2
+  for (int j = lane; j < quads; j += 32) {
+    const float4 v = mine[j];
+    its_top = fmaxf(its_top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+  }
+  Range r = nothing();
+  r.top = group_max<32>(its_top);
+  const float c = (float)(scale / 16);
+#pragma unroll 2
+  for (int j = lane; j < quads; j += 32) {
+    const float4 x = mine[j];
+    const float4 w = make_float4(near_weight(x.x, r.top, c), near_weight(x.y, r.top, c), near_weight(x.z, r.top, c), near_weight(x.w, r.top, c));
+    mine[j] = w;
+    r.sum += (double)((w.x + w.y) + (w.z + w.w));
+  }
+  r.sum = warp_sum(r.sum);
+  r.bad = r.sum != r.sum;
+  // (the logarithm is 2^-20 off, which the slack of 1.6 holds)
+  if (r.sum > 0.0) r.off = r.sum * (1.6 / (1 << 22) + 2.2 / (1 << 24) * (double)fmaxf(__log2f((float)most / (float)r.sum), 0.f));
+  return r;
+}
+// p, number by number, becomes max(p f - q g, 0); returns the sum.
+__device__ __noinline__ double near_residual(float4* mine, int apart, int quads, float f, float g) {
+  double sum = 0.0;
+#pragma unroll 2
+  for (int j = (int)(threadIdx.x & 31); j < quads; j += 32) {
+    float4 p = mine[j];
+    const float4 q = mine[apart + j];
+    p = make_float4(fmaxf(fmaf(p.x, f, -(q.x * g)), 0.f), fmaxf(fmaf(p.y, f, -(q.y * g)), 0.f), fmaxf(fmaf(p.z, f, -(q.z * g)), 0.f),
+                    fmaxf(fmaf(p.w, f, -(q.w * g)), 0.f));
+    mine[j] = p;
+    sum += (double)((p.x + p.y) + (p.z + p.w));
+  }
+  return warp_sum(sum);
+}
+// The weights of a range as they are in its warp's shared memory, from the logits once more.
+struct NearWeights {
+  const Shared& sh;
+  double scale, draft_scale;
+  int n;
+  struct InRange {
+    float top, draft_top, c, draft_c;
+    double factor, draft_factor;
+    const double* steps;
+    int n;
+    template <int N>
+    __device__ __forceinline__ void of(int, int, const float (&x)[N], const float (&y)[N], double (&p)[N]) const {
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        float w = near_weight(x[e], top, c);
+        if (n == 0) {
+          p[e] = (double)w * factor;
+          continue;
+        }
+        const float q = near_weight(y[e], draft_top, draft_c), g = (float)draft_factor;
+#pragma unroll 1
+        for (int k = 0; k < n; k++) w = fmaxf(fmaf(w, (float)(k ? steps[k] : steps[k] * factor), -(q * g)), 0.f);
+        p[e] = (double)w;
+      }
+    }
+    __device__ __forceinline__ double drafted(float y) const { return (double)near_weight(y, draft_top, draft_c) * draft_factor; }
+  };
+  __device__ __forceinline__ InRange in(int range) const {
+    const Command& c = sh.command;
+    InRange r = {sh.all_tops[0][range], sh.all_tops[1][range], (float)(scale / 16), (float)(draft_scale / 16), 0.0, 0.0, sh.steps, n};
+    r.factor = power(r.top, c.top, scale, sh.table);
+    r.draft_factor = power(r.draft_top, c.draft_top, draft_scale, sh.table) * c.draft_inverse;
+    return r;
+  }
+};
+
+// ------------------------------------------------------------------------------------------- both
+constexpr int NEAR = -2;                           // a draw that is too near to a border
+constexpr int32_t UNDECIDED = INT_MIN;           // `next` of a walk that the second kernel goes on with
+
 // Sums of the lanes up to this one.
 __device__ __forceinline__ double warp_scan(double x) {
   const int lane = threadIdx.x & 31;
@@ -303,10 +405,12 @@ __device__ __forceinline__ double warp_scan(double x) {
   }
   return x;
 }
-// The first token whose running sum passes u times all of it, or -1 where nothing weighs anything; the ranges' sums are in `run`.  All threads of
-// the leader: every warp finds the range, then each has neighbours of it.
-__device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const float* row, const float* draft, const Cut& cut, int vocab, int ranges,
-                                  float uniform) {
+// The first token whose running sum passes u times all of it, or -1 where nothing weighs anything; the ranges' sums are in `run`, and off by
+// up to `error` in all (0: in 64 bits).  All threads of the leader: every warp finds the range, then each has neighbours of it.
+// sh.found and sh.last are 0 before.
+template <class W>
+__device__ __noinline__ int drawn(Shared& sh, const W& every, const float* row, const float* draft, const Cut& cut, int vocab, int ranges, float uniform,
+                                  double error) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const double u = (double)fminf(fmaxf(uniform, 0.f), 0.999999940395355f);      // (NaN: 0)
   constexpr int PER = RANGES_MOST / 32, N = 2;     // ranges of a lane, all of one CTA; tokens of a thread
@@ -314,7 +418,7 @@ __device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const floa
 #pragma unroll
   for (int k = 0; k < PER; k++) {
     const int r = lane * PER + k;
-    mine[k] = r < ranges ? sh.run[r] * (weights.n ? 1.0 : sh.part_factors[r / WARPS]) : 0.0;
+    mine[k] = r < ranges ? sh.run[r] * (every.n ? 1.0 : sh.part_factors[r / WARPS]) : 0.0;
     sum += mine[k];
   }
   double up = warp_scan(sum), before = up - sum;
@@ -330,13 +434,12 @@ __device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const floa
     before += mine[k];
   }
   const unsigned have = __ballot_sync(0xffffffffu, range >= 0);
-  if (!have) return -1;
+  if (!have) return error > 0.0 ? NEAR : -1;
   const int who = __ffs((int)have) - 1;
   range = __shfl_sync(0xffffffffu, range, who);
   base = __shfl_sync(0xffffffffu, base, who);
+  const auto weights = every.in(range);
   const int lo = cut.logit(cut.first(range)), hi = min(cut.logit(cut.first(range + 1)), vocab);
-  // (found: tokens that pass, the first the largest, are above all that do not: the last that weighs anything, where roundings of 2^-53
-  // keep the goal from all)
 #pragma unroll 1
   for (int i0 = lo; i0 < hi; i0 += THREADS * N) {
     const int from = i0 + (int)threadIdx.x * N;
@@ -344,7 +447,7 @@ __device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const floa
 #pragma unroll
     for (int e = 0; e < N; e++) {
       x[e] = from + e < hi ? pdl_ld(row + from + e) : -INFINITY;
-      y[e] = from + e < hi && weights.n ? pdl_ld(draft + from + e) : -INFINITY;
+      y[e] = from + e < hi && every.n ? pdl_ld(draft + from + e) : -INFINITY;
     }
     double w[N];
     weights.of(from, 1, x, y, w);
@@ -360,19 +463,27 @@ __device__ __noinline__ int drawn(Shared& sh, const Weights& weights, const floa
       if (k < warp) running += of_warp;
       base += of_warp;
     }
-    int best = -1;
+    // the token that passes, the first the largest number; where roundings keep all from it, the last that weighs anything
+    uint32_t passes = 0, last = 0;
 #pragma unroll
     for (int e = 0; e < N; e++) {
+      if (w[e] > 0.0) {
+        last = (uint32_t)(from + e) + 1;
+        if (!passes && running + w[e] > goal)
+          passes = 2u * (uint32_t)((1 << 30) - (from + e)) + (error > 0.0 && (running + 2 * error > goal || running + w[e] < goal + 2 * error));
+      }
       running += w[e];
-      if (w[e] > 0.0 && best < 1 << 30) best = running > goal ? (1 << 30) + ((1 << 30) - 1 - (from + e)) : from + e;
     }
-    best = __reduce_max_sync(0xffffffffu, best);
-    if (lane == 0 && best >= 0) atomicMax(&sh.found, best);
+    passes = __reduce_max_sync(0xffffffffu, passes);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && passes) atomicMax(&sh.found, passes);
+    if (lane == 0 && last) atomicMax(&sh.last, last);
     __syncthreads();
-    if (sh.found >= 1 << 30) break;
+    if (sh.found) break;
   }
-  const int found = sh.found;
-  return found >= 1 << 30 ? (1 << 30) - 1 - (found - (1 << 30)) : found;
+  const uint32_t found = sh.found;
+  if (!found) return error > 0.0 ? NEAR : (int)sh.last - 1;
+  return found & 1 ? NEAR : (1 << 30) - (int)(found >> 1);
 }
 
 // The next child of new token `of` behind new token `after`, which has token `want` where `only` is set, or -1.  Every warp finds it.
@@ -395,13 +506,19 @@ __device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int r
   const float top = group_max<WARPS>(its.top);
   const int first = group_min<WARPS>(its.top == top ? its.first : 0x7fffffff);
   if (row && scale == 0.0) its.sum = its.first == first && its.top > -INFINITY ? 1.0 : 0.0;
-  else if (row) its.sum *= power(its.top, top, scale, sh.table);
+  else if (row) {
+    const double f = power(its.top, top, scale, sh.table);
+    its.sum *= f;
+    its.off *= f;
+    cluster_put(&sh.all_tops[side][rank * WARPS + r], 0, its.top);
+  }
   its.first = first;
   its.top = top;
   if (side == 0) cluster_put((row ? sh.run : sh.fresh) + rank * WARPS + r, 0, its.sum);
 #pragma unroll
   for (int w = 1; w < WARPS; w <<= 1) {
     its.sum += __shfl_xor_sync(0xffffffffu, its.sum, w);
+    its.off += __shfl_xor_sync(0xffffffffu, its.off, w);
     its.bad |= __shfl_xor_sync(0xffffffffu, its.bad, w);
   }
   if (r == 0) cluster_put(&sh.parts[side][rank], 0, its);
@@ -410,16 +527,32 @@ __device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int r
 // Warp 0 of the leader: where the walk stands, and what the last pass has to say about it.
 struct Walk {
   int at = 0, length = 1, child = 0, rejections = 0, next = -1;
-  double total = 0.0;
+  double total = 0.0, error = 0.0, draft_error = 0.0;
 };
 
-__global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyArgs a) {
+// FAST: in 32 bits.  Else, where a.goes_on, the walks that the other left undecided; all of them otherwise.
+template <bool FAST>
+__global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
   extern __shared__ float4 slices[];               // logits: each warp's of the target, then of the draft
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)a.parts), b = (int)(blockIdx.x / (unsigned)a.parts), ranges = a.parts * WARPS;
   if (threadIdx.x < 16) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 16);
+  if (threadIdx.x == 0) {
+    sh.steps = reinterpret_cast<double*>(slices + (a.draft ? 2 : 1) * WARPS * a.chunk);
+    sh.uniforms = reinterpret_cast<float*>(sh.steps + a.n_tokens);
+    sh.tokens = reinterpret_cast<int*>(sh.uniforms + a.n_tokens);
+    sh.parents = sh.tokens + a.n_tokens;
+    sh.path = sh.parents + a.n_tokens;
+  }
+  __syncthreads();
   pdl_wait();
+  Walk walk;
+  if (!FAST && a.goes_on) {
+    if (pdl_ld(a.next + b) != UNDECIDED) return;   // (all CTAs of the cluster)
+    walk.length = pdl_ld(a.accepted + b);
+    walk.at = pdl_ld(a.path + (int64_t)b * a.n_tokens + walk.length - 1);
+  }
   int count = a.counts ? pdl_ld(a.counts + b) : a.n_tokens;
   if (count < 0 || count > a.n_tokens) {
     if (threadIdx.x == 0) a.status[WDC_STATUS_DRAFT] = 1;
@@ -428,11 +561,15 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
   if (threadIdx.x == 0) {
     Command c = {};
     c.todo = ROW;
+    c.token = walk.at;
     c.with_draft = a.draft && count > 1;
     sh.command = c;
-    sh.path[0] = 0;
+    c.guess = -1;
+    if (walk.length == 1 && a.n_tokens > 0) sh.path[0] = 0;
   }
   if (rank == 0) {
+    if (walk.length > 1)
+      for (int i = threadIdx.x; i < walk.length; i += THREADS) sh.path[i] = pdl_ld(a.path + (int64_t)b * a.n_tokens + i);
     for (int i = threadIdx.x; i < count; i += THREADS) {
       const int64_t at = (int64_t)b * a.n_tokens + i;
       int parent = a.parents ? pdl_ld(a.parents + at) : i - 1;
@@ -450,7 +587,6 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
 
   float4* const mine = slices + warp * a.chunk;
   const int apart = WARPS * a.chunk;
-  Walk walk;
 #pragma unroll 1
   for (;;) {
     const int todo = sh.command.todo, standing = sh.command.token, with_draft = sh.command.with_draft;
@@ -460,6 +596,16 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
     const Cut cut(row, a.vocab, ranges);
     const int first = cut.first(rank * WARPS + warp), quads = cut.first(rank * WARPS + warp + 1) - first, i0 = 4 * first - cut.before;
     const bool same = (reinterpret_cast<uintptr_t>(row) >> 2 & 3) == (reinterpret_cast<uintptr_t>(draft) >> 2 & 3);
+    // The leader's next draft to test, and what the logits have for it: known before the pass, so that nothing waits for it behind it.
+    float target_logit[1] = {0.f}, draft_logit[1] = {0.f};
+    if (rank == 0 && warp == 0 && a.draft && count > 0) {
+      walk.child = child_of(sh, standing, todo == ROW ? standing : walk.child, count);
+      const int token = walk.child < 0 ? -1 : sh.tokens[walk.child];
+      if (token >= 0 && token < a.vocab) {
+        target_logit[0] = pdl_ld(row + token);
+        draft_logit[0] = pdl_ld(draft + token);
+      }
+    }
     if (count == 0) {
     } else if (todo == ROW) {
       if (a.chunks == 1) {
@@ -470,24 +616,46 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
       }
 #pragma unroll 1
       for (int side = 0; side <= (with_draft != 0); side++) {
-        const Range r = row_range(mine + side * apart, side ? draft : row, a.vocab, i0, quads, a.chunk, a.chunks, side == 0 || same,
-                                  side ? a.draft_scale : a.scale, sh.table);
-        if (lane == 0) sh.mine[side][warp] = r;
+        Range r;
+        if constexpr (FAST) r = near_range(mine + side * apart, quads, side ? a.draft_scale : a.scale, 4 * cut.each);
+        else r = row_range(mine + side * apart, side ? draft : row, a.vocab, i0, quads, a.chunk, a.chunks, side == 0 || same,
+                           side ? a.draft_scale : a.scale, sh.table);
+        if (lane == 0) {
+          sh.mine[side][warp] = r;
+          sh.tops[side][warp] = r.top;
+        }
       }
     } else {
       // the rejection that has just been: its step is the last
       if (threadIdx.x == 0) sh.steps[with_draft - 1] = sh.command.step;
       __syncthreads();
-      const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, with_draft};
-      const double sum = residual(mine, apart, row, draft, a.vocab, i0, quads, a.chunk, a.chunks, same, weights);
-      if (lane == 0) sh.mine[0][warp] = {sum, 0.f, 0, 0, 0};
+      double sum;
+      if constexpr (FAST) {
+        // (the first time p is still relative to the range's largest)
+        const Command& c = sh.command;
+        const double f = with_draft > 1 ? c.step : c.step * power(sh.tops[0][warp], c.top, a.scale, sh.table);
+        const double g = power(sh.tops[1][warp], c.draft_top, a.draft_scale, sh.table) * c.draft_inverse;
+        sum = near_residual(mine, apart, quads, (float)f, (float)g);
+      } else {
+        const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, with_draft};
+        sum = residual(mine, apart, row, draft, a.vocab, i0, quads, a.chunk, a.chunks, same, weights);
+      }
+      if (lane == 0) sh.mine[0][warp] = {sum, 0.0, 0.f, 0, 0, 0};
+    }
+    if (todo == ROW && sh.command.guess >= 0 && quads > 0) {
+      // while the leader decides, the rows of the first child on their way to L2, a line a lane
+      const int64_t from = 4 * (int64_t)first - cut.before, to = from + 4 * quads < a.vocab ? from + 4 * quads : a.vocab;
+      for (int64_t i = (from > 0 ? from : 0) + lane * 32; i < to; i += 32 * 32) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + b * a.logits_sb + sh.command.guess * a.logits_st + i));
+        if (a.draft) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.draft + b * a.draft_sb + sh.command.guess * a.draft_st + i));
+      }
     }
     __syncthreads();
     if (warp == 0 && count > 0) to_leader(sh, a, rank, todo == ROW, todo == ROW && with_draft);
     cluster_sync();
     if (rank == 0) {
       Command c = {};                              // (of warp 0, which decides; all threads draw)
-      bool test = false;
+      bool test = false, near = false;             // near: a decision that 32 bits do not make
       if (warp == 0) {
         c = sh.command;
         c.todo = STOP;
@@ -507,9 +675,11 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
             if (there && side == 0) sh.part_factors[part] = f;
           }
           its.sum *= f;
+          its.off *= f;
 #pragma unroll
           for (int w = 1; w < PARTS_MOST; w <<= 1) {
             its.sum += __shfl_xor_sync(0xffffffffu, its.sum, w);
+            if (FAST) its.off += __shfl_xor_sync(0xffffffffu, its.off, w);
             its.bad |= __shfl_xor_sync(0xffffffffu, its.bad, w);
           }
           const double total = __shfl_sync(0xffffffffu, its.sum, 0), draft_total = __shfl_sync(0xffffffffu, its.sum, PARTS_MOST);
@@ -521,39 +691,52 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
             c.draft_top = __shfl_sync(0xffffffffu, top, PARTS_MOST);
             c.draft_inverse = with_draft ? 1.0 / draft_total : 1.0;
             walk.total = total;
+            if (FAST) {
+              walk.error = __shfl_sync(0xffffffffu, its.off, 0);
+              walk.draft_error = 2 * __shfl_sync(0xffffffffu, its.off, PARTS_MOST) * c.draft_inverse + 4.0 / (1 << 24);
+            }
             walk.rejections = 0;
-            walk.child = standing;
             test = !none && a.draft;
             if (!none && !a.draft) draw = standing;
           } else {
+            if (FAST) {
+              walk.error = 2 * walk.error / walk.total + walk.draft_error + 8.0 / (1 << 24);
+              near = !(total > 4 * walk.error);
+            }
             if (total > 0.0) {
               for (int r = lane; r < ranges; r += 32) sh.run[r] = sh.fresh[r];
               walk.total = total;
               walk.rejections = with_draft;
             }
-            test = true;
+            test = !near;
           }
-          if (test) {
-            walk.child = child_of(sh, standing, walk.child, count);
-            if (walk.child < 0) draw = 0;
-          }
+          if (test && walk.child < 0) draw = 0;
         }
         __syncwarp();
         if (lane == 0) {
           sh.command = c;                          // (for the weights below; told to the others at the end)
           sh.command.with_draft = walk.rejections;
           sh.draw = draw;
-          sh.found = -1;
+          sh.draw_error = walk.error;
+          sh.found = sh.last = 0;
         }
         __syncwarp();
       }
       __syncthreads();
       if (sh.draw >= 0) {
-        const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, sh.command.with_draft};
-        const int token = drawn(sh, weights, row, draft, cut, a.vocab, ranges, sh.uniforms[sh.draw]);
+        int token;
+        if constexpr (FAST) {
+          const NearWeights weights = {sh, a.scale, a.draft_scale, sh.command.with_draft};
+          token = drawn(sh, weights, row, draft, cut, a.vocab, ranges, sh.uniforms[sh.draw], sh.draw_error);
+        } else {
+          const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, sh.command.with_draft};
+          token = drawn(sh, weights, row, draft, cut, a.vocab, ranges, sh.uniforms[sh.draw], 0.0);
+        }
         if (warp == 0) {
+          near = token == NEAR;
           walk.child = token < 0 || a.draft ? -1 : child_of(sh, standing, standing, count, true, token);
-          if (walk.child < 0) {
+          if (near) {
+          } else if (walk.child < 0) {
             walk.next = token;
           } else {
             walk.at = walk.child;
@@ -565,14 +748,22 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
         const double u = (double)fminf(fmaxf(sh.uniforms[walk.child], 0.f), 0.999999940395355f);
         bool stands = false;
         if (token >= 0 && token < a.vocab) {
-          const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, walk.rejections};
-          const float x[1] = {pdl_ld(row + token)}, y[1] = {pdl_ld(draft + token)};
           double p[1], q[1];
-          weights.of(token, 1, x, y, p);
-          weights.drafted(token, 1, y, q);
+          if constexpr (FAST) {
+            const NearWeights weights = {sh, a.scale, a.draft_scale, walk.rejections};
+            const auto its = weights.in((token + cut.before) / 4 / cut.each);
+            its.of(token, 1, target_logit, draft_logit, p);
+            q[0] = its.drafted(draft_logit[0]);
+            near = fabs(u * q[0] * walk.total - p[0]) <= 2 * walk.error + walk.total * walk.draft_error;
+          } else {
+            const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, walk.rejections};
+            weights.of(token, 1, target_logit, draft_logit, p);
+            weights.drafted(token, 1, draft_logit, q);
+          }
           stands = u * q[0] * walk.total < p[0];
         }
-        if (stands) {
+        if (near) {
+        } else if (stands) {
           walk.at = walk.child;
           c.todo = ROW;
         } else {
@@ -582,9 +773,11 @@ __global__ void __launch_bounds__(THREADS, 2) verify_drafts_kernel(const VerifyA
         }
       }
       if (warp == 0) {
+        if (near) walk.next = UNDECIDED;           // (and STOP)
         if (c.todo == ROW) {
           c.token = walk.at;
-          c.with_draft = a.draft && child_of(sh, walk.at, walk.at, count) >= 0;
+          c.guess = child_of(sh, walk.at, walk.at, count);
+          c.with_draft = a.draft && c.guess >= 0;
           if (lane == 0) sh.path[walk.length] = walk.at;
           walk.length++;
         }
@@ -629,32 +822,34 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
                         (const void*)uniforms, (const void*)path, (const void*)accepted, (const void*)next})
     WDC_REQUIRE(ctx, (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: buffers are not aligned", who);
   VerifyArgs a = {logits, draft_logits, uniforms, tokens, parents, counts, path, accepted, next, ctx->status_word,
-                  d->logits_sb, d->logits_st, d->draft_sb, d->draft_st, (int)d->tokens, (int)d->vocab, 1, 1, 1, 0.0, 0.0};
+                  d->logits_sb, d->logits_st, d->draft_sb, d->draft_st, (int)d->tokens, (int)d->vocab, 1, 0, 1, 1, 0.0, 0.0};
   const double to16 = 16 * 1.4426950408889634;     // 16 log2(e)
   if (d->temperature > 0.f) a.scale = to16 / d->temperature;
   if (d->draft_temperature > 0.f) a.draft_scale = to16 / d->draft_temperature;
   while (a.parts < PARTS_MOST && d->batch * a.parts < ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
-  // Shared memory for the logits of a warp's range, or for as many of them as there is room for.
+  // Shared memory for the logits of a warp's range, by more CTAs if need be; or for as many of them as there is room for.
   const int sides = draft_logits ? 2 : 1;
-  const int64_t each = ceil_div64((d->vocab + 6) / 4, a.parts * WARPS), most = SLICE_BYTES / (16 * WARPS * sides);
-  a.chunk = (int)(each < most ? each : most);
-  a.chunks = (int)ceil_div64(each, a.chunk);
+  const int64_t most = (SLICE_BYTES - TOKEN_BYTES * d->tokens) / (16 * WARPS * sides);
+  const auto each = [&]() { return ceil_div64((d->vocab + 6) / 4, a.parts * WARPS); };
+  const int parts = a.parts;
+  while (a.parts < PARTS_MOST && each() > most) a.parts *= 2;
+  if (each() > most) a.parts = parts;
+  a.chunk = (int)(each() < most ? each() : most);
+  a.chunks = (int)ceil_div64(each(), a.chunk);
   DeviceGuard g(ctx->device);
   static bool opted_in[64] = {};     // per device: more than 48 KB of dynamic shared memory needs the attribute
   WDC_REQUIRE(ctx, ctx->device >= 0 && ctx->device < 64, "%s: device index out of range", who);
   if (!opted_in[ctx->device]) {
-    WDC_CUDA(ctx, cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SLICE_BYTES));
+    WDC_CUDA(ctx, cudaFuncSetAttribute(verify_drafts_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SLICE_BYTES));
+    WDC_CUDA(ctx, cudaFuncSetAttribute(verify_drafts_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SLICE_BYTES));
     opted_in[ctx->device] = true;
   }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(d->batch * a.parts));
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = (size_t)(16 * WARPS * sides) * a.chunk;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-  attr[cfg.numAttrs].val.clusterDim.x = (unsigned)a.parts;
   attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
   cfg.numAttrs++;
   if (ctx->opt_pdl) {
@@ -662,6 +857,22 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs++;
   }
-  WDC_CUDA(ctx, cudaLaunchKernelEx(&cfg, verify_drafts_kernel, a));
+  const auto shape = [&]() {
+    cfg.gridDim = dim3((unsigned)(d->batch * a.parts));
+    cfg.dynamicSmemBytes = (size_t)(16 * WARPS * sides) * a.chunk + TOKEN_BYTES * d->tokens;
+    attr[0].val.clusterDim.x = (unsigned)a.parts;
+  };
+  shape();
+  // In 32 bits first, where all of a row's weights have room and there is something to weigh; then what that left undecided.
+  if (a.chunks == 1 && d->temperature > 0.f && (!draft_logits || d->draft_temperature > 0.f)) {
+    WDC_CUDA(ctx, cudaLaunchKernelEx(&cfg, verify_drafts_kernel<true>, a));
+    CACHE_TRY(wdc_check_launch(ctx, "verify_drafts_kernel"));
+    // (few walks have anything left to do, so that each may have many CTAs)
+    a.goes_on = 1;
+    while (a.parts < PARTS_MOST && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
+    a.chunk = (int)each();
+    shape();
+  }
+  WDC_CUDA(ctx, cudaLaunchKernelEx(&cfg, verify_drafts_kernel<false>, a));
   return wdc_check_launch(ctx, "verify_drafts_kernel");
 }
