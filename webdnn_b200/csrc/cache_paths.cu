@@ -20,25 +20,45 @@ __device__ __forceinline__ uint32_t largest_byte(uint32_t w) {
   w = __vmaxu4(w, w >> 16);
   return max(w & 255u, w >> 8 & 255u);
 }
-// Codes in units of `from` as codes in units of `to`.  A page that stands for NaN has codes of 0.
-__device__ __forceinline__ uint32_t again4(uint32_t w, float from, float to) {
+// Codes in units of `from` as codes in units of `to`, rint(code * from / to).  A page that stands for NaN has codes of 0.
+__device__ __noinline__ uint32_t divided4(uint32_t w, float from, float to) {
   uint32_t out = 0;
   if (!(to > 0.f && to < INFINITY)) return 0;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float r = rintf(__fdiv_rn(__fmul_rn((float)(int8_t)(w >> (8 * j)), from), to));
-    out |= (uint32_t)((int)fminf(fmaxf(r, -127.f), 127.f) & 255) << (8 * j);
+#pragma unroll 1
+  for (int j = 0; j < 32; j += 8) {
+    const float r = rintf(__fdiv_rn(__fmul_rn((float)(int8_t)(w >> j), from), to));
+    out |= (uint32_t)((int)fminf(fmaxf(r, -127.f), 127.f) & 255) << j;
   }
   return out;
 }
-__device__ __forceinline__ uint4 again16(uint4 v, float from, float to) {
-  return make_uint4(again4(v.x, from, to), again4(v.y, from, to), again4(v.z, from, to), again4(v.w, from, to));
+// Without a division where it cannot matter: the product with 1 / to is within 3e-5 of the quotient (at most 127, three roundings of 2^-24), so
+// where it is further than that from a half the nearest whole number is the same, and is read off the sum with 1.5 * 2^23.  (A code + 128
+// as the last byte of 2^23 is a float32 number.)  inverse: 0 where 1 / to might leave the normal range, or `to` is no number.
+__device__ __forceinline__ uint32_t again4(uint32_t w, float from, float to, float inverse) {
+  const float magic = 12582912.f, zero = 8388736.f;
+  const uint32_t biased = w ^ 0x80808080u;
+  float r[4], off = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float t = __fmul_rn(__fmul_rn(__uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7650 + j)) - zero, from), inverse);
+    r[j] = t + magic;
+    off = fmaxf(off, fabsf(t - (r[j] - magic)));
+  }
+  if (off < 0.4999f && inverse > 0.f)
+    return __byte_perm(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040), 0x5410);
+  return divided4(w, from, to);
+}
+__device__ __forceinline__ float inverse_of(float to) { return to > 1e-30f && to < INFINITY ? __frcp_rn(to) : 0.f; }
+__device__ __forceinline__ uint4 again16(uint4 v, float from, float to, float inverse) {
+  return make_uint4(again4(v.x, from, to, inverse), again4(v.y, from, to, inverse), again4(v.z, from, to, inverse), again4(v.w, from, to, inverse));
 }
 
-// A warp per sequence, layer, side and head; 2^(5 - lane_shift) tokens at a time.  A path rises, so a token's old place is never before
-// its new one: taken in order, with all of a step's loads before its stores, and page after page, nothing is overwritten before it is read.
-// A page's new scale is known from a first pass over the tokens that come to it.  Bound: a chain of dependent loads (path, page table,
-// scales, codes) that is the same for all.
+// A warp per sequence, layer, side and head; 2^(5 - lane_shift) tokens at a time, of 32 that the lanes have looked up.  A path rises, so a
+// token's old place is never before its new one: taken in order, with all of a step's loads before its stores, and page after page,
+// nothing is overwritten before it is read.
+// A page's new scale is known from a first pass over the tokens that come to it.  Bound: issue, of the codes that are rounded again (40
+// sequences, up to nine tokens, 30 layers of 8 heads of 128: 15.3 us; with a division each 17.8, two steps' loads together 15.7, four 18.8),
+// and the chain of dependent loads (path, page table, scales, codes) where they are few (2.7 us).
 __global__ void __launch_bounds__(32 * WARPS) cache_keep_kernel(const KeepArgs a) {
   pdl_wait();
   const int lane = threadIdx.x & 31, b = (int)blockIdx.y;
@@ -73,7 +93,33 @@ __global__ void __launch_bounds__(32 * WARPS) cache_keep_kernel(const KeepArgs a
   const auto block_of = [&](int page) { return (int64_t)page * kinds + kind; };
   const auto page_at = [&](int64_t index) { return cache_page(table, index, a.pages, a.status); };
   const auto piece_of = [&](int page, int in_page) {
-    return reinterpret_cast<uint4*>(codes + block_of(page) * block_bytes + ((int64_t)(in_page << a.lane_shift) + piece) * 16);
+    return reinterpret_cast<uint4*>(codes) + (block_of(page) << (a.page_shift + a.lane_shift)) + ((in_page << a.lane_shift) + piece);
+  };
+
+  // What a lane knows of a token of the path: where it comes from, and the page and scale of that.
+  int of = -1, at_in_page = 0;
+  float by = 0.f;
+  const auto look_up = [&](int i, int end, int page) {
+    of = -1;
+    if (i < end) {
+      const int from = start + path[i];
+      of = page_at(from >> a.page_shift);
+      at_in_page = from & (size - 1);
+      by = of >= 0 && of != page ? scales[block_of(of)] : 0.f;
+    }
+  };
+  // The piece of token k + mine of those that the lanes know of, where it comes from (or -1) and the scale there.
+  struct Source {
+    uint4 v;
+    int of;
+    float by;
+  };
+  const auto source = [&](int k, int not_of) {
+    const int token = (k + mine) & 31, at = __shfl_sync(0xffffffffu, at_in_page, token);
+    Source s = {make_uint4(0, 0, 0, 0), __shfl_sync(0xffffffffu, of, token), __shfl_sync(0xffffffffu, by, token)};
+    if (s.of == not_of) s.of = -1;
+    if (s.of >= 0) s.v = *piece_of(s.of, at);
+    return s;
   };
 
   for (int i0 = first; i0 < accepted;) {           // the kept tokens of one page: i0 .. i1 - 1
@@ -85,47 +131,38 @@ __global__ void __launch_bounds__(32 * WARPS) cache_keep_kernel(const KeepArgs a
     }
     const float before = scales[block_of(page)];
     float scale = before;
-    for (int i = i0; i < i1; i += together) {
-      float peak = 0.f;
-      if (i + mine < i1) {
-        const int from = start + path[i + mine], of = page_at(from >> a.page_shift);
-        if (of >= 0 && of != page) {
-          const uint4 v = *piece_of(of, from & (size - 1));
-          uint32_t most = largest_byte(abs_max4(v.x, abs_max4(v.y, abs_max4(v.z, abs_max4(v.w, 0)))));
-          const float by = scales[block_of(of)];
-          // (a scale that is no number or infinite stands for NaN)
-          peak = fabsf(by) < INFINITY ? __fdiv_rn(__fmul_rn((float)most, by), 127.f) : NAN;
-        }
+    uint32_t peak = 0;                             // of this lane, as bits: a NaN is above infinity
+    for (int c = i0; c < i1; c += 32) {
+      look_up(c + lane, i1, page);
+      if (!__any_sync(0xffffffffu, of >= 0 && of != page)) continue;
+      for (int k = 0; k < min(32, i1 - c); k += together) {
+        const Source s = source(k, page);
+        const uint32_t most = largest_byte(abs_max4(s.v.x, abs_max4(s.v.y, abs_max4(s.v.z, abs_max4(s.v.w, 0)))));
+        // (a scale that is no number or infinite stands for NaN)
+        if (s.of >= 0) peak = max(peak, __float_as_uint(fabsf(s.by) < INFINITY ? __fdiv_rn(__fmul_rn((float)most, s.by), 127.f) : NAN) & 0x7fffffffu);
       }
-      // the largest of all lanes', as bits: a NaN is above infinity
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(peak) & 0x7fffffffu);
-      const float fresh = __uint_as_float(top);
-      if (!(fresh <= scale) && fabsf(scale) < INFINITY) scale = fresh;
     }
+    const float fresh = __uint_as_float(__reduce_max_sync(0xffffffffu, peak));
+    if (!(fresh <= scale) && fabsf(scale) < INFINITY) scale = fresh;
     const bool grown = __float_as_uint(scale) != __float_as_uint(before);
+    const float inverse = inverse_of(scale);
     if (grown) {
       // what the page holds already: older tokens, and the first of the new ones, which stay where they are
       const int old = start + i0 - (index << a.page_shift);
       for (int t = mine; t < old; t += together) {
         uint4* at = piece_of(page, t);
-        *at = again16(*at, before, scale);
+        *at = again16(*at, before, scale, inverse);
       }
     }
-    for (int i = i0; i < i1; i += together) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const int p = i + mine < i1 ? path[i + mine] : 0;
-      bool moves = false;
-      if (i + mine < i1) {
-        const int from = start + p, of = page_at(from >> a.page_shift);
-        moves = of >= 0 && (grown || p != i + mine);
-        if (moves) {
-          v = *piece_of(of, from & (size - 1));
-          if (of != page || grown) v = again16(v, of == page ? before : scales[block_of(of)], scale);
-        }
+    for (int c = i0; c < i1; c += 32) {
+      if (i1 - i0 > 32) look_up(c + lane, i1, page);
+      for (int k = 0; k < min(32, i1 - c); k += together) {
+        const Source s = source(k, -1);
+        __syncwarp();
+        const bool stays = s.of == page;
+        if (s.of >= 0) *piece_of(page, (start + c + k + mine) & (size - 1)) = stays && !grown ? s.v : again16(s.v, stays ? before : s.by, scale, inverse);
+        __syncwarp();
       }
-      __syncwarp();
-      if (moves) *piece_of(page, (start + i + mine) & (size - 1)) = v;
-      __syncwarp();
     }
     if (grown && lane == 0) scales[block_of(page)] = scale;
     __syncwarp();
