@@ -162,29 +162,32 @@ __device__ __forceinline__ int group_min(int x) {
 // warp has `each` float4 of them.
 struct Cut {
   int before, quads, each;
-  __device__ Cut(const float* row, int vocab, int ranges) {
+  __device__ __forceinline__ Cut(const float* row, int vocab, int ranges_shift) {
     before = (int)(reinterpret_cast<uintptr_t>(row) >> 2 & 3);
-    quads = (int)(((int64_t)vocab + before + 3) / 4);
-    each = (quads + ranges - 1) / ranges;
+    quads = (vocab + before + 3) >> 2;
+    each = (quads + (1 << ranges_shift) - 1) >> ranges_shift;
   }
-  __device__ int first(int range) const { return (int)min((int64_t)range * each, (int64_t)quads); }
-  __device__ int logit(int quad) const { return max(4 * quad - before, 0); }
+  __device__ __forceinline__ int first(int range) const { return min(range * each, quads); }
+  __device__ __forceinline__ int logit(int quad) const { return max(4 * quad - before, 0); }
 };
 
 // `quads` float4 of a row, from logit i0 on, to shared memory, by asynchronous copies of a warp; -inf where the row has none, which is in the
 // first and the last.  whole: as they are in memory.
 __device__ __forceinline__ void fetch_quads(float4* to, const float* row, int vocab, int i0, int quads, bool whole) {
   const int lane = threadIdx.x & 31;
-  const bool cut_off = quads > 0 && (i0 < 0 || i0 + 4 * quads > vocab);
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(to);
+  const bool cut_off = quads > 0 && (i0 < 0 || i0 + 4 * quads > vocab);
   if (whole) {
-    const int inside = i0 < 0 ? 1 : 0, end = i0 + 4 * quads > vocab ? quads - 1 : quads;
-    const float* from = row + i0 + 4 * lane;
-    for (int j = lane; j < end; j += 32, from += 128)
-      if (j >= inside) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + 16 * j), "l"(from) : "memory");
+    const int end = i0 + 4 * quads > vocab ? quads - 1 : quads;
+    int j = i0 < 0 && lane == 0 ? 32 : lane;       // (the first float4 is cut off)
+    const float* from = row + i0 + 4 * j;
+    uint32_t at = base + 16 * j;
+#pragma unroll 4
+    for (; j < end; j += 32, from += 128, at += 512) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
     if (!cut_off) return;
   }
   // number by number: all of them, or the first and the last float4
+#pragma unroll 1
   for (int k = lane; k < 4 * quads; k += 32) {
     if (whole && k >= 4 && k < 4 * quads - 4) continue;
     const int i = i0 + k;
@@ -192,6 +195,7 @@ __device__ __forceinline__ void fetch_quads(float4* to, const float* row, int vo
     else reinterpret_cast<float*>(to)[k] = -INFINITY;
   }
 }
+
 // What a warp's range has: its float4, `quads` from logit i0 on, which are in `mine`, or are brought there a chunk at a time where they
 // are several chunks.  (A function of its own, which has the registers to itself.)
 __device__ __noinline__ Range row_range(float4* mine, const float* row, int vocab, int i0, int quads, int chunk, int chunks, bool whole, double scale,
@@ -315,31 +319,57 @@ __device__ __forceinline__ float exp2_of(float x) {      // results below 2^-126
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float near_weight(float x, float top, float c) { return exp2_of((x - (top == -INFINITY ? 0.f : top)) * c); }
-// A warp's logits in shared memory become weights relative to the largest of them.  (A NaN or +inf makes the sum NaN.)
-__device__ __noinline__ Range near_range(float4* mine, int quads, double scale, int most) {
-  const int lane = threadIdx.x & 31;
-  float its_top = -INFINITY;
+// (top: not -inf)
+__device__ __forceinline__ float near_weight(float x, float top, float c) { return exp2_of((x - top) * c); }
+// A warp's logits in shared memory become weights relative to the largest of them, both sides together (SIDES), so that one's exchanges
+// between lanes hide the other's.  (A NaN or +inf makes the sum NaN.)
+template <int SIDES>
+__device__ __noinline__ void near_ranges(Shared& sh, float4* mine, int apart, int quads, double scale, double draft_scale) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float top[SIDES], ref[SIDES];
+  const float c[2] = {(float)(scale / 16), (float)(draft_scale / 16)};
+#pragma unroll
+  for (int side = 0; side < SIDES; side++) top[side] = -INFINITY;
 #pragma unroll 2
   for (int j = lane; j < quads; j += 32) {
-    const float4 v = mine[j];
-    its_top = fmaxf(its_top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) {
+      const float4 v = mine[side * apart + j];
+      top[side] = fmaxf(top[side], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+    }
   }
-  Range r = nothing();
-  r.top = group_max<32>(its_top);
-  const float c = (float)(scale / 16);
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1)
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) top[side] = fmaxf(top[side], __shfl_xor_sync(0xffffffffu, top[side], w));
+  double sum[SIDES];
+#pragma unroll
+  for (int side = 0; side < SIDES; side++) {
+    ref[side] = top[side] == -INFINITY ? 0.f : top[side];
+    sum[side] = 0.0;
+  }
 #pragma unroll 2
   for (int j = lane; j < quads; j += 32) {
-    const float4 x = mine[j];
-    const float4 w = make_float4(near_weight(x.x, r.top, c), near_weight(x.y, r.top, c), near_weight(x.z, r.top, c), near_weight(x.w, r.top, c));
-    mine[j] = w;
-    r.sum += (double)((w.x + w.y) + (w.z + w.w));
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) {
+      const float4 x = mine[side * apart + j];
+      const float4 w = make_float4(near_weight(x.x, ref[side], c[side]), near_weight(x.y, ref[side], c[side]), near_weight(x.z, ref[side], c[side]),
+                                   near_weight(x.w, ref[side], c[side]));
+      mine[side * apart + j] = w;
+      sum[side] += (double)((w.x + w.y) + (w.z + w.w));
+    }
   }
-  r.sum = warp_sum(r.sum);
-  r.bad = r.sum != r.sum;
-  // (the logarithm is 2^-20 off, which the slack of 1.6 holds)
-  if (r.sum > 0.0) r.off = r.sum * (1.6 / (1 << 22) + 2.2 / (1 << 24) * (double)fmaxf(__log2f((float)most / (float)r.sum), 0.f));
-  return r;
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1)
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) sum[side] += __shfl_xor_sync(0xffffffffu, sum[side], w);
+  if (lane == 0) {
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) {
+      sh.mine[side][warp] = {sum[side], 0.0, top[side], 0x7fffffff, sum[side] != sum[side], 0};
+      sh.tops[side][warp] = top[side];
+    }
+  }
 }
 // p, number by number, becomes max(p f - q g, 0); returns the sum.
 __device__ __noinline__ double near_residual(float4* mine, int apart, int quads, float f, float g) {
@@ -387,6 +417,8 @@ struct NearWeights {
     InRange r = {sh.all_tops[0][range], sh.all_tops[1][range], (float)(scale / 16), (float)(draft_scale / 16), 0.0, 0.0, sh.steps, n};
     r.factor = power(r.top, c.top, scale, sh.table);
     r.draft_factor = power(r.draft_top, c.draft_top, draft_scale, sh.table) * c.draft_inverse;
+    if (r.top == -INFINITY) r.top = 0.f;
+    if (r.draft_top == -INFINITY) r.draft_top = 0.f;
     return r;
   }
 };
@@ -496,8 +528,8 @@ __device__ __forceinline__ int child_of(const Shared& sh, int of, int after, int
   return -1;
 }
 
-// A CTA's ranges, both sides at once, to the leader.  Warp 0.
-__device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int rank, bool row, bool with_draft) {
+// A CTA's ranges, of `most` logits each, both sides at once, to the leader.  Warp 0.
+__device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int rank, bool row, bool with_draft, int most) {
   const int lane = threadIdx.x & 31, side = lane / WARPS, r = lane % WARPS;
   Range its = nothing();
   if (side == 0 || with_draft) its = sh.mine[side][r];
@@ -508,8 +540,9 @@ __device__ __forceinline__ void to_leader(Shared& sh, const VerifyArgs& a, int r
   if (row && scale == 0.0) its.sum = its.first == first && its.top > -INFINITY ? 1.0 : 0.0;
   else if (row) {
     const double f = power(its.top, top, scale, sh.table);
+    // (E, where it is wanted; the logarithm is 2^-20 off, which the slack of 1.6 holds)
+    if (its.sum > 0.0) its.off = its.sum * f * (1.6 / (1 << 22) + 2.2 / (1 << 24) * (double)fmaxf(__log2f((float)most / (float)its.sum), 0.f));
     its.sum *= f;
-    its.off *= f;
     cluster_put(&sh.all_tops[side][rank * WARPS + r], 0, its.top);
   }
   its.first = first;
@@ -537,6 +570,7 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
   extern __shared__ float4 slices[];               // logits: each warp's of the target, then of the draft
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)a.parts), b = (int)(blockIdx.x / (unsigned)a.parts), ranges = a.parts * WARPS;
+  const int ranges_shift = 31 - __clz(ranges);     // (a power of two)
   if (threadIdx.x < 16) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 16);
   if (threadIdx.x == 0) {
     sh.steps = reinterpret_cast<double*>(slices + (a.draft ? 2 : 1) * WARPS * a.chunk);
@@ -593,7 +627,7 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
     if (todo == STOP) break;
     const float* row = a.logits + b * a.logits_sb + standing * a.logits_st;
     const float* draft = a.draft ? a.draft + b * a.draft_sb + standing * a.draft_st : nullptr;
-    const Cut cut(row, a.vocab, ranges);
+    const Cut cut(row, a.vocab, ranges_shift);
     const int first = cut.first(rank * WARPS + warp), quads = cut.first(rank * WARPS + warp + 1) - first, i0 = 4 * first - cut.before;
     const bool same = (reinterpret_cast<uintptr_t>(row) >> 2 & 3) == (reinterpret_cast<uintptr_t>(draft) >> 2 & 3);
     // The leader's next draft to test, and what the logits have for it: known before the pass, so that nothing waits for it behind it.
@@ -614,15 +648,15 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
       }
+      if constexpr (FAST) {
+        if (with_draft) near_ranges<2>(sh, mine, apart, quads, a.scale, a.draft_scale);
+        else near_ranges<1>(sh, mine, apart, quads, a.scale, a.draft_scale);
+      } else {
 #pragma unroll 1
-      for (int side = 0; side <= (with_draft != 0); side++) {
-        Range r;
-        if constexpr (FAST) r = near_range(mine + side * apart, quads, side ? a.draft_scale : a.scale, 4 * cut.each);
-        else r = row_range(mine + side * apart, side ? draft : row, a.vocab, i0, quads, a.chunk, a.chunks, side == 0 || same,
-                           side ? a.draft_scale : a.scale, sh.table);
-        if (lane == 0) {
-          sh.mine[side][warp] = r;
-          sh.tops[side][warp] = r.top;
+        for (int side = 0; side <= (with_draft != 0); side++) {
+          const Range r = row_range(mine + side * apart, side ? draft : row, a.vocab, i0, quads, a.chunk, a.chunks, side == 0 || same,
+                                    side ? a.draft_scale : a.scale, sh.table);
+          if (lane == 0) sh.mine[side][warp] = r;
         }
       }
     } else {
@@ -651,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
       }
     }
     __syncthreads();
-    if (warp == 0 && count > 0) to_leader(sh, a, rank, todo == ROW, todo == ROW && with_draft);
+    if (warp == 0 && count > 0) to_leader(sh, a, rank, todo == ROW, todo == ROW && with_draft, 4 * cut.each);
     cluster_sync();
     if (rank == 0) {
       Command c = {};                              // (of warp 0, which decides; all threads draw)
