@@ -293,6 +293,25 @@ def test_what_a_token_does_not_see_is_not_there(cuda_context, tokens, heads):
     cache.dispose()
 
 
+@pytest.mark.parametrize("heads,kv_heads,c,lengths,counts", [
+    (2, 1, 64, [30, 20, 9], [6, 1, 3]), (4, 1, 64, [3000], [3]), (16, 8, 128, [2100, 1999, 1500, 64], [64, 33, 1, 40]), (1, 1, 32, [400, 70], [60, 3])])
+def test_rows_behind_the_new_tokens_are_zero_whatever_the_cache_holds(cuda_context, heads, kv_heads, c, lengths, counts):
+    """Pages that stand for NaN, or whose values are infinite, are the business of the rows that are there."""
+    ctx, rng = cuda_context, np.random.default_rng(c + len(lengths))
+    cache = PagedCache(ctx, 1, sum(-(-n // 16) for n in lengths) + 3, kv_heads, c, 16)
+    codes, scales = random_pool(rng, cache)
+    table, tokens = tables(rng, cache, lengths), max(counts) + 4
+    q = rng.standard_normal((len(lengths), tokens, heads, c)).astype(f32)
+    parents = np.stack([random_tree(rng, tokens, "any") for _ in lengths])
+    for value in (np.nan, np.inf):
+        set_pool(cache, codes, np.full_like(scales, value))
+        for got in (run_attention(ctx, cache, q, table, lengths, counts), run_tree(ctx, cache, q, table, lengths, counts, parents)):
+            for b, n in enumerate(counts):
+                assert np.isnan(got[b, :n]).all() and np.array_equal(got[b, n:], np.zeros_like(got[b, n:]))
+    ctx.sync()
+    cache.dispose()
+
+
 def test_bad_parents_count_as_none_and_are_reported(cuda_context):
     ctx, rng = cuda_context, np.random.default_rng(4)
     cache = PagedCache(ctx, 1, 12, 2, 64, 16)
@@ -491,6 +510,48 @@ def test_drafts_do_not_change_what_is_said(cuda_context, with_draft):
     assert with_draft is False or (accepted > 1).mean() > 0.3
 
 
+@pytest.mark.parametrize("with_draft", [False, True])
+@pytest.mark.parametrize("vocab,spread", [(3001, 0.1), (3001, 3.0), (40009, 0.5)])
+def test_verdicts_beside_the_borders_of_tokens(cuda_context, vocab, spread, with_draft):
+    """Random numbers that are the float32 numbers next to a border of the running sum, and those that a draft stands or falls by: 32 bits
+    do not tell on which side they are."""
+    rng = np.random.default_rng(vocab)
+    batch, n = 60, 3
+    logits, draft, parents, tokens, uniforms = drafted(rng, batch, n, vocab, "chain", with_draft, spread=spread)
+    for b in range(batch):
+        p, u = chances(logits[b, 0], 1.0), rng.integers(-1, 2)
+        if with_draft and b % 2:
+            q = chances(draft[b, 0], 1.0)
+            tokens[b, 1] = np.where(p < q, q, 0).argmax()
+            border = p[tokens[b, 1]] / q[tokens[b, 1]]
+            uniforms[b, 1] = f32(border) * f32(1 + u * 2.0 ** -23)
+        else:
+            left = p
+            if with_draft:
+                tokens[b, 1], q = vocab, chances(draft[b, 0], 1.0)               # (never stands: a rejection, then a draw)
+                left = np.maximum(p - q, 0)
+            border = np.cumsum(left)[rng.integers(0, vocab)] / left.sum()
+            uniforms[b, 0] = min(f32(border) * f32(1 + u * 2.0 ** -23), f32(1 - 2.0 ** -24))
+    got = run_verify(cuda_context, logits, tokens, parents, None, uniforms, draft, 1.0)
+    cuda_context.sync()
+    assert_verdicts(got, logits, tokens, parents, None, uniforms, draft, 1.0)
+
+
+def test_results_of_verdicts_overlap_nothing(cuda_context):
+    ctx, rng = cuda_context, np.random.default_rng(15)
+    logits, _, parents, tokens, uniforms = drafted(rng, 3, 5, 50, "chain", False)
+    ints = [dev(ctx, np.asarray(a, np.int32)) for a in (tokens, parents, np.full(3, 5))]
+    floats = [dev(ctx, logits), dev(ctx, uniforms)]
+    out = [ctx.empty_tensor(d, "int32") for d in ([3, 5], [3], [3])]
+    for bad in ((ints[0], out[1], out[2]), (ints[1], out[1], out[2]), (out[0], ints[2], out[2]), (out[0], out[1], ints[2]), (out[0], out[1], out[1])):
+        with pytest.raises(CudaBackendError, match="overlaps"):
+            ctx.verify_drafts(floats[0], *ints, uniforms=floats[1], out=bad)
+    ctx.verify_drafts(floats[0], *ints, uniforms=floats[1], out=out)
+    ctx.sync()
+    assert_verdicts([t.get_data().reshape(t.dims) for t in out], logits, tokens, parents, None, uniforms, None, 1.0)
+    dispose(*out, *ints, *floats)
+
+
 def test_bad_parents_and_counts_of_verdicts_are_reported(cuda_context):
     ctx, rng = cuda_context, np.random.default_rng(14)
     logits, _, parents, tokens, uniforms = drafted(rng, 3, 5, 50, "chain", False)
@@ -589,6 +650,23 @@ def test_kept_paths_of_pages_without_numbers(cuda_context):
             assert np.abs(got[:, :, 11:13] * by[..., None, None] - want).max() <= (by.max() / 2) * (1 + 2.0 ** -14)
         ctx.sync()
         cache.dispose()
+
+
+def test_kept_paths_of_numbers_of_any_magnitude(cuda_context):
+    ctx, rng = cuda_context, np.random.default_rng(8)
+    cache = PagedCache(ctx, 1, 30, 2, 64, 16)
+    codes, scales = random_pool(rng, cache)
+    lengths, counts, accepted = [30] * 9, [20] * 9, [12] * 9
+    table = tables(rng, cache, lengths)
+    path = np.stack([np.pad(np.sort(rng.choice(20, 12, replace=False)), (0, 8), constant_values=-1) for _ in lengths])
+    for b, (first, second) in enumerate(((1e36, 1e35), (1e35, 1e36), (2e36, 1e30), (1e-30, 1e-36), (1e-36, 1e-30), (1e-40, 1e-42), (1e29, 1e31), (1e-29, 1e-31), (1e-45, 1e36))):
+        scales[0, table[b][0]], scales[0, table[b][1]] = first, second
+    set_pool(cache, codes, scales)
+    run_keep(ctx, cache, table, lengths, counts, path, accepted)
+    ctx.sync()
+    reference_keep(codes, scales, table, lengths, counts, path, accepted, 16)
+    assert np.array_equal(pool_scales(cache), scales) and np.array_equal(pool_codes(cache), codes)
+    cache.dispose()
 
 
 def test_paths_that_do_not_fit_leave_their_sequence_alone(cuda_context):

@@ -311,6 +311,8 @@ extern "C" int wdc_cache_append_rotary(wdc_context* ctx, const wdc_cache_append_
   WDC_REQUIRE(ctx, d->heads >= 0 && d->heads <= 65535 && !q == !q_out && (q || d->heads == 0 || !slots), "%s: bad queries", who);
   WDC_REQUIRE(ctx, cache_aligned(q, 16) && cache_aligned(q_out, 16) && cache_aligned(q_weight, 16) && cache_aligned(k_weight, 16),
               "%s: buffers are not aligned", who);
+  // (other heads are still to be read when the first are written)
+  WDC_REQUIRE(ctx, !q_out || (q_out != k && q_out != v), "%s: q_out is k or v", who);
   a.q = q; a.y = q_out; a.q_weight = q_weight; a.k_weight = k_weight;
   a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
   a.y_sb = d->y_sb; a.y_sh = d->y_sh; a.y_st = d->y_st;

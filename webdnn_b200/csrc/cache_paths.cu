@@ -33,7 +33,8 @@ __device__ __noinline__ uint32_t divided4(uint32_t w, float from, float to) {
 }
 // Without a division where it cannot matter: the product with 1 / to is within 3e-5 of the quotient (at most 127, three roundings of 2^-24), so
 // where it is further than that from a half the nearest whole number is the same, and is read off the sum with 1.5 * 2^23.  (A code + 128
-// as the last byte of 2^23 is a float32 number.)  inverse: 0 where 1 / to might leave the normal range, or `to` is no number.
+// as the last byte of 2^23 is a float32 number.)  inverse: 0 where 1 / to might leave the normal range, a code * from
+// might (`from` is at most 127 `to` where the code is not 0), or `to` is no number.
 __device__ __forceinline__ uint32_t again4(uint32_t w, float from, float to, float inverse) {
   const float magic = 12582912.f, zero = 8388736.f;
   const uint32_t biased = w ^ 0x80808080u;
@@ -48,7 +49,7 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float from, float to, flo
     return __byte_perm(__byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040), __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040), 0x5410);
   return divided4(w, from, to);
 }
-__device__ __forceinline__ float inverse_of(float to) { return to > 1e-30f && to < INFINITY ? __frcp_rn(to) : 0.f; }
+__device__ __forceinline__ float inverse_of(float to) { return to > 1e-30f && to < 1e30f ? __frcp_rn(to) : 0.f; }
 __device__ __forceinline__ uint4 again16(uint4 v, float from, float to, float inverse) {
   return make_uint4(again4(v.x, from, to, inverse), again4(v.y, from, to, inverse), again4(v.z, from, to, inverse), again4(v.w, from, to, inverse));
 }
