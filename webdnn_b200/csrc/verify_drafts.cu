@@ -502,7 +502,7 @@ __device__ __noinline__ int drawn(Shared& sh, const W& every, const float* row, 
       if (w[e] > 0.0) {
         last = (uint32_t)(from + e) + 1;
         if (!passes && running + w[e] > goal)
-          passes = 2u * (uint32_t)((1 << 30) - (from + e)) + (error > 0.0 && (running + 2 * error > goal || running + w[e] < goal + 2 * error));
+          passes = 2u * (uint32_t)((1 << 30) - (from + e)) + (error > 0.0 && (running + error > goal || running + w[e] < goal + error));
       }
       running += w[e];
     }
@@ -855,6 +855,20 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
   for (const void* p : {(const void*)logits, (const void*)draft_logits, (const void*)tokens, (const void*)parents, (const void*)counts,
                         (const void*)uniforms, (const void*)path, (const void*)accepted, (const void*)next})
     WDC_REQUIRE(ctx, (reinterpret_cast<uintptr_t>(p) & 3u) == 0, "%s: buffers are not aligned", who);
+  // (the second kernel reads what the first has read, after that has written its results)
+  const int64_t per_row = d->batch * d->tokens, row_end = d->tokens ? d->vocab : 0;
+  const auto extent = [&](int64_t sb, int64_t st) { return row_end ? (d->batch - 1) * sb + (d->tokens - 1) * st + row_end : 0; };
+  struct Words {
+    const void* at;
+    int64_t n;
+  };
+  const Words used[9] = {{path, per_row}, {accepted, d->batch}, {next, d->batch}, {tokens, per_row}, {parents, per_row}, {counts, d->batch}, {uniforms, per_row},
+                         {logits, extent(d->logits_sb, d->logits_st)}, {draft_logits, extent(d->draft_sb, d->draft_st)}};
+  for (int i = 0; i < 3; i++)
+    for (int j = i + 1; j < 9; j++) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(used[i].at), y = reinterpret_cast<uintptr_t>(used[j].at);
+      WDC_REQUIRE(ctx, !x || !y || x + 4 * used[i].n <= y || y + 4 * used[j].n <= x, "%s: a result overlaps another buffer", who);
+    }
   VerifyArgs a = {logits, draft_logits, uniforms, tokens, parents, counts, path, accepted, next, ctx->status_word,
                   d->logits_sb, d->logits_st, d->draft_sb, d->draft_st, (int)d->tokens, (int)d->vocab, 1, 0, 1, 1, 0.0, 0.0};
   const double to16 = 16 * 1.4426950408889634;     // 16 log2(e)
