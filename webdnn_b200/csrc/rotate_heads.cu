@@ -6,7 +6,7 @@
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 64;
 
 struct RotateArgs {
   const float *x, *weight;
@@ -20,9 +20,12 @@ struct RotateArgs {
 
 // A group of LANES lanes takes EACH heads of a row, SLOTS slots a lane.  y may be x: no two groups have a head.
 //
-// Bound: memory (9001 rows of 24 heads of 80, 139 MB: 29 us, 4.8 TB/s; of 16 heads of 128 25.8, 5.7 TB/s); the launch for few (1.7 us).
+// Bound: memory (9001 rows of 24 heads of 80, 139 MB: 26.8 us, 5.2 TB/s; of 16 heads of 128 25.1, 5.9 TB/s); the launch for few (1.6 us).
+// A CTA is a chain of loads, sums and stores, so small ones, which end at different times, keep the memory busy (us of these three and of
+// 500 rows of 8 heads of 128, by threads a CTA: 256 29.9, 26.1, 1.85, 2.09; 128 27.7, 25.2, 1.57, 2.06; 64 27.0, 25.1, 1.56, 2.06; 32 26.7, 25.0,
+// 1.64, 2.35).  CTAS: of 256 threads an SM, that many registers.
 template <int LANES, int SLOTS, int EACH, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS) rotate_heads_kernel(const RotateArgs a) {
+__global__ void __launch_bounds__(THREADS, CTAS * 256 / THREADS) rotate_heads_kernel(const RotateArgs a) {
   pdl_wait();
   const uint32_t item = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
   const bool there = item < a.items;
@@ -68,8 +71,9 @@ extern "C" int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, cons
   WDC_REQUIRE(ctx, cache_aligned(x, 16) && cache_aligned(y, 16) && cache_aligned(weight, 16), "wdc_rotate_heads: buffers are not aligned");
   DeviceGuard g(ctx->device);
   const int slots = (a.head_size / 4 + 1) / 2;
-  // Lanes, slots and heads a group by what was measured, us of 173 million numbers (floor 22): heads of 32 26.2 (two slots a lane 34.1), of
-  // 64 25.7 (two slots 26.5, two heads 27.1), of 128 25.8 (one slot 25.7, one head 27.5), of 80 29.2 (8 lanes of two slots 31.0, 16 of one 31.4).
+  // Lanes, slots and heads a group by what was measured with CTAs of 256 threads, us of 173 million numbers (floor 22): heads of 32 26.2 (two
+  // slots a lane 34.1), of 64 25.7 (two slots 26.5, two heads 27.1), of 128 25.8 (one slot 25.7, one head 27.5), of 80 29.2 (8 lanes of two
+  // slots 31.0, 16 of one 31.4, 2 of five 42).
   return slots <= 4    ? launch<4, 1, 4, 3>(ctx, a, d->rows)
          : slots <= 8  ? launch<8, 1, 4, 3>(ctx, a, d->rows)
          : slots <= 12 ? launch<4, 3, 2, 2>(ctx, a, d->rows)
