@@ -255,7 +255,6 @@ __device__ __noinline__ Range row_range(float4* mine, const float* row, int voca
 
 // The weight of tokens under the target's distribution after `n` rejections, not normalised.
 struct Weights {
-  __device__ __forceinline__ const Weights& in(int) const { return *this; }
   const Command& c;
   const double *table, *steps;
   double scale, draft_scale;
@@ -282,6 +281,20 @@ struct Weights {
 #pragma unroll
       for (int e = 0; e < N; e++) p[e] = fmax(fma(p[e], by, -q[e]), 0.0);
     }
+  }
+  // For a draw: of tokens from, from + 1, .. < hi of a range; 0 behind it.
+  __device__ __forceinline__ const Weights& in(int, const Cut&) const { return *this; }
+  template <int N>
+  __device__ __forceinline__ void take(const float* row, const float* draft, int from, int hi, double (&p)[N]) const {
+    float x[N], y[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      x[e] = from + e < hi ? pdl_ld(row + from + e) : -INFINITY;
+      y[e] = from + e < hi && n ? pdl_ld(draft + from + e) : -INFINITY;
+    }
+    of(from, 1, x, y, p);
+#pragma unroll
+    for (int e = 0; e < N; e++) p[e] = from + e < hi ? p[e] : 0.0;
   }
 };
 
@@ -385,9 +398,11 @@ __device__ __noinline__ double near_residual(float4* mine, int apart, int quads,
   }
   return warp_sum(sum);
 }
-// The weights of a range as they are in its warp's shared memory, from the logits once more.
+// The weights of a range: from the logits once more, as they are in its warp's shared memory, for a test; or those themselves.
 struct NearWeights {
   const Shared& sh;
+  const float4* slices;
+  int chunk;
   double scale, draft_scale;
   int n;
   struct InRange {
@@ -412,6 +427,27 @@ struct NearWeights {
     }
     __device__ __forceinline__ double drafted(float y) const { return (double)near_weight(y, draft_top, draft_c) * draft_factor; }
   };
+  // For a draw, in the shared memory of the CTA that has the range.
+  struct Taken {
+    uint32_t at;
+    int i0;
+    double factor;
+    template <int N>
+    __device__ __forceinline__ void take(const float*, const float*, int from, int hi, double (&p)[N]) const {
+      float w[N];
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        w[e] = 0.f;
+        if (from + e < hi) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w[e]) : "r"(at + 4 * (from + e - i0)) : "memory");
+      }
+#pragma unroll
+      for (int e = 0; e < N; e++) p[e] = (double)w[e] * factor;
+    }
+  };
+  __device__ __forceinline__ Taken in(int range, const Cut& cut) const {
+    return {cluster_at(slices + range % WARPS * chunk, range / WARPS), 4 * cut.first(range) - cut.before,
+            n ? 1.0 : power(sh.all_tops[0][range], sh.command.top, scale, sh.table)};
+  }
   __device__ __forceinline__ InRange in(int range) const {
     const Command& c = sh.command;
     InRange r = {sh.all_tops[0][range], sh.all_tops[1][range], (float)(scale / 16), (float)(draft_scale / 16), 0.0, 0.0, sh.steps, n};
@@ -470,21 +506,13 @@ __device__ __noinline__ int drawn(Shared& sh, const W& every, const float* row, 
   const int who = __ffs((int)have) - 1;
   range = __shfl_sync(0xffffffffu, range, who);
   base = __shfl_sync(0xffffffffu, base, who);
-  const auto weights = every.in(range);
+  const auto weights = every.in(range, cut);
   const int lo = cut.logit(cut.first(range)), hi = min(cut.logit(cut.first(range + 1)), vocab);
 #pragma unroll 1
   for (int i0 = lo; i0 < hi; i0 += THREADS * N) {
     const int from = i0 + (int)threadIdx.x * N;
-    float x[N], y[N];
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      x[e] = from + e < hi ? pdl_ld(row + from + e) : -INFINITY;
-      y[e] = from + e < hi && every.n ? pdl_ld(draft + from + e) : -INFINITY;
-    }
     double w[N];
-    weights.of(from, 1, x, y, w);
-#pragma unroll
-    for (int e = 0; e < N; e++) w[e] = from + e < hi ? w[e] : 0.0;
+    weights.take(row, draft, from, hi, w);
     const double scan = warp_scan(w[0] + w[1]);
     if (lane == 31) sh.warp_sums[warp] = scan;
     __syncthreads();
@@ -760,7 +788,7 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
       if (sh.draw >= 0) {
         int token;
         if constexpr (FAST) {
-          const NearWeights weights = {sh, a.scale, a.draft_scale, sh.command.with_draft};
+          const NearWeights weights = {sh, slices, a.chunk, a.scale, a.draft_scale, sh.command.with_draft};
           token = drawn(sh, weights, row, draft, cut, a.vocab, ranges, sh.uniforms[sh.draw], sh.draw_error);
         } else {
           const Weights weights = {sh.command, sh.table, sh.steps, a.scale, a.draft_scale, sh.command.with_draft};
@@ -784,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
         if (token >= 0 && token < a.vocab) {
           double p[1], q[1];
           if constexpr (FAST) {
-            const NearWeights weights = {sh, a.scale, a.draft_scale, walk.rejections};
+            const NearWeights weights = {sh, slices, a.chunk, a.scale, a.draft_scale, walk.rejections};
             const auto its = weights.in((token + cut.before) / 4 / cut.each);
             its.of(token, 1, target_logit, draft_logit, p);
             q[0] = its.drafted(draft_logit[0]);
