@@ -17,6 +17,11 @@
 //   which is concave: over n weights it is at most S log2(n / S);
 //   a rejection, p / S - q with q of sum 1:  E' = 2 E / S + Eq + 8 * 2^-24  (S is off by E itself; four roundings, and the sum's two).
 // In 64 bits the exponential is 2^(n / 16) from a table times a polynomial in what is left, 11 operations in all.
+//
+// Bound: what is serial, the chain of a pass (logits to shared memory, weights, sums, two barriers of the cluster, the leader's decision),
+// 12000 to 20000 cycles of which memory has a tenth; 28% of the issue slots are used.  One sequence of 5 new tokens, 32000 in the
+// vocabulary, drafts with their logits: 20 us; 16 of 25, 100003, without them: 48; 64 of 9, 50001, with them: 112, of which the 64-bit kernel
+// has 45 for four walks (64 bits alone: 28.7, 62 and 144).
 #include <limits.h>
 #include <math.h>
 
@@ -26,7 +31,7 @@ namespace {
 
 constexpr int WARPS = 16, THREADS = 32 * WARPS, PARTS_MOST = 8, RANGES_MOST = WARPS * PARTS_MOST;
 constexpr int TOKENS_MOST = 1024;
-constexpr int PART_LEAST = 2048;                   // logits of a CTA, where a row is cut into several
+constexpr int PART_LEAST = 1024;                   // logits of a CTA, where a row is cut into several
 constexpr int SLICE_BYTES = 106 * 1024;            // shared memory for a CTA's logits and what it has of tokens, two CTAs an SM
 
 struct VerifyArgs {
@@ -902,7 +907,9 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
   const double to16 = 16 * 1.4426950408889634;     // 16 log2(e)
   if (d->temperature > 0.f) a.scale = to16 / d->temperature;
   if (d->draft_temperature > 0.f) a.draft_scale = to16 / d->draft_temperature;
-  while (a.parts < PARTS_MOST && d->batch * a.parts < ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
+  // CTAs of a sequence: as many as fill the SMs once, of enough logits each.  Measured, us of 1 / 2 / 4 / 8, drafts with their logits: one sequence, 4000
+  // in the vocabulary, 20.2 / 18.8 / 18.5 / 18.6, 16000 34.5 / 34.6 / 30.7 / 28.1; 64 of 12000 88 / 74 / 78 / 97; 200 of 12000 75 / 76 / 110 / 176.
+  while (a.parts < PARTS_MOST && 2 * d->batch * a.parts <= ctx->sm_count && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
   // Shared memory for the logits of a warp's range, by more CTAs if need be; or for as many of them as there is room for.
   const int sides = draft_logits ? 2 : 1;
   const int64_t most = (SLICE_BYTES - TOKEN_BYTES * d->tokens) / (16 * WARPS * sides);
