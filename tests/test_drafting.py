@@ -250,6 +250,23 @@ def test_a_decision_that_fails_leaves_the_sequences_as_long_as_they_were(monkeyp
         assert decoder.cache.used_pages == 0 and not decoder.cache._sequences
 
 
+def test_temperatures_are_checked_and_few_graphs_are_kept(monkeypatch):
+    target, draft, made = decoders(monkeypatch, 50)
+    s = target.cache.add_sequence()
+    disposed = []
+    monkeypatch.setattr(Model, "dispose", lambda self: disposed.append(self))
+    for bad in (-1.0, 1e-9, 1e7, float("nan")):
+        with pytest.raises(ValueError):
+            target.decide([s], [[4]], [[-1]], np.zeros((1, 1)), bad)
+    assert len(made) == 2 and target.cache.length(s) == 0
+    for temperature in (0.0, 0.5, 1.0, 0.5, 1.5, 0.5, 2.0, 0.0):
+        target.decide([s], [[4]], [[-1]], np.zeros((1, 1)), temperature)
+    # (0.5 was used again before a fifth came, 0 was not)
+    assert len(made) == 2 + 6 and disposed == [made[2], made[4]] and list(target._deciding) == [1.5, 0.5, 2.0, 0.0]
+    target.close()
+    assert len(disposed) == 2 + 5
+
+
 def test_trees_that_do_not_fit_together_are_refused(monkeypatch):
     target, draft, made = decoders(monkeypatch, 50)
     s, r = target.cache.add_sequence(), target.cache.add_sequence()

@@ -36,7 +36,9 @@ class Decoder:
         self.table_pages = -(-positions // page_tokens)      # the same for every call, so that calls repeat
         self._graph = (vocab, d, heads, kv_heads, layers, ffn, positions, top, name, rotary)
         self.runner = self._load()
-        self._deciding: Dict[float, object] = {}             # runners that decide on drafts, by their temperature
+        self._deciding: Dict[float, object] = {}             # runners that decide on drafts, by their temperature: the last ones used
+
+    MAX_DECIDING = 4
 
     def _load(self, **how):
         return load(zoo.decoder(*self._graph, **how), backend_order=["cuda", "cpu"], backend_options={"cuda": {"context": self.context}})
@@ -106,12 +108,16 @@ class Decoder:
             raise ValueError(f"Decoder.decide: there are places for {self.positions} tokens")
         if ids.min() < 0 or ids.max() >= self.vocab:
             raise ValueError(f"Decoder.decide: tokens are 0 .. {self.vocab - 1}")
-        if temperature not in self._deciding:
-            self._deciding[temperature] = self._load(drafts=True, temperature=temperature)
+        if not (temperature == 0 or 1e-6 <= temperature <= 1e6):
+            raise ValueError("Decoder.decide: a temperature is 0, or 1e-6 to 1e6")
+        runner = self._deciding.pop(temperature, None) or self._load(drafts=True, temperature=temperature)
+        while len(self._deciding) >= self.MAX_DECIDING:      # (each has the weights once more)
+            self._deciding.pop(next(iter(self._deciding))).dispose()
+        self._deciding[temperature] = runner
         self.cache.extend(dict(zip(sequences, counts)))
         try:
             where = self.cache.batch(sequences, counts, self.table_pages)
-            outs = self._deciding[temperature].run([CPUTensor.from_array(ids), CPUTensor.from_array(places), *where, CPUTensor.from_array(above),
+            outs = runner.run([CPUTensor.from_array(ids), CPUTensor.from_array(places), *where, CPUTensor.from_array(above),
                                                     CPUTensor.from_array(uniforms)])
             path, accepted, following = (t.numpy().copy() for t in outs)
             if (following < 0).any():
