@@ -689,3 +689,27 @@ def test_paths_that_do_not_fit_leave_their_sequence_alone(cuda_context):
         ctx.sync()
     assert np.array_equal(pool_scales(cache), scales) and np.array_equal(pool_codes(cache), codes)
     cache.dispose()
+
+
+# -------------------------------------------------------------------------------------------------- verdicts: what has no say
+@pytest.mark.parametrize("batch,n,vocab,temperature,whole", [
+    (40, 2, 50, 1.0, False), (40, 5, 1003, 0.7, False), (30, 4, 1000, 1.0, True), (8, 6, 40009, 1.0, False), (3, 3, 300007, 1.3, False)])
+def test_drafts_that_never_stand_leave_the_target_where_both_are_equal(cuda_context, batch, n, vocab, temperature, whole):
+    """max(p - q, 0) of equal distributions is 0 everywhere, and p stays, however often a draft that never stands (a token outside of the
+    vocabulary, or one that weighs nothing on either side) is rejected: the next token is drawn from p."""
+    ctx, rng = cuda_context, np.random.default_rng(batch + vocab)
+    logits = (rng.standard_normal((batch, n, vocab)) * 2).astype(f32)
+    draft = logits.copy()
+    if whole:                                        # (whole numbers: equal distributions of different logits)
+        logits = np.rint(logits)
+        draft = logits + f32(5)
+    logits[:, :, 7] = draft[:, :, 7] = -np.inf
+    parents = np.tile(np.where(np.arange(n) == 0, -1, 0), (batch, 1))
+    tokens = rng.choice([-1, vocab, 7, 1 << 30], (batch, n))
+    uniforms = rng.random((batch, n)).astype(f32)
+    for wider in (0, 1):                             # (rows of the draft's that begin elsewhere in their 16 bytes)
+        got = run_verify(ctx, logits, tokens, parents, None, uniforms, np.pad(draft, [(0, 0), (0, 0), (0, wider)]), temperature, vocab=vocab)
+        ctx.sync()
+        assert_verdicts(got, logits, tokens, parents, None, uniforms, draft, temperature)
+        for b in range(batch):
+            assert got[1][b] == 1 and got[2][b] == taken_from(chances(logits[b, 0], temperature), uniforms[b, 0])

@@ -280,11 +280,12 @@ struct Weights {
     if (n == 0) return;
     double q[N];
     drafted(i, step, y, q);
+    // (both rounded before the difference: where the distributions are equal it is 0, and not what rounding q left out)
 #pragma unroll 1
     for (int k = 0; k < n; k++) {
       const double by = steps[k];
 #pragma unroll
-      for (int e = 0; e < N; e++) p[e] = fmax(fma(p[e], by, -q[e]), 0.0);
+      for (int e = 0; e < N; e++) p[e] = fmax(__dsub_rn(__dmul_rn(p[e], by), q[e]), 0.0);
     }
   }
   // For a draw: of tokens from, from + 1, .. < hi of a range; 0 behind it.
