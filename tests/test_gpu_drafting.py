@@ -713,3 +713,18 @@ def test_drafts_that_never_stand_leave_the_target_where_both_are_equal(cuda_cont
         assert_verdicts(got, logits, tokens, parents, None, uniforms, draft, temperature)
         for b in range(batch):
             assert got[1][b] == 1 and got[2][b] == taken_from(chances(logits[b, 0], temperature), uniforms[b, 0])
+
+
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_verdicts_of_sequences_without_tokens(cuda_context, with_draft):
+    """No rows are there, and no memory of them: nothing is asked for."""
+    ctx = cuda_context
+    empty = lambda *dims: ctx.empty_tensor(list(dims))  # noqa: E731
+    ints = [ctx.empty_tensor([3, 0], "int32"), ctx.empty_tensor([3, 0], "int32"), dev(ctx, np.zeros(3, np.int32))]
+    floats = [empty(3, 0, 40000), empty(3, 0), empty(3, 0, 40000)]
+    for counts in (None, ints[2]):
+        out = ctx.verify_drafts(floats[0], ints[0], ints[1], counts, floats[1], floats[2] if with_draft else None)
+        assert out[0].dims == [3, 0] and out[1].get_data().tolist() == [0] * 3 and out[2].get_data().tolist() == [-1] * 3
+        dispose(*out)
+    ctx.sync()
+    dispose(*ints, *floats)

@@ -631,8 +631,8 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
     c.todo = ROW;
     c.token = walk.at;
     c.with_draft = a.draft && count > 1;
-    sh.command = c;
     c.guess = -1;
+    sh.command = c;
     if (walk.length == 1 && a.n_tokens > 0) sh.path[0] = 0;
   }
   if (rank == 0) {
