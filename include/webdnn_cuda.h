@@ -438,7 +438,7 @@ int wdc_cache_attention_tree(wdc_context* ctx, const wdc_cache_attention_desc* d
  *   without draft_logits, a token is drawn from p with uniforms[i]; the first child that has this token stands and the walk goes on
  *   there; if none has, the drawn token is `next`.
  *   With draft_logits (strides draft_sb, draft_st; q = softmax(draft_logits / draft_temperature), from which the children of token i
- *   were drawn, each by itself), the children c are tried in order: c stands where uniforms[c] q(token) < p(token), else p becomes
+ *   were drawn, each by itself; rows behind tokens without children may hold anything), the children c are tried in order: c stands where uniforms[c] q(token) < p(token), else p becomes
  *   max(p - q, 0) over its sum (p stays where that is 0).  If none stands, `next` is drawn from p with uniforms[0].
  * A token drawn from p with u is the first whose running sum of p passes u times all of it.  uniforms is float32 [batch][tokens], 0
  * <= u < 1 (what is below counts as 0, what is not below 1 as 1 - 2^-24, NaN as 0); it may be NULL at temperature 0 without drafts.

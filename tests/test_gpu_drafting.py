@@ -728,3 +728,28 @@ def test_verdicts_of_sequences_without_tokens(cuda_context, with_draft):
         dispose(*out)
     ctx.sync()
     dispose(*ints, *floats)
+
+
+@pytest.mark.parametrize("missing", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("vocab", [5, 3001, 40009])
+def test_rows_of_drafts_behind_tokens_without_children_have_no_say(cuda_context, vocab, missing):
+    """A drafter need not run behind its last tokens.  Random numbers beside a border of a leaf's running sum, so that 32 bits do not decide
+    there; and sequences whose first token has no children, though others are there."""
+    ctx, rng = cuda_context, np.random.default_rng(vocab)
+    batch, n = 24, 4
+    logits, draft, _, tokens, uniforms = drafted(rng, batch, n, vocab, "star", True)
+    parents = np.tile([-1, 0, 1, 1], (batch, 1))
+    parents[::4] = -1
+    parents[1::4] = [-1, 0, 0, 0]
+    for b in range(batch):
+        for i in range(n):
+            if not (parents[b, i + 1:] == i).any():
+                draft[b, i] = missing
+        uniforms[b, 1:] = 0                          # (every draft that weighs anything stands)
+        leaf = 0 if b % 4 == 0 else 1 if b % 4 == 1 else 2
+        run = np.cumsum(chances(logits[b, leaf], 1.0))
+        uniforms[b, 0] = min(f32(run[rng.integers(0, vocab)] / run[-1]), f32(1 - 2.0 ** -24))
+    got = run_verify(ctx, logits, tokens, parents, None, uniforms, draft, 1.0)
+    ctx.sync()
+    assert_verdicts(got, logits, tokens, parents, None, uniforms, draft, 1.0)
+    assert got[1].tolist() == [1, 2, 3, 3] * (batch // 4) and (got[2] >= 0).all()

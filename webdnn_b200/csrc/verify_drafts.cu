@@ -626,31 +626,33 @@ __global__ void __launch_bounds__(THREADS, FAST ? 2 : 1) verify_drafts_kernel(co
     if (threadIdx.x == 0) a.status[WDC_STATUS_DRAFT] = 1;
     count = 0;
   }
-  if (threadIdx.x == 0) {
-    Command c = {};
-    c.todo = ROW;
-    c.token = walk.at;
-    c.with_draft = a.draft && count > 1;
-    c.guess = -1;
-    sh.command = c;
-    if (walk.length == 1 && a.n_tokens > 0) sh.path[0] = 0;
-  }
-  if (rank == 0) {
-    if (walk.length > 1)
-      for (int i = threadIdx.x; i < walk.length; i += THREADS) sh.path[i] = pdl_ld(a.path + (int64_t)b * a.n_tokens + i);
-    for (int i = threadIdx.x; i < count; i += THREADS) {
-      const int64_t at = (int64_t)b * a.n_tokens + i;
-      int parent = a.parents ? pdl_ld(a.parents + at) : i - 1;
-      if (parent < -1 || parent >= i) {
-        a.status[WDC_STATUS_DRAFT] = 1;
-        parent = -1;
-      }
-      sh.parents[i] = parent;
+  if (rank == 0 && walk.length > 1)
+    for (int i = threadIdx.x; i < walk.length; i += THREADS) sh.path[i] = pdl_ld(a.path + (int64_t)b * a.n_tokens + i);
+  for (int i = threadIdx.x; i < count; i += THREADS) {
+    const int64_t at = (int64_t)b * a.n_tokens + i;
+    int parent = a.parents ? pdl_ld(a.parents + at) : i - 1;
+    if (parent < -1 || parent >= i) {
+      a.status[WDC_STATUS_DRAFT] = 1;
+      parent = -1;
+    }
+    sh.parents[i] = parent;                        // (of every CTA: all of them know the first command)
+    if (rank == 0) {
       sh.tokens[i] = pdl_ld(a.tokens + at);
       sh.uniforms[i] = a.uniforms ? pdl_ld(a.uniforms + at) : 0.f;
     }
   }
   __syncthreads();
+  if (warp == 0) {
+    Command c = {};
+    c.todo = ROW;
+    c.token = walk.at;
+    c.guess = child_of(sh, walk.at, walk.at, count);
+    c.with_draft = a.draft && c.guess >= 0;        // (the draft's row behind a token without children has no say)
+    if (lane == 0) {
+      sh.command = c;
+      if (walk.length == 1 && a.n_tokens > 0) sh.path[0] = 0;
+    }
+  }
   cluster_sync();                                  // all CTAs of the cluster have begun
 
   float4* const mine = slices + warp * a.chunk;
