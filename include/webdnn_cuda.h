@@ -395,7 +395,8 @@ int wdc_cache_copy_pages(wdc_context* ctx, const wdc_cache_pages_desc* d, void* 
  *   with `interleaved` 2 i and 2 i + 1; cos and sin are [places][rotary / 2], of which the row's position names one (positions
  *   NULL: the row's number).  A position out of range counts as the nearest one.
  * Computed in 32 bits: a result is within 2^-20 (|a| + |b|) of it, or 2^-20 |n|; the squares of large or tiny numbers neither
- * overflow nor vanish.  y may be x (with the same strides); otherwise they do not overlap.
+ * overflow nor vanish.  y may be x (with the same strides); otherwise they do not
+ * overlap (else WDC_ERR_INVALID), though they may be columns of one buffer.  The heads of y do not overlap one another.
  * head_size is a multiple of 4 up to 256, rotary a multiple of 8 up to head_size, 0: none (else WDC_ERR_UNSUPPORTED). */
 typedef struct wdc_rotate_desc {
   int64_t rows, heads, head_size, rotary, places;

@@ -7,10 +7,13 @@ Tolerances, from the arithmetic that the operators promise:
 * rotated keys are computed in 64 bits and rounded once, so codes of rotated keys and kept paths are whole numbers, verdicts are decisions: equal;
 * attention of a tree: as that of a text (test_gpu_paged_cache).
 """
+from ctypes import byref
+
 import numpy as np
 import pytest
 
 from test_gpu_paged_cache import dev, pool_codes, pool_scales, random_pool, reference_append, run_attention, set_pool, tables
+from webdnn_b200 import lib
 from webdnn_b200.lib import CudaBackendError
 from webdnn_b200.paged_cache import PagedCache
 
@@ -753,3 +756,41 @@ def test_rows_of_drafts_behind_tokens_without_children_have_no_say(cuda_context,
     ctx.sync()
     assert_verdicts(got, logits, tokens, parents, None, uniforms, draft, 1.0)
     assert got[1].tolist() == [1, 2, 3, 3] * (batch // 4) and (got[2] >= 0).all()
+
+
+# -------------------------------------------------------------------------------------------------- results beside operands
+def test_heads_that_overlap_others_are_refused(cuda_context):
+    """What groups write in no order must not be what others still read; columns of one buffer are no overlap."""
+    ctx, rng = cuda_context, np.random.default_rng(21)
+    rows, heads, c, wide = 700, 3, 32, 200
+    x = rng.standard_normal((rows, wide)).astype(f32)
+    room = dev(ctx, np.concatenate([x.reshape(-1), np.zeros(4 * wide, f32)]))
+    cos, sin = tables_of(rows, 16)
+    tc, ts = dev(ctx, cos), dev(ctx, sin)
+
+    def call(y, y_st=wide, y_sh=c, n=rows):
+        desc = lib.RotateDesc(n, heads, c, 32, rows, wide, c, y_st, y_sh, 1e-6, 0)
+        ctx._call("wdc_rotate_heads", byref(desc), room.ptr, None, tc.ptr, ts.ptr, None, room.ptr + 4 * y)
+
+    width = heads * c
+    for bad in (dict(y=4), dict(y=c), dict(y=width - 4), dict(y=wide), dict(y=5 * wide), dict(y=5 * wide + width - 4), dict(y=wide - 4), dict(y=0, y_st=width),
+                dict(y=0, y_st=wide + 4), dict(y=width, y_st=width), dict(y=0, y_sh=c + 4), dict(y=width, y_sh=2 * c), dict(y=c, n=1)):
+        with pytest.raises(CudaBackendError, match="overlaps"):
+            call(**bad)
+    borrowed = ctx.borrow_tensor(room.ptr + 16, [rows, wide], "float32", owner=room)
+    whole = ctx.borrow_tensor(room.ptr, [rows, wide], "float32", owner=room)
+    with pytest.raises(CudaBackendError, match="overlaps"):
+        ctx.rotate_heads(whole, wide // 40, 40, out=borrowed)
+    ctx.sync()
+    assert np.array_equal(room.get_data()[:rows * wide].reshape(rows, wide), x)
+    want = x.copy()
+    call(width)                                      # beside x, and then in its place
+    got = room.get_data()[:rows * wide].reshape(rows, wide)
+    assert_heads(got[:, width:2 * width].reshape(rows, heads, c), x[:, :width].reshape(rows, heads, c), None, cos, sin, 1e-6, False)
+    want[:, width:2 * width] = got[:, width:2 * width]
+    assert np.array_equal(got, want)
+    call(0)
+    assert np.array_equal(room.get_data()[:rows * wide].reshape(rows, wide)[:, :width], got[:, width:2 * width])
+    call(wide, n=1)                                  # (one row, behind itself)
+    ctx.sync()
+    dispose(borrowed, whole, room, tc, ts)

@@ -200,6 +200,39 @@ __device__ __forceinline__ void rotate_heads_of(const HeadRotation& r, const flo
   }
 }
 
+// Heads in memory: `size` floats at every batch * stride[0] + row * stride[1] + head * stride[2].
+struct HeadRows {
+  const float* at;
+  int64_t count[3], stride[3], size;
+  bool any() const { return at && count[0] > 0 && count[1] > 0 && count[2] > 0; }
+  // Floats from the first to behind the last, of the strides that are no multiple of `pitch` (0: of all).
+  int64_t span(int64_t pitch) const {
+    int64_t n = size;
+    for (int i = 0; i < 3; i++)
+      if (count[i] > 1 && (pitch == 0 || stride[i] % pitch)) n += (count[i] - 1) * stride[i];
+    return n;
+  }
+  bool same(const HeadRows& o) const {
+    bool same = at == o.at;
+    for (int i = 0; i < 3; i++) same = same && (count[i] <= 1 || stride[i] == o.stride[i]);
+    return same;
+  }
+};
+// Whether heads that are written may be some of those that are read.  (Columns of one buffer, both in rows as wide as that, lie
+// beside one another.)
+static inline bool heads_overlap(const HeadRows& x, const HeadRows& y) {
+  if (!x.any() || !y.any()) return false;
+  const uintptr_t from_x = reinterpret_cast<uintptr_t>(x.at), from_y = reinterpret_cast<uintptr_t>(y.at);
+  if (from_x + 4 * x.span(0) <= from_y || from_y + 4 * y.span(0) <= from_x) return false;
+  const int64_t apart = from_y > from_x ? (int64_t)(from_y - from_x) / 4 : -((int64_t)(from_x - from_y) / 4);
+  for (const int64_t pitch : {x.stride[0], x.stride[1], x.stride[2], y.stride[0], y.stride[1], y.stride[2]}) {
+    if (pitch == 0) continue;
+    const int64_t behind = (apart % pitch + pitch) % pitch, x_wide = x.span(pitch), y_wide = y.span(pitch);
+    if (x_wide <= behind && y_wide <= pitch - behind) return false;
+  }
+  return true;
+}
+
 static inline int rotation_check(wdc_context* ctx, const char* who, HeadRotation& r, int64_t head_size, int64_t rotary, int64_t places,
                                  const float* cos, const float* sin, const int32_t* positions, float epsilon, int interleaved) {
   WDC_REQUIRE(ctx, rotary >= 0 && rotary <= head_size && places >= 0 && places < (1ll << 31), "%s: bad rotation", who);

@@ -69,6 +69,9 @@ extern "C" int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, cons
   CACHE_TRY(rotation_check(ctx, "wdc_rotate_heads", a.rotation, d->head_size, d->rotary, d->places, cos, sin, positions, d->epsilon, d->interleaved));
   WDC_REQUIRE(ctx, x && y, "wdc_rotate_heads: null argument");
   WDC_REQUIRE(ctx, cache_aligned(x, 16) && cache_aligned(y, 16) && cache_aligned(weight, 16), "wdc_rotate_heads: buffers are not aligned");
+  // (groups write in no order: what others are still to read would be gone)
+  const HeadRows from = {x, {1, d->rows, d->heads}, {0, d->x_st, d->x_sh}, d->head_size}, to = {y, {1, d->rows, d->heads}, {0, d->y_st, d->y_sh}, d->head_size};
+  WDC_REQUIRE(ctx, from.same(to) || !heads_overlap(from, to), "wdc_rotate_heads: y overlaps x and is not x");
   DeviceGuard g(ctx->device);
   const int slots = (a.head_size / 4 + 1) / 2;
   // Lanes, slots and heads a group by what was measured with CTAs of 256 threads, us of 173 million numbers (floor 22): heads of 32 26.2 (two
