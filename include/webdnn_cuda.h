@@ -408,8 +408,9 @@ int wdc_rotate_heads(wdc_context* ctx, const wdc_rotate_desc* d, const float* x,
                      const float* sin, const int32_t* positions, float* y);
 
 /* wdc_cache_append of keys that are normalised and rotated like wdc_rotate_heads' on the way, but in 64 bits and rounded once (their codes
- * hang on the last bit); where q is given, its heads are as wdc_rotate_heads' are, into q_out (rows of padding become zero).  Nothing of q is written unless q_out is q (with the same strides); otherwise they do not
- * overlap.  positions is int32 [batch][tokens] or NULL (a token's place in its sequence); one out of range counts as the nearest one. */
+ * hang on the last bit); where q is given, its heads are as wdc_rotate_heads' are, into q_out (rows of padding become
+ * zero).  q_out may be q (with the same strides); otherwise it overlaps neither q nor k nor v (else WDC_ERR_INVALID), though all may be
+ * columns of one buffer.  positions is int32 [batch][tokens] or NULL (a token's place in its sequence); one out of range counts as the nearest one. */
 typedef struct wdc_cache_append_rotary_desc {
   wdc_cache_append_desc append;
   int64_t heads; /* of q */

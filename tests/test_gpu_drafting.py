@@ -794,3 +794,58 @@ def test_heads_that_overlap_others_are_refused(cuda_context):
     call(wide, n=1)                                  # (one row, behind itself)
     ctx.sync()
     dispose(borrowed, whole, room, tc, ts)
+
+
+def test_queries_of_an_append_that_overlap_its_operands_are_refused(cuda_context):
+    """Keys are read by other groups than those that write queries.  Results that are columns of the operands' buffer are no overlap."""
+    ctx, rng = cuda_context, np.random.default_rng(22)
+    batch, tokens, heads, kv_heads, c, size = 3, 40, 4, 2, 32, 16
+    width, wide = heads * c, (2 * heads + 2 * kv_heads) * c
+    fused = rng.standard_normal((batch, tokens, wide)).astype(f32)          # q, k, v, and a place for the result
+    k0, v0, y0 = width, width + kv_heads * c, width + 2 * kv_heads * c
+    lengths, counts = [50, 40, 45], [40, 33, 1]
+    cache = PagedCache(ctx, 1, 20, kv_heads, c, size)
+    codes, scales = random_pool(rng, cache)
+    room, table = dev(ctx, np.concatenate([fused.reshape(-1), np.zeros(batch * tokens * wide, f32)])), tables(rng, cache, lengths)
+    where = [dev(ctx, np.asarray(a, np.int32)) for a in (table, lengths, counts)]
+    cos, sin = tables_of(60, 16)
+    tc, ts = dev(ctx, cos), dev(ctx, sin)
+
+    def call(y, q=0, y_sb=tokens * wide, y_st=wide, y_sh=c):
+        append = lib.CacheAppendDesc(20, kv_heads, size, c, batch, tokens, table.shape[1], tokens * wide, c, wide, tokens * wide, c, wide)
+        desc = lib.CacheAppendRotaryDesc(append, heads, tokens * wide, c, wide, y_sb, y_sh, y_st, 32, 60, 1e-6, 0)
+        ctx._call("wdc_cache_append_rotary", byref(desc), room.ptr + 4 * q, room.ptr + 4 * k0, room.ptr + 4 * v0, None, None, tc.ptr, ts.ptr, None,
+                  cache.codes.ptr, cache.scales.ptr, *[t.ptr for t in where], room.ptr + 4 * y)
+
+    behind = batch * tokens * wide
+    for bad in (dict(y=4), dict(y=k0), dict(y=k0 - c), dict(y=v0), dict(y=v0 + 4), dict(y=y0 - 4), dict(y=wide), dict(y=0, y_st=width), dict(y=0, y_sb=tokens * wide + 4),
+                dict(y=y0, y_st=width, y_sb=tokens * width), dict(y=behind - width - 4, y_st=width, y_sb=tokens * width), dict(y=y0, q=y0 - 4)):
+        with pytest.raises(CudaBackendError, match="overlaps"):
+            call(**bad)
+    # the call of a program whose queries come out where its keys are
+    whole = ctx.borrow_tensor(room.ptr, [batch, tokens, wide], "float32", owner=room)
+    out = ctx.borrow_tensor(room.ptr, [batch, tokens, width], "float32", owner=room)
+    keys = ctx.borrow_tensor(room.ptr, [batch, tokens, width], "float32", owner=room)
+    for args in (dict(q=whole, heads=heads, out=out), dict(q=dev(ctx, np.zeros((batch, tokens, width), f32)), out=keys)):
+        with pytest.raises((CudaBackendError, ValueError)):
+            cache.append_rotary(0, whole, whole, *where, cos=tc, sin=ts, k_column=k0, v_column=v0, **args)
+    ctx.sync()
+    assert np.array_equal(room.get_data()[:behind], fused.reshape(-1)) and np.array_equal(pool_codes(cache), codes)
+    positions = np.minimum((np.array(lengths) - counts)[:, None] + np.arange(tokens), 59)
+    there = np.arange(tokens) < np.array(counts)[:, None]
+    heads_of = lambda a, at, n: a[..., at:at + n * c].reshape(batch, tokens, n, c)  # noqa: E731
+    turned = rotated(heads_of(fused, k0, kv_heads), None, cos[positions], sin[positions], 0.0, False).astype(f32)
+    reference_append(codes[0], scales[0], turned, heads_of(fused, v0, kv_heads), table, lengths, counts, size)
+    results = []
+    for args in (dict(y=y0), dict(y=behind), dict(y=0)):     # beside the operands, behind them, in the queries' place
+        call(**args)
+        got = room.get_data()
+        results.append(heads_of(got[args["y"] // behind * behind:][:behind].reshape(fused.shape), args["y"] % behind, heads))
+        assert np.array_equal(pool_codes(cache), codes) and np.array_equal(pool_scales(cache), scales)
+        kept = got[:behind].reshape(fused.shape)
+        assert np.array_equal(kept[..., k0:y0], fused[..., k0:y0])
+    assert_heads(results[0][there], heads_of(fused, 0, heads)[there], None, cos[positions][there], sin[positions][there], 0.0, False)
+    assert not results[0][~there].any() and all(np.array_equal(results[0], r) for r in results[1:])
+    ctx.sync()
+    dispose(whole, out, keys, room, tc, ts, *where)
+    cache.dispose()

@@ -312,7 +312,13 @@ extern "C" int wdc_cache_append_rotary(wdc_context* ctx, const wdc_cache_append_
   WDC_REQUIRE(ctx, cache_aligned(q, 16) && cache_aligned(q_out, 16) && cache_aligned(q_weight, 16) && cache_aligned(k_weight, 16),
               "%s: buffers are not aligned", who);
   // (other heads are still to be read when the first are written)
-  WDC_REQUIRE(ctx, !q_out || (q_out != k && q_out != v), "%s: q_out is k or v", who);
+  const wdc_cache_append_desc& n = d->append;
+  const auto rows = [&](const float* at, int64_t heads, int64_t sb, int64_t st, int64_t sh) {
+    return HeadRows{at, {n.batch, n.tokens, heads}, {sb, st, sh}, n.head_size};
+  };
+  const HeadRows from = rows(q, d->heads, d->q_sb, d->q_st, d->q_sh), to = rows(q_out, d->heads, d->y_sb, d->y_st, d->y_sh);
+  WDC_REQUIRE(ctx, (from.same(to) || !heads_overlap(from, to)) && !heads_overlap(rows(k, n.kv_heads, n.k_sb, n.k_st, n.k_sh), to) &&
+              !heads_overlap(rows(v, n.kv_heads, n.v_sb, n.v_st, n.v_sh), to), "%s: q_out overlaps k or v, or q and is not q", who);
   a.q = q; a.y = q_out; a.q_weight = q_weight; a.k_weight = k_weight;
   a.q_sb = d->q_sb; a.q_sh = d->q_sh; a.q_st = d->q_st;
   a.y_sb = d->y_sb; a.y_sh = d->y_sh; a.y_st = d->y_st;
