@@ -288,3 +288,26 @@ def test_trees_that_do_not_fit_together_are_refused(monkeypatch):
     target.cache.release(s)
     target.cache.release(r)
     assert target.cache.used_pages == 0 and draft.cache.used_pages == 0
+
+
+@pytest.mark.parametrize("depth,width", [(8, 3), (30, 2), (2, 3)])
+def test_trees_beside_the_last_places_have_room(monkeypatch, depth, width):
+    """A tree has several tokens for a place: its pages may be more than those of a text that takes every place."""
+    target, draft, made = decoders(monkeypatch, 50, pages=30)
+    for prompt in (list(range(40)), list(range(49)) + [1] * 12, [3] * 69):
+        (text,) = target.generate([prompt], 70 - len(prompt), draft, depth, width)
+        want = [prompt[-1]]
+        while len(want) <= 70 - len(prompt):
+            want.append(following(want[-1]))
+        assert text == want[1:]
+    assert target.cache.used_pages == 0 and draft.cache.used_pages == 0
+    # and the table of every other call is as wide as before
+    s = target.cache.add_sequence()
+    tree = [4] * 70, [-1] + [0] * 69
+    assert target.decide([s], [tree[0]], [tree[1]], np.zeros((1, 70)))[0][0] == [0]
+    assert made[-1].calls[-1][2].shape == (1, 5)
+    for _ in range(60):
+        target.decide([s], [[4]], [[-1]], np.zeros((1, 1)))
+    assert target.decide([s], [tree[0]], [tree[1]], np.zeros((1, 70)))[0][0] == [0] and target.cache.length(s) == 62
+    assert made[-1].calls[-1][2].shape == (1, 9)
+    target.cache.release(s)

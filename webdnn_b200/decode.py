@@ -116,7 +116,9 @@ class Decoder:
         self._deciding[temperature] = runner
         self.cache.extend(dict(zip(sequences, counts)))
         try:
-            where = self.cache.batch(sequences, counts, self.table_pages)
+            # (a tree beside the last places has more tokens than there are places)
+            pages = max(len(self.cache.sequence_pages(s)) for s in sequences)
+            where = self.cache.batch(sequences, counts, max(self.table_pages, pages))
             outs = runner.run([CPUTensor.from_array(ids), CPUTensor.from_array(places), *where, CPUTensor.from_array(above),
                                                     CPUTensor.from_array(uniforms)])
             path, accepted, following = (t.numpy().copy() for t in outs)
