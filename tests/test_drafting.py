@@ -311,3 +311,24 @@ def test_trees_beside_the_last_places_have_room(monkeypatch, depth, width):
     assert target.decide([s], [tree[0]], [tree[1]], np.zeros((1, 70)))[0][0] == [0] and target.cache.length(s) == 62
     assert made[-1].calls[-1][2].shape == (1, 9)
     target.cache.release(s)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e6, 0.0, float(np.float32(1e-6))])
+def test_the_ends_of_temperatures_pass_through_a_graph(monkeypatch, temperature):
+    """A graph has them as float32, and 1e-6 is a little less there."""
+    from webdnn_b200 import onnx_io
+    model = onnx_io.decode_model(onnx_io.encode_model(zoo.decoder(50, 64, 2, 1, 1, 64, 128, 4, drafts=True, temperature=temperature)))
+    op = operators.CudaVerifyDrafts()
+    op.initialize(next(n for n in model.graph.node if n.op_type == "CudaVerifyDrafts").attribute)
+    context = FakeContext()
+    ints = lambda *dims: context.empty_tensor(list(dims), "int32")  # noqa: E731
+    given = [context.empty_tensor([2, 3, 50]), ints(2, 3), ints(2, 3), ints(2), context.empty_tensor([2, 3])]
+    assert len(op.run(context, given, 3)) == 3
+    op.temperature = op.draft_temperature = temperature
+    assert len(op.run(context, given, 3)) == 3
+    target, _, _ = decoders(monkeypatch, 50)
+    assert target.decide([target.cache.add_sequence()], [[4]], [[-1]], np.zeros((1, 1)), temperature) == [([0], following(4))]
+    for bad in (9.9e-7, 1.0001e6, 1e-50, 1e300, -1e-6, float("nan"), float("inf")):
+        op.temperature = bad
+        with pytest.raises(ValueError):
+            op.run(context, given, 3)

@@ -20,7 +20,7 @@ libwebdnn_cuda.so on the context's stream.
 from __future__ import annotations
 
 import ctypes
-from ctypes import byref, c_void_p
+from ctypes import byref, c_float, c_void_p
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
@@ -118,6 +118,11 @@ class EightbitCPUTensor(CPUTensor):
             from .tensor_loader import scaled_table
             self._decoded = scaled_table(self.scale)[self.codes]
         return self._decoded
+
+
+def is_temperature(t: float) -> bool:
+    """0, or 1e-6 to 1e6, as float32: a graph has 1e-6 as the nearest of those, which is smaller."""
+    return t == 0 or c_float(1e-6).value <= c_float(t).value <= 1e6
 
 
 def like_cpu_tensor(template: TensorImpl, data: np.ndarray) -> CPUTensor:
@@ -765,7 +770,7 @@ class WebDNNCudaContext:
             raise ValueError(f"{who}: draft_logits are [{batch}, {n}, {vocab} or more]")
         draft_temperature = temperature if draft_temperature is None else draft_temperature
         for t in (temperature, draft_temperature):
-            if not (t == 0 or 1e-6 <= t <= 1e6):
+            if not is_temperature(t):
                 raise ValueError(f"{who}: a temperature is 0, or 1e-6 to 1e6")
         if uniforms is None and (temperature != 0 or draft_logits is not None):
             raise ValueError(f"{who}: a temperature, or drafts with a distribution, need uniforms")

@@ -14,7 +14,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 
 from . import zoo
-from .backend import CPUTensor, WebDNNCudaContext
+from .backend import CPUTensor, WebDNNCudaContext, is_temperature
 from .paged_cache import PagedCache
 from .runner import load
 
@@ -108,7 +108,7 @@ class Decoder:
             raise ValueError(f"Decoder.decide: there are places for {self.positions} tokens")
         if ids.min() < 0 or ids.max() >= self.vocab:
             raise ValueError(f"Decoder.decide: tokens are 0 .. {self.vocab - 1}")
-        if not (temperature == 0 or 1e-6 <= temperature <= 1e6):
+        if not is_temperature(temperature):
             raise ValueError("Decoder.decide: a temperature is 0, or 1e-6 to 1e6")
         runner = self._deciding.pop(temperature, None) or self._load(drafts=True, temperature=temperature)
         while len(self._deciding) >= self.MAX_DECIDING:      # (each has the weights once more)
