@@ -332,3 +332,18 @@ def test_the_ends_of_temperatures_pass_through_a_graph(monkeypatch, temperature)
         op.temperature = bad
         with pytest.raises(ValueError):
             op.run(context, given, 3)
+
+
+@pytest.mark.parametrize("ids", [False, True])
+@pytest.mark.parametrize("dims", [[0, 5, 128], [2, 0, 128], [0, 2, 5, 64], [2, 2, 0, 64], [2, 0, 5, 64]])
+def test_rotary_embeddings_of_nothing_are_nothing(dims, ids):
+    op = operators.CudaRotaryEmbedding()
+    op.initialize(make_node("X", [], ["y"], num_heads=2).attribute)
+    context = FakeContext()
+    t = context.empty_tensor
+    tokens = [dims[0], dims[2] if len(dims) == 4 else dims[1]]
+    tables = [t([40, 32]), t([40, 32]), t(tokens, "int32")] if ids else [t([*tokens, 32]), t([*tokens, 32])]
+    (y,) = op.run(context, [t(dims), *tables], 1)
+    assert y.dims == dims and y.data_type == "float32" and not context.calls
+    with pytest.raises(ValueError):
+        op.run(context, [t(dims), t([40, 31]), *tables[1:]], 1)

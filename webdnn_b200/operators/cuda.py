@@ -478,6 +478,8 @@ class CudaRotaryEmbedding(OperatorImpl):
                 raise ValueError(f"RotaryEmbedding: cos_cache and sin_cache are {want}, not {cos.dims} and {sin.dims}")
             if positions is not None:
                 context.asserts_int_rows("RotaryEmbedding", "position_ids", positions, [batch, tokens])
+            if x.length == 0:
+                return [context.empty_tensor(x.dims)]
             # (a table that has a row for each token is a table of batch * tokens places)
             cos, sin = (t if positions is not None else t.alias([batch * tokens, pairs]) for t in (cos, sin))
             if x.ndim == 3:
