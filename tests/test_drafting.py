@@ -347,3 +347,16 @@ def test_rotary_embeddings_of_nothing_are_nothing(dims, ids):
     assert y.dims == dims and y.data_type == "float32" and not context.calls
     with pytest.raises(ValueError):
         op.run(context, [t(dims), t([40, 31]), *tables[1:]], 1)
+
+
+def test_random_numbers_in_64_bits_are_all_below_1(monkeypatch):
+    target, _, made = decoders(monkeypatch, 50)
+    s = target.cache.add_sequence()
+    given = np.array([[1 - 2.0 ** -25, np.nextafter(1.0, 0.0), 0.25]])
+    target.decide([s], [[4, 1, 2]], [[-1, 0, 0]], given)
+    assert made[-1].calls[-1][6].dtype == np.float32 and made[-1].calls[-1][6].tolist() == [[1 - 2.0 ** -24, 1 - 2.0 ** -24, 0.25]]
+    target.decide([s], [[4]], [[-1]], [[0]])
+    for bad in (1.0, 1 + 1e-12, -1e-300, np.nan):
+        with pytest.raises(ValueError):
+            target.decide([s], [[4]], [[-1]], [[bad]])
+    assert target.cache.length(s) == 2

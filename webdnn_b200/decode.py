@@ -95,9 +95,11 @@ class Decoder:
         if len(parents) != len(trees) or not all(len(p) == n and p[0] == -1 and all(0 <= a < i for i, a in enumerate(p) if i)
                                                  for p, n in zip(parents, counts)):
             raise ValueError("Decoder.decide: a token of a tree continues one before it, the first the text")
-        uniforms = np.asarray(uniforms, np.float32)
+        uniforms = np.asarray(uniforms)
         if uniforms.shape != (len(trees), width) or not ((uniforms >= 0) & (uniforms < 1)).all():
             raise ValueError(f"Decoder.decide: uniforms are [{len(trees)}, {width}], from 0 to below 1")
+        # (numbers next to 1 would be 1 as float32)
+        uniforms = np.minimum(uniforms.astype(np.float32), np.float32(1 - 2.0 ** -24))
         before = [self.cache.length(s) for s in sequences]
         ids, places, above = (np.zeros((len(trees), width), np.int32) for _ in range(3))
         for i, (n, tokens, tree) in enumerate(zip(before, trees, parents)):
