@@ -849,3 +849,15 @@ def test_queries_of_an_append_that_overlap_its_operands_are_refused(cuda_context
     ctx.sync()
     dispose(whole, out, keys, room, tc, ts, *where)
     cache.dispose()
+
+
+@pytest.mark.parametrize("wider", [1, 2, 3])
+@pytest.mark.parametrize("vocab", [37, 1002, 20011, 120001])
+def test_verdicts_of_rows_that_begin_at_different_places_in_16_bytes(cuda_context, vocab, wider):
+    rng = np.random.default_rng(vocab + wider)
+    logits, draft, parents, tokens, uniforms = drafted(rng, 6, 7, vocab, "any", True)
+    counts = np.array([7, 7, 6, 5, 7, 1], np.int32)
+    wide = np.concatenate([draft, np.full((6, 7, wider), np.nan, f32)], 2)
+    got = run_verify(cuda_context, logits, tokens, parents, counts, uniforms, wide, 0.9, vocab=vocab)
+    cuda_context.sync()
+    assert_verdicts(got, logits, tokens, parents, counts, uniforms, draft, 0.9)

@@ -275,3 +275,59 @@ def test_a_tape_that_moves_paths_is_not_repeated(cuda_context):
     ctx.sync()
     dispose(*ts)
     cache.dispose()
+
+
+# -------------------------------------------------------------------------------------------------- what the cache holds behind a decision
+@pytest.mark.parametrize("rotary", [False, True])
+def test_what_stands_is_where_its_text_has_it(cuda_context, rotary):
+    """Keys and values of the first layer, which only tokens and their places make, are those of the same text without drafts.  A number is
+    rounded to its page's scale when it comes, when that grows with a tree, when it is moved, and when that makes it grow: four times half a
+    step, and half of one in the other cache; S is the largest scale."""
+    rng = np.random.default_rng(9)
+    target = Decoder(cuda_context, vocab=300, d=128, heads=4, kv_heads=2, layers=2, ffn=128, positions=256, top=4, pages=200, page_tokens=16,
+                     name=f"stands {rotary}", rotary=rotary)
+    texts = [rng.integers(0, 300, n).tolist() for n in (12, 15, 16, 17, 31, 40)]
+    mine = [target.cache.add_sequence() for _ in texts]
+    target.step(mine, [t[:-1] for t in texts], [], [])
+    moved = 0
+    for step in range(3):
+        # the likeliest four behind each text, the likeliest last, and the same again behind each of those
+        trees, parents = [], []
+        for t in texts:
+            tree, above, level = [t[-1]], [-1], [(0, t)]
+            for _ in range(2):
+                probes = [target.cache.add_sequence() for _ in level]
+                *_, best, _ = target.step(probes, [x for _, x in level], [(i, len(x) - 1) for i, (_, x) in enumerate(level)], [0] * len(level))
+                for probe in probes:
+                    target.cache.release(probe)
+                following = []
+                for (at, x), ids in zip(level, best):
+                    for token in ids[::-1].tolist():
+                        following.append((len(tree), x + [token]))
+                        tree.append(token)
+                        above.append(at)
+                level = following
+            trees.append(tree)
+            parents.append(above)
+        found = target.decide(mine, trees, parents, np.zeros((len(texts), len(trees[0]))), 0.0)
+        for i, (path, token) in enumerate(found):
+            moved += path != list(range(len(path)))
+            texts[i] = texts[i] + [trees[i][j] for j in path[1:]] + [token]
+    assert moved >= 9                                # (of 18)
+    plain = [target.cache.add_sequence() for _ in texts]
+    target.step(plain, [t[:-1] for t in texts], [], [])
+    codes, scales = pool_codes(target.cache)[0].astype(np.float64), pool_scales(target.cache)[0].astype(np.float64)
+    whole = codes * scales[..., None, None]
+    for a, b, text in zip(mine, plain, texts):
+        assert target.cache.length(a) == target.cache.length(b) == len(text) - 1
+        rows = []
+        for s in (a, b):
+            pages = target.cache.sequence_pages(s)
+            rows.append(whole[pages].transpose(1, 2, 0, 3, 4).reshape(2, 2, -1, 32)[:, :, :len(text) - 1])
+        most = scales[target.cache.sequence_pages(a) + target.cache.sequence_pages(b)].max(0)[..., None, None]
+        assert (np.abs(rows[0] - rows[1]) <= 2.5 * most + 1e-5 * np.abs(rows[1]).max()).all()
+        # (and tokens that are elsewhere would not pass)
+        assert (np.abs(rows[0][:, :, 1:] - rows[1][:, :, :-1]) > 2.5 * most).any((0, 1, 3)).all()
+    for s in (*mine, *plain):
+        target.cache.release(s)
+    target.close()
