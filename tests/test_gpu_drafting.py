@@ -861,3 +861,24 @@ def test_verdicts_of_rows_that_begin_at_different_places_in_16_bytes(cuda_contex
     got = run_verify(cuda_context, logits, tokens, parents, counts, uniforms, wide, 0.9, vocab=vocab)
     cuda_context.sync()
     assert_verdicts(got, logits, tokens, parents, counts, uniforms, draft, 0.9)
+
+
+@pytest.mark.parametrize("c,heads,kv_heads,lengths,counts,width", [
+    (128, 32, 8, [900], [13], 512), (64, 16, 4, [900, 31], [11, 11], 700), (128, 16, 8, [300, 40, 0], [64, 40, 0], 300), (32, 4, 2, [70], [33], 900)])
+def test_trees_with_tables_that_are_wider_than_their_texts(cuda_context, c, heads, kv_heads, lengths, counts, width):
+    """Most parts of a tile have nothing to do, as with the tables of a program that has them as wide as its longest text may be."""
+    rng = np.random.default_rng(c + width)
+    cache = PagedCache(cuda_context, 1, sum(-(-n // 64) for n in lengths) + 3, kv_heads, c, 64)
+    codes, scales = random_pool(rng, cache)
+    table = tables(rng, cache, lengths)
+    table = np.pad(table, [(0, 0), (0, width - table.shape[1])], constant_values=-1)
+    q = rng.standard_normal((len(lengths), max(counts), heads, c)).astype(f32)
+    for kind in ("any", "chain"):
+        parents = np.stack([random_tree(rng, max(counts), kind) for _ in lengths])
+        got = run_tree(cuda_context, cache, q, table, lengths, counts, parents)
+        cuda_context.sync()
+        want, room = reference_tree(q, codes[0], scales[0], table, lengths, counts, 64, c ** -0.5, parents)
+        assert np.abs(got - want).max() <= room
+        for b, n in enumerate(counts):
+            assert not got[b, n:].any()
+    cache.dispose()

@@ -331,3 +331,12 @@ def test_what_stands_is_where_its_text_has_it(cuda_context, rotary):
     for s in (*mine, *plain):
         target.cache.release(s)
     target.close()
+
+
+def test_texts_are_drafted_up_to_the_last_place(cuda_context):
+    target = Decoder(cuda_context, vocab=300, d=128, heads=4, kv_heads=2, layers=1, ffn=128, positions=64, top=4, pages=60, page_tokens=16, name="last place")
+    prompts = [[1, 2, 3], list(range(40)), list(range(63))]
+    found = [target.generate([p], 64 - len(p), target, depth=5, width=4, temperature=t)[0] for p in prompts for t in (0.0, 1.0)]
+    assert [len(t) for t in found] == [61, 61, 24, 24, 1, 1] and all(0 <= x < 300 for t in found for x in t)
+    assert target.cache.used_pages == 0
+    target.close()
