@@ -444,7 +444,8 @@ int wdc_cache_attention_tree(wdc_context* ctx, const wdc_cache_attention_desc* d
  *   max(p - q, 0) over its sum (p stays where that is 0).  If none stands, `next` is drawn from p with uniforms[0].
  * A token drawn from p with u is the first whose running sum of p passes u times all of it.  uniforms is float32 [batch][tokens], 0
  * <= u < 1 (what is below counts as 0, what is not below 1 as 1 - 2^-24, NaN as 0); it may be NULL at temperature 0 without drafts.
- * The results are those of 64 bits: where 32 bits with a bound of their errors decide, they are used.  Results, which overlap neither
+ * The results are those of weights that are within 2^-42 of the exact ones, summed in 64 bits: where 32 bits with a bound of their
+ * errors decide, they are used.  Results, which overlap neither
  * one another nor what is read (else WDC_ERR_INVALID): path int32 [batch][tokens], the tokens that stand, 0 first, -1 behind them; accepted [batch], how
  * many; next [batch].  A distribution that does not exist (a NaN, +inf, or nothing above -inf) ends the walk with next = -1; a
  * drafted token outside 0 .. vocab - 1 never stands; a sequence whose count is 0 has accepted 0 and next -1, and so has one whose

@@ -108,8 +108,9 @@ __device__ __forceinline__ void append_queries(const RotaryAppendArgs& a, int pa
 //
 // With rotations a thread has float4 in twos, the slots of a head, whose channels are rotated together; and further CTAs take the
 // queries of as many tokens as a page has.  Bound: the CTAs' chains and their instructions (five prompts of up to 2001 tokens, 24 query, 8
-// key heads of 64: 33.2 us, 4.0 TB/s; 64 new tokens, 32 query, 8 key heads of 128: 3.9), so that 1024 threads an SM are worth the few
-// registers that they leave in local memory (33.2 against 34.6 of 768 and 42.8 of 512; heads of 128 in pages of 64 42.3, 44.1, 55.0).
+// key heads of 64: 33.2 us, 4.0 TB/s; 64 new tokens, 32 query, 8 key heads of 128: 3.9), so that 1024 threads an SM are worth the
+// registers that they leave in local memory, 252 bytes of stores and 292 of loads a thread that holds 8 float4 (33.2 against 34.6 of 768 and
+// 42.8 of 512; heads of 128 in pages of 64 42.3, 44.1, 55.0).  Without rotations there are none.
 template <int APPEND_THREADS, int HELD, class Args>
 __global__ void __launch_bounds__(APPEND_THREADS, std::is_same<Args, RotaryAppendArgs>::value ? 1024 / APPEND_THREADS : 0) cache_append_kernel(const Args a) {
   constexpr bool ROTARY = std::is_same<Args, RotaryAppendArgs>::value;

@@ -20,8 +20,9 @@ struct RotateArgs {
 
 // A group of LANES lanes takes EACH heads of a row, SLOTS slots a lane.  y may be x: no two groups have a head.
 //
-// Bound: memory (9001 rows of 24 heads of 80, 139 MB: 26.8 us, 5.2 TB/s; of 16 heads of 128 25.1, 5.9 TB/s); the launch for few (1.6 us).
-// A CTA is a chain of loads, sums and stores, so small ones, which end at different times, keep the memory busy (us of these three and of
+// Bound: the latency of loads (9001 rows of 24 heads of 80, 139 MB: 26.5 us, 5.2 TB/s, at 43% of what DRAM could and 35% of the issue slots: 128
+// registers a thread leave 3.6 warps a scheduler, which wait; of 16 heads of 128 25.1, 5.9 TB/s); the launch for few (1.7 us).
+// A CTA is a chain of loads, sums and stores, so small ones, which end at different times, leave fewer gaps (us of these three and of
 // 500 rows of 8 heads of 128, by threads a CTA: 256 29.9, 26.1, 1.85, 2.09; 128 27.7, 25.2, 1.57, 2.06; 64 27.0, 25.1, 1.56, 2.06; 32 26.7, 25.0,
 // 1.64, 2.35).  CTAS: of 256 threads an SM, that many registers.
 template <int LANES, int SLOTS, int EACH, int CTAS>

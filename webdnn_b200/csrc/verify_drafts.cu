@@ -16,12 +16,13 @@
 //   weights in 32 bits two more of 2^-24; so E = 1.6 * 2^-22 S + 2.2 * 2^-24 sum w |t|, S = sum w.  The last sum is that of -w log2 w,
 //   which is concave: over n weights it is at most S log2(n / S);
 //   a rejection, p / S - q with q of sum 1:  E' = 2 E / S + Eq + 8 * 2^-24  (S is off by E itself; four roundings, and the sum's two).
-// In 64 bits the exponential is 2^(n / 16) from a table times a polynomial in what is left, 11 operations in all.
+// In 64 bits the exponential is 2^(n / 16) from a table times a polynomial in what is left, 11 operations in all, within 2^-42.
 //
 // Bound: what is serial, the chain of a pass (logits to shared memory, weights, sums, two barriers of the cluster, the leader's decision),
 // 12000 to 20000 cycles of which memory has a tenth; 28% of the issue slots are used.  One sequence of 5 new tokens, 32000 in the
-// vocabulary, drafts with their logits: 20 us; 16 of 25, 100003, without them: 48; 64 of 9, 50001, with them: 112, of which the 64-bit kernel
-// has 45 for four walks (64 bits alone: 28.7, 62 and 144).
+// vocabulary, drafts with their logits: 20.6 us; 16 of 25, 100003, without them: 48.6; 64 of 9, 50001, with them: 112, of which the 64-bit kernel
+// has 45 for four walks (64 bits alone: 28.7, 62 and 144).  What 64 bits do alone: temperature 0 (16 of 25, 100003: 58), and drafts with their
+// logits above about 108000 tokens, whose rows have no room in shared memory (one sequence of 5: 25 us of 100000, 77 of 128256).
 #include <limits.h>
 #include <math.h>
 
@@ -953,7 +954,8 @@ extern "C" int wdc_verify_drafts(wdc_context* ctx, const wdc_verify_desc* d, con
   if (a.chunks == 1 && d->temperature > 0.f && (!draft_logits || d->draft_temperature > 0.f)) {
     WDC_CUDA(ctx, cudaLaunchKernelEx(&cfg, verify_drafts_kernel<true>, a));
     CACHE_TRY(wdc_check_launch(ctx, "verify_drafts_kernel"));
-    // (few walks have anything left to do, so that each may have many CTAs)
+    // (few walks have anything left to do, so that each may have many CTAs; the others pay for CTAs that begin, one an SM, and leave: of
+    // 50001 tokens 3 us for one sequence, 4 for 16, 6 for 64)
     a.goes_on = 1;
     while (a.parts < PARTS_MOST && d->vocab / (2 * a.parts) >= PART_LEAST) a.parts *= 2;
     a.chunk = (int)each();
